@@ -98,7 +98,7 @@ def main():
                     help="training rows of the CPU fit sample (10000: the whole table, about a minute of CPU work)")
     ap.add_argument("--rows-only", type=int, default=0,
                     help="profiling: after the fit, only predict this many rows 45 times (5 warm-up) and print the time")
-    ap.add_argument("--kv", choices=("f32", "i16", "i8"), default="f32", help="cache format of --rows-only")
+    ap.add_argument("--kv", choices=("f32", "i16", "i8", "i4"), default="f32", help="cache format of --rows-only")
     args = ap.parse_args()
     if args.gpus != 1:
         print(f"bench.py runs on one GPU only (asked for {args.gpus}); multi-GPU sharding is a design note, not built",
@@ -121,7 +121,7 @@ def main():
 
     if args.rows_only > 0:
         # a profiler's view of one batch size: the fit in the chosen format, then 45 predictions of that many rows
-        fmt = {"f32": abi.KV_F32, "i16": abi.KV_I16, "i8": abi.KV_I8}[args.kv]
+        fmt = abi.KV_NAMES[args.kv]
         n = min(args.rows_only, BATCH)
         fq = fitmod.fit_raw(gpu, w, x_train, y_train, CLASSES, CHUNK, fmt)
         vq = gpu.load(w, fmt, ROWS, CHUNK, fq.layers[0], fq.scales[0])

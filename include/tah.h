@@ -24,6 +24,7 @@
  * chunks of `chunk` training rows, the last one short; a chunk of rc rows is
  *     f32:     [K: d][rc] f32  then [V: d][rc] f32
  *     i16/i8:  [2d scales] f32, then [K: d][rc] ints, then [V: d][rc] ints     (value = int * scale[coordinate])
+ *     i4:      below, at TAH_KV_I4
  * and chunk ci starts at byte ci * record(d, chunk).
  */
 #ifndef TAH_H
@@ -45,8 +46,18 @@ enum {
     TAH_E_SINK = 5      /* the caller's layer sink returned non-zero; the fit stopped there */
 };
 
-/* Stored formats of in-context keys and values: the reference's Kv codes (src/fit.rs:102-127, Kv::from_code). */
-enum { TAH_KV_F32 = 0, TAH_KV_I16 = 1, TAH_KV_I8 = 2 };
+/* Stored formats of in-context keys and values: the reference's Kv codes (src/fit.rs:102-127, Kv::from_code), and
+ * TAH_KV_I4, which the reference does not have (its own readers refuse a bundle that holds it; tah_unpack gives the
+ * values back). A chunk of rc rows in 4 bits, with ng = (rc + 63) / 64 groups of 64 rows from the chunk's start:
+ *     [2d][ng] pairs of bfloat16 (step s, offset z), then [2d][(rc + 1) / 2] bytes of two codes, the even row's in the
+ *     low four bits; a code c from -8 to 7 is stored as c + 8 (the last row's unused four bits are 0)
+ *     value = z + s c, rounded to eleven significant bits
+ * which is 4.5 bits a number at chunks of 256. Packing takes, over a group's finite values, z midway between the least
+ * and the largest (bfloat16, to the nearest) and s the least bfloat16 whose sixteen codes reach both, so that a finite
+ * value is off by at most s / 2 and the eleven bits; a NaN is stored as z, an infinity as the group's last code. A group
+ * whose step would be below 2^-100 is held at its offset, and a magnitude over 2^126 as 2^126: what a packed record
+ * stands for is always finite. */
+enum { TAH_KV_F32 = 0, TAH_KV_I16 = 1, TAH_KV_I8 = 2, TAH_KV_I4 = 3 };
 
 /* One pre-norm attention block, x += attn(norm1 x); x += l2(gelu(l1(norm2 x))) (src/model.rs:27-98).
  * ss_hidden is 0 for a block without the scalable softmax ("QASSMax", src/model.rs:14-24, src/nn.rs:97-152). */
@@ -186,6 +197,17 @@ int tah_predict_rows_dev(tah_dev *dev, const tah_weights *w, const tah_model *mo
  * tah_pack: one stored chunk from its f32 keys and values c ([2d][rc]: the d key rows then the d value rows) to the
  * record of format kv_format, quantised on the card exactly as the reference's pack (src/fit.rs:549-576). */
 int tah_pack(tah_dev *dev, const float *c, int32_t d, int32_t rc, int32_t kv_format, uint8_t *out);
+/* A whole layer's records from its f32 keys and values in chunk layout (2 * rows * d floats), both on the card, as the
+ * fit forms them; the pointers 4-byte aligned. */
+int tah_pack_dev(tah_dev *dev, const float *kv_dev, int32_t d, int32_t rows, int32_t chunk, int32_t kv_format,
+                 uint8_t *records_dev);
+/* The way back, for any format: what a layer's records stand for, as f32 keys and values in chunk layout (2 * rows * d
+ * floats), which are also the layer's f32 records: a member in 4 bits becomes one that the reference reads. No
+ * counterpart in the reference, which widens inside its attention (src/predict.rs:459-499). */
+int tah_unpack(tah_dev *dev, const uint8_t *records, int32_t d, int32_t rows, int32_t chunk, int32_t kv_format,
+               float *kv);
+int tah_unpack_dev(tah_dev *dev, const uint8_t *records_dev, int32_t d, int32_t rows, int32_t chunk, int32_t kv_format,
+                   float *kv_dev);
 
 /* Attend::attend (src/fit.rs:46, Gpu src/gpu.rs:1471-1510): every training row's attention over all training rows
  * of one layer. q [rows][d] (already scaled), kv the layer's exact f32 keys and values in chunk layout

@@ -12,8 +12,8 @@ F32P = ctypes.POINTER(ctypes.c_float)
 U8P = ctypes.POINTER(ctypes.c_uint8)
 
 OK, E_ARG, E_BUDGET, E_DEVICE, E_DECLINED, E_SINK = 0, 1, 2, 3, 4, 5
-KV_F32, KV_I16, KV_I8 = 0, 1, 2
-KV_NAMES = {"f32": KV_F32, "i16": KV_I16, "i8": KV_I8}
+KV_F32, KV_I16, KV_I8, KV_I4 = 0, 1, 2, 3
+KV_NAMES = {"f32": KV_F32, "i16": KV_I16, "i8": KV_I8, "i4": KV_I4}
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libtah_hip.so")
@@ -41,7 +41,9 @@ LAYER_SINK = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int32, U8P
 
 
 def kv_record(kv_format: int, d: int, rc: int) -> int:
-    """`Kv::record` (`src/fit.rs:123-126`): bytes of one stored chunk of `rc` rows."""
+    """`Kv::record` (`src/fit.rs:123-126`): bytes of one stored chunk of `rc` rows (i4: `TAH_KV_I4` in tah.h)."""
+    if kv_format == KV_I4:
+        return 2 * d * (4 * ((rc + 63) // 64) + (rc + 1) // 2)
     w = {KV_F32: 4, KV_I16: 2, KV_I8: 1}[kv_format]
     return 2 * d * rc * w + (0 if kv_format == KV_F32 else 8 * d)
 
@@ -112,6 +114,9 @@ SIGNATURES = {
     "tah_fit_represent": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, F32P, F32P, ctypes.c_int32, ctypes.c_int32,
                                          ctypes.POINTER(ctypes.c_int32), ctypes.c_int32, F32P, F32P, F32P]),
     "tah_pack": (ctypes.c_int, [ctypes.c_void_p, F32P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, U8P]),
+    "tah_pack_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p] + [ctypes.c_int32] * 4 + [ctypes.c_void_p]),
+    "tah_unpack": (ctypes.c_int, [ctypes.c_void_p, U8P] + [ctypes.c_int32] * 4 + [F32P]),
+    "tah_unpack_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p] + [ctypes.c_int32] * 4 + [ctypes.c_void_p]),
     "tah_attend": (ctypes.c_int, [ctypes.c_void_p, F32P, F32P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                   ctypes.c_int32, F32P]),
     "tah_in_context": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, F32P, ctypes.c_int32, F32P, ctypes.c_int32,

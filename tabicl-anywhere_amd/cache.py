@@ -31,7 +31,7 @@ class Cache:
     @classmethod
     def open(cls, bundle: Bundle, prefix: str = "") -> "Cache":
         meta = bundle.i32s(f"{prefix}meta")
-        if meta.size != 7 or np.any(meta < 0) or meta[4] > 2:
+        if meta.size != 7 or np.any(meta < 0) or meta[4] > 3:
             raise BundleError(f"{prefix}meta: not a fitted member's description")
         tree = bundle.i32s(f"{prefix}tree")
         nodes = parse_tree(tree, int(meta[6]))

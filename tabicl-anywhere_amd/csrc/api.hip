@@ -157,10 +157,7 @@ static int guarded(tah_dev *dev, F &&f) {
     }
 }
 
-extern "C" size_t tah_kv_record(int32_t kv_format, int32_t d, int32_t rc) {
-    const size_t w = kv_format == TAH_KV_F32 ? 4 : (kv_format == TAH_KV_I16 ? 2 : 1);
-    return 2 * (size_t)d * rc * w + (kv_format == TAH_KV_F32 ? 0 : 8 * (size_t)d);
-}
+extern "C" size_t tah_kv_record(int32_t kv_format, int32_t d, int32_t rc) { return record_bytes(kv_format, d, rc); }
 
 static size_t layer_bytes(int fmt, int rows, int chunk, int d) {
     return (size_t)(rows / chunk) * tah_kv_record(fmt, d, chunk) + (rows % chunk ? tah_kv_record(fmt, d, rows % chunk) : 0);
@@ -578,7 +575,7 @@ static size_t model_layer_bytes(int kv_format, int rows, int chunk, int d, int h
 }
 
 extern "C" size_t tah_model_bytes(const tah_weights *w, int32_t kv_format, int32_t rows, int32_t chunk) {
-    if (!w || rows <= 0 || chunk <= 0 || kv_format < 0 || kv_format > 2) return 0;
+    if (!w || rows <= 0 || chunk <= 0 || !kv_known(kv_format)) return 0;
     const int d = w->d, layers = w->icl_layers;
     return (size_t)layers * model_layer_bytes(kv_format, rows, chunk, d, w->icl_heads) +
            align256(sizeof(float) * layers * d);
@@ -589,7 +586,7 @@ extern "C" int tah_model_load(tah_dev *dev, const tah_weights *w, int32_t kv_for
     if (!out || !w || !layer_records || !scales) return TAH_E_ARG;
     *out = nullptr;
     return guarded(dev, [&] {
-        if (rows <= 0 || chunk <= 0 || kv_format < 0 || kv_format > 2) throw ArgError{"model: bad rows, chunk or format"};
+        if (rows <= 0 || chunk <= 0 || !kv_known(kv_format)) throw ArgError{"model: bad rows, chunk or format"};
         for (int l = 0; l < w->icl_layers; l++)
             if (!layer_records[l]) throw ArgError{"model: missing layer records"};
         auto *m = new tah_model();
@@ -839,7 +836,7 @@ extern "C" int tah_stage_dev_noalloc(tah_dev *dev, const tah_weights *w, const t
 extern "C" int tah_pack(tah_dev *dev, const float *c, int32_t d, int32_t rc, int32_t kv_format, uint8_t *out) {
     if (!c || !out) return TAH_E_ARG;
     return guarded(dev, [&] {
-        if (d <= 0 || rc <= 0 || kv_format < 0 || kv_format > 2) throw ArgError{"pack: bad size or format"};
+        if (d <= 0 || rc <= 0 || !kv_known(kv_format)) throw ArgError{"pack: bad size or format"};
         Loans loans(dev);
         const size_t n = 2 * (size_t)d * rc, bytes = tah_kv_record(kv_format, d, rc);
         float *cd = loans.take<float>(n);
@@ -850,6 +847,57 @@ extern "C" int tah_pack(tah_dev *dev, const float *c, int32_t d, int32_t rc, int
         else
             pack(dev->stream, rc, d, rc, kv_format, cd, od);
         TAH_HIP(hipMemcpyAsync(out, od, bytes, hipMemcpyDeviceToHost, dev->stream));
+        TAH_HIP(hipStreamSynchronize(dev->stream));
+        return TAH_OK;
+    });
+}
+
+// Chunks are the kernels' grid in one dimension, coordinates in another.
+static void check_layer(const char *what, int d, int rows, int chunk, int kv_format, const void *a, const void *b) {
+    if (d <= 0 || rows < 0 || chunk <= 0 || !kv_known(kv_format)) throw ArgError{std::string(what) + ": bad size or format"};
+    if (2 * (long)d > 65535 || ((long)rows + chunk - 1) / chunk > 65535)
+        throw ArgError{std::string(what) + ": at most 32767 coordinates and 65535 chunks a call"};
+    if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) % 4)
+        throw ArgError{std::string(what) + ": the pointers have to be 4-byte aligned"};
+}
+
+extern "C" int tah_pack_dev(tah_dev *dev, const float *kv_dev, int32_t d, int32_t rows, int32_t chunk, int32_t kv_format,
+                            uint8_t *records_dev) {
+    if (!kv_dev || !records_dev) return TAH_E_ARG;
+    return guarded(dev, [&] {
+        check_layer("pack", d, rows, chunk, kv_format, kv_dev, records_dev);
+        if (rows > 0 && kv_format == TAH_KV_F32)
+            TAH_HIP(hipMemcpyAsync(records_dev, kv_dev, sizeof(float) * 2 * (size_t)rows * d, hipMemcpyDeviceToDevice,
+                                   dev->stream));
+        else
+            pack(dev->stream, rows, d, chunk, kv_format, kv_dev, records_dev);
+        return TAH_OK;
+    });
+}
+
+extern "C" int tah_unpack_dev(tah_dev *dev, const uint8_t *records_dev, int32_t d, int32_t rows, int32_t chunk,
+                              int32_t kv_format, float *kv_dev) {
+    if (!kv_dev || !records_dev) return TAH_E_ARG;
+    return guarded(dev, [&] {
+        check_layer("unpack", d, rows, chunk, kv_format, kv_dev, records_dev);
+        unpack(dev->stream, rows, d, chunk, kv_format, records_dev, kv_dev);
+        return TAH_OK;
+    });
+}
+
+extern "C" int tah_unpack(tah_dev *dev, const uint8_t *records, int32_t d, int32_t rows, int32_t chunk, int32_t kv_format,
+                          float *kv) {
+    if (!records || !kv) return TAH_E_ARG;
+    return guarded(dev, [&] {
+        check_layer("unpack", d, rows, chunk, kv_format, nullptr, nullptr);
+        if (rows == 0) return TAH_OK;
+        Loans loans(dev);
+        const size_t n = 2 * (size_t)rows * d, bytes = layer_bytes(kv_format, rows, chunk, d);
+        uint8_t *rd = loans.take<uint8_t>(bytes);
+        float *kd = loans.take<float>(n);
+        TAH_HIP(hipMemcpyAsync(rd, records, bytes, hipMemcpyHostToDevice, dev->stream));
+        unpack(dev->stream, rows, d, chunk, kv_format, rd, kd);
+        TAH_HIP(hipMemcpyAsync(kv, kd, n * sizeof(float), hipMemcpyDeviceToHost, dev->stream));
         TAH_HIP(hipStreamSynchronize(dev->stream));
         return TAH_OK;
     });
@@ -960,7 +1008,7 @@ static void copy_out(tah_dev *dev, void *dst, const void *src, size_t bytes) {
 }
 
 static void check_in_context(int rows, int kv_format, int chunk) {
-    if (rows <= 0 || chunk <= 0 || kv_format < 0 || kv_format > 2) throw ArgError{"in_context: bad rows, chunk or format"};
+    if (rows <= 0 || chunk <= 0 || !kv_known(kv_format)) throw ArgError{"in_context: bad rows, chunk or format"};
 }
 
 // The in-context stage of a fit from the rows h (on the card, taken over as working memory).

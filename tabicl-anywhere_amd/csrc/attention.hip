@@ -33,6 +33,7 @@
 
 #include "common.hpp"
 #include "device_math.hpp"
+#include "kv4.hpp"
 
 namespace tah {
 
@@ -61,11 +62,6 @@ __host__ __device__ inline KeyBlocks key_blocks(int rows, int chunk) {
     return k;
 }
 
-__host__ __device__ inline size_t record_bytes(int fmt, int d, int rc) {
-    const size_t w = fmt == TAH_KV_F32 ? 4 : (fmt == TAH_KV_I16 ? 2 : 1);
-    return 2 * (size_t)d * rc * w + (fmt == TAH_KV_F32 ? 0 : 8 * (size_t)d);
-}
-
 // Where key block kb lives: its chunk's record, the chunk's row count and the block's first row in it.
 struct Where {
     const uint8_t *rec;
@@ -86,6 +82,7 @@ __device__ inline Where locate(const KeyBlocks &k, int kb, const uint8_t *record
 template <int FMT>
 __device__ __forceinline__ float rec_value(const uint8_t *rec, int d, int rc, int c, int r) {
     if (FMT == TAH_KV_F32) return reinterpret_cast<const float *>(rec)[(size_t)c * rc + r];
+    if (FMT == TAH_KV_I4) return record_value4(rec, d, rc, c, r);
     const float sc = reinterpret_cast<const float *>(rec)[c];
     const uint8_t *body = rec + 8 * (size_t)d;
     if (FMT == TAH_KV_I16) return (float)reinterpret_cast<const int16_t *>(body)[(size_t)c * rc + r] * sc;
@@ -1906,6 +1903,11 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
         case TAH_KV_F32: launch<TAH_KV_F32>(s, a, p, q, records, have ? img : nullptr, out, part_o, part_ml); break;
         case TAH_KV_I16: launch<TAH_KV_I16>(s, a, p, q, records, have ? img : nullptr, out, part_o, part_ml); break;
         case TAH_KV_I8: launch<TAH_KV_I8>(s, a, p, q, records, have ? img : nullptr, out, part_o, part_ml); break;
+        case TAH_KV_I4:
+            hipLaunchKernelGGL(k_attn_decode<TAH_KV_I4>, dim3(p.splits, a.heads, p.groups), dim3(64), 0, s, a.nq, a.rows,
+                               a.chunk, a.d, a.heads, q, records, p.kb_per_split, part_o, part_ml, out);
+            TAH_LAUNCHED();
+            break;
         default: throw ArgError{"attention: unknown key/value format"};
     }
     if (p.splits > 1) {

@@ -150,6 +150,19 @@ struct tah_model {
 
 namespace tah {
 
+// ---- stored chunk records (include/tah.h) -------------------------------------------------------------------------
+constexpr int GROUP4 = 64;  // i4: rows that share a step and an offset
+__host__ __device__ inline int groups4(int rc) { return (rc + GROUP4 - 1) / GROUP4; }
+
+// bytes of one chunk of rc rows
+__host__ __device__ inline size_t record_bytes(int fmt, int d, int rc) {
+    if (fmt == TAH_KV_I4) return 2 * (size_t)d * (4 * (size_t)groups4(rc) + ((size_t)rc + 1) / 2);
+    const size_t w = fmt == TAH_KV_F32 ? 4 : (fmt == TAH_KV_I16 ? 2 : 1);
+    return 2 * (size_t)d * rc * w + (fmt == TAH_KV_F32 ? 0 : 8 * (size_t)d);
+}
+
+inline bool kv_known(int fmt) { return fmt >= TAH_KV_F32 && fmt <= TAH_KV_I4; }
+
 enum Epi { EPI_NONE = 0, EPI_GELU = 1, EPI_RESID = 2, EPI_QMOD = 3, EPI_SCALE = 4 };
 
 // Y[M][N] (leading dim ldy) = epi(X[M][K] (ldx) * W[N][K]^T + b[N]); EPI_RESID adds R (ldr, may alias Y).
@@ -257,7 +270,9 @@ struct AttnShape {
 size_t attention_work_bytes(const AttnShape &a);
 // Row-major keys and values kv [rows][2d] to f32 chunk records (2 * rows * d floats).
 void to_records(hipStream_t s, int rows, int d, int chunk, const float *kv, float *rec32);
-// f32 chunk records to i16/i8 records (the reference's quantiser, bit for bit).
+// f32 chunk records to i16/i8 records (the reference's quantiser, bit for bit) or i4 records; and any format's records to
+// f32 chunk records.
+void unpack(hipStream_t s, int rows, int d, int chunk, int fmt, const uint8_t *rec, float *rec32);
 void pack(hipStream_t s, int rows, int d, int chunk, int fmt, const float *rec32, uint8_t *recq);
 // Keys and values of one stored layer as tiles per (key block of 64, head), the form a fitted layer of head width 64
 // is held in on the card (its records are not kept) and the attention kernels read: f32 as fp16 hi/lo split images,

@@ -1,0 +1,66 @@
+// The 4-bit stored form of keys and values (TAH_KV_I4, include/tah.h): per coordinate and group of 64 rows of a chunk a
+// bfloat16 step s and offset z, per number a code c of -8 .. 7; value = z + s c rounded to eleven significant bits.
+//
+// Why so. A group's sixteen levels span its own range about its own middle: keys and values have a mean of their own per
+// coordinate (the median coordinate's is 0.2 to 0.75 of its spread in the published classifier), which levels about zero
+// would spend codes on (64 test rows of a fitted 900 x 12 table: probabilities move by 0.0012 on average and 0.010 at
+// worst; by 0.0018 and 0.014 with levels about zero and groups of 64, by 0.0019 and 0.021 with groups of 32 at the same
+// bits; in i8 by 0.0002 and 0.002). Groups are key blocks of the attention kernels, which then see one step and one offset
+// a coordinate. And eleven bits are what an fp16 operand of the matrix cores holds: a value times its head's power of two
+// goes in as one operand, exact, where an f32 or i16 value goes in as two halves; that rounding is 2^-12 of a value, far
+// below half a step.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "common.hpp"
+
+namespace tah {
+
+struct Step4 {
+    float s, z;  // bfloat16 values
+};
+
+// v rounded to eleven significant bits, ties to even (infinities stay)
+__device__ __forceinline__ float eleven_bits(float v) {
+    const uint32_t u = __float_as_uint(v);
+    return __uint_as_float((u + 0xFFFu + ((u >> 13) & 1u)) & 0xFFFFE000u);
+}
+
+// s c is exact in f32 (at most eleven bits)
+__device__ __forceinline__ float value4(Step4 st, int code) { return eleven_bits(fmaf(st.s, (float)code, st.z)); }
+
+// the step and offset of a group whose finite values lie from lo to hi (hi < lo: it has none)
+__device__ __forceinline__ Step4 step_for4(float lo, float hi) {
+#pragma clang fp contract(off)
+    Step4 st{0.0f, 0.0f};
+    if (!(lo <= hi)) return st;
+    lo = fminf(fmaxf(lo, -0x1p126f), 0x1p126f);  // so that no difference overflows
+    hi = fminf(fmaxf(hi, -0x1p126f), 0x1p126f);
+    const float mid = lo * (7.0f / 15.0f) + hi * (8.0f / 15.0f) + 0.0f;  // a zero is +0, whichever zeros lo and hi are
+    const uint32_t u = __float_as_uint(mid);
+    st.z = __uint_as_float((u + 0x7FFFu + ((u >> 16) & 1u)) & 0xFFFF0000u);
+    const float s = fmaxf((hi - st.z) * (1.0f / 7.0f), (st.z - lo) * 0.125f);
+    st.s = s < 0x1p-100f ? 0.0f : __uint_as_float((__float_as_uint(s) + 0xFFFFu) & 0xFFFF0000u);
+    return st;
+}
+
+// the code of a value: the nearest level (the quotient correctly rounded never meets a tie that the exact one does not:
+// a tie is a product of twelve bits with s, and a float beside it is off by more than half the quotient's last place)
+__device__ __forceinline__ int code4(Step4 st, float v) {
+    if (!(st.s > 0.0f) || v != v) return 0;
+    return (int)fminf(fmaxf(rintf(__fdiv_rn(v - st.z, st.s)), -8.0f), 7.0f);
+}
+
+__device__ __forceinline__ Step4 step_at4(const uint8_t *rec, int rc, int j, int g) {
+    const uint16_t *p = reinterpret_cast<const uint16_t *>(rec) + 2 * ((size_t)j * groups4(rc) + g);
+    return {__uint_as_float((uint32_t)p[0] << 16), __uint_as_float((uint32_t)p[1] << 16)};
+}
+
+// number (stacked coordinate j of 2d, row r) of a chunk's record
+__device__ __forceinline__ float record_value4(const uint8_t *rec, int d, int rc, int j, int r) {
+    const uint8_t b = rec[8 * (size_t)d * groups4(rc) + (size_t)j * ((rc + 1) / 2) + (r >> 1)];
+    return value4(step_at4(rec, rc, j, r / GROUP4), (int)(b >> 4 * (r & 1) & 15) - 8);
+}
+
+}  // namespace tah

@@ -9,8 +9,13 @@
 //   or 127, inv = 1 / s, code = round-half-away(v * inv) saturated to the integer range; the 2d scales first.
 //   One wavefront per coordinate row. Division is the correctly rounded one (__fdiv_rn), so the same f32 input
 //   gives the same scales and codes as the CPU.
+// * k_pack4: f32 records to i4 records.
+// * k_unpack: records of any format to f32 records.
+#include <algorithm>
+
 #include "common.hpp"
 #include "device_math.hpp"
+#include "kv4.hpp"
 
 namespace tah {
 
@@ -65,6 +70,48 @@ __global__ __launch_bounds__(256) void k_pack(int rows, int d, int chunk, const 
     }
 }
 
+// grid (groups of the layer, 2d / 4); 256 threads: a wavefront a group of one coordinate, a lane a row.
+__global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, int per_chunk, const float *__restrict__ rec32,
+                                               uint8_t *__restrict__ rec4) {
+    const int j = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (j >= 2 * d) return;
+    const int ci = blockIdx.x / per_chunk, g = blockIdx.x % per_chunk;
+    const int rc = min(chunk, rows - ci * chunk), r = g * GROUP4 + lane;
+    if (g * GROUP4 >= rc) return;
+    const bool in = r < rc;
+    const float v = in ? rec32[(size_t)ci * 2 * d * chunk + (size_t)j * rc + r] : 0.0f;
+    const bool fin = in && fabsf(v) < INFINITY;
+    const float lo = -wave_max(fin ? -v : -INFINITY), hi = wave_max(fin ? v : -INFINITY);
+    const Step4 st = step_for4(lo, hi);
+    const int code = in ? code4(st, v) + 8 : 0;
+    uint8_t *rec = rec4 + (size_t)ci * record_bytes(TAH_KV_I4, d, chunk);
+    if (lane < 2)
+        reinterpret_cast<uint16_t *>(rec)[2 * ((size_t)j * groups4(rc) + g) + lane] =
+            (uint16_t)(__float_as_uint(lane == 0 ? st.s : st.z) >> 16);
+    const int next = __shfl_down(code, 1);
+    if (in && !(lane & 1))
+        rec[8 * (size_t)d * groups4(rc) + (size_t)j * ((rc + 1) / 2) + (r >> 1)] = (uint8_t)(code | next << 4);
+}
+
+// grid (ceil(rows of a chunk / 256), 2d, chunks); 256 threads, a row each.
+template <int FMT>
+__global__ __launch_bounds__(256) void k_unpack(int rows, int d, int chunk, const uint8_t *__restrict__ rec,
+                                                float *__restrict__ rec32) {
+    const int j = blockIdx.y, ci = blockIdx.z, rc = min(chunk, rows - ci * chunk), r = blockIdx.x * 256 + threadIdx.x;
+    if (r >= rc) return;
+    const uint8_t *src = rec + (size_t)ci * record_bytes(FMT, d, chunk);
+    float v;
+    if constexpr (FMT == TAH_KV_I4) {
+        v = record_value4(src, d, rc, j, r);
+    } else {
+        const float s = reinterpret_cast<const float *>(src)[j];
+        const size_t at = (size_t)j * rc + r;
+        src += 8 * (size_t)d;
+        v = s * (FMT == TAH_KV_I16 ? (float)reinterpret_cast<const int16_t *>(src)[at] : (float)reinterpret_cast<const int8_t *>(src)[at]);
+    }
+    rec32[(size_t)ci * 2 * d * chunk + (size_t)j * rc + r] = v;
+}
+
 void to_records(hipStream_t s, int rows, int d, int chunk, const float *kv, float *rec32) {
     if (rows <= 0) return;
     dim3 grid((rows + 63) / 64, (2 * d + 63) / 64);
@@ -76,12 +123,30 @@ void pack(hipStream_t s, int rows, int d, int chunk, int fmt, const float *rec32
     if (rows <= 0 || fmt == TAH_KV_F32) return;
     const int n_chunks = (rows + chunk - 1) / chunk;
     dim3 grid(n_chunks, (2 * d + 3) / 4);
-    if (fmt == TAH_KV_I16)
+    if (fmt == TAH_KV_I4) {
+        const int per_chunk = groups4(chunk);
+        hipLaunchKernelGGL(k_pack4, dim3(n_chunks * per_chunk, grid.y), dim3(256), 0, s, rows, d, chunk, per_chunk, rec32, recq);
+    } else if (fmt == TAH_KV_I16)
         hipLaunchKernelGGL(k_pack<TAH_KV_I16>, grid, dim3(256), 0, s, rows, d, chunk, rec32, recq);
     else if (fmt == TAH_KV_I8)
         hipLaunchKernelGGL(k_pack<TAH_KV_I8>, grid, dim3(256), 0, s, rows, d, chunk, rec32, recq);
     else
         throw ArgError{"pack: unknown key/value format"};
+    TAH_LAUNCHED();
+}
+
+void unpack(hipStream_t s, int rows, int d, int chunk, int fmt, const uint8_t *rec, float *rec32) {
+    if (rows <= 0) return;
+    const int n_chunks = (rows + chunk - 1) / chunk;
+    const dim3 grid((std::min(chunk, rows) + 255) / 256, 2 * d, n_chunks);
+    if (fmt == TAH_KV_F32)
+        TAH_HIP(hipMemcpyAsync(rec32, rec, sizeof(float) * 2 * (size_t)rows * d, hipMemcpyDeviceToDevice, s));
+    else if (fmt == TAH_KV_I16)
+        hipLaunchKernelGGL(k_unpack<TAH_KV_I16>, grid, dim3(256), 0, s, rows, d, chunk, rec, rec32);
+    else if (fmt == TAH_KV_I8)
+        hipLaunchKernelGGL(k_unpack<TAH_KV_I8>, grid, dim3(256), 0, s, rows, d, chunk, rec, rec32);
+    else
+        hipLaunchKernelGGL(k_unpack<TAH_KV_I4>, grid, dim3(256), 0, s, rows, d, chunk, rec, rec32);
     TAH_LAUNCHED();
 }
 

@@ -295,6 +295,27 @@ class Gpu:
         self._check(self._l.tah_pack(self._h, _fp(c), int(d), int(rc), int(kv_format), out.ctypes.data_as(abi.U8P)))
         return out
 
+    def pack_dev(self, kv_ptr: int, d: int, rows: int, chunk: int, kv_format: int, records_ptr: int) -> None:
+        """A whole layer's records from its f32 keys and values in chunk layout, both in device memory."""
+        self._check(self._l.tah_pack_dev(self._h, kv_ptr, d, rows, chunk, kv_format, records_ptr))
+
+    def unpack(self, records, d: int, rows: int, chunk: int, kv_format: int) -> np.ndarray:
+        """What a layer's stored records stand for: its f32 keys and values in chunk layout (a flat array of
+        2 * rows * d, which are its f32 records)."""
+        records = np.ascontiguousarray(records, np.uint8).reshape(-1)
+        if d <= 0 or rows < 0 or chunk <= 0 or kv_format not in abi.KV_NAMES.values():
+            raise ValueError("unpack: bad size or format")
+        if records.size != abi.layer_bytes(kv_format, rows, chunk, d):
+            raise ValueError(f"unpack: expected {abi.layer_bytes(kv_format, rows, chunk, d)} bytes of records")
+        out = np.empty(2 * rows * d, np.float32)
+        self._check(self._l.tah_unpack(self._h, records.ctypes.data_as(abi.U8P), int(d), int(rows), int(chunk),
+                                       int(kv_format), _fp(out)))
+        return out
+
+    def unpack_dev(self, records_ptr: int, d: int, rows: int, chunk: int, kv_format: int, kv_ptr: int) -> None:
+        """`unpack` with the records and the values in device memory."""
+        self._check(self._l.tah_unpack_dev(self._h, records_ptr, d, rows, chunk, kv_format, kv_ptr))
+
     def attend(self, q, kv, rows: int, chunk: int, d: int, heads: int) -> np.ndarray:
         """`Attend::attend`: all rows' attention over the layer's exact f32 keys and values (chunk layout)."""
         q, kv = _f32(q), _f32(kv).reshape(-1)
