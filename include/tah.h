@@ -301,6 +301,23 @@ int tah_quantile_stats(tah_dev *dev, const float *q, int32_t rows, int32_t n, co
 int tah_quantile_stats_dev(tah_dev *dev, const float *q_dev, int32_t rows, int32_t n, const float *alphas,
                            int32_t n_alphas, float *stats_dev);
 
+/* ---- the classification head ------------------------------------------------------------------------------------
+ *
+ * Rows of class scores read as distributions at a softmax temperature (finish_proba, src/table.rs:70-78, in
+ * logarithms): scores [rows][n] (n from 1 to 2^24); given [rows][n_given] class ids whose log probabilities are wanted,
+ * top how many of the most probable classes (n_given and top at most 64, top at most n; either may be 0, its pointers
+ * then NULL). Writes stats [rows][1 + n_given + top]: the entropy in nats, log p of each given class, log p of the top
+ * most probable ones, falling; and ids [rows][top], those classes (the lower id first among equal scores, NaN after
+ * every number). A score of -inf is a class ruled out; a row of nothing else has entropy 0 and every log p -inf. A row
+ * with a NaN or +inf has NaN for all of them. A given id of -1 means none: its log p is NaN. Ids outside [-1, n) fail
+ * with TAH_E_ARG. No counterpart in the reference, which stops at the probabilities. */
+int tah_class_stats(tah_dev *dev, const float *scores, int32_t rows, int32_t n, float temperature,
+                    const int32_t *given, int32_t n_given, int32_t top, float *stats, int32_t *ids);
+/* The same with every array in device memory, and rows of scores ld floats apart (0: n); queued on the handle's stream.
+ * The given ids are not looked at beforehand: one outside [0, n) gives NaN. */
+int tah_class_stats_dev(tah_dev *dev, const float *scores_dev, int32_t rows, int32_t n, int64_t ld, float temperature,
+                        const int32_t *given_dev, int32_t n_given, int32_t top, float *stats_dev, int32_t *ids_dev);
+
 #ifdef __cplusplus
 }
 #endif

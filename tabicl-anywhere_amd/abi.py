@@ -10,6 +10,7 @@ import os
 
 F32P = ctypes.POINTER(ctypes.c_float)
 U8P = ctypes.POINTER(ctypes.c_uint8)
+I32P = ctypes.POINTER(ctypes.c_int32)
 
 OK, E_ARG, E_BUDGET, E_DEVICE, E_DECLINED, E_SINK = 0, 1, 2, 3, 4, 5
 KV_F32, KV_I16, KV_I8, KV_I4 = 0, 1, 2, 3
@@ -136,6 +137,11 @@ SIGNATURES = {
     "tah_probe_read": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int32)]),
     "tah_quantile_stats": (ctypes.c_int, [ctypes.c_void_p, F32P, ctypes.c_int32, ctypes.c_int32, F32P,
                                           ctypes.c_int32, F32P]),
+    "tah_class_stats": (ctypes.c_int, [ctypes.c_void_p, F32P, ctypes.c_int32, ctypes.c_int32, ctypes.c_float, I32P,
+                                       ctypes.c_int32, ctypes.c_int32, F32P, I32P]),
+    "tah_class_stats_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
+                                           ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_int32,
+                                           ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),
     "tah_quantile_stats_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, F32P,
                                               ctypes.c_int32, ctypes.c_void_p]),
 }

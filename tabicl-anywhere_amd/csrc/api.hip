@@ -960,6 +960,52 @@ extern "C" int tah_quantile_stats(tah_dev *dev, const float *q, int32_t rows, in
     });
 }
 
+// ---- the classification head -----------------------------------------------------------------------------------
+static void check_classes(int rows, int n, long ld, float temperature, const int32_t *given, int n_given, int top,
+                          const int32_t *ids) {
+    if (rows < 0 || n < 1 || n > 1 << 24 || ld < n)
+        throw ArgError{"class_stats: 1 to 2^24 classes a row, rows at least that far apart"};
+    if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.0f / temperature))
+        throw ArgError{"class_stats: the temperature has to be positive"};
+    if (n_given < 0 || n_given > 64 || top < 0 || top > 64 || top > n || (n_given > 0 && !given) || (top > 0 && !ids))
+        throw ArgError{"class_stats: at most 64 given classes and 64 of the most probable, no more than there are"};
+}
+
+extern "C" int tah_class_stats_dev(tah_dev *dev, const float *scores_dev, int32_t rows, int32_t n, int64_t ld,
+                                   float temperature, const int32_t *given_dev, int32_t n_given, int32_t top,
+                                   float *stats_dev, int32_t *ids_dev) {
+    if (!scores_dev || !stats_dev) return TAH_E_ARG;
+    return guarded(dev, [&] {
+        if (ld == 0) ld = n;
+        check_classes(rows, n, ld, temperature, given_dev, n_given, top, ids_dev);
+        class_stats(dev->stream, rows, n, (size_t)ld, scores_dev, temperature, given_dev, n_given, top, stats_dev, ids_dev);
+        return TAH_OK;
+    });
+}
+
+extern "C" int tah_class_stats(tah_dev *dev, const float *scores, int32_t rows, int32_t n, float temperature,
+                               const int32_t *given, int32_t n_given, int32_t top, float *stats, int32_t *ids) {
+    if (!scores || !stats) return TAH_E_ARG;
+    return guarded(dev, [&] {
+        check_classes(rows, n, n, temperature, given, n_given, top, ids);
+        for (size_t i = 0; i < (size_t)rows * n_given; i++)
+            if (given[i] < -1 || given[i] >= n) throw ArgError{"class_stats: a given class out of range"};
+        if (rows == 0) return TAH_OK;
+        Loans loans(dev);
+        const size_t nin = (size_t)rows * n, ng = (size_t)rows * n_given, nt = (size_t)rows * top;
+        const size_t nout = (size_t)rows * (1 + n_given + top);
+        float *xd = loans.take<float>(nin), *sd = loans.take<float>(nout);
+        int32_t *gd = loans.take<int32_t>(ng), *id = loans.take<int32_t>(nt);
+        TAH_HIP(hipMemcpyAsync(xd, scores, sizeof(float) * nin, hipMemcpyHostToDevice, dev->stream));
+        if (ng) TAH_HIP(hipMemcpyAsync(gd, given, sizeof(int32_t) * ng, hipMemcpyHostToDevice, dev->stream));
+        class_stats(dev->stream, rows, n, n, xd, temperature, gd, n_given, top, sd, id);
+        TAH_HIP(hipMemcpyAsync(stats, sd, sizeof(float) * nout, hipMemcpyDeviceToHost, dev->stream));
+        if (nt) TAH_HIP(hipMemcpyAsync(ids, id, sizeof(int32_t) * nt, hipMemcpyDeviceToHost, dev->stream));
+        TAH_HIP(hipStreamSynchronize(dev->stream));
+        return TAH_OK;
+    });
+}
+
 // The device's two pinned staging buffers for records and column caches on their way to the host, at least `bytes` each.
 static void staging(tah_dev *dev, size_t bytes) {
     for (int i = 0; i < 2; i++)

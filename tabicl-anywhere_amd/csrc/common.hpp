@@ -306,6 +306,11 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
 // (device) into stats [rows][3 + na].
 void quantile_stats(hipStream_t s, int rows, int n, const float *q, int na, const float *alphas, float *stats);
 
+// The classification head (class_stats.hip): rows of scores x (ld apart) to stats [rows][1 + n_given + top] and ids
+// [rows][top].
+void class_stats(hipStream_t s, int rows, int n, size_t ld, const float *x, float temperature, const int32_t *given,
+                 int n_given, int top, float *stats, int32_t *ids);
+
 // Column and row stages (stages.hip).
 // The input layer for n rows x [n][features]: cells [n][cls + features][e], the weights' class tokens first where
 // cls > 0 (cls 0: [n][features][e]); with kv (cls > 0) the class tokens' first-row-block keys and values cls_kv

@@ -286,6 +286,36 @@ class Gpu:
         self._check(self._l.tah_quantile_stats_dev(self._h, ctypes.c_void_p(q_ptr), int(rows), int(n), _fp(a),
                                                    int(a.size), ctypes.c_void_p(out_ptr)))
 
+    def class_stats(self, scores, given=None, top: int = 0, temperature: float = 1.0):
+        """Rows of class scores [rows][n] read as distributions at a softmax temperature. `given` ([rows] or [rows][k]
+        class ids, -1 for none) are classes whose log probabilities are wanted, `top` how many of the most probable ones.
+        Returns (stats [rows][1 + k + top] float32: entropy, log p of the given classes, log p of the top ones; ids
+        [rows][top] int32: the top classes, the lower id first among equals)."""
+        x = _f32(scores)
+        if x.ndim != 2:
+            raise ValueError("class_stats: scores must be [rows][n]")
+        rows, n = x.shape
+        g = np.zeros((rows, 0), np.int64) if given is None else np.asarray(given)
+        g = g[:, None] if g.ndim == 1 else g
+        if g.ndim != 2 or g.shape[0] != rows or g.dtype.kind not in "iu" or (g.size and (g.min() < -1 or g.max() >= n)):
+            raise ValueError(f"class_stats: given must be [rows] or [rows][k] class ids from -1 to {n - 1}")
+        g = np.ascontiguousarray(g, np.int32)
+        if not 0 <= top <= min(n, 64) or g.shape[1] > 64:
+            raise ValueError("class_stats: at most 64 given classes and 64 of the most probable, no more than there are")
+        stats = np.empty((rows, 1 + g.shape[1] + top), np.float32)
+        ids = np.empty((rows, top), np.int32)
+        ip = lambda a: a.ctypes.data_as(abi.I32P) if a.shape[1] else None
+        self._check(self._l.tah_class_stats(self._h, _fp(x), rows, n, float(temperature), ip(g), g.shape[1], int(top),
+                                            _fp(stats), ip(ids)))
+        return stats, ids
+
+    def class_stats_dev(self, scores_ptr: int, rows: int, n: int, given_ptr: int, n_given: int, top: int, stats_ptr: int,
+                        ids_ptr: int, temperature: float = 1.0, ld: int = 0) -> None:
+        """`class_stats` with every array in device memory, queued on the handle's stream; rows of scores `ld` floats
+        apart (0: n). A given id outside [0, n) gives NaN."""
+        self._check(self._l.tah_class_stats_dev(self._h, scores_ptr, rows, n, ld, temperature, given_ptr, n_given, top,
+                                                stats_ptr, ids_ptr))
+
     def pack(self, c, d: int, rc: int, kv_format: int) -> np.ndarray:
         """One stored chunk record from its f32 keys and values `c` ([2d][rc]), quantised on the card."""
         c = _f32(c).reshape(-1)

@@ -5,6 +5,7 @@
   (`src/table.rs:136-147`, `src/table.rs:245-256`);
 * `add_logits`: the members' raw scores summed in float64 in class order (`logit_sums`, `src/table.rs:242-272`);
 * `finish_proba`: temperature softmax over the sum (`src/table.rs:70-78`);
+* `class_report`: those distributions' entropies, the labels' log probabilities and the most probable classes;
 * `QuantileDist` and `add_regression`: a regression member's 999 (or 99) quantile outputs read as a distribution,
   and the members' means, variances, medians and quantiles averaged (`src/table.rs:292-346`, `src/table.rs:457-496`).
 
@@ -50,6 +51,42 @@ def finish_proba(sums: np.ndarray, members: int, temperature: float) -> np.ndarr
     inv = 1.0 / (members * temperature)
     out = np.exp((sums - sums.max(axis=1, keepdims=True)) * inv)
     return out / out.sum(axis=1, keepdims=True)
+
+
+def class_report(sums: np.ndarray, members: int, temperature: float, labels=None, top: int = 0, gpu=None):
+    """What `finish_proba`'s distributions say, in logarithms: per row of the summed scores the entropy (nats), the log
+    probability of the row's label (`labels`, class ids or -1 for none: NaN) and the `top` most probable classes with
+    theirs. Returns a dict of float64 "entropy" [n], "log_p" [n] (with labels), "top_log_p" [n][top] and int32 "top"
+    [n][top]. With a card (`hip.Gpu`) the rows are read there, the sums as float32 (`tah_class_stats`)."""
+    sums = np.asarray(sums, np.float64)
+    n, classes = sums.shape
+    if not 0 <= top <= classes:
+        raise ValueError(f"class_report: top must be from 0 to {classes}")
+    if labels is not None:
+        labels = np.asarray(labels)
+        if labels.shape != (n,) or labels.dtype.kind not in "iu" or (n and (labels.min() < -1 or labels.max() >= classes)):
+            raise ValueError("class_report: a class id (or -1) for every row")
+    if gpu is not None:
+        st, ids = gpu.class_stats(sums, labels, top, members * temperature)
+        st = st.astype(np.float64)
+        out = {"entropy": st[:, 0], "top": ids, "top_log_p": st[:, st.shape[1] - top:]}
+        if labels is not None:
+            out["log_p"] = st[:, 1]
+        return out
+    peak = sums.max(axis=1, keepdims=True)
+    with np.errstate(invalid="ignore"):  # inf - inf: a row that has no distribution
+        u = (sums - np.where(peak == -np.inf, 0.0, peak)) / (members * temperature)
+    e = np.exp(u)
+    total = e.sum(axis=1, keepdims=True)
+    logp = u - np.log(np.where(total > 0, total, 1.0))
+    logp[~(peak[:, 0] < np.inf)] = np.nan
+    ent = -np.sum(np.where(e > 0, e * np.where(e > 0, logp, 0.0), 0.0), axis=1) / np.maximum(total[:, 0], 1.0)
+    ids = np.argsort(np.where(np.isnan(sums), np.inf, -sums), axis=1, kind="stable")[:, :top].astype(np.int32)
+    out = {"entropy": np.where(peak[:, 0] < np.inf, ent, np.nan), "top": ids,
+           "top_log_p": np.take_along_axis(logp, ids.astype(np.int64), 1)}
+    if labels is not None:
+        out["log_p"] = np.where(labels < 0, np.nan, logp[np.arange(n), np.maximum(labels, 0)])
+    return out
 
 
 def _seq_sum(a) -> np.float32:
