@@ -94,7 +94,7 @@ __device__ __forceinline__ float rec_value(const uint8_t *rec, int d, int rc, in
 template <int FMT>
 __device__ __forceinline__ void load16(const uint8_t *rec, int d, int rc, int c, int o16, int nk_left, bool fast,
                                        float *dst) {
-    if (fast) {
+    if (FMT != TAH_KV_I4 && fast) {
         if (FMT == TAH_KV_F32) {
             const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(rec) + (size_t)c * rc + o16);
 #pragma unroll
@@ -162,7 +162,29 @@ constexpr int SCL = 768;  // bytes of one (chunk, head)'s scales
 constexpr int HALF16 = 8192 + 256;  // a half tile: 64 rows of codes, then 64 factors
 constexpr int IMG16 = 2 * HALF16;
 
-__host__ __device__ constexpr int img_bytes(int fmt) { return fmt == TAH_KV_F32 ? IMG : (fmt == TAH_KV_I16 ? IMG16 : IMG8); }
+// i4 caches: code tiles, 4.5 KB per (key block, head): the codes of the block's keys (2 KB) and their 64 steps and 64
+// offsets, then the same of its values, the steps and offsets as fp16 times the head's power of two (2^sk, 2^sv: from the
+// largest |K| and |V| the records stand for, kvmax, as for f32 images; exact down to 2^-28 of it). value = offset + step
+// code in fp16 is then one fused multiply-add with one rounding to eleven bits, what the record stands for.
+// The codes are in the order in which a wavefront reads them as operands of 16 x 16 x 32 products (k_attn_few4): two
+// kilobytes for 32 keys each, 16 bytes a lane, a word of eight codes an operand:
+//   keys: half s, lane (row, group g of eight coordinates), word 2 p + ks: key 32 s + 8 (row / 4) + 4 p + row % 4,
+//         coordinates 32 ks + 8 g .. + 7 (that order of the keys leaves a lane's scores as the values' next operand)
+//   values: half s, lane (row, g), word m: coordinate 16 m + row, keys 32 s + 8 g .. + 7
+// Code t of a word is at bits 4 (t / 2) + 16 (t % 2), + 8 stored: t and t + 1 then come out of it as a pair of halves.
+constexpr int HALF4 = 2048 + 256;
+constexpr int IMG4 = 2 * HALF4;
+
+// where the word of key r, coordinates 8 c .. 8 c + 7 lies; of coordinate r, keys 8 c .. 8 c + 7
+__device__ __forceinline__ int key_at4(int r, int c) {
+    const int row = 4 * (r >> 3 & 3) + (r & 3);
+    return 1024 * (r >> 5) + 16 * (row + 16 * (c & 3)) + 4 * (2 * (r >> 2 & 1) + (c >> 2));
+}
+__device__ __forceinline__ int value_at4(int r, int c) { return 1024 * (c >> 2) + 16 * ((r & 15) + 16 * (c & 3)) + 4 * (r >> 4); }
+
+__host__ __device__ constexpr int img_bytes(int fmt) {
+    return fmt == TAH_KV_F32 ? IMG : (fmt == TAH_KV_I16 ? IMG16 : (fmt == TAH_KV_I8 ? IMG8 : IMG4));
+}
 
 __host__ __device__ inline size_t image_bytes_of(int rows, int chunk, int heads, int fmt) {
     return (size_t)key_blocks(rows, chunk).n_kb * heads * img_bytes(fmt);
@@ -670,6 +692,49 @@ __global__ __launch_bounds__(256) void k_kv_tiles16(int rows, int chunk, int d, 
     }
 }
 
+// grid (key blocks, heads); 256 threads: one code tile of an i4 layer. kvmax (k_kv_absmax) holds the head's largest |K| and
+// |V|. Past a short block's end the codes are 0 (stored 8): finite numbers, whose scores are masked.
+__global__ __launch_bounds__(256) void k_kv_tiles4(int rows, int chunk, int d, int heads, const uint8_t *__restrict__ records,
+                                                   const uint32_t *__restrict__ kvmax, uint8_t *__restrict__ tiles) {
+    __shared__ uint8_t codes[2][64][KB + 4];  // [keys, values][coordinate][key]
+    const int kb = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+    const KeyBlocks kbs = key_blocks(rows, chunk);
+    const Where w = locate(kbs, kb, records, TAH_KV_I4, d, chunk);
+    const uint8_t *body = w.rec + 8 * (size_t)d * groups4(w.rc);
+    uint8_t *tile = tiles + ((size_t)kb * heads + h) * IMG4;
+    for (int u = tid; u < 2 * 64 * 32; u += 256) {
+        const int which = u >> 11, c = u >> 5 & 63, b = u & 31;
+        const int j = which * d + h * 64 + c;
+        const uint8_t two = 2 * b < w.nk ? body[(size_t)j * ((w.rc + 1) / 2) + w.o / 2 + b] : 0x88;
+        codes[which][c][2 * b] = two & 15;
+        codes[which][c][2 * b + 1] = 2 * b + 1 < w.nk ? two >> 4 : 8;
+    }
+    if (tid < 128) {
+        const int c = tid & 63, which = tid >> 6, e = shift_for(kvmax[h * 2 + which]);
+        const Step4 st = step_at4(w.rec, w.rc, which * d + h * 64 + c, w.o / KB);
+        const _Float16 s = (_Float16)ldexpf(st.s, e), z = (_Float16)ldexpf(st.z, e);
+        _Float16 *f = reinterpret_cast<_Float16 *>(tile + which * HALF4 + 2048);
+        if (which == 0) {
+            f[c] = s;
+            f[64 + c] = z;
+        } else {
+            f[8 * (c & 15) + 2 * (c >> 4)] = s;
+            f[8 * (c & 15) + 2 * (c >> 4) + 1] = z;
+        }
+    }
+    __syncthreads();
+    for (int u = tid; u < 1024; u += 256) {
+        const int which = u >> 9, r = u >> 3 & 63, c = u & 7;
+        uint32_t word = 0;
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+            const uint32_t code = which == 0 ? codes[0][8 * c + t][r] : codes[1][r][8 * c + t];
+            word |= code << (4 * (t >> 1) + 16 * (t & 1));
+        }
+        *reinterpret_cast<uint32_t *>(tile + which * HALF4 + (which == 0 ? key_at4(r, c) : value_at4(r, c))) = word;
+    }
+}
+
 // ---- split-fp16 MFMA kernel: head width 64 over tile images --------------------------------------------------
 // A flat grid of qtiles x heads x splits workgroups of WAVES wavefronts x 32 queries (the flat index remapped so that
 // the query tiles sharing a (head, key range) run on the same XCD: workgroup i is dispatched to XCD i % 8, and the
@@ -711,13 +776,6 @@ __device__ __forceinline__ void half_image_to_lds(const uint8_t *src, uint8_t *d
     }
 }
 
-// i16 staging (k_attn_split64 with STAGED): half a code tile (8 KB of codes and its 256 bytes of factors, keys or
-// values) into a staging slot's half by DMA: 528 copies of 16 bytes, the last 16 by wavefront 0.
-template <int WAVES>
-__device__ __forceinline__ void stage_half16(const uint8_t *src, uint8_t *dst, int tid) {
-    half_image_to_lds<WAVES, HALF16>(src, dst, tid);
-}
-
 // A staging slot's key codes into the split image kdst (K hi, K lo) and its value codes into vdst (V hi, V lo), either
 // null for none: the dequantised values (code times its coordinate's factor, in f32) split into fp16 halves, written
 // swizzled as the images are; each thread takes 16 bytes (8 codes) of a 128-byte row at a time.
@@ -748,6 +806,31 @@ __device__ __forceinline__ void convert16(const uint8_t *st, uint8_t *kdst, uint
     }
 }
 
+// The same for a 4-bit code tile (a halves' layout above k_kv_tiles4): the numbers as fp16, one plane each.
+template <int WAVES>
+__device__ __forceinline__ void convert4(const uint8_t *st, uint8_t *kdst, uint8_t *vdst, int tid) {
+#pragma unroll
+    for (int i = 0; i < 512 / (64 * WAVES); i++) {
+        const int u = tid + 64 * WAVES * i, r = u >> 3, c = u & 7;
+        const int off = r * 128 + swz(r, c) * 16;
+        if (kdst) {
+            // key r, coordinates 8 c .. 8 c + 7, each with its own step and offset
+            const halfx8 s = *reinterpret_cast<const halfx8 *>(st + 2048 + 16 * c);
+            const halfx8 z = *reinterpret_cast<const halfx8 *>(st + 2176 + 16 * c);
+            *reinterpret_cast<halfx8 *>(kdst + off) = values4(*reinterpret_cast<const uint32_t *>(st + key_at4(r, c)), s, z);
+        }
+        if (vdst) {
+            // coordinate r, keys 8 c .. 8 c + 7, one step and offset
+            const uint8_t *sv = st + HALF4;
+            const halfx2 f = *reinterpret_cast<const halfx2 *>(sv + 2048 + 16 * (r & 15) + 4 * (r >> 4));
+            const _Float16 s = f[0], z = f[1];
+            *reinterpret_cast<halfx8 *>(vdst + off) =
+                values4(*reinterpret_cast<const uint32_t *>(sv + value_at4(r, c)), halfx8{s, s, s, s, s, s, s, s},
+                        halfx8{z, z, z, z, z, z, z, z});
+        }
+    }
+}
+
 template <bool B>
 struct Flag {
     static constexpr bool value = B;
@@ -766,6 +849,9 @@ struct Flag {
 // in f32) and writes them split into the same LDS images as an f32 layer's, which the rest of the kernel reads
 // unchanged. In step kb the staging slot of its parity holds keys kb + 2 and values kb + 1 (converted then), and the
 // copies bring keys kb + 3 and values kb + 2 into the other.
+//
+// An i4 cache's code tiles (FOUR) go the same way, but what they stand for is exact in fp16: the LDS images have one
+// plane, as the i8 code images, and the products are two a term, with neither scales to follow nor a query to split again.
 template <int WAVES, int FMT>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows, int chunk, int d, int heads,
                                                                const float *__restrict__ q,
@@ -775,10 +861,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
                                                                int qtiles, int splits, float *__restrict__ part_o,
                                                                float *__restrict__ part_ml, float *__restrict__ out) {
     constexpr bool CODES = FMT == TAH_KV_I8;    // fp16 code images, scales applied in the kernel
-    constexpr bool STAGED = FMT == TAH_KV_I16;  // int16 code tiles dequantised into split images in the kernel
-    constexpr int HB = CODES ? IMG8 / 2 : IMG / 2;  // bytes of an LDS image's keys (or values)
+    constexpr bool FOUR = FMT == TAH_KV_I4;     // 4-bit code tiles dequantised into fp16 images in the kernel
+    constexpr bool STAGED = FMT == TAH_KV_I16 || FOUR;  // code tiles dequantised into images in the kernel
+    constexpr bool SINGLE = CODES || FOUR;          // keys and values are one fp16 plane
+    constexpr int HB = SINGLE ? IMG8 / 2 : IMG / 2;  // bytes of an LDS image's keys (or values)
     constexpr int IS = img_bytes(FMT);              // bytes of a tile in memory
-    constexpr int SG = IMG16;                       // STAGED: a staging slot, a whole code tile
+    constexpr int SG = IS, SH = IS / 2;             // STAGED: a staging slot, a whole code tile; half of it
     __shared__ __align__(16) uint8_t kt[2][HB], vt[2][HB];
     __shared__ __align__(16) float sb[CODES ? 4 : 1][192];  // CODES: scale ring, [chunk % 4][key, value, ratio]
     // CODES: each lane's 32 query coordinates, kept for the per-chunk splits: [wavefront][8 chunks of 4][lane][4];
@@ -805,12 +893,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
                                              reinterpret_cast<uint8_t *>(&sb[ci & 3][0]), 16, 0, 0);
     };
     // STAGED: block kb's key codes and key factors into staging slot sl; its value codes and value factors
-    auto stage_keys = [&](int kb, int sl) { stage_half16<WAVES>(head_images + kb * kb_stride, side + sl * SG, tid); };
+    auto stage_keys = [&](int kb, int sl) {
+        half_image_to_lds<WAVES, SH>(head_images + kb * kb_stride, side + sl * SG, tid);
+    };
     auto stage_values = [&](int kb, int sl) {
-        stage_half16<WAVES>(head_images + kb * kb_stride + HALF16, side + sl * SG + HALF16, tid);
+        half_image_to_lds<WAVES, SH>(head_images + kb * kb_stride + SH, side + sl * SG + SH, tid);
     };
     auto convert = [&](int sl, int kdst, int vdst) {
-        convert16<WAVES>(side + sl * SG, kdst >= 0 ? kt[kdst] : nullptr, vdst >= 0 ? vt[vdst] : nullptr, tid);
+        const uint8_t *st = side + sl * SG;
+        uint8_t *kd = kdst >= 0 ? kt[kdst] : nullptr, *vd = vdst >= 0 ? vt[vdst] : nullptr;
+        if constexpr (FOUR) convert4<WAVES>(st, kd, vd, tid);
+        else convert16<WAVES>(st, kd, vd, tid);
     };
     if (kb0 < kb1) {
         if constexpr (STAGED) {
@@ -977,7 +1070,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
                 const int r = 32 * kh + krow;
                 const int off = r * 128 + swz(r, 2 * dc + g) * 16;
                 khi[dc][kh] = *reinterpret_cast<const halfx8 *>(tile + off);
-                if constexpr (!CODES) klo[dc][kh] = *reinterpret_cast<const halfx8 *>(tile + 8192 + off);
+                if constexpr (!SINGLE) klo[dc][kh] = *reinterpret_cast<const halfx8 *>(tile + 8192 + off);
             }
 #pragma unroll
         for (int dc = 0; dc < 4; dc++)
@@ -985,7 +1078,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
             for (int kh = 0; kh < 2; kh++) {
                 sc[kh] = mfma16(khi[dc][kh], qh[dc], dc == 0 ? zero : sc[kh]);
                 sc[kh] = mfma16(khi[dc][kh], ql[dc], sc[kh]);
-                if constexpr (!CODES) sc[kh] = mfma16(klo[dc][kh], qh[dc], sc[kh]);
+                if constexpr (!SINGLE) sc[kh] = mfma16(klo[dc][kh], qh[dc], sc[kh]);
             }
         return tl_q;
     };
@@ -1055,7 +1148,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
                     const int r = 32 * db + r32;
                     const int voff = r * 128 + swz(r, 4 * kh + 2 * hh + g) * 16;
                     const halfx8 vhi = *reinterpret_cast<const halfx8 *>(vtile + voff);
-                    if constexpr (CODES) {
+                    if constexpr (SINGLE) {
                         acc_o[db] = mfma16(vhi, ph[kh][hh], acc_o[db]);
                         acc_o[db] = mfma16(vhi, pl[kh][hh], acc_o[db]);
                     } else {
@@ -1066,7 +1159,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
                     }
                 }
         l += ps;
-        if constexpr (NEXT && CODES) {
+        if constexpr (NEXT && SINGLE) {
             // one region: 8 key and 8 value operand reads, 16 + 16 products and the weights' VALU work
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
             __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
@@ -1643,10 +1736,10 @@ struct AttnPlan {
 };
 
 bool kv_images_apply(int kv_format, int d, int heads) {
-    return kv_format >= TAH_KV_F32 && kv_format <= TAH_KV_I8 && heads > 0 && d == 64 * heads;
+    return kv_known(kv_format) && heads > 0 && d == 64 * heads;
 }
 
-// The tiles, then (256-aligned) a 256-byte slot for f32 and i16's maxima, then the i8 scales.
+// The tiles, then (256-aligned) a 256-byte slot for f32, i16 and i4's maxima, then the i8 scales.
 size_t kv_images_bytes(int rows, int chunk, int heads, int kv_format) {
     const size_t chunks = key_blocks(rows, chunk).n_chunks;
     const size_t tail = kv_format == TAH_KV_I8 ? chunks * heads * SCL : 0;
@@ -1679,6 +1772,11 @@ void kv_images(hipStream_t s, int rows, int chunk, int d, int heads, int kv_form
             hipLaunchKernelGGL(k_kv_tiles16, dim3(k.n_kb, heads), dim3(256), 0, s, rows, chunk, d, heads, records,
                                img.kvmax, img.images);
             break;
+        case TAH_KV_I4:
+            launch_absmax<TAH_KV_I4>(s, rows, chunk, d, heads, records, img);
+            hipLaunchKernelGGL(k_kv_tiles4, dim3(k.n_kb, heads), dim3(256), 0, s, rows, chunk, d, heads, records, img.kvmax,
+                               img.images);
+            break;
         default:
             hipLaunchKernelGGL(k_kv_codes, dim3(k.n_kb, heads), dim3(256), 0, s, rows, chunk, d, heads, records,
                                img.images, img.scales);
@@ -1703,7 +1801,7 @@ static AttnPlan plan(const AttnShape &a, bool images) {
     const KeyBlocks k = key_blocks(a.rows, a.chunk);
     const int hd = a.d / a.heads;
     const bool tiles = hd == 64 && images && kv_images_apply(a.kv_format, a.d, a.heads);
-    p.few = tiles && a.nq <= FEW_Q && (a.kv_format != TAH_KV_I16 || a.nq >= FEW16_FROM);
+    p.few = tiles && a.nq <= FEW_Q && a.kv_format != TAH_KV_I4 && (a.kv_format != TAH_KV_I16 || a.nq >= FEW16_FROM);
     p.split16 = tiles && (p.few || a.nq >= split16_min_q(a.kv_format));
     // k_attn_split64: 256 queries a workgroup (one a compute unit, one wave of them) from 768 queries on, else 128
     // (at 512 / 640 rows f32 1.376 / 1.740 -> 1.368 / 1.717 ms and i8 1.337 / 1.705 -> 1.330 / 1.676 ms with the
@@ -1892,6 +1990,10 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
             case TAH_KV_I16:
                 if (p.waves == 8) launch_split<8, TAH_KV_I16>(s, a, p, q, *img, out, part_o, part_ml);
                 else launch_split<4, TAH_KV_I16>(s, a, p, q, *img, out, part_o, part_ml);
+                break;
+            case TAH_KV_I4:
+                if (p.waves == 8) launch_split<8, TAH_KV_I4>(s, a, p, q, *img, out, part_o, part_ml);
+                else launch_split<4, TAH_KV_I4>(s, a, p, q, *img, out, part_o, part_ml);
                 break;
             default:
                 if (p.waves == 8) launch_split<8, TAH_KV_I8>(s, a, p, q, *img, out, part_o, part_ml);

@@ -14,6 +14,7 @@
 #include <hip/hip_runtime.h>
 
 #include "common.hpp"
+#include "device_math.hpp"
 
 namespace tah {
 
@@ -61,6 +62,29 @@ __device__ __forceinline__ Step4 step_at4(const uint8_t *rec, int rc, int j, int
 __device__ __forceinline__ float record_value4(const uint8_t *rec, int d, int rc, int j, int r) {
     const uint8_t b = rec[8 * (size_t)d * groups4(rc) + (size_t)j * ((rc + 1) / 2) + (r >> 1)];
     return value4(step_at4(rec, rc, j, r / GROUP4), (int)(b >> 4 * (r & 1) & 15) - 8);
+}
+
+// A tile word's eight codes (code t at bits 4 (t / 2) + 16 (t % 2), 8 more than it is) as the fp16 numbers z + s c, each
+// rounded once. Four bits or'ed into the significand of 1024 are 1024 + n, or 1024 + 16 n from the next four, so that a
+// pair of codes is a half each in two instructions (three for all four pairs' shifts), exact; then one packed
+// multiply-add.
+__device__ __forceinline__ halfx8 values4(uint32_t word, halfx8 s, halfx8 z) {
+    const halfx2 down = {(_Float16)-1032.0f, (_Float16)-1032.0f}, down16 = {(_Float16)-72.0f, (_Float16)-72.0f};
+    const halfx2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+    const uint32_t high = word >> 8;
+    halfx2 c[4];
+    c[0] = __builtin_bit_cast(halfx2, (word & 0x000F000Fu) | 0x64006400u) + down;
+    c[1] = __builtin_elementwise_fma(__builtin_bit_cast(halfx2, (word & 0x00F000F0u) | 0x64006400u), sixteenth, down16);
+    c[2] = __builtin_bit_cast(halfx2, (high & 0x000F000Fu) | 0x64006400u) + down;
+    c[3] = __builtin_elementwise_fma(__builtin_bit_cast(halfx2, (high & 0x00F000F0u) | 0x64006400u), sixteenth, down16);
+    halfx8 v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const halfx2 x = __builtin_elementwise_fma(c[i], halfx2{s[2 * i], s[2 * i + 1]}, halfx2{z[2 * i], z[2 * i + 1]});
+        v[2 * i] = x[0];
+        v[2 * i + 1] = x[1];
+    }
+    return v;
 }
 
 }  // namespace tah
