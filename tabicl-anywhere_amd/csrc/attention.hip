@@ -1618,6 +1618,182 @@ __global__ __launch_bounds__(256, 1) void k_attn_few(int nq, int rows, int chunk
     }
 }
 
+// ---- few-query kernel over 4-bit code tiles: head width 64, 1 to 16 queries -------------------------------------------
+// grid heads x splits (workgroup i: head i % heads, key range i / heads); 256 threads. Each wavefront takes key blocks of
+// its own (kb0 + w, kb0 + w + 4, ..): a tile is 4.5 KB in the order of its operands, so a block is nine 16-byte loads a
+// lane straight into registers, the next block's issued before this one's arithmetic, and there is no LDS and no barrier
+// until the four softmax states are merged. The products are 16 x 16 x 32 with the queries as columns: S = K Q^T by 16
+// (two for each of four sets of 16 keys and two halves of the coordinates), O^T += V^T P^T by 16. The order of the keys
+// within a tile leaves a lane's eight scores of each 32 keys as the operand that the values' product takes.
+__global__ __launch_bounds__(256, 2) void k_attn_few4(int nq, int rows, int chunk, int d, int heads,
+                                                      const float *__restrict__ q, const uint8_t *__restrict__ tiles,
+                                                      const uint32_t *__restrict__ kvmax, int kb_per_split, int splits,
+                                                      float *__restrict__ part_o, float *__restrict__ part_ml,
+                                                      float *__restrict__ out) {
+    __shared__ float mref[4][16], msum[4][16], macc[4][64][17];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int qi = lane & 15, lg = lane >> 4;
+    const int h = blockIdx.x % heads, split = blockIdx.x / heads;
+    const KeyBlocks kbs = key_blocks(rows, chunk);
+    const int kb0 = split * kb_per_split, kb1 = min(kbs.n_kb, kb0 + kb_per_split);
+    const uint8_t *head_tiles = tiles + (size_t)h * IMG4;
+    const size_t kb_stride = (size_t)heads * IMG4;
+    struct Block {
+        u32x4 k[2], v[2];  // codes, 32 keys each
+        halfx8 ks[2], kz[2];  // the keys' steps and offsets at coordinates 32 ks + 8 lg ..
+        u32x4 vf;             // the values' (step, offset) at coordinates 16 m + lane % 16
+    };
+    auto fetch = [&](int kb) {
+        Block b;
+        const uint8_t *t = head_tiles + (size_t)kb * kb_stride;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            b.k[s] = *reinterpret_cast<const u32x4 *>(t + 1024 * s + 16 * lane);
+            b.v[s] = *reinterpret_cast<const u32x4 *>(t + HALF4 + 1024 * s + 16 * lane);
+            b.ks[s] = *reinterpret_cast<const halfx8 *>(t + 2048 + 64 * s + 16 * lg);
+            b.kz[s] = *reinterpret_cast<const halfx8 *>(t + 2176 + 64 * s + 16 * lg);
+        }
+        b.vf = *reinterpret_cast<const u32x4 *>(t + HALF4 + 2048 + 16 * qi);
+        return b;
+    };
+    Block cur;
+    int kb = kb0 + wave;
+    if (kb < kb1) cur = fetch(kb);
+    // query qi's coordinates 32 ks + 8 lg + t, scaled to a maximum near 2^14 and split
+    halfx8 qh[2], ql[2];
+    float qv[2][8];
+    {
+        const float *src = q + (size_t)min(qi, nq - 1) * d + h * 64 + 8 * lg;
+        const float live = qi < nq ? 1.0f : 0.0f;
+        float qmax = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            load8(src + 32 * ks, qv[ks]);
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+                qv[ks][t] *= live;
+                qmax = fmaxf(qmax, fabsf(qv[ks][t]));
+            }
+        }
+        qmax = max32(max16(qmax));
+        const int eq = shift_for_max(qmax);
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) split8(qv[ks], ldexpf(1.0f, eq), qh[ks], ql[ks]);
+        qv[0][0] = ldexpf(LOG2E, -(shift_for(kvmax[h * 2]) + eq));
+    }
+    const float to_log2 = qv[0][0];
+    float ref = -INFINITY, l = 0.0f;
+    floatx4 acc[4];  // O^T: coordinate 16 m + 4 lg + i of query qi, times 2^sv
+#pragma unroll
+    for (int m = 0; m < 4; m++) acc[m] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (; kb < kb1; kb += 4) {
+        Block next;
+        if (kb + 4 < kb1) next = fetch(kb + 4);
+        const int ci = kb / kbs.bpc;
+        const int nk = min(KB, (ci == kbs.n_chunks - 1 ? kbs.last_rc : chunk) - (kb % kbs.bpc) * KB);
+        float sc[16];  // 8 s + 4 p + i: key 32 s + 8 lg + 4 p + i
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                floatx4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ks = 0; ks < 2; ks++) {
+                    const halfx8 k = values4(cur.k[s][2 * p + ks], cur.ks[ks], cur.kz[ks]);
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[ks], a, 0, 0, 0);
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[ks], a, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[8 * s + 4 * p + i] = a[i];
+            }
+        if (nk < KB) {
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (32 * (j >> 3) + 8 * lg + (j & 7) >= nk) sc[j] = -INFINITY;
+        }
+        float mb = sc[0];
+#pragma unroll
+        for (int j = 1; j < 16; j++) mb = fmaxf(mb, sc[j]);
+        mb = max32(max16(mb)) * to_log2;
+        const bool grow = mb > ref + 3.0f;
+        if (__any(grow)) {
+            const float nref = grow ? mb : ref;
+            const float alpha = exp2_hw(ref - nref);
+            l *= alpha;
+#pragma unroll
+            for (int m = 0; m < 4; m++) acc[m] *= alpha;
+            ref = nref;
+        }
+        const float off = 12.0f - ref;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            u32x4 hw, lw;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const float p0 = exp2_hw(fmaf(sc[8 * s + 2 * t], to_log2, off));
+                const float p1 = exp2_hw(fmaf(sc[8 * s + 2 * t + 1], to_log2, off));
+                l += p0 + p1;
+                uint32_t hi, lo;
+                split2(p0, p1, hi, lo);
+                hw[t] = hi;
+                lw[t] = lo;
+            }
+            const halfx8 ph = __builtin_bit_cast(halfx8, hw), pl = __builtin_bit_cast(halfx8, lw);
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                const uint32_t word = cur.vf[m];
+                const halfx2 f = __builtin_bit_cast(halfx2, word);
+                const _Float16 fs = f[0], fz = f[1];
+                const halfx8 v = values4(cur.v[s][m], halfx8{fs, fs, fs, fs, fs, fs, fs, fs},
+                                         halfx8{fz, fz, fz, fz, fz, fz, fz, fz});
+                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, acc[m], 0, 0, 0);
+                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc[m], 0, 0, 0);
+            }
+        }
+        cur = next;
+    }
+    // the four wavefronts' (maximum, sum, weighted sums), merged as the split merge merges key ranges
+    const float lw = sum32(sum16(l));
+    if (lg == 0) {
+        mref[wave][qi] = ref;
+        msum[wave][qi] = lw;
+    }
+#pragma unroll
+    for (int m = 0; m < 4; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) macc[wave][16 * m + 4 * lg + i][qi] = acc[m][i];
+    __syncthreads();
+    // thread t: query t / 16, coordinates 4 (t % 16) .. + 3
+    const int oq = tid >> 4, oc = 4 * (tid & 15);
+    if (oq >= nq) return;
+    const float unscale = ldexpf(1.0f, -shift_for(kvmax[h * 2 + 1]));
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; w++)
+        if (msum[w][oq] > 0.0f) m = fmaxf(m, mref[w][oq]);
+    float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const float ls = msum[w][oq];
+        const float f = ls > 0.0f ? exp2_hw(mref[w][oq] - m) : 0.0f;
+        L += ls * f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] += macc[w][oc + j][oq] * f;
+    }
+    if (splits == 1) {
+        const float fo = unscale / L;
+        *reinterpret_cast<float4 *>(out + (size_t)oq * d + h * 64 + oc) = make_float4(o[0] * fo, o[1] * fo, o[2] * fo, o[3] * fo);
+    } else {
+        const size_t at = ((size_t)split * nq + oq) * heads + h;
+        *reinterpret_cast<float4 *>(part_o + at * 64 + oc) =
+            make_float4(o[0] * unscale, o[1] * unscale, o[2] * unscale, o[3] * unscale);
+        if (oc == 0) {
+            part_ml[at * 2] = m;
+            part_ml[at * 2 + 1] = L;
+        }
+    }
+}
+
 // ---- split merge: Soft::merge then Soft::finish ---------------------------------------------------------------
 // grid nq * heads; 64 threads. The largest running maximum first (lanes over splits), then one pass over the
 // splits accumulating each one's weight sum and weighted values rescaled to it; loads are independent across
@@ -1801,8 +1977,18 @@ static AttnPlan plan(const AttnShape &a, bool images) {
     const KeyBlocks k = key_blocks(a.rows, a.chunk);
     const int hd = a.d / a.heads;
     const bool tiles = hd == 64 && images && kv_images_apply(a.kv_format, a.d, a.heads);
-    p.few = tiles && a.nq <= FEW_Q && a.kv_format != TAH_KV_I4 && (a.kv_format != TAH_KV_I16 || a.nq >= FEW16_FROM);
+    p.few = tiles && a.nq <= FEW_Q && (a.kv_format != TAH_KV_I16 || a.nq >= FEW16_FROM);
     p.split16 = tiles && (p.few || a.nq >= split16_min_q(a.kv_format));
+    if (p.few && a.kv_format == TAH_KV_I4) {
+        // a wavefront a block, up to two workgroups a compute unit; more blocks then in as many ranges
+        p.waves = 4;
+        p.groups = 1;
+        const int most = std::max(1, 512 / a.heads);
+        const int want = std::min((k.n_kb + 3) / 4, most);
+        p.kb_per_split = (k.n_kb + want - 1) / want;
+        p.splits = (k.n_kb + p.kb_per_split - 1) / p.kb_per_split;
+        return p;
+    }
     // k_attn_split64: 256 queries a workgroup (one a compute unit, one wave of them) from 768 queries on, else 128
     // (at 512 / 640 rows f32 1.376 / 1.740 -> 1.368 / 1.717 ms and i8 1.337 / 1.705 -> 1.330 / 1.676 ms with the
     // smaller tiles than from 512; from 1,024 or 1,536 queries f32 was slower at 768 to 1,280); an i16 layer's (whose
@@ -1966,7 +2152,10 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
     }
     if (p.few) {
         const dim3 grid(a.heads * p.splits);
-        if (a.kv_format == TAH_KV_I16)
+        if (a.kv_format == TAH_KV_I4)
+            hipLaunchKernelGGL(k_attn_few4, grid, dim3(256), 0, s, a.nq, a.rows, a.chunk, a.d, a.heads, q, img->images,
+                               img->kvmax, p.kb_per_split, p.splits, part_o, part_ml, out);
+        else if (a.kv_format == TAH_KV_I16)
             hipLaunchKernelGGL((k_attn_few<FEW_Q / 16, TAH_KV_I16>), grid, dim3(256), 0, s, a.nq, a.rows, a.chunk, a.d,
                                a.heads, q, img->images, img->kvmax, img->scales, p.kb_per_split, p.splits, part_o,
                                part_ml, out);
