@@ -1625,16 +1625,16 @@ __global__ __launch_bounds__(256, 1) void k_attn_few(int nq, int rows, int chunk
 // until the four softmax states are merged. The products are 16 x 16 x 32 with the queries as columns: S = K Q^T by 16
 // (two for each of four sets of 16 keys and two halves of the coordinates), O^T += V^T P^T by 16. The order of the keys
 // within a tile leaves a lane's eight scores of each 32 keys as the operand that the values' product takes.
-__global__ __launch_bounds__(256, 2) void k_attn_few4(int nq, int rows, int chunk, int d, int heads,
-                                                      const float *__restrict__ q, const uint8_t *__restrict__ tiles,
-                                                      const uint32_t *__restrict__ kvmax, int kb_per_split, int splits,
-                                                      float *__restrict__ part_o, float *__restrict__ part_ml,
-                                                      float *__restrict__ out) {
-    __shared__ float mref[4][16], msum[4][16], macc[4][64][17];
+constexpr int FEW4_WAVES = 8;
+__global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlocks kbs, int chunk, const float *__restrict__ q,
+                                                      const uint8_t *__restrict__ tiles, const uint32_t *__restrict__ kvmax,
+                                                      int kb_per_split, float *__restrict__ part_o,
+                                                      float *__restrict__ part_ml, float *__restrict__ out) {
+    constexpr int W = FEW4_WAVES;
+    __shared__ float mref[W][16], msum[W][16], macc[W][64][17];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qi = lane & 15, lg = lane >> 4;
-    const int h = blockIdx.x % heads, split = blockIdx.x / heads;
-    const KeyBlocks kbs = key_blocks(rows, chunk);
+    const int h = blockIdx.x, heads = gridDim.x, split = blockIdx.y, splits = gridDim.y, d = 64 * heads;
     const int kb0 = split * kb_per_split, kb1 = min(kbs.n_kb, kb0 + kb_per_split);
     const uint8_t *head_tiles = tiles + (size_t)h * IMG4;
     const size_t kb_stride = (size_t)heads * IMG4;
@@ -1656,9 +1656,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_few4(int nq, int rows, int chun
         b.vf = *reinterpret_cast<const u32x4 *>(t + HALF4 + 2048 + 16 * qi);
         return b;
     };
-    Block cur;
+    Block cur[2];
     int kb = kb0 + wave;
-    if (kb < kb1) cur = fetch(kb);
+    if (kb < kb1) cur[0] = fetch(kb);
+    int in_chunk = kb % kbs.bpc, ci = kb / kbs.bpc;  // kept along, without a division a block
+    const int over = W % kbs.bpc, past = W / kbs.bpc;
     // query qi's coordinates 32 ks + 8 lg + t, scaled to a maximum near 2^14 and split
     halfx8 qh[2], ql[2];
     float qv[2][8];
@@ -1686,11 +1688,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_few4(int nq, int rows, int chun
     floatx4 acc[4];  // O^T: coordinate 16 m + 4 lg + i of query qi, times 2^sv
 #pragma unroll
     for (int m = 0; m < 4; m++) acc[m] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (; kb < kb1; kb += 4) {
-        Block next;
-        if (kb + 4 < kb1) next = fetch(kb + 4);
-        const int ci = kb / kbs.bpc;
-        const int nk = min(KB, (ci == kbs.n_chunks - 1 ? kbs.last_rc : chunk) - (kb % kbs.bpc) * KB);
+    auto step = [&](const Block &cur) {
+        const int nk = min(KB, (ci == kbs.n_chunks - 1 ? kbs.last_rc : chunk) - in_chunk * KB);
         float sc[16];  // 8 s + 4 p + i: key 32 s + 8 lg + 4 p + i
 #pragma unroll
         for (int s = 0; s < 2; s++)
@@ -1750,9 +1749,24 @@ __global__ __launch_bounds__(256, 2) void k_attn_few4(int nq, int rows, int chun
                 acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc[m], 0, 0, 0);
             }
         }
-        cur = next;
+    };
+    // two blocks a round, so that the registers' roles are fixed
+    while (kb < kb1) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (kb + W < kb1) cur[u ^ 1] = fetch(kb + W);
+            step(cur[u]);
+            kb += W;
+            in_chunk += over;
+            ci += past;
+            if (in_chunk >= kbs.bpc) {
+                in_chunk -= kbs.bpc;
+                ci++;
+            }
+            if (kb >= kb1) break;
+        }
     }
-    // the four wavefronts' (maximum, sum, weighted sums), merged as the split merge merges key ranges
+    // the wavefronts' (maximum, sum, weighted sums), merged as the split merge merges key ranges
     const float lw = sum32(sum16(l));
     if (lg == 0) {
         mref[wave][qi] = ref;
@@ -1765,15 +1779,15 @@ __global__ __launch_bounds__(256, 2) void k_attn_few4(int nq, int rows, int chun
     __syncthreads();
     // thread t: query t / 16, coordinates 4 (t % 16) .. + 3
     const int oq = tid >> 4, oc = 4 * (tid & 15);
-    if (oq >= nq) return;
+    if (oq >= min(nq, 16)) return;
     const float unscale = ldexpf(1.0f, -shift_for(kvmax[h * 2 + 1]));
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; w++)
+    for (int w = 0; w < W; w++)
         if (msum[w][oq] > 0.0f) m = fmaxf(m, mref[w][oq]);
     float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < W; w++) {
         const float ls = msum[w][oq];
         const float f = ls > 0.0f ? exp2_hw(mref[w][oq] - m) : 0.0f;
         L += ls * f;
@@ -1905,6 +1919,53 @@ __global__ __launch_bounds__(256) void k_attn_merge_w(int items, int splits, con
     out[(size_t)i * 64 + lane] = O / L;
 }
 
+// Split merge for few (query, head) pairs and up to MERGE_FEW key ranges: a workgroup a pair, its wavefronts the ranges of
+// one residue each, lane = coordinate, every load issued before the sums; the four states through LDS.
+constexpr int MERGE_FEW = 32;
+__global__ __launch_bounds__(256) void k_attn_merge_few(int items, int splits, const float *__restrict__ part_o,
+                                                        const float *__restrict__ part_ml, float *__restrict__ out) {
+    __shared__ float wm[4], wl[4], wo[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x;
+    float2 ml[MERGE_FEW / 4];
+    float po[MERGE_FEW / 4];
+#pragma unroll
+    for (int u = 0; u < MERGE_FEW / 4; u++) {
+        // past the last range: its own values reread and given no weight
+        const int s = 4 * u + wave;
+        const size_t at = (size_t)min(s, splits - 1) * items + i;
+        ml[u] = *reinterpret_cast<const float2 *>(part_ml + at * 2);
+        po[u] = part_o[at * 64 + lane];
+        if (s >= splits) ml[u].y = 0.0f;
+    }
+    float M = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < MERGE_FEW / 4; u++)
+        if (ml[u].y > 0.0f) M = fmaxf(M, ml[u].x);
+    float L = 0.0f, O = 0.0f;
+#pragma unroll
+    for (int u = 0; u < MERGE_FEW / 4; u++) {
+        const float f = ml[u].y > 0.0f ? exp2_hw(ml[u].x - M) : 0.0f;
+        L += ml[u].y * f;
+        O += po[u] * f;
+    }
+    wo[wave][lane] = O;
+    if (lane == 0) {
+        wm[wave] = M;
+        wl[wave] = L;
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    const float m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    L = O = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const float f = wl[u] > 0.0f ? exp2_hw(wm[u] - m) : 0.0f;
+        L += wl[u] * f;
+        O += wo[u][lane] * f;
+    }
+    out[(size_t)i * 64 + lane] = O / L;
+}
+
 // ---- planning and launch --------------------------------------------------------------------------------------
 struct AttnPlan {
     bool split16, few;  // few: k_attn_few (any tiles, at most FEW_Q queries; i16 from FEW16_FROM)
@@ -1983,8 +2044,8 @@ static AttnPlan plan(const AttnShape &a, bool images) {
         // a wavefront a block, up to two workgroups a compute unit; more blocks then in as many ranges
         p.waves = 4;
         p.groups = 1;
-        const int most = std::max(1, 512 / a.heads);
-        const int want = std::min((k.n_kb + 3) / 4, most);
+        const int most = std::max(1, 256 / a.heads);
+        const int want = k.n_kb <= 2 * FEW4_WAVES ? 1 : std::min((k.n_kb + FEW4_WAVES - 1) / FEW4_WAVES, most);
         p.kb_per_split = (k.n_kb + want - 1) / want;
         p.splits = (k.n_kb + p.kb_per_split - 1) / p.kb_per_split;
         return p;
@@ -2153,8 +2214,9 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
     if (p.few) {
         const dim3 grid(a.heads * p.splits);
         if (a.kv_format == TAH_KV_I4)
-            hipLaunchKernelGGL(k_attn_few4, grid, dim3(256), 0, s, a.nq, a.rows, a.chunk, a.d, a.heads, q, img->images,
-                               img->kvmax, p.kb_per_split, p.splits, part_o, part_ml, out);
+            hipLaunchKernelGGL(k_attn_few4, dim3(a.heads, p.splits), dim3(64 * FEW4_WAVES), 0, s, a.nq,
+                               key_blocks(a.rows, a.chunk), a.chunk, q, img->images, img->kvmax, p.kb_per_split, part_o,
+                               part_ml, out);
         else if (a.kv_format == TAH_KV_I16)
             hipLaunchKernelGGL((k_attn_few<FEW_Q / 16, TAH_KV_I16>), grid, dim3(256), 0, s, a.nq, a.rows, a.chunk, a.d,
                                a.heads, q, img->images, img->kvmax, img->scales, p.kb_per_split, p.splits, part_o,
@@ -2202,7 +2264,10 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
         default: throw ArgError{"attention: unknown key/value format"};
     }
     if (p.splits > 1) {
-        if (a.d == 64 * a.heads && p.splits <= MERGE64_MAX)  // many queries, few splits (else lanes over splits win)
+        if (p.few && a.kv_format == TAH_KV_I4 && p.splits <= MERGE_FEW)
+            hipLaunchKernelGGL(k_attn_merge_few, dim3(a.nq * a.heads), dim3(256), 0, s, a.nq * a.heads, p.splits, part_o,
+                               part_ml, out);
+        else if (a.d == 64 * a.heads && p.splits <= MERGE64_MAX)  // many queries, few splits (else lanes over splits win)
             hipLaunchKernelGGL(k_attn_merge64, dim3((a.nq * a.heads + 15) / 16), dim3(256), 0, s, a.nq * a.heads,
                                a.heads, p.splits, part_o, part_ml, out);
         else if (a.d == 64 * a.heads)

@@ -71,12 +71,15 @@ __device__ __forceinline__ float record_value4(const uint8_t *rec, int d, int rc
 __device__ __forceinline__ halfx8 values4(uint32_t word, halfx8 s, halfx8 z) {
     const halfx2 down = {(_Float16)-1032.0f, (_Float16)-1032.0f}, down16 = {(_Float16)-72.0f, (_Float16)-72.0f};
     const halfx2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+    // in registers: as literals the and and the or would be an instruction each
+    uint32_t low = 0x000F000Fu, up = 0x00F000F0u, base = 0x64006400u;
+    asm("" : "+s"(low), "+s"(up), "+v"(base));
     const uint32_t high = word >> 8;
     halfx2 c[4];
-    c[0] = __builtin_bit_cast(halfx2, (word & 0x000F000Fu) | 0x64006400u) + down;
-    c[1] = __builtin_elementwise_fma(__builtin_bit_cast(halfx2, (word & 0x00F000F0u) | 0x64006400u), sixteenth, down16);
-    c[2] = __builtin_bit_cast(halfx2, (high & 0x000F000Fu) | 0x64006400u) + down;
-    c[3] = __builtin_elementwise_fma(__builtin_bit_cast(halfx2, (high & 0x00F000F0u) | 0x64006400u), sixteenth, down16);
+    c[0] = __builtin_bit_cast(halfx2, (word & low) | base) + down;
+    c[1] = __builtin_elementwise_fma(__builtin_bit_cast(halfx2, (word & up) | base), sixteenth, down16);
+    c[2] = __builtin_bit_cast(halfx2, (high & low) | base) + down;
+    c[3] = __builtin_elementwise_fma(__builtin_bit_cast(halfx2, (high & up) | base), sixteenth, down16);
     halfx8 v;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
