@@ -304,7 +304,7 @@ int tah_quantile_stats_dev(tah_dev *dev, const float *q_dev, int32_t rows, int32
 /* ---- the classification head ------------------------------------------------------------------------------------
  *
  * Rows of class scores read as distributions at a softmax temperature (finish_proba, src/table.rs:70-78, in
- * logarithms): scores [rows][n] (n from 1 to 2^24); given [rows][n_given] class ids whose log probabilities are wanted,
+ * logarithms): scores [rows][n] (n from 1 to 2^20); given [rows][n_given] class ids whose log probabilities are wanted,
  * top how many of the most probable classes (n_given and top at most 64, top at most n; either may be 0, its pointers
  * then NULL). Writes stats [rows][1 + n_given + top]: the entropy in nats, log p of each given class, log p of the top
  * most probable ones, falling; and ids [rows][top], those classes (the lower id first among equal scores, NaN after

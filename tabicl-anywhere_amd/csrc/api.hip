@@ -963,8 +963,8 @@ extern "C" int tah_quantile_stats(tah_dev *dev, const float *q, int32_t rows, in
 // ---- the classification head -----------------------------------------------------------------------------------
 static void check_classes(int rows, int n, long ld, float temperature, const int32_t *given, int n_given, int top,
                           const int32_t *ids) {
-    if (rows < 0 || n < 1 || n > 1 << 24 || ld < n)
-        throw ArgError{"class_stats: 1 to 2^24 classes a row, rows at least that far apart"};
+    if (rows < 0 || n < 1 || n > 1 << 20 || ld < n)
+        throw ArgError{"class_stats: 1 to 2^20 classes a row, rows at least that far apart"};
     if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.0f / temperature))
         throw ArgError{"class_stats: the temperature has to be positive"};
     if (n_given < 0 || n_given > 64 || top < 0 || top > 64 || top > n || (n_given > 0 && !given) || (top > 0 && !ids))
@@ -978,7 +978,10 @@ extern "C" int tah_class_stats_dev(tah_dev *dev, const float *scores_dev, int32_
     return guarded(dev, [&] {
         if (ld == 0) ld = n;
         check_classes(rows, n, ld, temperature, given_dev, n_given, top, ids_dev);
-        class_stats(dev->stream, rows, n, (size_t)ld, scores_dev, temperature, given_dev, n_given, top, stats_dev, ids_dev);
+        Loans loans(dev);
+        const size_t work = class_stats_work_bytes(rows, n, top);
+        class_stats(dev->stream, rows, n, (size_t)ld, scores_dev, temperature, given_dev, n_given, top, stats_dev, ids_dev,
+                    work ? loans.take<uint8_t>(work) : nullptr);
         return TAH_OK;
     });
 }
@@ -998,7 +1001,9 @@ extern "C" int tah_class_stats(tah_dev *dev, const float *scores, int32_t rows, 
         int32_t *gd = loans.take<int32_t>(ng), *id = loans.take<int32_t>(nt);
         TAH_HIP(hipMemcpyAsync(xd, scores, sizeof(float) * nin, hipMemcpyHostToDevice, dev->stream));
         if (ng) TAH_HIP(hipMemcpyAsync(gd, given, sizeof(int32_t) * ng, hipMemcpyHostToDevice, dev->stream));
-        class_stats(dev->stream, rows, n, n, xd, temperature, gd, n_given, top, sd, id);
+        const size_t work = class_stats_work_bytes(rows, n, top);
+        class_stats(dev->stream, rows, n, n, xd, temperature, gd, n_given, top, sd, id,
+                    work ? loans.take<uint8_t>(work) : nullptr);
         TAH_HIP(hipMemcpyAsync(stats, sd, sizeof(float) * nout, hipMemcpyDeviceToHost, dev->stream));
         if (nt) TAH_HIP(hipMemcpyAsync(ids, id, sizeof(int32_t) * nt, hipMemcpyDeviceToHost, dev->stream));
         TAH_HIP(hipStreamSynchronize(dev->stream));

@@ -8,6 +8,7 @@
 // (m, s, t) of two parts join as the online softmax's do: with m1 >= m2 and g = (m1 - m2) / T,
 //     s = s1 + e^-g (s2 + 1),    t = t1 + e^-g (t2 + g (s2 + 1)).
 // Classes in order: larger scores first, the lower id among equals (-0 and 0 are equal), NaN after every number.
+#include <algorithm>
 #include <cmath>
 
 #include "common.hpp"
@@ -20,32 +21,39 @@ struct ClassDist {
     bool bad;  // a NaN among the scores
 };
 
+// e^x for x <= 0 on the hardware's exp2 (1 ulp; x log2 e rounded: 2^-24 of it in the exponent)
+__device__ __forceinline__ float exp_below(float x) { return exp2_hw(x * LOG2E); }
+
 __device__ __forceinline__ ClassDist join(ClassDist a, ClassDist b, float inv) {
     const bool swap = b.m > a.m;
     const float m = swap ? b.m : a.m, m2 = swap ? a.m : b.m;
     const float s1 = swap ? b.s : a.s, t1 = swap ? b.t : a.t, s2 = (swap ? a.s : b.s) + 1.0f, t2 = swap ? a.t : b.t;
-    const float g = (m - m2) * inv, f = __expf(-g);
+    const float g = (m - m2) * inv, f = exp_below(-g);
     // nothing but -inf in the lesser part, or too far below to count (g times 0 would be NaN where g is infinite)
     const bool none = m2 == -INFINITY || f == 0.0f;
     return {m, none ? s1 : fmaf(f, s2, s1), none ? t1 : fmaf(f, fmaf(g, s2, t2), t1), a.bad || b.bad};
 }
 
-__device__ __forceinline__ ClassDist join_lane(ClassDist a, int mask, float inv) {
-    return join(a, {__shfl_xor(a.m, mask), __shfl_xor(a.s, mask), __shfl_xor(a.t, mask), (bool)__shfl_xor((int)a.bad, mask)}, inv);
-}
-
-// a score and its id as a number that orders as the classes do; never 0
-__device__ __forceinline__ uint64_t class_key(float x, int id) {
+// a score as a number that orders as the scores do: a NaN 1, and 0 is left for none
+__device__ __forceinline__ uint32_t score_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
-    const uint32_t k = x != x ? 0u : u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
-    return (uint64_t)k << 32 | (0xFFFFFFFFu - (uint32_t)id);
+    return x != x ? 1u : u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
+__device__ __forceinline__ float score_of(uint32_t k) {
+    return k == 1u ? NAN : __uint_as_float((k >> 31) ? (k ^ 0x80000000u) : ~k);
+}
+// with its class: a number that orders as the classes do
+__device__ __forceinline__ uint64_t class_key(uint32_t k, int id) { return (uint64_t)k << 32 | (0xFFFFFFFFu - (uint32_t)id); }
+__device__ __forceinline__ int class_of(uint64_t key) { return (int)(0xFFFFFFFFu - (uint32_t)key); }
 
 struct ClassOut {
     const int32_t *given;  // [rows][n_given]
     int n_given, top;
     float *stats;   // [rows][1 + n_given + top]
     int32_t *ids;   // [rows][top]
+    ClassOut from(size_t row) const {
+        return {given + row * n_given, n_given, top, stats + row * (1 + n_given + top), ids + row * top};
+    }
 };
 
 // What a row's distribution says of one score.
@@ -59,54 +67,350 @@ __device__ __forceinline__ float entropy(const ClassDist &c) {
     return c.m == -INFINITY ? 0.0f : log1pf(c.s) + c.t / (1.0f + c.s);
 }
 
-// grid rows; 256 threads.
-__global__ __launch_bounds__(256) void k_class_stats(int n, size_t ld, const float *__restrict__ x, float inv, ClassOut o) {
-    __shared__ ClassDist part[4];
-    __shared__ uint64_t best[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const size_t row = blockIdx.x;
-    const float *src = x + row * ld;
-    ClassDist c{-INFINITY, 0.0f, 0.0f, false};
-    for (int i = tid; i < n; i += 256) c = join(c, {src[i], 0.0f, 0.0f, src[i] != src[i]}, inv);
-    for (int mask = 1; mask < 64; mask <<= 1) c = join_lane(c, mask, inv);
-    if (lane == 0) part[wave] = c;
+// ---- up to 64 classes: a lane a row -----------------------------------------------------------------------------------
+// grid ceil(rows / 64); 64 threads. The scores of 64 rows come in whole lines and are turned in LDS (an odd pitch: the
+// lanes' reads meet no bank twice; -inf past n), each lane then keeps its row's N >= n scores in registers, so
+// that nothing is exchanged between lanes: a row of ten classes takes a lane about 150 instructions, where a wavefront or a
+// workgroup a row spent most of its own on reductions (200,000 rows of seven: 664 us a workgroup a row). The most probable
+// classes by one scan of the keys each.
+template <int N>
+__global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t ld, const float *__restrict__ x, float inv,
+                                                         ClassOut o) {
+    constexpr int PITCH = N + 1;
+    __shared__ float turned[64 * PITCH];
+    const int lane = threadIdx.x, row0 = blockIdx.x * 64, here = min(64, rows - row0);
+    const float per = 1.0f / (float)n;
+    const float *src = x + (size_t)row0 * ld;
+    if (n < N) {
+#pragma unroll
+        for (int i = 0; i < N; i++) turned[lane * PITCH + i] = -INFINITY;
+        __syncthreads();
+    }
+    for (int e = lane; e < here * n; e += 64) {
+        // e + 1/2 over n is at least 1 / (2 n) from a whole number and below 64: far more than the product's rounding
+        const int r = (int)(((float)e + 0.5f) * per), i = e - r * n;
+        turned[r * PITCH + i] = src[r * ld + i];
+    }
     __syncthreads();
-    c = join(join(part[0], part[1], inv), join(part[2], part[3], inv), inv);
+    if (lane >= here) return;
+    const float *mine = turned + lane * PITCH;
+    uint32_t k[N];
+    ClassDist c{-INFINITY, 0.0f, 0.0f, false};
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float v = mine[i];
+        k[i] = i < n ? score_key(v) : 0u;
+        c.bad = c.bad || v != v;
+        if (v > c.m) {
+            c.m = v;
+            at = i;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        // the maximum's own term left out; a score of -inf weighs nothing (0 times infinity would be NaN)
+        const float u = (mine[i] - c.m) * inv, e = i == at ? 0.0f : exp_below(u);
+        c.s += e;
+        c.t -= e > 0.0f ? e * u : 0.0f;
+    }
+    const size_t row = (size_t)row0 + lane;
+    float *st = o.stats + row * (1 + o.n_given + o.top);
+    st[0] = entropy(c);
+    for (int i = 0; i < o.n_given; i++) {
+        const int id = o.given[row * o.n_given + i];
+        st[1 + i] = id >= 0 && id < n ? log_p(c, mine[id], inv) : NAN;
+    }
+    for (int r = 0; r < o.top; r++) {
+        uint32_t best = 0;
+        int id = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const bool more = k[i] > best;
+            best = more ? k[i] : best;
+            id = more ? i : id;
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) k[i] = i == id ? 0u : k[i];
+        st[1 + o.n_given + r] = log_p(c, score_of(best), inv);
+        o.ids[row * o.top + r] = id;
+    }
+}
+
+// ---- a wavefront's scores, E a lane -----------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    // as floats' bit patterns would not do: an unsigned maximum in pairs of lanes 1, 2, 4, 8, 16 and 32 apart
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, false));
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((uint32_t)a[0], (uint32_t)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((uint32_t)b[0], (uint32_t)b[1]);
+}
+
+// the largest of the lanes' keys
+__device__ __forceinline__ uint64_t wave_best(uint64_t key) {
+    const uint32_t hi = wave_max_u32((uint32_t)(key >> 32));
+    const uint32_t lo = wave_max_u32((uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
+    return (uint64_t)hi << 32 | lo;
+}
+
+// The distribution of the keys k (E a lane, 0 for none) of a wavefront, in every lane. Class ids: id(r) of entry r.
+template <int E>
+__device__ __forceinline__ ClassDist wave_dist(const uint32_t (&k)[E], float inv) {
+    uint32_t mk = 0;
+    bool bad = false;
+#pragma unroll
+    for (int r = 0; r < E; r++) {
+        mk = max(mk, k[r]);
+        bad = bad || k[r] == 1u;
+    }
+    const uint32_t best = wave_max_u32(mk);
+    ClassDist c{best > 1u ? score_of(best) : -INFINITY, 0.0f, 0.0f, __any(bad) != 0};
+    // every term, then the sum without one of the largest: each of those is exactly 1, so they are counted apart
+    int tops = 0;
+    float s = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int r = 0; r < E; r++) {
+        const float u = (score_of(k[r] > 1u ? k[r] : 0x007FFFFFu) - c.m) * inv, e = exp_below(u);
+        const bool is_top = k[r] == best && k[r] > 1u;
+        tops += is_top;
+        s += is_top || !(e > 0.0f) ? 0.0f : e;
+        t -= is_top || !(e > 0.0f) ? 0.0f : e * u;
+    }
+    c.s = wave_sum(s) + (float)max((int)wave_sum((float)tops) - 1, 0);
+    c.t = wave_sum(t);
+    if (c.m == -INFINITY) c.s = c.t = 0.0f;
+    return c;
+}
+
+// The top largest keys of a wavefront in order: lane r's result is the r-th (top at most 64). Each lane keeps its own
+// largest left; the one whose key is taken looks for its next.
+template <int E, class Id>
+__device__ __forceinline__ uint64_t wave_top(uint32_t (&k)[E], int top, int lane, Id &&id) {
+    uint64_t mine = 0, got = 0;
+    auto next = [&] {
+        uint32_t best = 0;
+        int at = 0;
+#pragma unroll
+        for (int r = 0; r < E; r++) {
+            const bool more = k[r] > best;
+            best = more ? k[r] : best;
+            at = more ? r : at;
+        }
+#pragma unroll
+        for (int r = 0; r < E; r++) k[r] = r == at ? 0u : k[r];
+        mine = best ? class_key(best, id(at)) : 0;
+    };
+    next();
+    for (int r = 0; r < top; r++) {
+        const uint64_t best = wave_best(mine);
+        if (lane == r) got = best;
+        if (mine == best && best) next();
+    }
+    return got;
+}
+
+// ---- up to 1,024 classes: a wavefront a row ------------------------------------------------------------------------------
+// grid ceil(rows / 4); 256 threads. Entry r of a lane is class 64 r + lane: the row is read once, in whole lines, and kept.
+template <int E>
+__global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_t ld, const float *__restrict__ x, float inv,
+                                                          ClassOut o) {
+    const int lane = threadIdx.x & 63;
+    const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= (size_t)rows) return;
+    const float *src = x + row * ld;
+    uint32_t k[E];
+#pragma unroll
+    for (int r = 0; r < E; r++) k[r] = 64 * r + lane < n ? score_key(src[64 * r + lane]) : 0u;
+    const ClassDist c = wave_dist(k, inv);
+    float *st = o.stats + row * (1 + o.n_given + o.top);
+    if (lane == 0) st[0] = entropy(c);
+    if (lane < o.n_given) {
+        const int id = o.given[row * o.n_given + lane];
+        st[1 + lane] = id >= 0 && id < n ? log_p(c, src[id], inv) : NAN;
+    }
+    if (o.top == 0) return;
+    const uint64_t key = wave_top(k, o.top, lane, [&](int r) { return 64 * r + lane; });
+    if (lane < o.top) {
+        st[1 + o.n_given + lane] = log_p(c, score_of((uint32_t)(key >> 32)), inv);
+        o.ids[row * o.top + lane] = class_of(key);
+    }
+}
+
+// ---- more classes: a workgroup a segment of a row ------------------------------------------------------------------------
+// A segment's state: its distribution, then its top keys in order.
+struct SegState {
+    ClassDist c;
+};
+constexpr int SEG = 8192, SEG_E = SEG / 256;
+
+__host__ __device__ inline size_t seg_bytes(int top) { return sizeof(SegState) + 8 * (size_t)top; }
+
+__device__ __forceinline__ void write_row(const ClassDist &c, const ClassOut &o, size_t row, int n, const float *src,
+                                          float inv, int tid) {
     float *st = o.stats + row * (1 + o.n_given + o.top);
     if (tid == 0) st[0] = entropy(c);
-    for (int i = tid; i < o.n_given; i += 256) {
-        const int id = o.given[row * o.n_given + i];
-        st[1 + i] = id >= 0 && id < n ? log_p(c, src[id], inv) : NAN;
+    if (tid < o.n_given) {
+        const int id = o.given[row * o.n_given + tid];
+        st[1 + tid] = id >= 0 && id < n ? log_p(c, src[id], inv) : NAN;
     }
-    uint64_t last = ~0ull;
-    for (int r = 0; r < o.top; r++) {
-        uint64_t k = 0;
-        for (int i = tid; i < n; i += 256) {
-            const uint64_t u = class_key(src[i], i);
-            if (u < last && u > k) k = u;
+}
+
+// The place of key among `lists` lists of `each` falling keys (in LDS, 0 past a list's end): how many are larger.
+__device__ __forceinline__ int place_of(uint64_t key, const uint64_t *keys, int lists, int each) {
+    int place = 0;
+    for (int l = 0; l < lists; l++) {
+        int lo = 0, hi = each;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (keys[l * each + mid] > key) lo = mid + 1;
+            else hi = mid;
         }
-        for (int mask = 1; mask < 64; mask <<= 1) {
-            const uint64_t u = __shfl_xor(k, mask);
-            k = u > k ? u : k;
+        place += lo;
+    }
+    return place;
+}
+
+// grid (segments, rows); 256 threads: each keeps 32 scores of its segment in registers, so that the row is read once. Every
+// wavefront takes its 2,048 scores' distribution and most probable classes; the four are joined in LDS, the segments of a
+// row by k_class_stats_join (a row of one segment is written here).
+__global__ __launch_bounds__(256) void k_class_stats_seg(int n, size_t ld, const float *__restrict__ x, float inv,
+                                                         uint8_t *__restrict__ state, ClassOut o) {
+    __shared__ ClassDist part[4];
+    __shared__ uint64_t keys[4 * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = blockIdx.x, segs = gridDim.x;
+    const size_t row = blockIdx.y;
+    const float *src = x + row * ld;
+    const int base = seg * SEG;
+    uint32_t k[SEG_E];
+    // entry 4 r + j of a thread: class base + 4 (256 r + tid) + j
+    const bool whole = base + SEG <= n && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+#pragma unroll
+    for (int r = 0; r < SEG_E / 4; r++) {
+        const int i = base + 4 * (256 * r + tid);
+        if (whole) {
+            const float4 v = *reinterpret_cast<const float4 *>(src + i);
+            k[4 * r] = score_key(v.x);
+            k[4 * r + 1] = score_key(v.y);
+            k[4 * r + 2] = score_key(v.z);
+            k[4 * r + 3] = score_key(v.w);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) k[4 * r + j] = i + j < n ? score_key(src[i + j]) : 0u;
         }
-        __syncthreads();
-        if (lane == 0) best[wave] = k;
-        __syncthreads();
-        for (int w = 0; w < 4; w++) k = best[w] > k ? best[w] : k;
-        last = k;
-        if (tid == 0) {
-            const int id = (int)(0xFFFFFFFFu - (uint32_t)k);
-            st[1 + o.n_given + r] = log_p(c, src[id], inv);
-            o.ids[row * o.top + r] = id;
+    }
+    const ClassDist w = wave_dist(k, inv);
+    if (lane == 0) part[wave] = w;
+    if (o.top > 0) {
+        const uint64_t key = wave_top(k, o.top, lane, [&](int e) { return base + 4 * (256 * (e >> 2) + tid) + (e & 3); });
+        if (lane < o.top) keys[wave * o.top + lane] = key;
+    }
+    __syncthreads();
+    const ClassDist c = join(join(part[0], part[1], inv), join(part[2], part[3], inv), inv);
+    uint8_t *mine = state + (row * segs + seg) * seg_bytes(o.top);
+    if (segs == 1) write_row(c, o, row, n, src, inv, tid);
+    else if (tid == 0) reinterpret_cast<SegState *>(mine)->c = c;
+    if (tid < 4 * o.top) {
+        const uint64_t key = keys[tid];
+        const int place = key ? place_of(key, keys, 4, o.top) : o.top;
+        if (place < o.top) {
+            if (segs == 1) {
+                o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = log_p(c, score_of((uint32_t)(key >> 32)), inv);
+                o.ids[row * o.top + place] = class_of(key);
+            } else {
+                reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[place] = key;
+            }
+        }
+    }
+    // a last segment of fewer classes than top: nothing in the places past them
+    const int live = min(SEG, n - base);
+    if (segs > 1 && tid >= live && tid < o.top) reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[tid] = 0;
+}
+
+// grid rows; 256 threads: the segments of a row joined; segs top keys of LDS.
+__global__ __launch_bounds__(256) void k_class_stats_join(int n, size_t ld, const float *__restrict__ x, float inv, int segs,
+                                                          const uint8_t *__restrict__ state, ClassOut o) {
+    extern __shared__ uint64_t all[];
+    const int tid = threadIdx.x;
+    const size_t row = blockIdx.x;
+    const uint8_t *rows_state = state + row * segs * seg_bytes(o.top);
+    for (int i = tid; i < segs * o.top; i += 256) {
+        const int s = i / o.top;
+        all[i] = reinterpret_cast<const uint64_t *>(rows_state + s * seg_bytes(o.top) + sizeof(SegState))[i - s * o.top];
+    }
+    ClassDist c{-INFINITY, 0.0f, 0.0f, false};
+    for (int s = 0; s < segs; s++) c = join(c, reinterpret_cast<const SegState *>(rows_state + s * seg_bytes(o.top))->c, inv);
+    write_row(c, o, row, n, x + row * ld, inv, tid);
+    __syncthreads();
+    for (int i = tid; i < segs * o.top; i += 256) {
+        const uint64_t key = all[i];
+        if (!key) continue;
+        const int place = place_of(key, all, segs, o.top);
+        if (place < o.top) {
+            o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = log_p(c, score_of((uint32_t)(key >> 32)), inv);
+            o.ids[row * o.top + place] = class_of(key);
         }
     }
 }
 
+static int segments(int n) { return (n + SEG - 1) / SEG; }
+
+// Rows whose segments' states fit 32 MB (a launch's grid takes 65,535 of them).
+static int rows_at_once(int n, int top) {
+    return (int)std::max<size_t>(1, std::min<size_t>(65535, (size_t(32) << 20) / (segments(n) * seg_bytes(top))));
+}
+
+size_t class_stats_work_bytes(int rows, int n, int top) {
+    if (n <= 1024 || segments(n) == 1) return 0;
+    return (size_t)std::min(rows, rows_at_once(n, top)) * segments(n) * seg_bytes(top);
+}
+
+template <int N>
+static void launch_rows(hipStream_t s, int rows, int n, size_t ld, const float *x, float inv, const ClassOut &o) {
+    hipLaunchKernelGGL(k_class_stats_rows<N>, dim3((rows - 1) / 64 + 1), dim3(64), 0, s, rows, n, ld, x, inv,
+                       o);
+}
+template <int E>
+static void launch_wave(hipStream_t s, int rows, int n, size_t ld, const float *x, float inv, const ClassOut &o) {
+    constexpr int MOST = 1 << 24;  // rows a launch: a grid holds fewer than 2^32 threads
+    for (int r0 = 0; r0 < rows; r0 += std::min(MOST, rows - r0)) {
+        const int here = std::min(MOST, rows - r0);
+        hipLaunchKernelGGL(k_class_stats_wave<E>, dim3((here + 3) / 4), dim3(256), 0, s, here, n, ld, x + r0 * ld, inv,
+                           o.from(r0));
+    }
+}
+
+// work: class_stats_work_bytes(rows, n, top) bytes.
 void class_stats(hipStream_t s, int rows, int n, size_t ld, const float *x, float temperature, const int32_t *given,
-                 int n_given, int top, float *stats, int32_t *ids) {
+                 int n_given, int top, float *stats, int32_t *ids, void *work) {
     if (rows <= 0) return;
-    hipLaunchKernelGGL(k_class_stats, dim3(rows), dim3(256), 0, s, n, ld, x, 1.0f / temperature,
-                       ClassOut{given, n_given, top, stats, ids});
+    const float inv = 1.0f / temperature;
+    ClassOut o{given, n_given, top, stats, ids};
+    // the fewest entries a lane that hold a row
+    if (n <= 8) launch_rows<8>(s, rows, n, ld, x, inv, o);
+    else if (n <= 16) launch_rows<16>(s, rows, n, ld, x, inv, o);
+    else if (n <= 32) launch_rows<32>(s, rows, n, ld, x, inv, o);
+    else if (n <= 64) launch_rows<64>(s, rows, n, ld, x, inv, o);
+    else if (n <= 128) launch_wave<2>(s, rows, n, ld, x, inv, o);
+    else if (n <= 256) launch_wave<4>(s, rows, n, ld, x, inv, o);
+    else if (n <= 512) launch_wave<8>(s, rows, n, ld, x, inv, o);
+    else if (n <= 1024) launch_wave<16>(s, rows, n, ld, x, inv, o);
+    else {
+        const int segs = segments(n), most = rows_at_once(n, top);
+        for (int r0 = 0; r0 < rows; r0 += most) {
+            const int here = std::min(most, rows - r0);
+            const float *xr = x + r0 * ld;
+            const ClassOut at = o.from(r0);
+            hipLaunchKernelGGL(k_class_stats_seg, dim3(segs, here), dim3(256), 0, s, n, ld, xr, inv,
+                               static_cast<uint8_t *>(work), at);
+            if (segs > 1)
+                hipLaunchKernelGGL(k_class_stats_join, dim3(here), dim3(256), (size_t)segs * top * 8, s, n, ld, xr, inv, segs,
+                                   static_cast<const uint8_t *>(work), at);
+        }
+    }
     TAH_LAUNCHED();
 }
 

@@ -307,9 +307,10 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
 void quantile_stats(hipStream_t s, int rows, int n, const float *q, int na, const float *alphas, float *stats);
 
 // The classification head (class_stats.hip): rows of scores x (ld apart) to stats [rows][1 + n_given + top] and ids
-// [rows][top].
+// [rows][top]; work holds class_stats_work_bytes.
+size_t class_stats_work_bytes(int rows, int n, int top);
 void class_stats(hipStream_t s, int rows, int n, size_t ld, const float *x, float temperature, const int32_t *given,
-                 int n_given, int top, float *stats, int32_t *ids);
+                 int n_given, int top, float *stats, int32_t *ids, void *work);
 
 // Column and row stages (stages.hip).
 // The input layer for n rows x [n][features]: cells [n][cls + features][e], the weights' class tokens first where

@@ -125,7 +125,7 @@ def gpu():
 @pytest.mark.parametrize("rows,n,k,top", [(1, 1, 1, 1), (1, 2, 0, 0), (300, 2, 1, 2), (1000, 3, 0, 3), (65, 10, 2, 10),
                                           (130, 16, 1, 1), (130, 17, 1, 17), (64, 64, 3, 5), (9, 65, 64, 64),
                                           (70, 999, 1, 20), (37, 1024, 0, 64), (20, 1025, 1, 3), (11, 5000, 2, 64),
-                                          (9, 16384, 1, 7), (10, 16385, 1, 64), (9, 70001, 1, 33), (1, 300000, 1, 64)])
+                                          (9, 16384, 1, 7), (10, 16385, 1, 64), (9, 70001, 1, 33), (1, 300000, 1, 64), (2, 1 << 20, 1, 64), (3, 8193, 1, 40), (200, 24, 2, 24), (99, 40, 1, 40)])
 def test_class_stats(gpu, kind, rows, n, k, top):
     say(f"class stats {rows} x {n}, {k} given, {top} best, {kind}")
     rng = np.random.default_rng(rows * 7 + n)
@@ -186,14 +186,15 @@ def test_class_stats_refused(gpu):
         with pytest.raises(ValueError):
             gpu.class_stats(x, given, top, temperature)
     b = dm.DeviceBuffer(4096)
-    for args in ((None, 2, 5, b.ptr, 1, 1, b.ptr, b.ptr), (b.ptr, -1, 5, b.ptr, 1, 1, b.ptr, b.ptr),
-                 (b.ptr, 2, 0, b.ptr, 1, 0, b.ptr, b.ptr), (b.ptr, 2, 5, None, 1, 1, b.ptr, b.ptr),
-                 (b.ptr, 2, 5, b.ptr, 1, 1, b.ptr, None), (b.ptr, 2, 5, b.ptr, 65, 1, b.ptr, b.ptr),
-                 (b.ptr, 2, 5, b.ptr, 1, 6, b.ptr, b.ptr), (b.ptr, 2, (1 << 24) + 1, b.ptr, 1, 1, b.ptr, b.ptr)):
+    # no rows: a call that was let through would read nothing
+    for args in ((None, 0, 5, b.ptr, 1, 1, b.ptr, b.ptr), (b.ptr, -1, 5, b.ptr, 1, 1, b.ptr, b.ptr),
+                 (b.ptr, 0, 0, b.ptr, 1, 0, b.ptr, b.ptr), (b.ptr, 0, 5, None, 1, 1, b.ptr, b.ptr),
+                 (b.ptr, 0, 5, b.ptr, 1, 1, b.ptr, None), (b.ptr, 0, 5, b.ptr, 65, 1, b.ptr, b.ptr),
+                 (b.ptr, 0, 5, b.ptr, 1, 6, b.ptr, b.ptr), (b.ptr, 0, (1 << 20) + 1, b.ptr, 1, 1, b.ptr, b.ptr)):
         with pytest.raises(ValueError):
             gpu.class_stats_dev(*args)
     with pytest.raises(ValueError):
-        gpu.class_stats_dev(b.ptr, 2, 5, b.ptr, 1, 1, b.ptr, b.ptr, ld=4)
+        gpu.class_stats_dev(b.ptr, 0, 5, b.ptr, 1, 1, b.ptr, b.ptr, ld=4)
     b.free()
     st, ids = gpu.class_stats(np.zeros((0, 5), np.float32), None, 2)
     assert st.shape == (0, 3) and ids.shape == (0, 2)

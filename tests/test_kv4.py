@@ -159,7 +159,7 @@ def test_layers_refused(gpu):
     b = dm.DeviceBuffer(4096)
     for d, rows, chunk, fmt, ptr in ((0, 4, 8, abi.KV_I4, b.ptr), (16, -1, 8, abi.KV_I4, b.ptr), (16, 4, 0, abi.KV_I4, b.ptr),
                                      (16, 4, 8, 4, b.ptr), (16, 4, 8, -1, b.ptr), (16, 4, 8, abi.KV_I4, b.ptr + 1),
-                                     (16, 4, 8, abi.KV_I4, None)):
+                                     (16, 0, 8, abi.KV_I4, None)):
         with pytest.raises(ValueError):
             gpu.pack_dev(ptr, d, rows, chunk, fmt, b.ptr)
         with pytest.raises(ValueError):
