@@ -34,6 +34,11 @@ __device__ __forceinline__ ClassDist join(ClassDist a, ClassDist b, float inv) {
     return {m, none ? s1 : fmaf(f, s2, s1), none ? t1 : fmaf(f, fmaf(g, s2, t2), t1), a.bad || b.bad};
 }
 
+__device__ __forceinline__ ClassDist join_lane(ClassDist a, int mask, float inv) {
+    const ClassDist b{__shfl_xor(a.m, mask), __shfl_xor(a.s, mask), __shfl_xor(a.t, mask), (bool)__shfl_xor((int)a.bad, mask)};
+    return join(a, b, inv);
+}
+
 // a score as a number that orders as the scores do: a NaN 1, and 0 is left for none
 __device__ __forceinline__ uint32_t score_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
@@ -157,39 +162,99 @@ __device__ __forceinline__ uint64_t wave_best(uint64_t key) {
     return (uint64_t)hi << 32 | lo;
 }
 
-// The distribution of the keys k (E a lane, 0 for none) of a wavefront, in every lane. Class ids: id(r) of entry r.
+// The distribution of a wavefront's scores v (E a lane, -inf past the last), in every lane.
 template <int E>
-__device__ __forceinline__ ClassDist wave_dist(const uint32_t (&k)[E], float inv) {
-    uint32_t mk = 0;
+__device__ __forceinline__ ClassDist wave_dist(const float (&v)[E], float inv) {
+    float own = -INFINITY;
     bool bad = false;
 #pragma unroll
     for (int r = 0; r < E; r++) {
-        mk = max(mk, k[r]);
-        bad = bad || k[r] == 1u;
+        own = fmaxf(own, v[r]);
+        bad = bad || v[r] != v[r];
     }
-    const uint32_t best = wave_max_u32(mk);
-    ClassDist c{best > 1u ? score_of(best) : -INFINITY, 0.0f, 0.0f, __any(bad) != 0};
-    // every term, then the sum without one of the largest: each of those is exactly 1, so they are counted apart
+    ClassDist c{wave_max(own), 0.0f, 0.0f, __any(bad) != 0};
+    if (c.m == -INFINITY) return c;
+    // in units of log 2; the terms of the largest score are exactly 1 and are counted apart. From 2^-200 down a term is 0
+    const float inv2 = inv * LOG2E;
     int tops = 0;
     float s = 0.0f, t = 0.0f;
 #pragma unroll
     for (int r = 0; r < E; r++) {
-        const float u = (score_of(k[r] > 1u ? k[r] : 0x007FFFFFu) - c.m) * inv, e = exp_below(u);
-        const bool is_top = k[r] == best && k[r] > 1u;
-        tops += is_top;
-        s += is_top || !(e > 0.0f) ? 0.0f : e;
-        t -= is_top || !(e > 0.0f) ? 0.0f : e * u;
+        const float u = fmaxf((v[r] - c.m) * inv2, -200.0f), e = exp2_hw(u);
+        const bool is_top = v[r] == c.m;
+        tops += __popcll(__ballot(is_top));
+        const float w = is_top ? 0.0f : e;
+        s += w;
+        t = fmaf(-w, u, t);
     }
-    c.s = wave_sum(s) + (float)max((int)wave_sum((float)tops) - 1, 0);
-    c.t = wave_sum(t);
-    if (c.m == -INFINITY) c.s = c.t = 0.0f;
+    c.s = wave_sum(s) + (float)(tops - 1);
+    c.t = wave_sum(t) * 0.69314718055994530942f;
     return c;
 }
 
-// The top largest keys of a wavefront in order: lane r's result is the r-th (top at most 64). Each lane keeps its own
-// largest left; the one whose key is taken looks for its next.
+// The top largest scores of a wavefront as keys in order: lane r's result is the r-th (top at most 64). live: how many
+// entries of a lane are scores. Class ids: id(r) of entry r.
+//
+// A bound that top lanes' own largest scores reach, and few more, by halving (the least and the largest of them, as keys,
+// apart): top scores reach it, so nothing below it is among the top. What reaches it goes into a list in LDS, whose entries
+// are placed by counting the larger ones. Where that does not serve (too many equal scores, or rising ones in few lanes; a
+// bound of -inf; NaN among the top) the keys are taken one by one: each lane keeps its own largest left, and the one whose
+// key is taken looks for its next (64 x 100,000 with twenty: 39 us, 16 us by the bound).
+constexpr int LIST = 256;
 template <int E, class Id>
-__device__ __forceinline__ uint64_t wave_top(uint32_t (&k)[E], int top, int lane, Id &&id) {
+__device__ __forceinline__ uint64_t wave_top(const float (&v)[E], const ClassDist &c, int live, int top, int lane,
+                                             uint64_t *list, Id &&id) {
+    float own = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < E; r++) own = fmaxf(own, v[r]);
+    const uint32_t key = score_key(own);
+    uint32_t lo = ~wave_max_u32(~key), hi = score_key(c.m);
+    for (int i = 0; i < 14 && lo < hi; i++) {
+        const uint32_t mid = hi - (hi - lo) / 2;
+        if (__popcll(__ballot(key >= mid)) >= top) lo = mid;
+        else hi = mid - 1;
+    }
+    if (lo > score_key(-INFINITY)) {
+        const float bound = score_of(lo);
+        int n = 0;
+#pragma unroll
+        for (int r = 0; r < E; r++) {
+            const bool in = v[r] >= bound;
+            const uint64_t who = __ballot(in);
+            if (who) {
+                const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+                if (in && at < LIST) list[at] = class_key(score_key(v[r]), id(r));
+                n += __popcll(who);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (n >= top && n <= LIST) {
+            uint64_t mine[LIST / 64];
+            int place[LIST / 64];
+#pragma unroll
+            for (int u = 0; u < LIST / 64; u++) {
+                if (64 * u >= n) break;
+                mine[u] = 64 * u + lane < n ? list[64 * u + lane] : 0;
+                place[u] = 0;
+#pragma unroll 4
+                for (int j = 0; j < n; j++) place[u] += list[j] > mine[u];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();  // every entry is read before the first is written over
+#pragma unroll
+            for (int u = 0; u < LIST / 64; u++) {
+                if (64 * u >= n) break;
+                if (mine[u] && place[u] < top) list[place[u]] = mine[u];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            return lane < top ? list[lane] : 0;
+        }
+    }
+    uint32_t k[E];
+#pragma unroll
+    for (int r = 0; r < E; r++) k[r] = r < live ? score_key(v[r]) : 0u;
     uint64_t mine = 0, got = 0;
     auto next = [&] {
         uint32_t best = 0;
@@ -218,14 +283,15 @@ __device__ __forceinline__ uint64_t wave_top(uint32_t (&k)[E], int top, int lane
 template <int E>
 __global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_t ld, const float *__restrict__ x, float inv,
                                                           ClassOut o) {
+    __shared__ uint64_t list[4][LIST];
     const int lane = threadIdx.x & 63;
     const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= (size_t)rows) return;
     const float *src = x + row * ld;
-    uint32_t k[E];
+    float v[E];
 #pragma unroll
-    for (int r = 0; r < E; r++) k[r] = 64 * r + lane < n ? score_key(src[64 * r + lane]) : 0u;
-    const ClassDist c = wave_dist(k, inv);
+    for (int r = 0; r < E; r++) v[r] = 64 * r + lane < n ? src[64 * r + lane] : -INFINITY;
+    const ClassDist c = wave_dist(v, inv);
     float *st = o.stats + row * (1 + o.n_given + o.top);
     if (lane == 0) st[0] = entropy(c);
     if (lane < o.n_given) {
@@ -233,7 +299,8 @@ __global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_
         st[1 + lane] = id >= 0 && id < n ? log_p(c, src[id], inv) : NAN;
     }
     if (o.top == 0) return;
-    const uint64_t key = wave_top(k, o.top, lane, [&](int r) { return 64 * r + lane; });
+    const uint64_t key = wave_top(v, c, (n - lane + 63) / 64, o.top, lane, list[threadIdx.x >> 6],
+                                  [&](int r) { return 64 * r + lane; });
     if (lane < o.top) {
         st[1 + o.n_given + lane] = log_p(c, score_of((uint32_t)(key >> 32)), inv);
         o.ids[row * o.top + lane] = class_of(key);
@@ -280,32 +347,35 @@ __device__ __forceinline__ int place_of(uint64_t key, const uint64_t *keys, int 
 __global__ __launch_bounds__(256) void k_class_stats_seg(int n, size_t ld, const float *__restrict__ x, float inv,
                                                          uint8_t *__restrict__ state, ClassOut o) {
     __shared__ ClassDist part[4];
-    __shared__ uint64_t keys[4 * 64];
+    __shared__ uint64_t keys[4 * 64], list[4][LIST];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = blockIdx.x, segs = gridDim.x;
     const size_t row = blockIdx.y;
     const float *src = x + row * ld;
     const int base = seg * SEG;
-    uint32_t k[SEG_E];
+    float v[SEG_E];
     // entry 4 r + j of a thread: class base + 4 (256 r + tid) + j
     const bool whole = base + SEG <= n && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
 #pragma unroll
     for (int r = 0; r < SEG_E / 4; r++) {
         const int i = base + 4 * (256 * r + tid);
         if (whole) {
-            const float4 v = *reinterpret_cast<const float4 *>(src + i);
-            k[4 * r] = score_key(v.x);
-            k[4 * r + 1] = score_key(v.y);
-            k[4 * r + 2] = score_key(v.z);
-            k[4 * r + 3] = score_key(v.w);
+            const float4 x4 = *reinterpret_cast<const float4 *>(src + i);
+            v[4 * r] = x4.x;
+            v[4 * r + 1] = x4.y;
+            v[4 * r + 2] = x4.z;
+            v[4 * r + 3] = x4.w;
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) k[4 * r + j] = i + j < n ? score_key(src[i + j]) : 0u;
+            for (int j = 0; j < 4; j++) v[4 * r + j] = i + j < n ? src[i + j] : -INFINITY;
         }
     }
-    const ClassDist w = wave_dist(k, inv);
+    const ClassDist w = wave_dist(v, inv);
     if (lane == 0) part[wave] = w;
     if (o.top > 0) {
-        const uint64_t key = wave_top(k, o.top, lane, [&](int e) { return base + 4 * (256 * (e >> 2) + tid) + (e & 3); });
+        // entries of this thread that are scores: those of its whole fours, then what its last one has
+        const int left = max(0, min(SEG, n - base) - 4 * tid), live = left / 1024 * 4 + min(4, left % 1024);
+        const uint64_t key = wave_top(v, w, live, o.top, lane, list[wave],
+                                      [&](int e) { return base + 4 * (256 * (e >> 2) + tid) + (e & 3); });
         if (lane < o.top) keys[wave * o.top + lane] = key;
     }
     __syncthreads();
@@ -330,25 +400,35 @@ __global__ __launch_bounds__(256) void k_class_stats_seg(int n, size_t ld, const
     if (segs > 1 && tid >= live && tid < o.top) reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[tid] = 0;
 }
 
-// grid rows; 256 threads: the segments of a row joined; segs top keys of LDS.
-__global__ __launch_bounds__(256) void k_class_stats_join(int n, size_t ld, const float *__restrict__ x, float inv, int segs,
+// grid rows; 512 threads: the segments of a row joined; segs top keys of LDS.
+__global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, const float *__restrict__ x, float inv, int segs,
                                                           const uint8_t *__restrict__ state, ClassOut o) {
     extern __shared__ uint64_t all[];
     const int tid = threadIdx.x;
     const size_t row = blockIdx.x;
     const uint8_t *rows_state = state + row * segs * seg_bytes(o.top);
-    for (int i = tid; i < segs * o.top; i += 256) {
+    const int total = segs * o.top;
+    for (int i = tid; i < total; i += 512) {
         const int s = i / o.top;
         all[i] = reinterpret_cast<const uint64_t *>(rows_state + s * seg_bytes(o.top) + sizeof(SegState))[i - s * o.top];
     }
     ClassDist c{-INFINITY, 0.0f, 0.0f, false};
-    for (int s = 0; s < segs; s++) c = join(c, reinterpret_cast<const SegState *>(rows_state + s * seg_bytes(o.top))->c, inv);
+    for (int s = tid & 63; s < segs; s += 64)
+        c = join(c, reinterpret_cast<const SegState *>(rows_state + s * seg_bytes(o.top))->c, inv);
+    for (int mask = 1; mask < 64; mask <<= 1) c = join_lane(c, mask, inv);
     write_row(c, o, row, n, x + row * ld, inv, tid);
     __syncthreads();
-    for (int i = tid; i < segs * o.top; i += 256) {
+    for (int i = tid; i < total; i += 512) {
         const uint64_t key = all[i];
         if (!key) continue;
-        const int place = place_of(key, all, segs, o.top);
+        int place = 0;
+        if (total <= 1024) {
+            // reads of one address, none waiting for another
+#pragma unroll 8
+            for (int j = 0; j < total; j++) place += all[j] > key;
+        } else {
+            place = place_of(key, all, segs, o.top);
+        }
         if (place < o.top) {
             o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = log_p(c, score_of((uint32_t)(key >> 32)), inv);
             o.ids[row * o.top + place] = class_of(key);
@@ -407,7 +487,7 @@ void class_stats(hipStream_t s, int rows, int n, size_t ld, const float *x, floa
             hipLaunchKernelGGL(k_class_stats_seg, dim3(segs, here), dim3(256), 0, s, n, ld, xr, inv,
                                static_cast<uint8_t *>(work), at);
             if (segs > 1)
-                hipLaunchKernelGGL(k_class_stats_join, dim3(here), dim3(256), (size_t)segs * top * 8, s, n, ld, xr, inv, segs,
+                hipLaunchKernelGGL(k_class_stats_join, dim3(here), dim3(512), (size_t)segs * top * 8, s, n, ld, xr, inv, segs,
                                    static_cast<const uint8_t *>(work), at);
         }
     }
