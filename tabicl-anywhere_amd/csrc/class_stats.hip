@@ -193,13 +193,51 @@ __device__ __forceinline__ ClassDist wave_dist(const float (&v)[E], float inv) {
 }
 
 // The top largest scores of a wavefront as keys in order: lane r's result is the r-th (top at most 64). live: how many
-// entries of a lane are scores. Class ids: id(r) of entry r.
-//
-// A bound that top lanes' own largest scores reach, and few more, by halving (the least and the largest of them, as keys,
-// apart): top scores reach it, so nothing below it is among the top. What reaches it goes into a list in LDS, whose entries
+// entries of a lane are scores. Class ids: id(r) of entry r. Taken one by one: each lane keeps its own largest left, and
+// the one whose key is taken looks for its next.
+template <int E, class Id>
+__device__ __forceinline__ uint64_t wave_top_each(const float (&v)[E], int live, int top, int lane, Id &&id) {
+    uint32_t k[E];
+#pragma unroll
+    for (int r = 0; r < E; r++) k[r] = r < live ? score_key(v[r]) : 0u;
+    uint64_t mine = 0, got = 0;
+    auto next = [&] {
+        uint32_t best = 0;
+        int at = 0;
+#pragma unroll
+        for (int r = 0; r < E; r++) {
+            const bool more = k[r] > best;
+            best = more ? k[r] : best;
+            at = more ? r : at;
+        }
+#pragma unroll
+        for (int r = 0; r < E; r++) k[r] = r == at ? 0u : k[r];
+        mine = best ? class_key(best, id(at)) : 0;
+    };
+    next();
+    for (int r = 0; r < top; r++) {
+        const uint64_t best = wave_best(mine);
+        if (lane == r) got = best;
+        if (mine == best && best) next();
+    }
+    return got;
+}
+
+// The least key that at least top of the lanes' keys reach, or a little less: halved down from the largest of them (hi).
+__device__ __forceinline__ uint32_t bound_of(uint32_t key, uint32_t hi, int top) {
+    uint32_t lo = ~wave_max_u32(~key);
+    for (int i = 0; i < 14 && lo < hi; i++) {
+        const uint32_t mid = hi - (hi - lo) / 2;
+        if (__popcll(__ballot(key >= mid)) >= top) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// The same sooner. A bound that top lanes' own largest scores reach, and few more, (bound_of): top scores reach it, so nothing below it is among the top. What reaches it goes into a list in LDS, whose entries
 // are placed by counting the larger ones. Where that does not serve (too many equal scores, or rising ones in few lanes; a
-// bound of -inf; NaN among the top) the keys are taken one by one: each lane keeps its own largest left, and the one whose
-// key is taken looks for its next (64 x 100,000 with twenty: 39 us, 16 us by the bound).
+// bound of -inf; NaN among the top) the keys are taken one by one (3,000 x 1,001 with ten: 15.2 us,
+// 8.2 by the bound).
 constexpr int LIST = 256;
 template <int E, class Id>
 __device__ __forceinline__ uint64_t wave_top(const float (&v)[E], const ClassDist &c, int live, int top, int lane,
@@ -207,13 +245,7 @@ __device__ __forceinline__ uint64_t wave_top(const float (&v)[E], const ClassDis
     float own = -INFINITY;
 #pragma unroll
     for (int r = 0; r < E; r++) own = fmaxf(own, v[r]);
-    const uint32_t key = score_key(own);
-    uint32_t lo = ~wave_max_u32(~key), hi = score_key(c.m);
-    for (int i = 0; i < 14 && lo < hi; i++) {
-        const uint32_t mid = hi - (hi - lo) / 2;
-        if (__popcll(__ballot(key >= mid)) >= top) lo = mid;
-        else hi = mid - 1;
-    }
+    const uint32_t lo = bound_of(score_key(own), score_key(c.m), top);
     if (lo > score_key(-INFINITY)) {
         const float bound = score_of(lo);
         int n = 0;
@@ -252,30 +284,7 @@ __device__ __forceinline__ uint64_t wave_top(const float (&v)[E], const ClassDis
             return lane < top ? list[lane] : 0;
         }
     }
-    uint32_t k[E];
-#pragma unroll
-    for (int r = 0; r < E; r++) k[r] = r < live ? score_key(v[r]) : 0u;
-    uint64_t mine = 0, got = 0;
-    auto next = [&] {
-        uint32_t best = 0;
-        int at = 0;
-#pragma unroll
-        for (int r = 0; r < E; r++) {
-            const bool more = k[r] > best;
-            best = more ? k[r] : best;
-            at = more ? r : at;
-        }
-#pragma unroll
-        for (int r = 0; r < E; r++) k[r] = r == at ? 0u : k[r];
-        mine = best ? class_key(best, id(at)) : 0;
-    };
-    next();
-    for (int r = 0; r < top; r++) {
-        const uint64_t best = wave_best(mine);
-        if (lane == r) got = best;
-        if (mine == best && best) next();
-    }
-    return got;
+    return wave_top_each(v, live, top, lane, id);
 }
 
 // ---- up to 1,024 classes: a wavefront a row ------------------------------------------------------------------------------
@@ -312,7 +321,7 @@ __global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_
 struct SegState {
     ClassDist c;
 };
-constexpr int SEG = 8192, SEG_E = SEG / 256;
+constexpr int SEG_T = 512, SEG = 32 * SEG_T, SEG_E = SEG / SEG_T, SEG_LIST = 512;
 
 __host__ __device__ inline size_t seg_bytes(int top) { return sizeof(SegState) + 8 * (size_t)top; }
 
@@ -341,23 +350,30 @@ __device__ __forceinline__ int place_of(uint64_t key, const uint64_t *keys, int 
     return place;
 }
 
-// grid (segments, rows); 256 threads: each keeps 32 scores of its segment in registers, so that the row is read once. Every
-// wavefront takes its 2,048 scores' distribution and most probable classes; the four are joined in LDS, the segments of a
-// row by k_class_stats_join (a row of one segment is written here).
-__global__ __launch_bounds__(256) void k_class_stats_seg(int n, size_t ld, const float *__restrict__ x, float inv,
-                                                         uint8_t *__restrict__ state, ClassOut o) {
-    __shared__ ClassDist part[4];
-    __shared__ uint64_t keys[4 * 64], list[4][LIST];
+// grid (segments, rows); 512 threads: each keeps 32 scores of its segment in registers, so that the row is read once. The
+// wavefronts' distributions are joined in LDS, the segments of a row by k_class_stats_join (a row of one segment is written
+// here). The most probable classes as wave_top has them, but of the workgroup: the bound from the largest scores of its 64
+// groups of eight lanes, one list. Loads and arithmetic hardly overlap, since all workgroups start together: 64 x 100,000
+// is 25.6 MB.
+__global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, size_t ld, const float *__restrict__ x, float inv,
+                                                           uint8_t *__restrict__ state, ClassOut o) {
+    constexpr int W = SEG_T / 64;
+    __shared__ ClassDist part[W];
+    __shared__ float group[64];
+    __shared__ uint64_t list[SEG_LIST];
+    __shared__ int listed;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = blockIdx.x, segs = gridDim.x;
     const size_t row = blockIdx.y;
     const float *src = x + row * ld;
     const int base = seg * SEG;
+    if (tid == 0) listed = 0;
     float v[SEG_E];
-    // entry 4 r + j of a thread: class base + 4 (256 r + tid) + j
+    // entry 4 r + j of a thread: class base + 4 (512 r + tid) + j
+    auto id = [&](int e) { return base + 4 * (SEG_T * (e >> 2) + tid) + (e & 3); };
     const bool whole = base + SEG <= n && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
 #pragma unroll
     for (int r = 0; r < SEG_E / 4; r++) {
-        const int i = base + 4 * (256 * r + tid);
+        const int i = id(4 * r);
         if (whole) {
             const float4 x4 = *reinterpret_cast<const float4 *>(src + i);
             v[4 * r] = x4.x;
@@ -369,35 +385,76 @@ __global__ __launch_bounds__(256) void k_class_stats_seg(int n, size_t ld, const
             for (int j = 0; j < 4; j++) v[4 * r + j] = i + j < n ? src[i + j] : -INFINITY;
         }
     }
+    if (o.top > 0) {
+        float own = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < SEG_E; r++) own = fmaxf(own, v[r]);
+        own = fmaxf(own, dpp<0xb1>(own));   // lanes 1 apart
+        own = fmaxf(own, dpp<0x4e>(own));   // 2 apart
+        own = fmaxf(own, dpp<0x141>(own));  // the other four of eight
+        if ((lane & 7) == 0) group[tid >> 3] = own;
+    }
     const ClassDist w = wave_dist(v, inv);
     if (lane == 0) part[wave] = w;
-    if (o.top > 0) {
-        // entries of this thread that are scores: those of its whole fours, then what its last one has
-        const int left = max(0, min(SEG, n - base) - 4 * tid), live = left / 1024 * 4 + min(4, left % 1024);
-        const uint64_t key = wave_top(v, w, live, o.top, lane, list[wave],
-                                      [&](int e) { return base + 4 * (256 * (e >> 2) + tid) + (e & 3); });
-        if (lane < o.top) keys[wave * o.top + lane] = key;
-    }
     __syncthreads();
-    const ClassDist c = join(join(part[0], part[1], inv), join(part[2], part[3], inv), inv);
+    ClassDist c = part[0];
+#pragma unroll
+    for (int i = 1; i < W; i++) c = join(c, part[i], inv);
     uint8_t *mine = state + (row * segs + seg) * seg_bytes(o.top);
     if (segs == 1) write_row(c, o, row, n, src, inv, tid);
     else if (tid == 0) reinterpret_cast<SegState *>(mine)->c = c;
-    if (tid < 4 * o.top) {
-        const uint64_t key = keys[tid];
-        const int place = key ? place_of(key, keys, 4, o.top) : o.top;
-        if (place < o.top) {
-            if (segs == 1) {
-                o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = log_p(c, score_of((uint32_t)(key >> 32)), inv);
-                o.ids[row * o.top + place] = class_of(key);
-            } else {
-                reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[place] = key;
+    if (o.top == 0) return;
+    auto put = [&](uint64_t key, int place) {
+        if (segs == 1) {
+            o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = log_p(c, score_of((uint32_t)(key >> 32)), inv);
+            o.ids[row * o.top + place] = class_of(key);
+        } else {
+            reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[place] = key;
+        }
+    };
+    const uint32_t lo = bound_of(score_key(group[lane]), score_key(c.m), o.top);
+    const bool bounded = lo > score_key(-INFINITY);
+    if (bounded) {
+        const float bound = score_of(lo);
+#pragma unroll
+        for (int r = 0; r < SEG_E; r++) {
+            const bool in = v[r] >= bound;
+            const uint64_t who = __ballot(in);
+            if (who) {
+                int from = 0;
+                if (lane == 0) from = atomicAdd(&listed, __popcll(who));
+                from = __builtin_amdgcn_readfirstlane(from);
+                const int at = from + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+                if (in && at < SEG_LIST) list[at] = class_key(score_key(v[r]), id(r));
             }
         }
     }
+    __syncthreads();
+    const int got = listed;
+    if (bounded && got >= o.top && got <= SEG_LIST) {
+        if (tid < got) {
+            const uint64_t key = list[tid];
+            int place = 0;
+#pragma unroll 8
+            for (int j = 0; j < got; j++) place += list[j] > key;
+            if (place < o.top) put(key, place);
+        }
+        return;
+    }
+    __syncthreads();  // the list is free
+    // entries of this thread that are scores: those of its whole fours, then what its last one has
+    const int left = max(0, min(SEG, n - base) - 4 * tid), live = left / (4 * SEG_T) * 4 + min(4, left % (4 * SEG_T));
+    static_assert(W * 64 <= SEG_LIST, "every wavefront's keys fit the list");
+    const uint64_t key = wave_top_each(v, live, o.top, lane, id);
+    if (lane < o.top) list[wave * o.top + lane] = key;
+    __syncthreads();
+    if (tid < W * o.top) {
+        const uint64_t k = list[tid];
+        const int place = k ? place_of(k, list, W, o.top) : o.top;
+        if (place < o.top) put(k, place);
+    }
     // a last segment of fewer classes than top: nothing in the places past them
-    const int live = min(SEG, n - base);
-    if (segs > 1 && tid >= live && tid < o.top) reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[tid] = 0;
+    if (segs > 1 && tid >= n - base && tid < o.top) reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[tid] = 0;
 }
 
 // grid rows; 512 threads: the segments of a row joined; segs top keys of LDS.
@@ -484,7 +541,7 @@ void class_stats(hipStream_t s, int rows, int n, size_t ld, const float *x, floa
             const int here = std::min(most, rows - r0);
             const float *xr = x + r0 * ld;
             const ClassOut at = o.from(r0);
-            hipLaunchKernelGGL(k_class_stats_seg, dim3(segs, here), dim3(256), 0, s, n, ld, xr, inv,
+            hipLaunchKernelGGL(k_class_stats_seg, dim3(segs, here), dim3(SEG_T), 0, s, n, ld, xr, inv,
                                static_cast<uint8_t *>(work), at);
             if (segs > 1)
                 hipLaunchKernelGGL(k_class_stats_join, dim3(here), dim3(512), (size_t)segs * top * 8, s, n, ld, xr, inv, segs,
