@@ -61,16 +61,19 @@ struct ClassOut {
     }
 };
 
-// What a row's distribution says of one score.
-__device__ __forceinline__ float log_p(const ClassDist &c, float x, float inv) {
-    if (c.bad || !(c.m < INFINITY)) return NAN;
-    if (c.m == -INFINITY) return -INFINITY;  // every class ruled out
-    return (x - c.m) * inv - log1pf(c.s);
-}
-__device__ __forceinline__ float entropy(const ClassDist &c) {
-    if (c.bad || !(c.m < INFINITY)) return NAN;
-    return c.m == -INFINITY ? 0.0f : log1pf(c.s) + c.t / (1.0f + c.s);
-}
+// What a row's distribution says: its entropy, and of one score.
+struct ClassLogs {
+    float entropy, from, logs;  // log p = (x - from) / T - logs
+    __device__ __forceinline__ ClassLogs(const ClassDist &c) : from(c.m), logs(log1pf(c.s)) {
+        entropy = logs + c.t / (1.0f + c.s);
+        if (c.m == -INFINITY) {
+            // every class ruled out: -inf - 0
+            entropy = from = logs = 0.0f;
+        }
+        if (c.bad || !(c.m < INFINITY)) entropy = logs = NAN;
+    }
+    __device__ __forceinline__ float log_p(float x, float inv) const { return (x - from) * inv - logs; }
+};
 
 // ---- up to 64 classes: a lane a row -----------------------------------------------------------------------------------
 // grid ceil(rows / 64); 64 threads. The scores of 64 rows come in whole lines and are turned in LDS (an odd pitch: the
@@ -84,17 +87,23 @@ __global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t
     constexpr int PITCH = N + 1;
     __shared__ float turned[64 * PITCH];
     const int lane = threadIdx.x, row0 = blockIdx.x * 64, here = min(64, rows - row0);
-    const float per = 1.0f / (float)n;
     const float *src = x + (size_t)row0 * ld;
     if (n < N) {
 #pragma unroll
         for (int i = 0; i < N; i++) turned[lane * PITCH + i] = -INFINITY;
         __syncthreads();
     }
+    // entry e of the 64 rows' here * n: row r, class i, 64 entries on at each turn
+    const int rows_on = 64 / n, on = 64 - rows_on * n;
+    int r = lane / n, i = lane - r * n;
     for (int e = lane; e < here * n; e += 64) {
-        // e + 1/2 over n is at least 1 / (2 n) from a whole number and below 64: far more than the product's rounding
-        const int r = (int)(((float)e + 0.5f) * per), i = e - r * n;
         turned[r * PITCH + i] = src[r * ld + i];
+        r += rows_on;
+        i += on;
+        if (i >= n) {
+            i -= n;
+            r++;
+        }
     }
     __syncthreads();
     if (lane >= here) return;
@@ -121,10 +130,11 @@ __global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t
     }
     const size_t row = (size_t)row0 + lane;
     float *st = o.stats + row * (1 + o.n_given + o.top);
-    st[0] = entropy(c);
+    const ClassLogs says(c);
+    st[0] = says.entropy;
     for (int i = 0; i < o.n_given; i++) {
         const int id = o.given[row * o.n_given + i];
-        st[1 + i] = id >= 0 && id < n ? log_p(c, mine[id], inv) : NAN;
+        st[1 + i] = id >= 0 && id < n ? says.log_p(mine[id], inv) : NAN;
     }
     for (int r = 0; r < o.top; r++) {
         uint32_t best = 0;
@@ -137,7 +147,7 @@ __global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t
         }
 #pragma unroll
         for (int i = 0; i < N; i++) k[i] = i == id ? 0u : k[i];
-        st[1 + o.n_given + r] = log_p(c, score_of(best), inv);
+        st[1 + o.n_given + r] = says.log_p(score_of(best), inv);
         o.ids[row * o.top + r] = id;
     }
 }
@@ -302,16 +312,17 @@ __global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_
     for (int r = 0; r < E; r++) v[r] = 64 * r + lane < n ? src[64 * r + lane] : -INFINITY;
     const ClassDist c = wave_dist(v, inv);
     float *st = o.stats + row * (1 + o.n_given + o.top);
-    if (lane == 0) st[0] = entropy(c);
+    const ClassLogs says(c);
+    if (lane == 0) st[0] = says.entropy;
     if (lane < o.n_given) {
         const int id = o.given[row * o.n_given + lane];
-        st[1 + lane] = id >= 0 && id < n ? log_p(c, src[id], inv) : NAN;
+        st[1 + lane] = id >= 0 && id < n ? says.log_p(src[id], inv) : NAN;
     }
     if (o.top == 0) return;
     const uint64_t key = wave_top(v, c, (n - lane + 63) / 64, o.top, lane, list[threadIdx.x >> 6],
                                   [&](int r) { return 64 * r + lane; });
     if (lane < o.top) {
-        st[1 + o.n_given + lane] = log_p(c, score_of((uint32_t)(key >> 32)), inv);
+        st[1 + o.n_given + lane] = says.log_p(score_of((uint32_t)(key >> 32)), inv);
         o.ids[row * o.top + lane] = class_of(key);
     }
 }
@@ -325,13 +336,13 @@ constexpr int SEG_T = 512, SEG = 32 * SEG_T, SEG_E = SEG / SEG_T, SEG_LIST = 512
 
 __host__ __device__ inline size_t seg_bytes(int top) { return sizeof(SegState) + 8 * (size_t)top; }
 
-__device__ __forceinline__ void write_row(const ClassDist &c, const ClassOut &o, size_t row, int n, const float *src,
+__device__ __forceinline__ void write_row(const ClassLogs &says, const ClassOut &o, size_t row, int n, const float *src,
                                           float inv, int tid) {
     float *st = o.stats + row * (1 + o.n_given + o.top);
-    if (tid == 0) st[0] = entropy(c);
+    if (tid == 0) st[0] = says.entropy;
     if (tid < o.n_given) {
         const int id = o.given[row * o.n_given + tid];
-        st[1 + tid] = id >= 0 && id < n ? log_p(c, src[id], inv) : NAN;
+        st[1 + tid] = id >= 0 && id < n ? says.log_p(src[id], inv) : NAN;
     }
 }
 
@@ -350,13 +361,13 @@ __device__ __forceinline__ int place_of(uint64_t key, const uint64_t *keys, int 
     return place;
 }
 
-// grid (segments, rows); 512 threads: each keeps 32 scores of its segment in registers, so that the row is read once. The
+// grid (segments, rows); 512 threads: each keeps up to 32 scores of its segment (len, a multiple of 4) in registers, so that the row is read once. The
 // wavefronts' distributions are joined in LDS, the segments of a row by k_class_stats_join (a row of one segment is written
 // here). The most probable classes as wave_top has them, but of the workgroup: the bound from the largest scores of its 64
 // groups of eight lanes, one list. Loads and arithmetic hardly overlap, since all workgroups start together: 64 x 100,000
 // is 25.6 MB.
-__global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, size_t ld, const float *__restrict__ x, float inv,
-                                                           uint8_t *__restrict__ state, ClassOut o) {
+__global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_t ld, const float *__restrict__ x,
+                                                           float inv, uint8_t *__restrict__ state, ClassOut o) {
     constexpr int W = SEG_T / 64;
     __shared__ ClassDist part[W];
     __shared__ float group[64];
@@ -365,16 +376,16 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, size_t ld, con
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = blockIdx.x, segs = gridDim.x;
     const size_t row = blockIdx.y;
     const float *src = x + row * ld;
-    const int base = seg * SEG;
+    const int base = seg * len, end = min(n, base + len);
     if (tid == 0) listed = 0;
     float v[SEG_E];
     // entry 4 r + j of a thread: class base + 4 (512 r + tid) + j
     auto id = [&](int e) { return base + 4 * (SEG_T * (e >> 2) + tid) + (e & 3); };
-    const bool whole = base + SEG <= n && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+    const bool fours = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
 #pragma unroll
     for (int r = 0; r < SEG_E / 4; r++) {
         const int i = id(4 * r);
-        if (whole) {
+        if (fours && i + 4 <= end) {
             const float4 x4 = *reinterpret_cast<const float4 *>(src + i);
             v[4 * r] = x4.x;
             v[4 * r + 1] = x4.y;
@@ -382,7 +393,7 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, size_t ld, con
             v[4 * r + 3] = x4.w;
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[4 * r + j] = i + j < n ? src[i + j] : -INFINITY;
+            for (int j = 0; j < 4; j++) v[4 * r + j] = i + j < end ? src[i + j] : -INFINITY;
         }
     }
     if (o.top > 0) {
@@ -401,12 +412,13 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, size_t ld, con
 #pragma unroll
     for (int i = 1; i < W; i++) c = join(c, part[i], inv);
     uint8_t *mine = state + (row * segs + seg) * seg_bytes(o.top);
-    if (segs == 1) write_row(c, o, row, n, src, inv, tid);
+    const ClassLogs says(c);
+    if (segs == 1) write_row(says, o, row, n, src, inv, tid);
     else if (tid == 0) reinterpret_cast<SegState *>(mine)->c = c;
     if (o.top == 0) return;
     auto put = [&](uint64_t key, int place) {
         if (segs == 1) {
-            o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = log_p(c, score_of((uint32_t)(key >> 32)), inv);
+            o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = says.log_p(score_of((uint32_t)(key >> 32)), inv);
             o.ids[row * o.top + place] = class_of(key);
         } else {
             reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[place] = key;
@@ -443,7 +455,7 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, size_t ld, con
     }
     __syncthreads();  // the list is free
     // entries of this thread that are scores: those of its whole fours, then what its last one has
-    const int left = max(0, min(SEG, n - base) - 4 * tid), live = left / (4 * SEG_T) * 4 + min(4, left % (4 * SEG_T));
+    const int left = max(0, end - base - 4 * tid), live = left / (4 * SEG_T) * 4 + min(4, left % (4 * SEG_T));
     static_assert(W * 64 <= SEG_LIST, "every wavefront's keys fit the list");
     const uint64_t key = wave_top_each(v, live, o.top, lane, id);
     if (lane < o.top) list[wave * o.top + lane] = key;
@@ -454,7 +466,7 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, size_t ld, con
         if (place < o.top) put(k, place);
     }
     // a last segment of fewer classes than top: nothing in the places past them
-    if (segs > 1 && tid >= n - base && tid < o.top) reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[tid] = 0;
+    if (segs > 1 && tid >= end - base && tid < o.top) reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[tid] = 0;
 }
 
 // grid rows; 512 threads: the segments of a row joined; segs top keys of LDS.
@@ -473,7 +485,8 @@ __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, cons
     for (int s = tid & 63; s < segs; s += 64)
         c = join(c, reinterpret_cast<const SegState *>(rows_state + s * seg_bytes(o.top))->c, inv);
     for (int mask = 1; mask < 64; mask <<= 1) c = join_lane(c, mask, inv);
-    write_row(c, o, row, n, x + row * ld, inv, tid);
+    const ClassLogs says(c);
+    write_row(says, o, row, n, x + row * ld, inv, tid);
     __syncthreads();
     for (int i = tid; i < total; i += 512) {
         const uint64_t key = all[i];
@@ -487,22 +500,37 @@ __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, cons
             place = place_of(key, all, segs, o.top);
         }
         if (place < o.top) {
-            o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = log_p(c, score_of((uint32_t)(key >> 32)), inv);
+            o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = says.log_p(score_of((uint32_t)(key >> 32)), inv);
             o.ids[row * o.top + place] = class_of(key);
         }
     }
 }
 
-static int segments(int n) { return (n + SEG - 1) / SEG; }
-
-// Rows whose segments' states fit 32 MB (a launch's grid takes 65,535 of them).
-static int rows_at_once(int n, int top) {
-    return (int)std::max<size_t>(1, std::min<size_t>(65535, (size_t(32) << 20) / (segments(n) * seg_bytes(top))));
+// Rows of more than 1,024 classes: how they are cut. At least as many segments as registers hold, and so many more that the
+// workgroups fill whole rounds of the 256 compute units (64 x 100,000: 8 segments, two workgroups each, where 7 left some
+// with one; 18.0 -> 17.0 us), while a segment keeps 2,048 classes. Rows at a time whose segments' states fit 32 MB (and a
+// launch's grid).
+struct ClassCut {
+    int segs, len, rows;
+};
+static ClassCut cut(int rows, int n, int top) {
+    const int least = (n + SEG - 1) / SEG;
+    long segs = least;
+    if (least > 1 || rows < 256) {
+        const long round = ((long)rows * least + 255) / 256 * 256;
+        segs = std::max<long>(least, std::min<long>({round / rows, n / 2048, 64}));
+    }
+    ClassCut c;
+    c.len = (int)(((n + segs - 1) / segs + 3) / 4 * 4);
+    c.segs = (n + c.len - 1) / c.len;
+    c.rows = (int)std::max<size_t>(1, std::min<size_t>(65535, (size_t(32) << 20) / (c.segs * seg_bytes(top))));
+    return c;
 }
 
 size_t class_stats_work_bytes(int rows, int n, int top) {
-    if (n <= 1024 || segments(n) == 1) return 0;
-    return (size_t)std::min(rows, rows_at_once(n, top)) * segments(n) * seg_bytes(top);
+    if (n <= 1024) return 0;
+    const ClassCut c = cut(rows, n, top);
+    return c.segs == 1 ? 0 : (size_t)std::min(rows, c.rows) * c.segs * seg_bytes(top);
 }
 
 template <int N>
@@ -536,12 +564,13 @@ void class_stats(hipStream_t s, int rows, int n, size_t ld, const float *x, floa
     else if (n <= 512) launch_wave<8>(s, rows, n, ld, x, inv, o);
     else if (n <= 1024) launch_wave<16>(s, rows, n, ld, x, inv, o);
     else {
-        const int segs = segments(n), most = rows_at_once(n, top);
-        for (int r0 = 0; r0 < rows; r0 += most) {
-            const int here = std::min(most, rows - r0);
+        const ClassCut c = cut(rows, n, top);
+        const int segs = c.segs;
+        for (int r0 = 0; r0 < rows; r0 += c.rows) {
+            const int here = std::min(c.rows, rows - r0);
             const float *xr = x + r0 * ld;
             const ClassOut at = o.from(r0);
-            hipLaunchKernelGGL(k_class_stats_seg, dim3(segs, here), dim3(SEG_T), 0, s, n, ld, xr, inv,
+            hipLaunchKernelGGL(k_class_stats_seg, dim3(segs, here), dim3(SEG_T), 0, s, n, c.len, ld, xr, inv,
                                static_cast<uint8_t *>(work), at);
             if (segs > 1)
                 hipLaunchKernelGGL(k_class_stats_join, dim3(here), dim3(512), (size_t)segs * top * 8, s, n, ld, xr, inv, segs,
