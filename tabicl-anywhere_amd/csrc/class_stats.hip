@@ -233,12 +233,13 @@ __device__ __forceinline__ uint64_t wave_top_each(const float (&v)[E], int live,
     return got;
 }
 
-// The least key that at least top of the lanes' keys reach, or a little less: halved down from the largest of them (hi).
-__device__ __forceinline__ uint32_t bound_of(uint32_t key, uint32_t hi, int top) {
-    uint32_t lo = ~wave_max_u32(~key);
+// The largest key that at least top of the lanes' keys (two a lane) reach, or a little less: halved between the least and
+// the largest of them (hi).
+__device__ __forceinline__ uint32_t bound_of(uint32_t key, uint32_t other, uint32_t hi, int top) {
+    uint32_t lo = ~wave_max_u32(~min(key, other));
     for (int i = 0; i < 14 && lo < hi; i++) {
         const uint32_t mid = hi - (hi - lo) / 2;
-        if (__popcll(__ballot(key >= mid)) >= top) lo = mid;
+        if (__popcll(__ballot(key >= mid)) + __popcll(__ballot(other >= mid)) >= top) lo = mid;
         else hi = mid - 1;
     }
     return lo;
@@ -255,7 +256,7 @@ __device__ __forceinline__ uint64_t wave_top(const float (&v)[E], const ClassDis
     float own = -INFINITY;
 #pragma unroll
     for (int r = 0; r < E; r++) own = fmaxf(own, v[r]);
-    const uint32_t lo = bound_of(score_key(own), score_key(c.m), top);
+    const uint32_t lo = bound_of(score_key(own), 0xFFFFFFFFu, score_key(c.m), top + 64);  // one a lane: 64 that always do
     if (lo > score_key(-INFINITY)) {
         const float bound = score_of(lo);
         int n = 0;
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_
 struct SegState {
     ClassDist c;
 };
-constexpr int SEG_T = 512, SEG = 32 * SEG_T, SEG_E = SEG / SEG_T, SEG_LIST = 512;
+constexpr int SEG_T = 512, SEG = 32 * SEG_T, SEG_E = SEG / SEG_T, SEG_LIST = 1024;
 
 __host__ __device__ inline size_t seg_bytes(int top) { return sizeof(SegState) + 8 * (size_t)top; }
 
@@ -363,14 +364,14 @@ __device__ __forceinline__ int place_of(uint64_t key, const uint64_t *keys, int 
 
 // grid (segments, rows); 512 threads: each keeps up to 32 scores of its segment (len, a multiple of 4) in registers, so that the row is read once. The
 // wavefronts' distributions are joined in LDS, the segments of a row by k_class_stats_join (a row of one segment is written
-// here). The most probable classes as wave_top has them, but of the workgroup: the bound from the largest scores of its 64
-// groups of eight lanes, one list. Loads and arithmetic hardly overlap, since all workgroups start together: 64 x 100,000
+// here). The most probable classes as wave_top has them, but of the workgroup: the bound from the largest scores of its 128
+// groups of four lanes, one list. Loads and arithmetic hardly overlap, since all workgroups start together: 64 x 100,000
 // is 25.6 MB.
 __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_t ld, const float *__restrict__ x,
                                                            float inv, uint8_t *__restrict__ state, ClassOut o) {
     constexpr int W = SEG_T / 64;
     __shared__ ClassDist part[W];
-    __shared__ float group[64];
+    __shared__ float group[SEG_T / 4];
     __shared__ uint64_t list[SEG_LIST];
     __shared__ int listed;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = blockIdx.x, segs = gridDim.x;
@@ -402,8 +403,7 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
         for (int r = 0; r < SEG_E; r++) own = fmaxf(own, v[r]);
         own = fmaxf(own, dpp<0xb1>(own));   // lanes 1 apart
         own = fmaxf(own, dpp<0x4e>(own));   // 2 apart
-        own = fmaxf(own, dpp<0x141>(own));  // the other four of eight
-        if ((lane & 7) == 0) group[tid >> 3] = own;
+        if ((lane & 3) == 0) group[tid >> 2] = own;
     }
     const ClassDist w = wave_dist(v, inv);
     if (lane == 0) part[wave] = w;
@@ -424,7 +424,8 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
             reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[place] = key;
         }
     };
-    const uint32_t lo = bound_of(score_key(group[lane]), score_key(c.m), o.top);
+    static_assert(SEG_T / 4 == 128, "two groups a lane");
+    const uint32_t lo = bound_of(score_key(group[lane]), score_key(group[64 + lane]), score_key(c.m), o.top);
     const bool bounded = lo > score_key(-INFINITY);
     if (bounded) {
         const float bound = score_of(lo);
@@ -444,8 +445,8 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
     __syncthreads();
     const int got = listed;
     if (bounded && got >= o.top && got <= SEG_LIST) {
-        if (tid < got) {
-            const uint64_t key = list[tid];
+        for (int i = tid; i < got; i += SEG_T) {
+            const uint64_t key = list[i];
             int place = 0;
 #pragma unroll 8
             for (int j = 0; j < got; j++) place += list[j] > key;
@@ -469,33 +470,52 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
     if (segs > 1 && tid >= end - base && tid < o.top) reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[tid] = 0;
 }
 
-// grid rows; 512 threads: the segments of a row joined; segs top keys of LDS.
+// grid rows; 512 threads: the segments of a row joined; segs (at most 64) lists of top falling keys, in LDS. With j =
+// ceil(top / segs), the ceil(top / j)-th largest of the lists' j-th entries is a bound that top keys reach; what reaches it
+// is placed by counting (all of it, 960 keys of one row, took 25 us of LDS reads).
+constexpr int JOIN_LIST = 512;
 __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, const float *__restrict__ x, float inv, int segs,
                                                           const uint8_t *__restrict__ state, ClassOut o) {
     extern __shared__ uint64_t all[];
-    const int tid = threadIdx.x;
+    __shared__ uint64_t list[JOIN_LIST];
+    __shared__ int listed;
+    const int tid = threadIdx.x, lane = tid & 63, total = segs * o.top;
     const size_t row = blockIdx.x;
     const uint8_t *rows_state = state + row * segs * seg_bytes(o.top);
-    const int total = segs * o.top;
+    if (tid == 0) listed = 0;
     for (int i = tid; i < total; i += 512) {
         const int s = i / o.top;
         all[i] = reinterpret_cast<const uint64_t *>(rows_state + s * seg_bytes(o.top) + sizeof(SegState))[i - s * o.top];
     }
     ClassDist c{-INFINITY, 0.0f, 0.0f, false};
-    for (int s = tid & 63; s < segs; s += 64)
-        c = join(c, reinterpret_cast<const SegState *>(rows_state + s * seg_bytes(o.top))->c, inv);
+    if (lane < segs) c = reinterpret_cast<const SegState *>(rows_state + lane * seg_bytes(o.top))->c;
     for (int mask = 1; mask < 64; mask <<= 1) c = join_lane(c, mask, inv);
     const ClassLogs says(c);
     write_row(says, o, row, n, x + row * ld, inv, tid);
+    if (o.top == 0) return;
     __syncthreads();
+    const int j = (o.top + segs - 1) / segs, need = (o.top + j - 1) / j;
+    // lanes past the lists count as reaching any bound
+    const uint32_t entry = lane < segs ? (uint32_t)(all[lane * o.top + j - 1] >> 32) : 0xFFFFFFFFu;
+    const uint32_t bound = bound_of(entry, 0xFFFFFFFFu, wave_max_u32(lane < segs ? entry : 0u), need + 64 + 64 - segs);
     for (int i = tid; i < total; i += 512) {
         const uint64_t key = all[i];
+        if (key && (uint32_t)(key >> 32) >= bound) {
+            const int at = atomicAdd(&listed, 1);
+            if (at < JOIN_LIST) list[at] = key;
+        }
+    }
+    __syncthreads();
+    const int got = listed;
+    const bool few = got <= JOIN_LIST;  // else equal scores without end
+    const uint64_t *keys = few ? list : all;
+    for (int i = tid; i < (few ? got : total); i += 512) {
+        const uint64_t key = keys[i];
         if (!key) continue;
         int place = 0;
-        if (total <= 1024) {
-            // reads of one address, none waiting for another
+        if (few) {
 #pragma unroll 8
-            for (int j = 0; j < total; j++) place += all[j] > key;
+            for (int u = 0; u < got; u++) place += list[u] > key;
         } else {
             place = place_of(key, all, segs, o.top);
         }
