@@ -852,11 +852,11 @@ extern "C" int tah_pack(tah_dev *dev, const float *c, int32_t d, int32_t rc, int
     });
 }
 
-// Chunks are the kernels' grid in one dimension, coordinates in another.
 static void check_layer(const char *what, int d, int rows, int chunk, int kv_format, const void *a, const void *b) {
     if (d <= 0 || rows < 0 || chunk <= 0 || !kv_known(kv_format)) throw ArgError{std::string(what) + ": bad size or format"};
-    if (2 * (long)d > 65535 || ((long)rows + chunk - 1) / chunk > 65535)
-        throw ArgError{std::string(what) + ": at most 32767 coordinates and 65535 chunks a call"};
+    // the kernels number a chunk's fours of rows, and i16 and i8 packing its coordinates in a grid's second dimension
+    if ((std::min(chunk, std::max(rows, 1)) + 3L) / 4 * 2 * d > 0x7FFFFFFF - 1024 || d > 131070)
+        throw ArgError{std::string(what) + ": a chunk of more numbers than a call takes"};
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) % 4)
         throw ArgError{std::string(what) + ": the pointers have to be 4-byte aligned"};
 }

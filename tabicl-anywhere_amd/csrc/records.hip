@@ -70,46 +70,142 @@ __global__ __launch_bounds__(256) void k_pack(int rows, int d, int chunk, const 
     }
 }
 
-// grid (groups of the layer, 2d / 4); 256 threads: a wavefront a group of one coordinate, a lane a row.
-__global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, int per_chunk, const float *__restrict__ rec32,
+// ---- i4 records and back ------------------------------------------------------------------------------------------------
+// Both are bound by memory (a number is 4 bytes and 9/16 of one), so the numbers move 16 bytes a lane where the records
+// allow it: a lane takes four consecutive rows of a coordinate, 16 lanes a group of 64, UNITS groups in turn with their
+// loads issued together. Records whose rows do not start on whole words (odd chunks) take the same path by single loads.
+constexpr int UNITS = 4;
+
+// grid (groups of a full chunk / 64, chunks); 256 threads.
+__global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const float *__restrict__ rec32,
                                                uint8_t *__restrict__ rec4) {
-    const int j = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (j >= 2 * d) return;
-    const int ci = blockIdx.x / per_chunk, g = blockIdx.x % per_chunk;
-    const int rc = min(chunk, rows - ci * chunk), r = g * GROUP4 + lane;
-    if (g * GROUP4 >= rc) return;
-    const bool in = r < rc;
-    const float v = in ? rec32[(size_t)ci * 2 * d * chunk + (size_t)j * rc + r] : 0.0f;
-    const bool fin = in && fabsf(v) < INFINITY;
-    const float lo = -wave_max(fin ? -v : -INFINITY), hi = wave_max(fin ? v : -INFINITY);
-    const Step4 st = step_for4(lo, hi);
-    const int code = in ? code4(st, v) + 8 : 0;
-    uint8_t *rec = rec4 + (size_t)ci * record_bytes(TAH_KV_I4, d, chunk);
-    if (lane < 2)
-        reinterpret_cast<uint16_t *>(rec)[2 * ((size_t)j * groups4(rc) + g) + lane] =
-            (uint16_t)(__float_as_uint(lane == 0 ? st.s : st.z) >> 16);
-    const int next = __shfl_down(code, 1);
-    if (in && !(lane & 1))
-        rec[8 * (size_t)d * groups4(rc) + (size_t)j * ((rc + 1) / 2) + (r >> 1)] = (uint8_t)(code | next << 4);
+    const int n_chunks = (rows + chunk - 1) / chunk;
+    for (int ci = blockIdx.y; ci < n_chunks; ci += gridDim.y) {
+        const int rc = min(chunk, rows - ci * chunk), G = groups4(rc), half = (rc + 1) / 2, in16 = 4 * (threadIdx.x & 15);
+        const float *src = rec32 + (size_t)ci * 2 * d * chunk;
+        uint8_t *rec = rec4 + (size_t)ci * record_bytes(TAH_KV_I4, d, chunk), *codes = rec + 8 * (size_t)d * G;
+        const bool fours = rc % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+        const bool pairs = half % 2 == 0 && (reinterpret_cast<uintptr_t>(codes) & 1) == 0;
+        float v[UNITS][4];
+        int j[UNITS], g[UNITS];
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            const int unit = (blockIdx.x * UNITS + u) * 16 + (threadIdx.x >> 4);
+            j[u] = unit / G;
+            g[u] = unit - j[u] * G;
+            const int r = 64 * g[u] + in16;
+            const float *at = src + (size_t)j[u] * rc + r;
+#pragma unroll
+            for (int t = 0; t < 4; t++) v[u][t] = NAN;  // what is past the end takes no part
+            if (j[u] >= 2 * d) continue;
+            if (fours && r < rc) {
+                const float4 x = *reinterpret_cast<const float4 *>(at);
+                v[u][0] = x.x; v[u][1] = x.y; v[u][2] = x.z; v[u][3] = x.w;
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    if (r + t < rc) v[u][t] = at[t];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            // the group's least and largest number (NaN passed over); again without the infinities where there are any
+            auto range = [&](bool all, float &lo, float &hi) {
+                lo = INFINITY;
+                hi = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const float x = all || fabsf(v[u][t]) < INFINITY ? v[u][t] : NAN;
+                    lo = fminf(lo, x);
+                    hi = fmaxf(hi, x);
+                }
+                lo = row16_reduce(lo, fminf);
+                hi = row16_reduce(hi, fmaxf);
+            };
+            float lo, hi;
+            range(true, lo, hi);
+            if (__any(fmaxf(fabsf(lo), fabsf(hi)) == INFINITY)) range(false, lo, hi);
+            const Step4 st = step_for4(lo, hi);
+            if (j[u] >= 2 * d) continue;
+            const int r = 64 * g[u] + in16, left = rc - r;
+            if (in16 == 0) {
+                uint16_t *sp = reinterpret_cast<uint16_t *>(rec) + 2 * ((size_t)j[u] * G + g[u]);
+                sp[0] = (uint16_t)(__float_as_uint(st.s) >> 16);
+                sp[1] = (uint16_t)(__float_as_uint(st.z) >> 16);
+            }
+            if (left <= 0) continue;
+            uint32_t word = 0;
+#pragma unroll
+            for (int t = 0; t < 4; t++) word |= (t < left ? (uint32_t)(code4(st, v[u][t]) + 8) : 0u) << 4 * t;
+            uint8_t *cp = codes + (size_t)j[u] * half + r / 2;
+            if (pairs && left > 2) {
+                *reinterpret_cast<uint16_t *>(cp) = (uint16_t)word;
+            } else {
+                cp[0] = (uint8_t)word;
+                if (left > 2) cp[1] = (uint8_t)(word >> 8);
+            }
+        }
+    }
 }
 
-// grid (ceil(rows of a chunk / 256), 2d, chunks); 256 threads, a row each.
+// What four consecutive rows (from a multiple of 4) of coordinate j of a chunk's record stand for; rows past the end not
+// looked at.
+template <int FMT>
+__device__ __forceinline__ void values_of(const uint8_t *rec, int d, int rc, int j, int r, bool whole, float (&v)[4]) {
+    if constexpr (FMT == TAH_KV_I4) {
+        const Step4 st = step_at4(rec, rc, j, r / GROUP4);
+        const int half = (rc + 1) / 2;
+        const uint8_t *cp = rec + 8 * (size_t)d * groups4(rc) + (size_t)j * half + r / 2;
+        uint32_t word;
+        if (whole) word = *reinterpret_cast<const uint16_t *>(cp);
+        else word = cp[0] | (r + 2 < rc ? cp[1] : 0) << 8;
+#pragma unroll
+        for (int t = 0; t < 4; t++) v[t] = value4(st, (int)(word >> 4 * t & 15) - 8);
+    } else {
+        const float s = reinterpret_cast<const float *>(rec)[j];
+        const size_t at = (size_t)j * rc + r;
+        const uint8_t *body = rec + 8 * (size_t)d;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            if (r + t < rc)
+                v[t] = s * (FMT == TAH_KV_I16 ? (float)reinterpret_cast<const int16_t *>(body)[at + t]
+                                              : (float)reinterpret_cast<const int8_t *>(body)[at + t]);
+    }
+}
+
+// grid (fours of rows of a full chunk / 1,024, chunks); 256 threads.
 template <int FMT>
 __global__ __launch_bounds__(256) void k_unpack(int rows, int d, int chunk, const uint8_t *__restrict__ rec,
                                                 float *__restrict__ rec32) {
-    const int j = blockIdx.y, ci = blockIdx.z, rc = min(chunk, rows - ci * chunk), r = blockIdx.x * 256 + threadIdx.x;
-    if (r >= rc) return;
-    const uint8_t *src = rec + (size_t)ci * record_bytes(FMT, d, chunk);
-    float v;
-    if constexpr (FMT == TAH_KV_I4) {
-        v = record_value4(src, d, rc, j, r);
-    } else {
-        const float s = reinterpret_cast<const float *>(src)[j];
-        const size_t at = (size_t)j * rc + r;
-        src += 8 * (size_t)d;
-        v = s * (FMT == TAH_KV_I16 ? (float)reinterpret_cast<const int16_t *>(src)[at] : (float)reinterpret_cast<const int8_t *>(src)[at]);
+    const int n_chunks = (rows + chunk - 1) / chunk;
+    for (int ci = blockIdx.y; ci < n_chunks; ci += gridDim.y) {
+        const int rc = min(chunk, rows - ci * chunk), Q = (rc + 3) / 4;
+        const uint8_t *src = rec + (size_t)ci * record_bytes(FMT, d, chunk);
+        float *dst = rec32 + (size_t)ci * 2 * d * chunk;
+        const bool fours = rc % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+        const bool whole = rc % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 1) == 0;  // two bytes of codes at once
+        float v[UNITS][4];
+        int j[UNITS], r[UNITS];
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            const int unit = (blockIdx.x * UNITS + u) * 256 + threadIdx.x;
+            j[u] = unit / Q;
+            r[u] = 4 * (unit - j[u] * Q);
+            if (j[u] < 2 * d) values_of<FMT>(src, d, rc, j[u], r[u], whole, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            if (j[u] >= 2 * d) continue;
+            float *to = dst + (size_t)j[u] * rc + r[u];
+            if (fours) {
+                *reinterpret_cast<float4 *>(to) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    if (r[u] + t < rc) to[t] = v[u][t];
+            }
+        }
     }
-    rec32[(size_t)ci * 2 * d * chunk + (size_t)j * rc + r] = v;
 }
 
 void to_records(hipStream_t s, int rows, int d, int chunk, const float *kv, float *rec32) {
@@ -124,8 +220,9 @@ void pack(hipStream_t s, int rows, int d, int chunk, int fmt, const float *rec32
     const int n_chunks = (rows + chunk - 1) / chunk;
     dim3 grid(n_chunks, (2 * d + 3) / 4);
     if (fmt == TAH_KV_I4) {
-        const int per_chunk = groups4(chunk);
-        hipLaunchKernelGGL(k_pack4, dim3(n_chunks * per_chunk, grid.y), dim3(256), 0, s, rows, d, chunk, per_chunk, rec32, recq);
+        const size_t units = 2 * (size_t)d * groups4(std::min(chunk, rows));
+        hipLaunchKernelGGL(k_pack4, dim3((units + 16 * UNITS - 1) / (16 * UNITS), std::min(n_chunks, 65535)), dim3(256), 0, s,
+                           rows, d, chunk, rec32, recq);
     } else if (fmt == TAH_KV_I16)
         hipLaunchKernelGGL(k_pack<TAH_KV_I16>, grid, dim3(256), 0, s, rows, d, chunk, rec32, recq);
     else if (fmt == TAH_KV_I8)
@@ -138,7 +235,8 @@ void pack(hipStream_t s, int rows, int d, int chunk, int fmt, const float *rec32
 void unpack(hipStream_t s, int rows, int d, int chunk, int fmt, const uint8_t *rec, float *rec32) {
     if (rows <= 0) return;
     const int n_chunks = (rows + chunk - 1) / chunk;
-    const dim3 grid((std::min(chunk, rows) + 255) / 256, 2 * d, n_chunks);
+    const size_t fours = 2 * (size_t)d * ((std::min(chunk, rows) + 3) / 4);
+    const dim3 grid((fours + 256 * UNITS - 1) / (256 * UNITS), std::min(n_chunks, 65535));
     if (fmt == TAH_KV_F32)
         TAH_HIP(hipMemcpyAsync(rec32, rec, sizeof(float) * 2 * (size_t)rows * d, hipMemcpyDeviceToDevice, s));
     else if (fmt == TAH_KV_I16)
