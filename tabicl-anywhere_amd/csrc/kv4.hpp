@@ -46,11 +46,30 @@ __device__ __forceinline__ Step4 step_for4(float lo, float hi) {
     return st;
 }
 
-// the code of a value: the nearest level (the quotient correctly rounded never meets a tie that the exact one does not:
-// a tie is a product of twelve bits with s, and a float beside it is off by more than half the quotient's last place)
+// The code of a value: the nearest level of (v - z) / s, a tie to the even one. The quotient correctly rounded never meets a
+// tie that the exact one does not: a tie is a product of twelve bits with s, and a float beside it is off by more than half
+// the quotient's last place.
 __device__ __forceinline__ int code4(Step4 st, float v) {
     if (!(st.s > 0.0f) || v != v) return 0;
     return (int)fminf(fmaxf(rintf(__fdiv_rn(v - st.z, st.s)), -8.0f), 7.0f);
+}
+
+// The same of four values with one reciprocal: it is off by 2^-22 of the quotient at most, so that away from a tie the
+// nearest level is the same; where a lane of the wavefront is near one (one in 2^16 values), by the division.
+__device__ __forceinline__ void codes4(Step4 st, const float (&v)[4], int (&code)[4]) {
+    const bool some = st.s > 0.0f;
+    const float inv = some ? __builtin_amdgcn_rcpf(st.s) : 0.0f;
+    bool near = false;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const float x = (v[t] - st.z) * inv, q = rintf(x);
+        near = near || fabsf(x - q) > 0.5f - 0x1p-16f;
+        code[t] = some && v[t] == v[t] ? (int)fminf(fmaxf(q, -8.0f), 7.0f) : 0;
+    }
+    if (__any(near)) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) code[t] = code4(st, v[t]);
+    }
 }
 
 __device__ __forceinline__ Step4 step_at4(const uint8_t *rec, int rc, int j, int g) {

@@ -88,11 +88,18 @@ __global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const
         const bool pairs = half % 2 == 0 && (reinterpret_cast<uintptr_t>(codes) & 1) == 0;
         float v[UNITS][4];
         int j[UNITS], g[UNITS];
+        // the units of a thread are 16 apart
+        const int unit = blockIdx.x * UNITS * 16 + (threadIdx.x >> 4), over = 16 / G, past = 16 - over * G;
+        j[0] = unit / G;
+        g[0] = unit - j[0] * G;
+#pragma unroll
+        for (int u = 1; u < UNITS; u++) {
+            g[u] = g[u - 1] + past;
+            j[u] = j[u - 1] + over + (g[u] >= G);
+            g[u] -= g[u] >= G ? G : 0;
+        }
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
-            const int unit = (blockIdx.x * UNITS + u) * 16 + (threadIdx.x >> 4);
-            j[u] = unit / G;
-            g[u] = unit - j[u] * G;
             const int r = 64 * g[u] + in16;
             const float *at = src + (size_t)j[u] * rc + r;
 #pragma unroll
@@ -134,9 +141,11 @@ __global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const
                 sp[1] = (uint16_t)(__float_as_uint(st.z) >> 16);
             }
             if (left <= 0) continue;
+            int code[4];
+            codes4(st, v[u], code);
             uint32_t word = 0;
 #pragma unroll
-            for (int t = 0; t < 4; t++) word |= (t < left ? (uint32_t)(code4(st, v[u][t]) + 8) : 0u) << 4 * t;
+            for (int t = 0; t < 4; t++) word |= (t < left ? (uint32_t)(code[t] + 8) : 0u) << 4 * t;
             uint8_t *cp = codes + (size_t)j[u] * half + r / 2;
             if (pairs && left > 2) {
                 *reinterpret_cast<uint16_t *>(cp) = (uint16_t)word;
@@ -153,7 +162,13 @@ __global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const
 template <int FMT>
 __device__ __forceinline__ void values_of(const uint8_t *rec, int d, int rc, int j, int r, bool whole, float (&v)[4]) {
     if constexpr (FMT == TAH_KV_I4) {
-        const Step4 st = step_at4(rec, rc, j, r / GROUP4);
+        Step4 st;
+        if (whole) {
+            const uint32_t sz = reinterpret_cast<const uint32_t *>(rec)[(size_t)j * groups4(rc) + r / GROUP4];
+            st = {__uint_as_float(sz << 16), __uint_as_float(sz & 0xFFFF0000u)};
+        } else {
+            st = step_at4(rec, rc, j, r / GROUP4);
+        }
         const int half = (rc + 1) / 2;
         const uint8_t *cp = rec + 8 * (size_t)d * groups4(rc) + (size_t)j * half + r / 2;
         uint32_t word;
@@ -183,14 +198,22 @@ __global__ __launch_bounds__(256) void k_unpack(int rows, int d, int chunk, cons
         const uint8_t *src = rec + (size_t)ci * record_bytes(FMT, d, chunk);
         float *dst = rec32 + (size_t)ci * 2 * d * chunk;
         const bool fours = rc % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
-        const bool whole = rc % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 1) == 0;  // two bytes of codes at once
+        const bool whole = rc % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 3) == 0;  // steps and codes by whole words
         float v[UNITS][4];
         int j[UNITS], r[UNITS];
+        // the fours of a thread are 256 apart
+        const int unit = blockIdx.x * UNITS * 256 + threadIdx.x, over = 256 / Q, past = 256 - over * Q;
+        j[0] = unit / Q;
+        r[0] = unit - j[0] * Q;
+#pragma unroll
+        for (int u = 1; u < UNITS; u++) {
+            r[u] = r[u - 1] + past;
+            j[u] = j[u - 1] + over + (r[u] >= Q);
+            r[u] -= r[u] >= Q ? Q : 0;
+        }
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
-            const int unit = (blockIdx.x * UNITS + u) * 256 + threadIdx.x;
-            j[u] = unit / Q;
-            r[u] = 4 * (unit - j[u] * Q);
+            r[u] *= 4;
             if (j[u] < 2 * d) values_of<FMT>(src, d, rc, j[u], r[u], whole, v[u]);
         }
 #pragma unroll
