@@ -1625,15 +1625,17 @@ __global__ __launch_bounds__(256, 1) void k_attn_few(int nq, int rows, int chunk
 // until the four softmax states are merged. The products are 16 x 16 x 32 with the queries as columns: S = K Q^T by 16
 // (two for each of four sets of 16 keys and two halves of the coordinates), O^T += V^T P^T by 16. The order of the keys
 // within a tile leaves a lane's eight scores of each 32 keys as the operand that the values' product takes.
+constexpr int FEW4_Q = 512;
 constexpr int FEW4_WAVES = 8;
+template <int G>
 __global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlocks kbs, int chunk, const float *__restrict__ q,
                                                       const uint8_t *__restrict__ tiles, const uint32_t *__restrict__ kvmax,
                                                       int kb_per_split, float *__restrict__ part_o,
                                                       float *__restrict__ part_ml, float *__restrict__ out) {
-    constexpr int W = FEW4_WAVES;
-    __shared__ float mref[W][16], msum[W][16], macc[W][64][17];
+    constexpr int W = FEW4_WAVES, NQ = 16 * G;
+    __shared__ float mref[W][NQ], msum[W][NQ], macc[W][64][NQ + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int qi = lane & 15, lg = lane >> 4;
+    const int qi = lane & 15, lg = lane >> 4, q0 = blockIdx.z * NQ;
     const int h = blockIdx.x, heads = gridDim.x, split = blockIdx.y, splits = gridDim.y, d = 64 * heads;
     const int kb0 = split * kb_per_split, kb1 = min(kbs.n_kb, kb0 + kb_per_split);
     const uint8_t *head_tiles = tiles + (size_t)h * IMG4;
@@ -1661,83 +1663,102 @@ __global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlo
     if (kb < kb1) cur[0] = fetch(kb);
     int in_chunk = kb % kbs.bpc, ci = kb / kbs.bpc;  // kept along, without a division a block
     const int over = W % kbs.bpc, past = W / kbs.bpc;
-    // query qi's coordinates 32 ks + 8 lg + t, scaled to a maximum near 2^14 and split
-    halfx8 qh[2], ql[2];
-    float qv[2][8];
-    {
-        const float *src = q + (size_t)min(qi, nq - 1) * d + h * 64 + 8 * lg;
-        const float live = qi < nq ? 1.0f : 0.0f;
-        float qmax = 0.0f;
+    // query 16 g + qi's coordinates 32 ks + 8 lg + t, scaled to a maximum near 2^14 and split
+    halfx8 qh[G][2], ql[G][2];
+    float to_log2[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const int at = q0 + 16 * g + qi;
+        const float *src = q + (size_t)min(at, nq - 1) * d + h * 64 + 8 * lg;
+        float qv[2][8], qmax = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
             load8(src + 32 * ks, qv[ks]);
 #pragma unroll
             for (int t = 0; t < 8; t++) {
-                qv[ks][t] *= live;
+                qv[ks][t] = at < nq ? qv[ks][t] : 0.0f;
                 qmax = fmaxf(qmax, fabsf(qv[ks][t]));
             }
         }
         qmax = max32(max16(qmax));
         const int eq = shift_for_max(qmax);
 #pragma unroll
-        for (int ks = 0; ks < 2; ks++) split8(qv[ks], ldexpf(1.0f, eq), qh[ks], ql[ks]);
-        qv[0][0] = ldexpf(LOG2E, -(shift_for(kvmax[h * 2]) + eq));
+        for (int ks = 0; ks < 2; ks++) split8(qv[ks], ldexpf(1.0f, eq), qh[g][ks], ql[g][ks]);
+        to_log2[g] = ldexpf(LOG2E, -(shift_for(kvmax[h * 2]) + eq));
     }
-    const float to_log2 = qv[0][0];
-    float ref = -INFINITY, l = 0.0f;
-    floatx4 acc[4];  // O^T: coordinate 16 m + 4 lg + i of query qi, times 2^sv
+    float ref[G], l[G];
+    floatx4 acc[G][4];  // O^T: coordinate 16 m + 4 lg + i of query 16 g + qi, times 2^sv
 #pragma unroll
-    for (int m = 0; m < 4; m++) acc[m] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int g = 0; g < G; g++) {
+        ref[g] = -INFINITY;
+        l[g] = 0.0f;
+#pragma unroll
+        for (int m = 0; m < 4; m++) acc[g][m] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     auto step = [&](const Block &cur) {
         const int nk = min(KB, (ci == kbs.n_chunks - 1 ? kbs.last_rc : chunk) - in_chunk * KB);
-        float sc[16];  // 8 s + 4 p + i: key 32 s + 8 lg + 4 p + i
+        float sc[G][16];  // 8 s + 4 p + i: key 32 s + 8 lg + 4 p + i
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int p = 0; p < 2; p++) {
-                floatx4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+                floatx4 a[G];
+#pragma unroll
+                for (int g = 0; g < G; g++) a[g] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int ks = 0; ks < 2; ks++) {
-                    const halfx8 k = values4(cur.k[s][2 * p + ks], cur.ks[ks], cur.kz[ks]);
-                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[ks], a, 0, 0, 0);
-                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[ks], a, 0, 0, 0);
+                    const halfx8 kv = values4(cur.k[s][2 * p + ks], cur.ks[ks], cur.kz[ks]);
+#pragma unroll
+                    for (int g = 0; g < G; g++) a[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, qh[g][ks], a[g], 0, 0, 0);
+#pragma unroll
+                    for (int g = 0; g < G; g++) a[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, ql[g][ks], a[g], 0, 0, 0);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) sc[8 * s + 4 * p + i] = a[i];
+                for (int g = 0; g < G; g++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sc[g][8 * s + 4 * p + i] = a[g][i];
             }
-        if (nk < KB) {
+        halfx8 ph[G][2], pl[G][2];
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (32 * (j >> 3) + 8 * lg + (j & 7) >= nk) sc[j] = -INFINITY;
-        }
-        float mb = sc[0];
+        for (int g = 0; g < G; g++) {
+            if (nk < KB) {
 #pragma unroll
-        for (int j = 1; j < 16; j++) mb = fmaxf(mb, sc[j]);
-        mb = max32(max16(mb)) * to_log2;
-        const bool grow = mb > ref + 3.0f;
-        if (__any(grow)) {
-            const float nref = grow ? mb : ref;
-            const float alpha = exp2_hw(ref - nref);
-            l *= alpha;
-#pragma unroll
-            for (int m = 0; m < 4; m++) acc[m] *= alpha;
-            ref = nref;
-        }
-        const float off = 12.0f - ref;
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-            u32x4 hw, lw;
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const float p0 = exp2_hw(fmaf(sc[8 * s + 2 * t], to_log2, off));
-                const float p1 = exp2_hw(fmaf(sc[8 * s + 2 * t + 1], to_log2, off));
-                l += p0 + p1;
-                uint32_t hi, lo;
-                split2(p0, p1, hi, lo);
-                hw[t] = hi;
-                lw[t] = lo;
+                for (int j = 0; j < 16; j++)
+                    if (32 * (j >> 3) + 8 * lg + (j & 7) >= nk) sc[g][j] = -INFINITY;
             }
-            const halfx8 ph = __builtin_bit_cast(halfx8, hw), pl = __builtin_bit_cast(halfx8, lw);
+            float mb = sc[g][0];
+#pragma unroll
+            for (int j = 1; j < 16; j++) mb = fmaxf(mb, sc[g][j]);
+            mb = max32(max16(mb)) * to_log2[g];
+            const bool grow = mb > ref[g] + 3.0f;
+            if (__any(grow)) {
+                const float nref = grow ? mb : ref[g];
+                const float alpha = exp2_hw(ref[g] - nref);
+                l[g] *= alpha;
+#pragma unroll
+                for (int m = 0; m < 4; m++) acc[g][m] *= alpha;
+                ref[g] = nref;
+            }
+            const float off = 12.0f - ref[g];
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                u32x4 hw, lw;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const float p0 = exp2_hw(fmaf(sc[g][8 * s + 2 * t], to_log2[g], off));
+                    const float p1 = exp2_hw(fmaf(sc[g][8 * s + 2 * t + 1], to_log2[g], off));
+                    l[g] += p0 + p1;
+                    uint32_t hi, lo;
+                    split2(p0, p1, hi, lo);
+                    hw[t] = hi;
+                    lw[t] = lo;
+                }
+                ph[g][s] = __builtin_bit_cast(halfx8, hw);
+                pl[g][s] = __builtin_bit_cast(halfx8, lw);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int m = 0; m < 4; m++) {
                 const uint32_t word = cur.vf[m];
@@ -1745,10 +1766,11 @@ __global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlo
                 const _Float16 fs = f[0], fz = f[1];
                 const halfx8 v = values4(cur.v[s][m], halfx8{fs, fs, fs, fs, fs, fs, fs, fs},
                                          halfx8{fz, fz, fz, fz, fz, fz, fz, fz});
-                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, acc[m], 0, 0, 0);
-                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc[m], 0, 0, 0);
+#pragma unroll
+                for (int g = 0; g < G; g++) acc[g][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[g][s], acc[g][m], 0, 0, 0);
+#pragma unroll
+                for (int g = 0; g < G; g++) acc[g][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[g][s], acc[g][m], 0, 0, 0);
             }
-        }
     };
     // two blocks a round, so that the registers' roles are fixed
     while (kb < kb1) {
@@ -1767,32 +1789,35 @@ __global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlo
         }
     }
     // the wavefronts' (maximum, sum, weighted sums), merged as the split merge merges key ranges
-    const float lw = sum32(sum16(l));
-    if (lg == 0) {
-        mref[wave][qi] = ref;
-        msum[wave][qi] = lw;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const float lw = sum32(sum16(l[g]));
+        if (lg == 0) {
+            mref[wave][16 * g + qi] = ref[g];
+            msum[wave][16 * g + qi] = lw;
+        }
+#pragma unroll
+        for (int m = 0; m < 4; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) macc[wave][16 * m + 4 * lg + i][16 * g + qi] = acc[g][m][i];
     }
-#pragma unroll
-    for (int m = 0; m < 4; m++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) macc[wave][16 * m + 4 * lg + i][qi] = acc[m][i];
     __syncthreads();
     // thread t: query t / 16, coordinates 4 (t % 16) .. + 3
-    const int oq = tid >> 4, oc = 4 * (tid & 15);
-    if (oq >= min(nq, 16)) return;
+    const int lq = tid >> 4, oc = 4 * (tid & 15), oq = q0 + lq;
+    if (lq >= NQ || oq >= nq) return;
     const float unscale = ldexpf(1.0f, -shift_for(kvmax[h * 2 + 1]));
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < W; w++)
-        if (msum[w][oq] > 0.0f) m = fmaxf(m, mref[w][oq]);
+        if (msum[w][lq] > 0.0f) m = fmaxf(m, mref[w][lq]);
     float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < W; w++) {
-        const float ls = msum[w][oq];
-        const float f = ls > 0.0f ? exp2_hw(mref[w][oq] - m) : 0.0f;
+        const float ls = msum[w][lq];
+        const float f = ls > 0.0f ? exp2_hw(mref[w][lq] - m) : 0.0f;
         L += ls * f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) o[j] += macc[w][oc + j][oq] * f;
+        for (int j = 0; j < 4; j++) o[j] += macc[w][oc + j][lq] * f;
     }
     if (splits == 1) {
         const float fo = unscale / L;
@@ -2038,13 +2063,13 @@ static AttnPlan plan(const AttnShape &a, bool images) {
     const KeyBlocks k = key_blocks(a.rows, a.chunk);
     const int hd = a.d / a.heads;
     const bool tiles = hd == 64 && images && kv_images_apply(a.kv_format, a.d, a.heads);
-    p.few = tiles && a.nq <= FEW_Q && (a.kv_format != TAH_KV_I16 || a.nq >= FEW16_FROM);
+    p.few = tiles && a.nq <= (a.kv_format == TAH_KV_I4 ? FEW4_Q : FEW_Q) && (a.kv_format != TAH_KV_I16 || a.nq >= FEW16_FROM);
     p.split16 = tiles && (p.few || a.nq >= split16_min_q(a.kv_format));
     if (p.few && a.kv_format == TAH_KV_I4) {
         // a wavefront a block, up to two workgroups a compute unit; more blocks then in as many ranges
-        p.waves = 4;
-        p.groups = 1;
-        const int most = std::max(1, 256 / a.heads);
+        p.waves = a.nq <= 16 ? 1 : 2;  // groups of 16 queries a workgroup
+        p.groups = (a.nq + 16 * p.waves - 1) / (16 * p.waves);
+        const int most = std::max(1, 256 / (a.heads * p.groups));
         const int want = k.n_kb <= 2 * FEW4_WAVES ? 1 : std::min((k.n_kb + FEW4_WAVES - 1) / FEW4_WAVES, most);
         p.kb_per_split = (k.n_kb + want - 1) / want;
         p.splits = (k.n_kb + p.kb_per_split - 1) / p.kb_per_split;
@@ -2213,10 +2238,13 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
     }
     if (p.few) {
         const dim3 grid(a.heads * p.splits);
-        if (a.kv_format == TAH_KV_I4)
-            hipLaunchKernelGGL(k_attn_few4, dim3(a.heads, p.splits), dim3(64 * FEW4_WAVES), 0, s, a.nq,
-                               key_blocks(a.rows, a.chunk), a.chunk, q, img->images, img->kvmax, p.kb_per_split, part_o,
-                               part_ml, out);
+        const dim3 grid4(a.heads, p.splits, p.groups);
+        if (a.kv_format == TAH_KV_I4 && p.waves == 1)
+            hipLaunchKernelGGL(k_attn_few4<1>, grid4, dim3(64 * FEW4_WAVES), 0, s, a.nq, key_blocks(a.rows, a.chunk),
+                               a.chunk, q, img->images, img->kvmax, p.kb_per_split, part_o, part_ml, out);
+        else if (a.kv_format == TAH_KV_I4)
+            hipLaunchKernelGGL(k_attn_few4<2>, grid4, dim3(64 * FEW4_WAVES), 0, s, a.nq, key_blocks(a.rows, a.chunk),
+                               a.chunk, q, img->images, img->kvmax, p.kb_per_split, part_o, part_ml, out);
         else if (a.kv_format == TAH_KV_I16)
             hipLaunchKernelGGL((k_attn_few<FEW_Q / 16, TAH_KV_I16>), grid, dim3(256), 0, s, a.nq, a.rows, a.chunk, a.d,
                                a.heads, q, img->images, img->kvmax, img->scales, p.kb_per_split, p.splits, part_o,
@@ -2264,7 +2292,7 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
         default: throw ArgError{"attention: unknown key/value format"};
     }
     if (p.splits > 1) {
-        if (p.few && a.kv_format == TAH_KV_I4 && p.splits <= MERGE_FEW)
+        if (p.few && a.kv_format == TAH_KV_I4 && p.splits <= MERGE_FEW && (p.splits > MERGE64_MAX || a.nq <= 16))
             hipLaunchKernelGGL(k_attn_merge_few, dim3(a.nq * a.heads), dim3(256), 0, s, a.nq * a.heads, p.splits, part_o,
                                part_ml, out);
         else if (a.d == 64 * a.heads && p.splits <= MERGE64_MAX)  // many queries, few splits (else lanes over splits win)
