@@ -1625,7 +1625,6 @@ __global__ __launch_bounds__(256, 1) void k_attn_few(int nq, int rows, int chunk
 // until the four softmax states are merged. The products are 16 x 16 x 32 with the queries as columns: S = K Q^T by 16
 // (two for each of four sets of 16 keys and two halves of the coordinates), O^T += V^T P^T by 16. The order of the keys
 // within a tile leaves a lane's eight scores of each 32 keys as the operand that the values' product takes.
-constexpr int FEW4_Q = 512;
 constexpr int FEW4_WAVES = 8;
 template <int G>
 __global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlocks kbs, int chunk, const float *__restrict__ q,
@@ -2058,23 +2057,61 @@ KvImages kv_images_at(uint8_t *base, int rows, int chunk, int heads, int kv_form
     return img;
 }
 
+// 4-bit tiles: which kernel, and into how many ranges the keys go. Both run in rounds of one workgroup a compute unit; a
+// range count is worth looking at where it fills a whole number of rounds. A round of k_attn_few4 takes 2.6 us a block of
+// its eight wavefronts' turns and one and a half more, the merge of ranges as much again; one of k_attn_split64 2 us a
+// block and eight and a half more (queries x rows, 8 heads, measured by the one and the other: 512 x 10,000 33 and 42 us, 600 x 2,000
+// 15 and 21, 1,024 x 10,000 55 and 56, 1,536 x 10,000 106 and 77, 2,048 x 2,000 30 and 34, 2,048 x 10,000 107 and 95).
+static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
+    auto ranges = [&](int per, int least_blocks, auto cost_of, float &cost) {
+        int best = 1;
+        cost = cost_of((per + 255) / 256, k.n_kb, false);
+        for (int rounds = 1; rounds <= 8; rounds++) {
+            const int s = std::min(256 * rounds / per, (k.n_kb + least_blocks - 1) / least_blocks);
+            if (s < 2) continue;
+            const float c = cost_of((per * s + 255) / 256, (k.n_kb + s - 1) / s, true);
+            if (c < cost) {
+                cost = c;
+                best = s;
+            }
+        }
+        return best;
+    };
+    AttnPlan p{};
+    p.few = true;
+    p.waves = a.nq <= 16 ? 1 : 2;  // groups of 16 queries a workgroup
+    p.groups = (a.nq + 16 * p.waves - 1) / (16 * p.waves);
+    float few_cost, many_cost;
+    // one range while a wavefront has no more than two blocks: a second one's merge takes longer
+    int splits = ranges(a.heads * p.groups, FEW4_WAVES,
+                        [](int rounds, int blocks, bool merge) {
+                            return 2.6f * (rounds * ((blocks + FEW4_WAVES - 1) / FEW4_WAVES + 1.5f) + (merge ? 1.5f : 0.0f));
+                        },
+                        few_cost);
+    if (a.nq > 128) {
+        const int tiles = (a.nq + 255) / 256;
+        const int s = ranges(a.heads * tiles, 2, [](int rounds, int blocks, bool) { return 2.0f * rounds * (blocks + 8.5f); }, many_cost);
+        if (many_cost < few_cost) {
+            p.few = false;
+            p.split16 = true;
+            p.waves = 8;
+            p.groups = tiles;
+            splits = s;
+        }
+    }
+    p.kb_per_split = (k.n_kb + splits - 1) / splits;
+    p.splits = (k.n_kb + p.kb_per_split - 1) / p.kb_per_split;
+    return p;
+}
+
 static AttnPlan plan(const AttnShape &a, bool images) {
     AttnPlan p;
     const KeyBlocks k = key_blocks(a.rows, a.chunk);
     const int hd = a.d / a.heads;
     const bool tiles = hd == 64 && images && kv_images_apply(a.kv_format, a.d, a.heads);
-    p.few = tiles && a.nq <= (a.kv_format == TAH_KV_I4 ? FEW4_Q : FEW_Q) && (a.kv_format != TAH_KV_I16 || a.nq >= FEW16_FROM);
+    if (tiles && a.kv_format == TAH_KV_I4) return plan4(a, k);
+    p.few = tiles && a.nq <= FEW_Q && (a.kv_format != TAH_KV_I16 || a.nq >= FEW16_FROM);
     p.split16 = tiles && (p.few || a.nq >= split16_min_q(a.kv_format));
-    if (p.few && a.kv_format == TAH_KV_I4) {
-        // a wavefront a block, up to two workgroups a compute unit; more blocks then in as many ranges
-        p.waves = a.nq <= 16 ? 1 : 2;  // groups of 16 queries a workgroup
-        p.groups = (a.nq + 16 * p.waves - 1) / (16 * p.waves);
-        const int most = std::max(1, 256 / (a.heads * p.groups));
-        const int want = k.n_kb <= 2 * FEW4_WAVES ? 1 : std::min((k.n_kb + FEW4_WAVES - 1) / FEW4_WAVES, most);
-        p.kb_per_split = (k.n_kb + want - 1) / want;
-        p.splits = (k.n_kb + p.kb_per_split - 1) / p.kb_per_split;
-        return p;
-    }
     // k_attn_split64: 256 queries a workgroup (one a compute unit, one wave of them) from 768 queries on, else 128
     // (at 512 / 640 rows f32 1.376 / 1.740 -> 1.368 / 1.717 ms and i8 1.337 / 1.705 -> 1.330 / 1.676 ms with the
     // smaller tiles than from 512; from 1,024 or 1,536 queries f32 was slower at 768 to 1,280); an i16 layer's (whose
@@ -2271,8 +2308,7 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
                 else launch_split<4, TAH_KV_I16>(s, a, p, q, *img, out, part_o, part_ml);
                 break;
             case TAH_KV_I4:
-                if (p.waves == 8) launch_split<8, TAH_KV_I4>(s, a, p, q, *img, out, part_o, part_ml);
-                else launch_split<4, TAH_KV_I4>(s, a, p, q, *img, out, part_o, part_ml);
+                launch_split<8, TAH_KV_I4>(s, a, p, q, *img, out, part_o, part_ml);
                 break;
             default:
                 if (p.waves == 8) launch_split<8, TAH_KV_I8>(s, a, p, q, *img, out, part_o, part_ml);
