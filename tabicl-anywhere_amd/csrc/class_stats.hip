@@ -10,11 +10,14 @@
 // Classes in order: larger scores first, the lower id among equals (-0 and 0 are equal), NaN after every number.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 #include "device_math.hpp"
 
 namespace tah {
+
+constexpr float LN2 = 0.69314718055994530942f;
 
 struct ClassDist {
     float m, s, t;
@@ -75,64 +78,71 @@ struct ClassLogs {
     __device__ __forceinline__ float log_p(float x, float inv) const { return (x - from) * inv - logs; }
 };
 
-// ---- up to 64 classes: a lane a row -----------------------------------------------------------------------------------
-// grid ceil(rows / 64); 64 threads. The scores of 64 rows come in whole lines and are turned in LDS (an odd pitch: the
-// lanes' reads meet no bank twice; -inf past n), each lane then keeps its row's N >= n scores in registers, so
-// that nothing is exchanged between lanes: a row of ten classes takes a lane about 150 instructions, where a wavefront or a
-// workgroup a row spent most of its own on reductions (200,000 rows of seven: 664 us a workgroup a row). The most probable
-// classes by one scan of the keys each.
-template <int N>
+// ---- up to 64 classes: one to eight lanes a row --------------------------------------------------------------------------
+// v combined over the L lanes of a row (neighbours, L a power of two up to 8).
+template <int L, class T, class F>
+__device__ __forceinline__ T row_lanes(T v, F &&f) {
+    static_assert(sizeof(T) == 4, "one register");
+    auto there = [](T x, auto ctrl) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    if (L > 1) v = f(v, there(v, std::integral_constant<int, 0xb1>()));   // lanes 1 apart
+    if (L > 2) v = f(v, there(v, std::integral_constant<int, 0x4e>()));   // 2 apart
+    if (L > 4) v = f(v, there(v, std::integral_constant<int, 0x141>()));  // mirrored in eights: of the other four
+    return v;
+}
+
+// grid ceil(rows / (64 / L)); 64 threads. Each of a row's L lanes keeps N / L of its N >= n scores in registers, read where
+// they lie: a wavefront's loads meet the same few lines again and again, in L1 (turned in LDS first, whole lines at a time:
+// 200,000 x 7 6.9 us for 5.8, 100,000 x 20 10.9 for 8.9). A row of ten classes takes two lanes about 150 instructions, where
+// a wavefront or a workgroup a row spent most of its own on reductions (200,000 x 7: 664 us a workgroup a row). The most
+// probable classes by one scan of the keys each. Instructions bound it: 100,000 x 50 with five best 14.6 us, 1.4 TB/s.
+template <int N, int L>
 __global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t ld, const float *__restrict__ x, float inv,
                                                          ClassOut o) {
-    constexpr int PITCH = N + 1;
-    __shared__ float turned[64 * PITCH];
-    const int lane = threadIdx.x, row0 = blockIdx.x * 64, here = min(64, rows - row0);
-    const float *src = x + (size_t)row0 * ld;
-    if (n < N) {
-#pragma unroll
-        for (int i = 0; i < N; i++) turned[lane * PITCH + i] = -INFINITY;
-        __syncthreads();
-    }
-    // entry e of the 64 rows' here * n: row r, class i, 64 entries on at each turn
-    const int rows_on = 64 / n, on = 64 - rows_on * n;
-    int r = lane / n, i = lane - r * n;
-    for (int e = lane; e < here * n; e += 64) {
-        turned[r * PITCH + i] = src[r * ld + i];
-        r += rows_on;
-        i += on;
-        if (i >= n) {
-            i -= n;
-            r++;
-        }
-    }
-    __syncthreads();
-    if (lane >= here) return;
-    const float *mine = turned + lane * PITCH;
-    uint32_t k[N];
+    constexpr int R = 64 / L, E = N / L;
+    const int part = threadIdx.x % L;
+    const size_t row = (size_t)blockIdx.x * R + threadIdx.x / L;
+    if (row >= (size_t)rows) return;
+    const float *mine = x + row * ld;
+    // entry i of a lane: class L i + part
+    float v[E];
+    uint32_t k[E];
     ClassDist c{-INFINITY, 0.0f, 0.0f, false};
-    int at = 0;
+    int bad = 0;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const float v = mine[i];
-        k[i] = i < n ? score_key(v) : 0u;
-        c.bad = c.bad || v != v;
-        if (v > c.m) {
-            c.m = v;
-            at = i;
-        }
+    for (int i = 0; i < E; i++) {
+        const int at = L * i + part;
+        v[i] = -INFINITY;
+        if (L * (i + 1) <= n || at < n) v[i] = mine[at];  // the first is the same for all lanes
     }
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        // the maximum's own term left out; a score of -inf weighs nothing (0 times infinity would be NaN)
-        const float u = (mine[i] - c.m) * inv, e = i == at ? 0.0f : exp_below(u);
-        c.s += e;
-        c.t -= e > 0.0f ? e * u : 0.0f;
+    for (int i = 0; i < E; i++) {
+        k[i] = L * i + part < n ? score_key(v[i]) : 0u;
+        bad |= v[i] != v[i];
+        c.m = fmaxf(c.m, v[i]);
     }
-    const size_t row = (size_t)row0 + lane;
+    c.m = row_lanes<L>(c.m, [](float a, float b) { return fmaxf(a, b); });
+    c.bad = row_lanes<L>(bad, [](int a, int b) { return a | b; }) != 0;
+    // in units of log 2; the largest scores' terms are exactly 1 and are counted apart. From 2^-200 down a term is 0
+    const float inv2 = inv * LOG2E;
+    int tops = 0;
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        const float u = fmaxf((v[i] - c.m) * inv2, -200.0f);
+        const bool is_top = v[i] == c.m;
+        const float w = is_top ? 0.0f : exp2_hw(u);
+        tops += is_top;
+        c.s += w;
+        c.t = fmaf(-w, u, c.t);
+    }
+    const auto add = [](auto a, auto b) { return a + b; };
+    c.s = row_lanes<L>(c.s, add) + (float)(row_lanes<L>(tops, add) - 1);
+    c.t = row_lanes<L>(c.t, add) * LN2;
     float *st = o.stats + row * (1 + o.n_given + o.top);
     const ClassLogs says(c);
-    st[0] = says.entropy;
-    for (int i = 0; i < o.n_given; i++) {
+    if (part == 0) st[0] = says.entropy;
+    for (int i = part; i < o.n_given; i += L) {
         const int id = o.given[row * o.n_given + i];
         st[1 + i] = id >= 0 && id < n ? says.log_p(mine[id], inv) : NAN;
     }
@@ -140,15 +150,19 @@ __global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t
         uint32_t best = 0;
         int id = 0;
 #pragma unroll
-        for (int i = 0; i < N; i++) {
+        for (int i = 0; i < E; i++) {
             const bool more = k[i] > best;
             best = more ? k[i] : best;
-            id = more ? i : id;
+            id = more ? L * i + part : id;
         }
+        const uint32_t most = row_lanes<L>(best, [](uint32_t a, uint32_t b) { return max(a, b); });
+        id = row_lanes<L>(best == most ? id : N, [](int a, int b) { return min(a, b); });
 #pragma unroll
-        for (int i = 0; i < N; i++) k[i] = i == id ? 0u : k[i];
-        st[1 + o.n_given + r] = says.log_p(score_of(best), inv);
-        o.ids[row * o.top + r] = id;
+        for (int i = 0; i < E; i++) k[i] = L * i + part == id ? 0u : k[i];
+        if (r % L == part) {
+            st[1 + o.n_given + r] = says.log_p(score_of(most), inv);
+            o.ids[row * o.top + r] = id;
+        }
     }
 }
 
@@ -198,7 +212,7 @@ __device__ __forceinline__ ClassDist wave_dist(const float (&v)[E], float inv) {
         t = fmaf(-w, u, t);
     }
     c.s = wave_sum(s) + (float)(tops - 1);
-    c.t = wave_sum(t) * 0.69314718055994530942f;
+    c.t = wave_sum(t) * LN2;
     return c;
 }
 
@@ -553,10 +567,14 @@ size_t class_stats_work_bytes(int rows, int n, int top) {
     return c.segs == 1 ? 0 : (size_t)std::min(rows, c.rows) * c.segs * seg_bytes(top);
 }
 
-template <int N>
+template <int N, int L>
 static void launch_rows(hipStream_t s, int rows, int n, size_t ld, const float *x, float inv, const ClassOut &o) {
-    hipLaunchKernelGGL(k_class_stats_rows<N>, dim3((rows - 1) / 64 + 1), dim3(64), 0, s, rows, n, ld, x, inv,
-                       o);
+    constexpr int R = 64 / L, MOST = 1 << 26;  // rows a launch: a grid holds fewer than 2^32 threads
+    for (int r0 = 0; r0 < rows; r0 += std::min(MOST, rows - r0)) {
+        const int here = std::min(MOST, rows - r0);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_class_stats_rows<N, L>), dim3((here + R - 1) / R), dim3(64), 0, s, here, n, ld,
+                           x + r0 * ld, inv, o.from(r0));
+    }
 }
 template <int E>
 static void launch_wave(hipStream_t s, int rows, int n, size_t ld, const float *x, float inv, const ClassOut &o) {
@@ -574,11 +592,12 @@ void class_stats(hipStream_t s, int rows, int n, size_t ld, const float *x, floa
     if (rows <= 0) return;
     const float inv = 1.0f / temperature;
     ClassOut o{given, n_given, top, stats, ids};
-    // the fewest entries a lane that hold a row
-    if (n <= 8) launch_rows<8>(s, rows, n, ld, x, inv, o);
-    else if (n <= 16) launch_rows<16>(s, rows, n, ld, x, inv, o);
-    else if (n <= 32) launch_rows<32>(s, rows, n, ld, x, inv, o);
-    else if (n <= 64) launch_rows<64>(s, rows, n, ld, x, inv, o);
+    // eight scores a lane (sixteen: 1,000 x 50 4.0 -> 5.1 us, 100,000 x 50 14.6 -> 15.0; four: 200,000 x 7 5.8 -> 6.7, 100,000 x
+    // 20 8.9 -> 11.3), past 64 classes the fewest entries a lane that hold a row
+    if (n <= 8) launch_rows<8, 1>(s, rows, n, ld, x, inv, o);
+    else if (n <= 16) launch_rows<16, 2>(s, rows, n, ld, x, inv, o);
+    else if (n <= 32) launch_rows<32, 4>(s, rows, n, ld, x, inv, o);
+    else if (n <= 64) launch_rows<64, 8>(s, rows, n, ld, x, inv, o);
     else if (n <= 128) launch_wave<2>(s, rows, n, ld, x, inv, o);
     else if (n <= 256) launch_wave<4>(s, rows, n, ld, x, inv, o);
     else if (n <= 512) launch_wave<8>(s, rows, n, ld, x, inv, o);
