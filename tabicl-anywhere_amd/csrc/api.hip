@@ -857,6 +857,8 @@ static void check_layer(const char *what, int d, int rows, int chunk, int kv_for
     // the kernels number a chunk's fours of rows, and i16 and i8 packing its coordinates in a grid's second dimension
     if ((std::min(chunk, std::max(rows, 1)) + 3L) / 4 * 2 * d > 0x7FFFFFFF - 1024 || d > 131070)
         throw ArgError{std::string(what) + ": a chunk of more numbers than a call takes"};
+    // a grid holds fewer than 2^32 threads, and i16 and i8 packing has 256 of them a chunk
+    if (rows > 0 && (rows - 1) / chunk >= (1 << 24) - 1) throw ArgError{std::string(what) + ": at most 2^24 - 1 chunks"};
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) % 4)
         throw ArgError{std::string(what) + ": the pointers have to be 4-byte aligned"};
 }
@@ -978,6 +980,10 @@ extern "C" int tah_class_stats_dev(tah_dev *dev, const float *scores_dev, int32_
     return guarded(dev, [&] {
         if (ld == 0) ld = n;
         check_classes(rows, n, ld, temperature, given_dev, n_given, top, ids_dev);
+        if ((reinterpret_cast<uintptr_t>(scores_dev) | reinterpret_cast<uintptr_t>(given_dev) |
+             reinterpret_cast<uintptr_t>(stats_dev) | reinterpret_cast<uintptr_t>(ids_dev)) % 4)
+            throw ArgError{"class_stats: the pointers have to be 4-byte aligned"};
+        if (rows == 0) return TAH_OK;
         Loans loans(dev);
         const size_t work = class_stats_work_bytes(rows, n, top);
         class_stats(dev->stream, rows, n, (size_t)ld, scores_dev, temperature, given_dev, n_given, top, stats_dev, ids_dev,

@@ -78,8 +78,8 @@ struct ClassLogs {
     __device__ __forceinline__ float log_p(float x, float inv) const { return (x - from) * inv - logs; }
 };
 
-// ---- up to 64 classes: one to eight lanes a row --------------------------------------------------------------------------
-// v combined over the L lanes of a row (neighbours, L a power of two up to 8).
+// ---- up to 256 classes: one to 32 lanes a row ----------------------------------------------------------------------------
+// v combined over the L lanes of a row (neighbours, L a power of two up to 32).
 template <int L, class T, class F>
 __device__ __forceinline__ T row_lanes(T v, F &&f) {
     static_assert(sizeof(T) == 4, "one register");
@@ -89,6 +89,13 @@ __device__ __forceinline__ T row_lanes(T v, F &&f) {
     if (L > 1) v = f(v, there(v, std::integral_constant<int, 0xb1>()));   // lanes 1 apart
     if (L > 2) v = f(v, there(v, std::integral_constant<int, 0x4e>()));   // 2 apart
     if (L > 4) v = f(v, there(v, std::integral_constant<int, 0x141>()));  // mirrored in eights: of the other four
+    if (L > 8) v = f(v, there(v, std::integral_constant<int, 0x140>()));  // mirrored in sixteens: of the other eight
+    if (L > 16) {
+        const auto both = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v),
+                                                           false, false);
+        const unsigned a = both[0], b = both[1];  // a bit cast of a vector's element takes its first
+        v = f(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+    }
     return v;
 }
 
@@ -259,10 +266,10 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t key, uint32_t other, uint3
     return lo;
 }
 
-// The same sooner. A bound that top lanes' own largest scores reach, and few more, (bound_of): top scores reach it, so nothing below it is among the top. What reaches it goes into a list in LDS, whose entries
-// are placed by counting the larger ones. Where that does not serve (too many equal scores, or rising ones in few lanes; a
-// bound of -inf; NaN among the top) the keys are taken one by one (3,000 x 1,001 with ten: 15.2 us,
-// 8.2 by the bound).
+// The same sooner. A bound that top lanes' own largest scores reach, and few more (bound_of): top scores reach it, so nothing
+// below it is among the top. What reaches it goes into a list in LDS, whose entries are placed by counting the larger ones.
+// Where that does not serve (too many equal scores, or rising ones in few lanes; a bound of -inf; NaN among the top) the keys
+// are taken one by one (3,000 x 1,001 with ten best: 15.2 us for all rows so, 7.9 by the bound).
 constexpr int LIST = 256;
 template <int E, class Id>
 __device__ __forceinline__ uint64_t wave_top(const float (&v)[E], const ClassDist &c, int live, int top, int lane,
@@ -312,7 +319,7 @@ __device__ __forceinline__ uint64_t wave_top(const float (&v)[E], const ClassDis
     return wave_top_each(v, live, top, lane, id);
 }
 
-// ---- up to 1,024 classes: a wavefront a row ------------------------------------------------------------------------------
+// ---- up to 1,024 classes, many of them wanted: a wavefront a row ------------------------------------------------------------------------------
 // grid ceil(rows / 4); 256 threads. Entry r of a lane is class 64 r + lane: the row is read once, in whole lines, and kept.
 template <int E>
 __global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_t ld, const float *__restrict__ x, float inv,
@@ -347,7 +354,7 @@ __global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_
 struct SegState {
     ClassDist c;
 };
-constexpr int SEG_T = 512, SEG = 32 * SEG_T, SEG_E = SEG / SEG_T, SEG_LIST = 1024;
+constexpr int SEG_T = 512, SEG = 32 * SEG_T, SEG_LIST = 1024;
 
 __host__ __device__ inline size_t seg_bytes(int top) { return sizeof(SegState) + 8 * (size_t)top; }
 
@@ -376,11 +383,12 @@ __device__ __forceinline__ int place_of(uint64_t key, const uint64_t *keys, int 
     return place;
 }
 
-// grid (segments, rows); 512 threads: each keeps up to 32 scores of its segment (len, a multiple of 4) in registers, so that the row is read once. The
-// wavefronts' distributions are joined in LDS, the segments of a row by k_class_stats_join (a row of one segment is written
-// here). The most probable classes as wave_top has them, but of the workgroup: the bound from the largest scores of its 128
-// groups of four lanes, one list. Loads and arithmetic hardly overlap, since all workgroups start together: 64 x 100,000
-// is 25.6 MB.
+// grid (segments, rows); 512 threads: each keeps up to E scores of its segment (len, a multiple of 4) in registers, so that
+// the row is read once. The wavefronts' distributions are joined in LDS, the segments of a row by k_class_stats_join (a row of
+// one segment is written here). The most probable classes as wave_top has them, but of the workgroup: the bound from the
+// largest scores of its 128 groups of four lanes, one list (a list a wavefront, then joined: 64 x 100,000 with 20 best
+// 22 us for 18). Loads and arithmetic hardly overlap, since all workgroups start together.
+template <int E>
 __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_t ld, const float *__restrict__ x,
                                                            float inv, uint8_t *__restrict__ state, ClassOut o) {
     constexpr int W = SEG_T / 64;
@@ -393,12 +401,12 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
     const float *src = x + row * ld;
     const int base = seg * len, end = min(n, base + len);
     if (tid == 0) listed = 0;
-    float v[SEG_E];
+    float v[E];
     // entry 4 r + j of a thread: class base + 4 (512 r + tid) + j
     auto id = [&](int e) { return base + 4 * (SEG_T * (e >> 2) + tid) + (e & 3); };
     const bool fours = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
 #pragma unroll
-    for (int r = 0; r < SEG_E / 4; r++) {
+    for (int r = 0; r < E / 4; r++) {
         const int i = id(4 * r);
         if (fours && i + 4 <= end) {
             const float4 x4 = *reinterpret_cast<const float4 *>(src + i);
@@ -414,7 +422,7 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
     if (o.top > 0) {
         float own = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < SEG_E; r++) own = fmaxf(own, v[r]);
+        for (int r = 0; r < E; r++) own = fmaxf(own, v[r]);
         own = fmaxf(own, dpp<0xb1>(own));   // lanes 1 apart
         own = fmaxf(own, dpp<0x4e>(own));   // 2 apart
         if ((lane & 3) == 0) group[tid >> 2] = own;
@@ -444,7 +452,7 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
     if (bounded) {
         const float bound = score_of(lo);
 #pragma unroll
-        for (int r = 0; r < SEG_E; r++) {
+        for (int r = 0; r < E; r++) {
             const bool in = v[r] >= bound;
             const uint64_t who = __ballot(in);
             if (who) {
@@ -540,22 +548,17 @@ __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, cons
     }
 }
 
-// Rows of more than 1,024 classes: how they are cut. At least as many segments as registers hold, and so many more that the
-// workgroups fill whole rounds of the 256 compute units (64 x 100,000: 8 segments, two workgroups each, where 7 left some
-// with one; 18.0 -> 17.0 us), while a segment keeps 2,048 classes. Rows at a time whose segments' states fit 32 MB (and a
-// launch's grid).
+// Rows of more than 1,024 classes: how they are cut. As few segments as registers hold them in: more of them, to fill whole
+// rounds of the compute units, gave the join more to do than they saved (1 x 100,000 with 20 best in 7 and in 48 segments 14.0
+// and 14.8 us, 64 x 16,384 in 1 and in 4 8.9 and 14.9, 64 x 100,000 in 7 and in 8 alike). Rows at a time whose segments'
+// states fit 32 MB (and a launch's grid).
 struct ClassCut {
     int segs, len, rows;
 };
-static ClassCut cut(int rows, int n, int top) {
-    const int least = (n + SEG - 1) / SEG;
-    long segs = least;
-    if (least > 1 || rows < 256) {
-        const long round = ((long)rows * least + 255) / 256 * 256;
-        segs = std::max<long>(least, std::min<long>({round / rows, n / 2048, 64}));
-    }
+static ClassCut cut(int n, int top) {
     ClassCut c;
-    c.len = (int)(((n + segs - 1) / segs + 3) / 4 * 4);
+    c.segs = (n + SEG - 1) / SEG;
+    c.len = ((n + c.segs - 1) / c.segs + 3) / 4 * 4;
     c.segs = (n + c.len - 1) / c.len;
     c.rows = (int)std::max<size_t>(1, std::min<size_t>(65535, (size_t(32) << 20) / (c.segs * seg_bytes(top))));
     return c;
@@ -563,7 +566,7 @@ static ClassCut cut(int rows, int n, int top) {
 
 size_t class_stats_work_bytes(int rows, int n, int top) {
     if (n <= 1024) return 0;
-    const ClassCut c = cut(rows, n, top);
+    const ClassCut c = cut(n, top);
     return c.segs == 1 ? 0 : (size_t)std::min(rows, c.rows) * c.segs * seg_bytes(top);
 }
 
@@ -586,31 +589,44 @@ static void launch_wave(hipStream_t s, int rows, int n, size_t ld, const float *
     }
 }
 
+// the fewest scores a thread that hold a segment (1,000 x 2,000 by 32 a thread 17.8 us, by 8 10.8;
+// 1,000 x 5,000 by 32 18.7, by 16 14.1)
+static void launch_seg(hipStream_t s, int segs, int rows, int n, int len, size_t ld, const float *x, float inv, uint8_t *state,
+                       const ClassOut &o) {
+    const dim3 grid(segs, rows), block(SEG_T);
+    if (len <= 8 * SEG_T) hipLaunchKernelGGL(k_class_stats_seg<8>, grid, block, 0, s, n, len, ld, x, inv, state, o);
+    else if (len <= 16 * SEG_T) hipLaunchKernelGGL(k_class_stats_seg<16>, grid, block, 0, s, n, len, ld, x, inv, state, o);
+    else hipLaunchKernelGGL(k_class_stats_seg<32>, grid, block, 0, s, n, len, ld, x, inv, state, o);
+}
+
 // work: class_stats_work_bytes(rows, n, top) bytes.
 void class_stats(hipStream_t s, int rows, int n, size_t ld, const float *x, float temperature, const int32_t *given,
                  int n_given, int top, float *stats, int32_t *ids, void *work) {
     if (rows <= 0) return;
     const float inv = 1.0f / temperature;
     ClassOut o{given, n_given, top, stats, ids};
-    // eight scores a lane (sixteen: 1,000 x 50 4.0 -> 5.1 us, 100,000 x 50 14.6 -> 15.0; four: 200,000 x 7 5.8 -> 6.7, 100,000 x
-    // 20 8.9 -> 11.3), past 64 classes the fewest entries a lane that hold a row
+    // Eight scores a lane (sixteen: 1,000 x 50 4.0 -> 5.1 us, 100,000 x 50 14.6 -> 15.0; four: 200,000 x 7 5.8 -> 6.7, 100,000 x
+    // 20 8.9 -> 11.3), up to 256 classes while few of them are wanted one by one (20,000 x 100, a wavefront a row against this:
+    // five best 15.5 -> 7.7 us, 20 best 16.9 and 16.1; 20,000 x 200: 17.2 -> 12.9, 18.7 and 29.2; 200 x 100, 20 best 4.7 and
+    // 7.2). Else a wavefront a row, the fewest entries a lane that hold it.
     if (n <= 8) launch_rows<8, 1>(s, rows, n, ld, x, inv, o);
     else if (n <= 16) launch_rows<16, 2>(s, rows, n, ld, x, inv, o);
     else if (n <= 32) launch_rows<32, 4>(s, rows, n, ld, x, inv, o);
     else if (n <= 64) launch_rows<64, 8>(s, rows, n, ld, x, inv, o);
+    else if (n <= 128 && top <= 8) launch_rows<128, 16>(s, rows, n, ld, x, inv, o);
+    else if (n <= 256 && top <= 8) launch_rows<256, 32>(s, rows, n, ld, x, inv, o);
     else if (n <= 128) launch_wave<2>(s, rows, n, ld, x, inv, o);
     else if (n <= 256) launch_wave<4>(s, rows, n, ld, x, inv, o);
     else if (n <= 512) launch_wave<8>(s, rows, n, ld, x, inv, o);
     else if (n <= 1024) launch_wave<16>(s, rows, n, ld, x, inv, o);
     else {
-        const ClassCut c = cut(rows, n, top);
+        const ClassCut c = cut(n, top);
         const int segs = c.segs;
         for (int r0 = 0; r0 < rows; r0 += c.rows) {
             const int here = std::min(c.rows, rows - r0);
             const float *xr = x + r0 * ld;
             const ClassOut at = o.from(r0);
-            hipLaunchKernelGGL(k_class_stats_seg, dim3(segs, here), dim3(SEG_T), 0, s, n, c.len, ld, xr, inv,
-                               static_cast<uint8_t *>(work), at);
+            launch_seg(s, segs, here, n, c.len, ld, xr, inv, static_cast<uint8_t *>(work), at);
             if (segs > 1)
                 hipLaunchKernelGGL(k_class_stats_join, dim3(here), dim3(512), (size_t)segs * top * 8, s, n, ld, xr, inv, segs,
                                    static_cast<const uint8_t *>(work), at);

@@ -9,8 +9,8 @@
 //   or 127, inv = 1 / s, code = round-half-away(v * inv) saturated to the integer range; the 2d scales first.
 //   One wavefront per coordinate row. Division is the correctly rounded one (__fdiv_rn), so the same f32 input
 //   gives the same scales and codes as the CPU.
-// * k_pack4: f32 records to i4 records.
-// * k_unpack: records of any format to f32 records.
+// * k_pack4: f32 records to i4 records (kv4.hpp).
+// * k_unpack: records of i16, i8 or i4 to f32 records.
 #include <algorithm>
 
 #include "common.hpp"
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void k_pack(int rows, int d, int chunk, const 
                                                uint8_t *__restrict__ recq) {
     const int ci = blockIdx.x, j = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (j >= 2 * d) return;
-    const int n_chunks = (rows + chunk - 1) / chunk;
+    const int n_chunks = (rows - 1) / chunk + 1;
     const int rc = ci == n_chunks - 1 ? rows - (n_chunks - 1) * chunk : chunk;
     const float *src = rec32 + (size_t)ci * 2 * d * chunk + (size_t)j * rc;
     constexpr size_t W = FMT == TAH_KV_I16 ? 2 : 1;
@@ -79,7 +79,7 @@ constexpr int UNITS = 4;
 // grid (groups of a full chunk / 64, chunks); 256 threads.
 __global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const float *__restrict__ rec32,
                                                uint8_t *__restrict__ rec4) {
-    const int n_chunks = (rows + chunk - 1) / chunk;
+    const int n_chunks = (rows - 1) / chunk + 1;
     for (int ci = blockIdx.y; ci < n_chunks; ci += gridDim.y) {
         const int rc = min(chunk, rows - ci * chunk), G = groups4(rc), half = (rc + 1) / 2, in16 = 4 * (threadIdx.x & 15);
         const float *src = rec32 + (size_t)ci * 2 * d * chunk;
@@ -192,7 +192,7 @@ __device__ __forceinline__ void values_of(const uint8_t *rec, int d, int rc, int
 template <int FMT>
 __global__ __launch_bounds__(256) void k_unpack(int rows, int d, int chunk, const uint8_t *__restrict__ rec,
                                                 float *__restrict__ rec32) {
-    const int n_chunks = (rows + chunk - 1) / chunk;
+    const int n_chunks = (rows - 1) / chunk + 1;
     for (int ci = blockIdx.y; ci < n_chunks; ci += gridDim.y) {
         const int rc = min(chunk, rows - ci * chunk), Q = (rc + 3) / 4;
         const uint8_t *src = rec + (size_t)ci * record_bytes(FMT, d, chunk);
@@ -240,7 +240,7 @@ void to_records(hipStream_t s, int rows, int d, int chunk, const float *kv, floa
 
 void pack(hipStream_t s, int rows, int d, int chunk, int fmt, const float *rec32, uint8_t *recq) {
     if (rows <= 0 || fmt == TAH_KV_F32) return;
-    const int n_chunks = (rows + chunk - 1) / chunk;
+    const int n_chunks = (rows - 1) / chunk + 1;
     dim3 grid(n_chunks, (2 * d + 3) / 4);
     if (fmt == TAH_KV_I4) {
         const size_t units = 2 * (size_t)d * groups4(std::min(chunk, rows));
@@ -257,7 +257,7 @@ void pack(hipStream_t s, int rows, int d, int chunk, int fmt, const float *rec32
 
 void unpack(hipStream_t s, int rows, int d, int chunk, int fmt, const uint8_t *rec, float *rec32) {
     if (rows <= 0) return;
-    const int n_chunks = (rows + chunk - 1) / chunk;
+    const int n_chunks = (rows - 1) / chunk + 1;
     const size_t fours = 2 * (size_t)d * ((std::min(chunk, rows) + 3) / 4);
     const dim3 grid((fours + 256 * UNITS - 1) / (256 * UNITS), std::min(n_chunks, 65535));
     if (fmt == TAH_KV_F32)

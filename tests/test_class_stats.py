@@ -125,7 +125,10 @@ def gpu():
 @pytest.mark.parametrize("rows,n,k,top", [(1, 1, 1, 1), (1, 2, 0, 0), (300, 2, 1, 2), (1000, 3, 0, 3), (65, 10, 2, 10),
                                           (130, 16, 1, 1), (130, 17, 1, 17), (64, 64, 3, 5), (9, 65, 64, 64),
                                           (70, 999, 1, 20), (37, 1024, 0, 64), (20, 1025, 1, 3), (11, 5000, 2, 64),
-                                          (9, 16384, 1, 7), (10, 16385, 1, 64), (9, 70001, 1, 33), (1, 300000, 1, 64), (2, 1 << 20, 1, 64), (3, 8193, 1, 40), (200, 24, 2, 24), (99, 40, 1, 40)])
+                                          (9, 16384, 1, 7), (10, 16385, 1, 64), (9, 70001, 1, 33), (1, 300000, 1, 64), (2, 1 << 20, 1, 64), (3, 8193, 1, 40), (200, 24, 2, 24), (99, 40, 1, 40),
+                                          (41, 33, 1, 5), (77, 100, 2, 8), (77, 128, 0, 0), (50, 129, 1, 3), (33, 256, 1, 8),
+                                          (33, 200, 3, 9), (31, 257, 1, 5), (40, 600, 1, 10), (5, 4096, 1, 20), (5, 4097, 0, 64),
+                                          (4, 8192, 2, 3)])
 def test_class_stats(gpu, kind, rows, n, k, top):
     say(f"class stats {rows} x {n}, {k} given, {top} best, {kind}")
     rng = np.random.default_rng(rows * 7 + n)
@@ -195,9 +198,15 @@ def test_class_stats_refused(gpu):
             gpu.class_stats_dev(*args)
     with pytest.raises(ValueError):
         gpu.class_stats_dev(b.ptr, 0, 5, b.ptr, 1, 1, b.ptr, b.ptr, ld=4)
+    for off in ((1, 0, 0, 0), (0, 2, 0, 0), (0, 0, 3, 0), (0, 0, 0, 1)):
+        with pytest.raises(ValueError):
+            gpu.class_stats_dev(b.ptr + off[0], 0, 5, b.ptr + off[1], 1, 1, b.ptr + off[2], b.ptr + off[3])
+    for n in (1, 5, 1024, 2000, 1 << 20):  # no rows: nothing to do, however many classes
+        gpu.class_stats_dev(b.ptr, 0, n, b.ptr, 1, 1, b.ptr, b.ptr)
+        st, ids = gpu.class_stats(np.zeros((0, n), np.float32), None, 1)
+        assert st.shape == (0, 2) and ids.shape == (0, 1)
+    gpu.sync()
     b.free()
-    st, ids = gpu.class_stats(np.zeros((0, 5), np.float32), None, 2)
-    assert st.shape == (0, 3) and ids.shape == (0, 2)
 
 
 @pytest.mark.gpu

@@ -155,11 +155,32 @@ def test_a_layer_on_the_card(gpu, fmt, d, rows, chunk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [abi.KV_F32, abi.KV_I16, abi.KV_I8, abi.KV_I4])
+def test_a_chunk_longer_than_any_table(gpu, fmt):
+    """Chunks of up to 2^31 - 1 rows: a shorter table is one chunk of its own length."""
+    d, rows = 48, 77
+    kv = np.random.default_rng(5).standard_normal(2 * rows * d).astype(np.float32)
+    size = abi.layer_bytes(fmt, rows, rows, d)
+    src, dst, back = dm.DeviceBuffer.of(kv), dm.DeviceBuffer(size), dm.DeviceBuffer(kv.nbytes)
+    got = []
+    for chunk in (rows, 2 ** 31 - 1):
+        gpu.pack_dev(src.ptr, d, rows, chunk, fmt, dst.ptr)
+        gpu.unpack_dev(dst.ptr, d, rows, chunk, fmt, back.ptr)
+        gpu.sync()
+        got.append((dst.download(size, np.uint8), back.download(kv.size)))
+    assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1])
+    assert np.array_equal(got[0][0], gpu.pack(kv, d, rows, fmt))
+    for b in (src, dst, back):
+        b.free()
+
+
+@pytest.mark.gpu
 def test_layers_refused(gpu):
     b = dm.DeviceBuffer(4096)
     for d, rows, chunk, fmt, ptr in ((0, 4, 8, abi.KV_I4, b.ptr), (16, -1, 8, abi.KV_I4, b.ptr), (16, 4, 0, abi.KV_I4, b.ptr),
                                      (16, 4, 8, 4, b.ptr), (16, 4, 8, -1, b.ptr), (16, 4, 8, abi.KV_I4, b.ptr + 1),
-                                     (16, 0, 8, abi.KV_I4, None)):
+                                     (16, 0, 8, abi.KV_I4, None), (1, 1 << 24, 1, abi.KV_I4, b.ptr + 2),
+                                     (1 << 20, 0, 1 << 20, abi.KV_I4, b.ptr)):
         with pytest.raises(ValueError):
             gpu.pack_dev(ptr, d, rows, chunk, fmt, b.ptr)
         with pytest.raises(ValueError):
