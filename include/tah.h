@@ -121,7 +121,11 @@ int tah_sync(tah_dev *dev);
 /* The device handle's HIP stream (a hipStream_t), for callers that time or order work around _dev calls. A call may
    fork part of its work onto a second stream of the handle (the column and row stages of 768 rows or more, as two
    halves); it joins that stream back into this one before it returns, so that ordering on this stream orders all of
-   the call's work (a graph captured on it takes the fork and the join with it). */
+   the call's work (a graph captured on it takes the fork and the join with it). Working memory a captured call takes
+   stays the handle's: make the call once before capturing it (memory cannot be allocated meanwhile), replay such graphs
+   on this stream, in order with the handle's own calls, and none after tah_release or after a call that the budget made
+   give idle memory back. tah_pack_dev, tah_unpack_dev, tah_class_stats_dev up to 16,384 classes and
+   tah_stage_dev_noalloc take none. */
 void *tah_stream(tah_dev *dev);
 
 /* ---- weights: GpuWeights::new / bytes (src/gpu.rs:1838-2027). Copies every tensor the card uses. */
@@ -131,12 +135,13 @@ size_t tah_weights_bytes(const tah_weights *w);
 void tah_weights_free(tah_weights *w);
 
 /* ---- fitted model on the card: VramModel::model_bytes / load (src/gpu.rs:2064-2116), but from the bundle's own
- * chunk records as they are stored (n{j}_kv{l}), any of the three formats, no re-layout on the host.
+ * chunk records as they are stored (n{j}_kv{l}), any of the four formats, no re-layout on the host.
  * layer_records[l] points at layer l's bytes (tah_kv_record summed over its chunks); scales is n{j}_scale,
  * [layers][d]. A layer of head width 64 is held once, as the tiles the card makes of its records (f32: split-fp16
- * images; i16: the codes with their dequantisation factors; i8: the codes as fp16 with the scales), which every
- * attention kernel reads; other head widths keep the records. tah_model_bytes (like Gpu::model_bytes, from the
- * weights' shape) counts what the layers are held as, and the scales; 0 without weights. */
+ * images; i16: the codes with their dequantisation factors; i8: the codes as fp16 with the scales; i4: the codes with
+ * their steps and offsets as fp16), which every attention kernel reads; other head widths keep the records.
+ * tah_model_bytes (like Gpu::model_bytes, from the weights' shape) counts what the layers are held as, and the scales; 0
+ * without weights. */
 size_t tah_model_bytes(const tah_weights *w, int32_t kv_format, int32_t rows, int32_t chunk);
 int tah_model_load(tah_dev *dev, const tah_weights *w, int32_t kv_format, int32_t rows, int32_t chunk,
                    const uint8_t *const *layer_records, const float *scales, tah_model **out);

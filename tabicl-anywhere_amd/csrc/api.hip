@@ -576,6 +576,7 @@ static size_t model_layer_bytes(int kv_format, int rows, int chunk, int d, int h
 
 extern "C" size_t tah_model_bytes(const tah_weights *w, int32_t kv_format, int32_t rows, int32_t chunk) {
     if (!w || rows <= 0 || chunk <= 0 || !kv_known(kv_format)) return 0;
+    chunk = std::min(chunk, rows);  // no chunk is longer than the table
     const int d = w->d, layers = w->icl_layers;
     return (size_t)layers * model_layer_bytes(kv_format, rows, chunk, d, w->icl_heads) +
            align256(sizeof(float) * layers * d);
@@ -589,6 +590,7 @@ extern "C" int tah_model_load(tah_dev *dev, const tah_weights *w, int32_t kv_for
         if (rows <= 0 || chunk <= 0 || !kv_known(kv_format)) throw ArgError{"model: bad rows, chunk or format"};
         for (int l = 0; l < w->icl_layers; l++)
             if (!layer_records[l]) throw ArgError{"model: missing layer records"};
+        chunk = std::min(chunk, rows);
         auto *m = new tah_model();
         m->dev = dev;
         m->ordinal = dev->ordinal;

@@ -1,6 +1,6 @@
 // In-context attention of query rows over one stored layer of training-row keys and values: the bundle's chunk
-// records (f32, or i16/i8 codes with per-chunk, per-coordinate scales, dequantised on the card), or the tile images
-// made of them. This replaces the reference's streaming loop (src/predict.rs:427-533 with Soft::update/update_int,
+// records (f32, i16/i8 codes with per-chunk, per-coordinate scales, or i4 codes with a step and an offset per 64 rows and
+// coordinate, dequantised on the card), or the tile images made of them. This replaces the reference's streaming loop (src/predict.rs:427-533 with Soft::update/update_int,
 // src/nn.rs:194-258) and its WGSL attend/merge shaders (src/gpu.rs:492-627).
 //
 // Keys are visited in blocks of 64 that never straddle a stored chunk. Each workgroup keeps, per query and head,
@@ -19,12 +19,14 @@
 //  * k_attn_few: head width 64, 1 to 16 queries over f32 images and i8 code images (2 to 16 over i16 code tiles):
 //    the four wavefronts of a workgroup split each key block, with the queries as the 16 columns of 16 x 16
 //    products, and merge their softmax states at the end.
+//  * k_attn_few4: head width 64 over i4 code tiles, up to where k_attn_split64's larger query tiles are quicker (plan4):
+//    eight wavefronts with key blocks of their own, tiles straight into registers, 16 or 32 queries a workgroup.
 //  * k_attn_decode_w: head width 64 and few queries (or no images), from the records: 256 threads per (six key
 //    blocks, head, 8 queries), each wavefront streaming a key block at a time with no barrier (lane = key for the
 //    scores, lane = coordinate for the weighted sum), integer codes scaled through the query and the sums.
 //  * k_attn_decode: any other head width up to 64 (the tiny test models): the same with one wavefront.
 // All of them leave the running maximum in log2 units (score * log2 e) for the split merge (head width 64:
-// k_attn_merge64 for few key ranges, k_attn_merge_w for many; k_attn_merge otherwise).
+// k_attn_merge64 for few key ranges, k_attn_merge_w for many, k_attn_merge_few for few pairs; k_attn_merge otherwise).
 #include <algorithm>
 
 #include <atomic>
@@ -852,6 +854,8 @@ struct Flag {
 //
 // An i4 cache's code tiles (FOUR) go the same way, but what they stand for is exact in fp16: the LDS images have one
 // plane, as the i8 code images, and the products are two a term, with neither scales to follow nor a query to split again.
+// 2,048 queries over 10,000 rows 95 us: 883 TFLOP/s of fp16 products. The matrix units are busy 38% of the time; the widening
+// and the weights' exponentials and splits take the issue slots beside them.
 template <int WAVES, int FMT>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows, int chunk, int d, int heads,
                                                                const float *__restrict__ q,
@@ -1618,19 +1622,26 @@ __global__ __launch_bounds__(256, 1) void k_attn_few(int nq, int rows, int chunk
     }
 }
 
-// ---- few-query kernel over 4-bit code tiles: head width 64, 1 to 16 queries -------------------------------------------
-// grid heads x splits (workgroup i: head i % heads, key range i / heads); 256 threads. Each wavefront takes key blocks of
-// its own (kb0 + w, kb0 + w + 4, ..): a tile is 4.5 KB in the order of its operands, so a block is nine 16-byte loads a
-// lane straight into registers, the next block's issued before this one's arithmetic, and there is no LDS and no barrier
-// until the four softmax states are merged. The products are 16 x 16 x 32 with the queries as columns: S = K Q^T by 16
-// (two for each of four sets of 16 keys and two halves of the coordinates), O^T += V^T P^T by 16. The order of the keys
-// within a tile leaves a lane's eight scores of each 32 keys as the operand that the values' product takes.
+// ---- 4-bit code tiles straight into registers: head width 64 -------------------------------------------------------------
+// grid (heads, key ranges, groups of 16 G queries); 512 threads. Each wavefront takes key blocks of its own (kb0 + w,
+// kb0 + w + 8, ..): a tile is 4.5 KB in the order of its operands, so a block is nine 16-byte loads a lane straight into
+// registers, the next block's issued before this one's arithmetic, and there is no LDS and no barrier until the eight softmax
+// states are merged. The products are 16 x 16 x 32 with the queries as columns: S = K Q^T (two for each of four sets of 16
+// keys and two halves of the coordinates, a group), O^T += V^T P^T by as many. The order of the keys within a tile leaves a
+// lane's eight scores of each 32 keys as the operand that the values' product takes. What fp16 holds of a key or value is
+// exact, so a term is two products (query or weight high and low), for f32's error.
+//
+// Few queries: the tiles' bytes and latency bound it (one query over 100,000 rows of 8 heads, 57.6 MB of tiles, 17.7 us with
+// the merge: 3.3 TB/s; over 1,000 rows 7.1 us, one range). Many: widening codes is repeated by every workgroup, so two groups
+// a workgroup share it (G 2 from 17 queries: 100 over 5,003 rows of 4 heads 11.3 us), until a tile of 256 queries wins.
 constexpr int FEW4_WAVES = 8;
 template <int G>
-__global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlocks kbs, int chunk, const float *__restrict__ q,
-                                                      const uint8_t *__restrict__ tiles, const uint32_t *__restrict__ kvmax,
-                                                      int kb_per_split, float *__restrict__ part_o,
-                                                      float *__restrict__ part_ml, float *__restrict__ out) {
+__global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlocks kbs, int chunk,
+                                                                  const float *__restrict__ q,
+                                                                  const uint8_t *__restrict__ tiles,
+                                                                  const uint32_t *__restrict__ kvmax, int kb_per_split,
+                                                                  float *__restrict__ part_o, float *__restrict__ part_ml,
+                                                                  float *__restrict__ out) {
     constexpr int W = FEW4_WAVES, NQ = 16 * G;
     __shared__ float mref[W][NQ], msum[W][NQ], macc[W][64][NQ + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1944,7 +1955,8 @@ __global__ __launch_bounds__(256) void k_attn_merge_w(int items, int splits, con
 }
 
 // Split merge for few (query, head) pairs and up to MERGE_FEW key ranges: a workgroup a pair, its wavefronts the ranges of
-// one residue each, lane = coordinate, every load issued before the sums; the four states through LDS.
+// one residue each, lane = coordinate, every load issued before the sums; the four states through LDS (one query over
+// 100,000 i4 rows 19.0 -> 17.7 us with the other merges' replaced, 16 over 50,000 15.0 -> 13.6).
 constexpr int MERGE_FEW = 32;
 __global__ __launch_bounds__(256) void k_attn_merge_few(int items, int splits, const float *__restrict__ part_o,
                                                         const float *__restrict__ part_ml, float *__restrict__ out) {
@@ -1992,7 +2004,7 @@ __global__ __launch_bounds__(256) void k_attn_merge_few(int items, int splits, c
 
 // ---- planning and launch --------------------------------------------------------------------------------------
 struct AttnPlan {
-    bool split16, few;  // few: k_attn_few (any tiles, at most FEW_Q queries; i16 from FEW16_FROM)
+    bool split16, few;  // few: k_attn_few (any tiles, at most FEW_Q queries; i16 from FEW16_FROM), i4: k_attn_few4<waves>
     int splits, kb_per_split, groups, waves;
 };
 
@@ -2060,7 +2072,7 @@ KvImages kv_images_at(uint8_t *base, int rows, int chunk, int heads, int kv_form
 // 4-bit tiles: which kernel, and into how many ranges the keys go. Both run in rounds of one workgroup a compute unit; a
 // range count is worth looking at where it fills a whole number of rounds. A round of k_attn_few4 takes 2.6 us a block of
 // its eight wavefronts' turns and one and a half more, the merge of ranges as much again; one of k_attn_split64 2 us a
-// block and eight and a half more (queries x rows, 8 heads, measured by the one and the other: 512 x 10,000 33 and 42 us, 600 x 2,000
+// block and eight and a half more (queries x rows, 8 heads, by the one and the other: 512 x 10,000 33 and 42 us, 600 x 2,000
 // 15 and 21, 1,024 x 10,000 55 and 56, 1,536 x 10,000 106 and 77, 2,048 x 2,000 30 and 34, 2,048 x 10,000 107 and 95).
 static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
     auto ranges = [&](int per, int least_blocks, auto cost_of, float &cost) {
@@ -2080,7 +2092,7 @@ static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
     AttnPlan p{};
     p.few = true;
     p.waves = a.nq <= 16 ? 1 : 2;  // groups of 16 queries a workgroup
-    p.groups = (a.nq + 16 * p.waves - 1) / (16 * p.waves);
+    p.groups = std::max(1, (a.nq + 16 * p.waves - 1) / (16 * p.waves));
     float few_cost, many_cost;
     // one range while a wavefront has no more than two blocks: a second one's merge takes longer
     int splits = ranges(a.heads * p.groups, FEW4_WAVES,

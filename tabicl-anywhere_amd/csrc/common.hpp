@@ -272,14 +272,15 @@ size_t attention_work_bytes(const AttnShape &a);
 void to_records(hipStream_t s, int rows, int d, int chunk, const float *kv, float *rec32);
 // f32 chunk records to i16/i8 records (the reference's quantiser, bit for bit) or i4 records; and any format's records to
 // f32 chunk records.
-void unpack(hipStream_t s, int rows, int d, int chunk, int fmt, const uint8_t *rec, float *rec32);
 void pack(hipStream_t s, int rows, int d, int chunk, int fmt, const float *rec32, uint8_t *recq);
+void unpack(hipStream_t s, int rows, int d, int chunk, int fmt, const uint8_t *rec, float *rec32);
 // Keys and values of one stored layer as tiles per (key block of 64, head), the form a fitted layer of head width 64
 // is held in on the card (its records are not kept) and the attention kernels read: f32 as fp16 hi/lo split images,
-// i16 as code tiles with dequantisation factors, i8 as fp16 code images with the chunks' scales (attention.hip).
+// i16 as code tiles with dequantisation factors, i8 as fp16 code images with the chunks' scales, i4 as code tiles with
+// steps and offsets in fp16 (attention.hip).
 struct KvImages {
     uint8_t *images = nullptr;
-    uint32_t *kvmax = nullptr;  // f32 and i16: the heads' largest |K|, |V| (dequantised)
+    uint32_t *kvmax = nullptr;  // f32, i16 and i4: the heads' largest |K|, |V| (dequantised)
     float *scales = nullptr;    // i8: per (chunk, head) the key scales, value scales and ratios
     int fmt = TAH_KV_F32;       // the stored format the tiles were made from
 };
