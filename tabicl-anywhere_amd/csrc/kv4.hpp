@@ -54,27 +54,32 @@ __device__ __forceinline__ int code4(Step4 st, float v) {
     return (int)fminf(fmaxf(rintf(__fdiv_rn(v - st.z, st.s)), -8.0f), 7.0f);
 }
 
-// The same of four values with one reciprocal: it is off by 2^-22 of the quotient at most, so that away from a tie the
-// nearest level is the same; where a lane of the wavefront is near one (one in 2^16 values), by the division.
-__device__ __forceinline__ void codes4(Step4 st, const float (&v)[4], int (&code)[4]) {
-    const bool some = st.s > 0.0f;
-    const float inv = some ? __builtin_amdgcn_rcpf(st.s) : 0.0f;
-    bool near = false;
+// The same of four values, eight more than each in four bits, with one reciprocal: it is off by 2^-22 of the quotient at
+// most, so that away from a tie the nearest level is the same; where a lane of the wavefront is near one (one in 2^16
+// values), by the division.
+__device__ __forceinline__ uint32_t codes4(Step4 st, const float (&v)[4]) {
+    const float inv = st.s > 0.0f ? __builtin_amdgcn_rcpf(st.s) : 0.0f;
+    float far = 0.0f;  // from the nearest level, a NaN passed over
+    int code[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         const float x = (v[t] - st.z) * inv, q = rintf(x);
-        near = near || fabsf(x - q) > 0.5f - 0x1p-16f;
-        code[t] = some && v[t] == v[t] ? (int)fminf(fmaxf(q, -8.0f), 7.0f) : 0;
+        far = fmaxf(far, fabsf(x - q));
+        // the instruction takes a NaN to 0 and clamps what does not fit, which the language leaves open
+        asm("v_cvt_i32_f32 %0, %1" : "=v"(code[t]) : "v"(q));
+        code[t] = min(max(code[t], -8), 7);
     }
-    if (__any(near)) {
+    if (__any(far > 0.5f - 0x1p-16f)) {
 #pragma unroll
         for (int t = 0; t < 4; t++) code[t] = code4(st, v[t]);
     }
+    return (uint32_t)(code[0] + 16 * (code[1] + 16 * (code[2] + 16 * code[3])) + 0x8888);
 }
 
 __device__ __forceinline__ Step4 step_at4(const uint8_t *rec, int rc, int j, int g) {
-    const uint16_t *p = reinterpret_cast<const uint16_t *>(rec) + 2 * ((size_t)j * groups4(rc) + g);
-    return {__uint_as_float((uint32_t)p[0] << 16), __uint_as_float((uint32_t)p[1] << 16)};
+    uint32_t sz;  // a record starts on an even byte
+    __builtin_memcpy(&sz, rec + 4 * ((size_t)j * groups4(rc) + g), 4);
+    return {__uint_as_float(sz << 16), __uint_as_float(sz & 0xFFFF0000u)};
 }
 
 // number (stacked coordinate j of 2d, row r) of a chunk's record

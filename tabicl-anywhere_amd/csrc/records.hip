@@ -71,10 +71,35 @@ __global__ __launch_bounds__(256) void k_pack(int rows, int d, int chunk, const 
 }
 
 // ---- i4 records and back ------------------------------------------------------------------------------------------------
-// Both are bound by memory (a number is 4 bytes and 9/16 of one), so the numbers move 16 bytes a lane where the records
-// allow it: a lane takes four consecutive rows of a coordinate, 16 lanes a group of 64, UNITS groups in turn with their
-// loads issued together. Records whose rows do not start on whole words (odd chunks) take the same path by single loads.
-constexpr int UNITS = 4;
+// A number is 4 bytes and 9/16 of one. It moves 16 bytes at a time: a lane takes four consecutive rows of a coordinate, 16
+// lanes a group of 64, UNITS groups in turn with their loads issued together (10,000 x 512 in chunks of 256 unpacked with 1, 2
+// and 4: 11.9, 9.2 and 9.9 us; packed 12.5, 11.0 and 12.0). Chunks of any length do so: fours that start off a 16-byte line
+// are loads and stores of 4-byte alignment, only a coordinate's last rows go one by one. Unpacked numbers are written past the
+// caches, which hold the records and would be turned over (40,000 x 512: 61.7 -> 30.4 us).
+//
+// 10,000 x 512 (46.7 MB): unpacked 8.2 us, 5.7 TB/s, a large copy's rate; packed 11.0 us, bound by its instructions, about 120
+// a lane's four numbers: the range of 16 lanes, the step, four quotients, their ties.
+constexpr int UNITS = 2;
+typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
+
+// The least lo and largest hi of 16 lanes (neither a NaN), in all of them: lanes 1, 2, 4 and 8 apart. Written out because the
+// compiler moves and cleans a lane's neighbour in two instructions of their own before each comparison; a register written
+// is read across lanes two instructions later at the soonest.
+__device__ __forceinline__ void row16_range(float &lo, float &hi) {
+    asm("s_nop 1\n\t"
+        "v_min_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+        "v_max_f32_dpp %1, %1, %1 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 0\n\t"
+        "v_min_f32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+        "v_max_f32_dpp %1, %1, %1 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 0\n\t"
+        "v_min_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+        "v_max_f32_dpp %1, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 0\n\t"
+        "v_min_f32_dpp %0, %0, %0 row_mirror row_mask:0xf bank_mask:0xf\n\t"
+        "v_max_f32_dpp %1, %1, %1 row_mirror row_mask:0xf bank_mask:0xf"
+        : "+v"(lo), "+v"(hi));
+}
 
 // grid (groups of a full chunk / 64, chunks); 256 threads.
 __global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const float *__restrict__ rec32,
@@ -84,8 +109,6 @@ __global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const
         const int rc = min(chunk, rows - ci * chunk), G = groups4(rc), half = (rc + 1) / 2, in16 = 4 * (threadIdx.x & 15);
         const float *src = rec32 + (size_t)ci * 2 * d * chunk;
         uint8_t *rec = rec4 + (size_t)ci * record_bytes(TAH_KV_I4, d, chunk), *codes = rec + 8 * (size_t)d * G;
-        const bool fours = rc % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-        const bool pairs = half % 2 == 0 && (reinterpret_cast<uintptr_t>(codes) & 1) == 0;
         float v[UNITS][4];
         int j[UNITS], g[UNITS];
         // the units of a thread are 16 apart
@@ -105,9 +128,10 @@ __global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const
 #pragma unroll
             for (int t = 0; t < 4; t++) v[u][t] = NAN;  // what is past the end takes no part
             if (j[u] >= 2 * d) continue;
-            if (fours && r < rc) {
-                const float4 x = *reinterpret_cast<const float4 *>(at);
-                v[u][0] = x.x; v[u][1] = x.y; v[u][2] = x.z; v[u][3] = x.w;
+            if (r + 4 <= rc) {
+                const Four x = *reinterpret_cast<const Four *>(at);
+#pragma unroll
+                for (int t = 0; t < 4; t++) v[u][t] = x[t];
             } else {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
@@ -126,8 +150,7 @@ __global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const
                     lo = fminf(lo, x);
                     hi = fmaxf(hi, x);
                 }
-                lo = row16_reduce(lo, fminf);
-                hi = row16_reduce(hi, fmaxf);
+                row16_range(lo, hi);
             };
             float lo, hi;
             range(true, lo, hi);
@@ -136,23 +159,15 @@ __global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const
             if (j[u] >= 2 * d) continue;
             const int r = 64 * g[u] + in16, left = rc - r;
             if (in16 == 0) {
-                uint16_t *sp = reinterpret_cast<uint16_t *>(rec) + 2 * ((size_t)j[u] * G + g[u]);
-                sp[0] = (uint16_t)(__float_as_uint(st.s) >> 16);
-                sp[1] = (uint16_t)(__float_as_uint(st.z) >> 16);
+                const uint32_t sz = __float_as_uint(st.s) >> 16 | __float_as_uint(st.z);
+                __builtin_memcpy(rec + 4 * ((size_t)j[u] * G + g[u]), &sz, 4);
             }
             if (left <= 0) continue;
-            int code[4];
-            codes4(st, v[u], code);
-            uint32_t word = 0;
-#pragma unroll
-            for (int t = 0; t < 4; t++) word |= (t < left ? (uint32_t)(code[t] + 8) : 0u) << 4 * t;
+            uint32_t word = codes4(st, v[u]);
+            if (left < 4) word &= (1u << 4 * left) - 1;
             uint8_t *cp = codes + (size_t)j[u] * half + r / 2;
-            if (pairs && left > 2) {
-                *reinterpret_cast<uint16_t *>(cp) = (uint16_t)word;
-            } else {
-                cp[0] = (uint8_t)word;
-                if (left > 2) cp[1] = (uint8_t)(word >> 8);
-            }
+            if (left > 2) __builtin_memcpy(cp, &word, 2);
+            else cp[0] = (uint8_t)word;
         }
     }
 }
@@ -160,20 +175,14 @@ __global__ __launch_bounds__(256) void k_pack4(int rows, int d, int chunk, const
 // What four consecutive rows (from a multiple of 4) of coordinate j of a chunk's record stand for; rows past the end not
 // looked at.
 template <int FMT>
-__device__ __forceinline__ void values_of(const uint8_t *rec, int d, int rc, int j, int r, bool whole, float (&v)[4]) {
+__device__ __forceinline__ void values_of(const uint8_t *rec, int d, int rc, int j, int r, float (&v)[4]) {
     if constexpr (FMT == TAH_KV_I4) {
-        Step4 st;
-        if (whole) {
-            const uint32_t sz = reinterpret_cast<const uint32_t *>(rec)[(size_t)j * groups4(rc) + r / GROUP4];
-            st = {__uint_as_float(sz << 16), __uint_as_float(sz & 0xFFFF0000u)};
-        } else {
-            st = step_at4(rec, rc, j, r / GROUP4);
-        }
+        const Step4 st = step_at4(rec, rc, j, r / GROUP4);
         const int half = (rc + 1) / 2;
         const uint8_t *cp = rec + 8 * (size_t)d * groups4(rc) + (size_t)j * half + r / 2;
-        uint32_t word;
-        if (whole) word = *reinterpret_cast<const uint16_t *>(cp);
-        else word = cp[0] | (r + 2 < rc ? cp[1] : 0) << 8;
+        uint32_t word = 0;
+        if (r + 2 < rc) __builtin_memcpy(&word, cp, 2);
+        else word = cp[0];
 #pragma unroll
         for (int t = 0; t < 4; t++) v[t] = value4(st, (int)(word >> 4 * t & 15) - 8);
     } else {
@@ -197,8 +206,6 @@ __global__ __launch_bounds__(256) void k_unpack(int rows, int d, int chunk, cons
         const int rc = min(chunk, rows - ci * chunk), Q = (rc + 3) / 4;
         const uint8_t *src = rec + (size_t)ci * record_bytes(FMT, d, chunk);
         float *dst = rec32 + (size_t)ci * 2 * d * chunk;
-        const bool fours = rc % 4 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
-        const bool whole = rc % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 3) == 0;  // steps and codes by whole words
         float v[UNITS][4];
         int j[UNITS], r[UNITS];
         // the fours of a thread are 256 apart
@@ -214,14 +221,14 @@ __global__ __launch_bounds__(256) void k_unpack(int rows, int d, int chunk, cons
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
             r[u] *= 4;
-            if (j[u] < 2 * d) values_of<FMT>(src, d, rc, j[u], r[u], whole, v[u]);
+            if (j[u] < 2 * d) values_of<FMT>(src, d, rc, j[u], r[u], v[u]);
         }
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
             if (j[u] >= 2 * d) continue;
             float *to = dst + (size_t)j[u] * rc + r[u];
-            if (fours) {
-                *reinterpret_cast<float4 *>(to) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+            if (r[u] + 4 <= rc) {
+                __builtin_nontemporal_store(Four{v[u][0], v[u][1], v[u][2], v[u][3]}, reinterpret_cast<Four *>(to));
             } else {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
