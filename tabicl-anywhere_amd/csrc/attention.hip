@@ -1625,18 +1625,20 @@ __global__ __launch_bounds__(256, 1) void k_attn_few(int nq, int rows, int chunk
 // ---- 4-bit code tiles straight into registers: head width 64 -------------------------------------------------------------
 // grid (heads, key ranges, groups of 16 G queries); 512 threads. Each wavefront takes key blocks of its own (kb0 + w,
 // kb0 + w + 8, ..): a tile is 4.5 KB in the order of its operands, so a block is nine 16-byte loads a lane straight into
-// registers, the next block's issued before this one's arithmetic, and there is no LDS and no barrier until the eight softmax
-// states are merged. The products are 16 x 16 x 32 with the queries as columns: S = K Q^T (two for each of four sets of 16
-// keys and two halves of the coordinates, a group), O^T += V^T P^T by as many. The order of the keys within a tile leaves a
-// lane's eight scores of each 32 keys as the operand that the values' product takes. What fp16 holds of a key or value is
-// exact, so a term is two products (query or weight high and low), for f32's error.
+// registers, and there is no LDS and no barrier until the eight softmax states are merged. The products are 16 x 16 x 32 with
+// the queries as columns: S = K Q^T (two for each of four sets of 16 keys and two halves of the coordinates, a group), O^T +=
+// V^T P^T by as many, the four accumulators in turn so that none waits for its own last product. The order of the keys within
+// a tile leaves a lane's eight scores of each 32 keys as the operand that the values' product takes. What fp16 holds of a key
+// or value is exact, so a term is two products (query or weight high and low), for f32's error.
 //
-// Few queries: the tiles' bytes and latency bound it (one query over 100,000 rows of 8 heads, 57.6 MB of tiles, 17.7 us with
-// the merge: 3.3 TB/s; over 1,000 rows 7.1 us, one range). Many: widening codes is repeated by every workgroup, so two groups
-// a workgroup share it (G 2 from 17 queries: 100 over 5,003 rows of 4 heads 11.3 us), until a tile of 256 queries wins.
+// Few queries: one over 100,000 rows of 8 heads (57.6 MB of tiles) takes 17.8 us with the merge, 3.2 TB/s, where a wavefront's
+// turn of one block (350 vector instructions, 208 of them widening codes, and 32 products) is twice its loads' time; the next
+// block's loads issued ahead of it change nothing there and hold registers (16 over 50,000 rows 13.6 -> 12.9 us without). Over
+// 1,000 rows 6.8 us, one range. Many: widening is repeated by every workgroup, so two groups share it (G 2 from 17 queries:
+// 100 over 5,003 rows of 4 heads 11.0 us), until a tile of 256 queries wins.
 constexpr int FEW4_WAVES = 8;
 template <int G>
-__global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlocks kbs, int chunk,
+__global__ __launch_bounds__(64 * FEW4_WAVES, G == 1 ? 4 : 2) void k_attn_few4(int nq, KeyBlocks kbs, int chunk,
                                                                   const float *__restrict__ q,
                                                                   const uint8_t *__restrict__ tiles,
                                                                   const uint32_t *__restrict__ kvmax, int kb_per_split,
@@ -1668,9 +1670,7 @@ __global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlo
         b.vf = *reinterpret_cast<const u32x4 *>(t + HALF4 + 2048 + 16 * qi);
         return b;
     };
-    Block cur[2];
     int kb = kb0 + wave;
-    if (kb < kb1) cur[0] = fetch(kb);
     int in_chunk = kb % kbs.bpc, ci = kb / kbs.bpc;  // kept along, without a division a block
     const int over = W % kbs.bpc, past = W / kbs.bpc;
     // query 16 g + qi's coordinates 32 ks + 8 lg + t, scaled to a maximum near 2^14 and split
@@ -1708,26 +1708,30 @@ __global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlo
     auto step = [&](const Block &cur) {
         const int nk = min(KB, (ci == kbs.n_chunks - 1 ? kbs.last_rc : chunk) - in_chunk * KB);
         float sc[G][16];  // 8 s + 4 p + i: key 32 s + 8 lg + 4 p + i
+        const floatx4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+        floatx4 a[4][G];  // set 2 s + p of 16 keys
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+        for (int ks = 0; ks < 2; ks++) {
+            halfx8 kv[4];
 #pragma unroll
-            for (int p = 0; p < 2; p++) {
-                floatx4 a[G];
-#pragma unroll
-                for (int g = 0; g < G; g++) a[g] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int ks = 0; ks < 2; ks++) {
-                    const halfx8 kv = values4(cur.k[s][2 * p + ks], cur.ks[ks], cur.kz[ks]);
-#pragma unroll
-                    for (int g = 0; g < G; g++) a[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, qh[g][ks], a[g], 0, 0, 0);
-#pragma unroll
-                    for (int g = 0; g < G; g++) a[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, ql[g][ks], a[g], 0, 0, 0);
-                }
+            for (int sp = 0; sp < 4; sp++) {
+                kv[sp] = values4(cur.k[sp >> 1][2 * (sp & 1) + ks], cur.ks[ks], cur.kz[ks]);
 #pragma unroll
                 for (int g = 0; g < G; g++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sc[g][8 * s + 4 * p + i] = a[g][i];
+                    a[sp][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[sp], qh[g][ks], ks ? a[sp][g] : none, 0, 0, 0);
             }
+#pragma unroll
+            for (int sp = 0; sp < 4; sp++)
+#pragma unroll
+                for (int g = 0; g < G; g++)
+                    a[sp][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[sp], ql[g][ks], a[sp][g], 0, 0, 0);
+        }
+#pragma unroll
+        for (int sp = 0; sp < 4; sp++)
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[g][4 * sp + i] = a[sp][g][i];
         halfx8 ph[G][2], pl[G][2];
 #pragma unroll
         for (int g = 0; g < G; g++) {
@@ -1768,34 +1772,33 @@ __global__ __launch_bounds__(64 * FEW4_WAVES, 2) void k_attn_few4(int nq, KeyBlo
             }
         }
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+        for (int s = 0; s < 2; s++) {
+            halfx8 v[4];
 #pragma unroll
             for (int m = 0; m < 4; m++) {
                 const uint32_t word = cur.vf[m];
                 const halfx2 f = __builtin_bit_cast(halfx2, word);
                 const _Float16 fs = f[0], fz = f[1];
-                const halfx8 v = values4(cur.v[s][m], halfx8{fs, fs, fs, fs, fs, fs, fs, fs},
-                                         halfx8{fz, fz, fz, fz, fz, fz, fz, fz});
+                v[m] = values4(cur.v[s][m], halfx8{fs, fs, fs, fs, fs, fs, fs, fs},
+                               halfx8{fz, fz, fz, fz, fz, fz, fz, fz});
 #pragma unroll
-                for (int g = 0; g < G; g++) acc[g][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[g][s], acc[g][m], 0, 0, 0);
-#pragma unroll
-                for (int g = 0; g < G; g++) acc[g][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[g][s], acc[g][m], 0, 0, 0);
+                for (int g = 0; g < G; g++)
+                    acc[g][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[m], ph[g][s], acc[g][m], 0, 0, 0);
             }
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+#pragma unroll
+                for (int g = 0; g < G; g++)
+                    acc[g][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[m], pl[g][s], acc[g][m], 0, 0, 0);
+        }
     };
-    // two blocks a round, so that the registers' roles are fixed
-    while (kb < kb1) {
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            if (kb + W < kb1) cur[u ^ 1] = fetch(kb + W);
-            step(cur[u]);
-            kb += W;
-            in_chunk += over;
-            ci += past;
-            if (in_chunk >= kbs.bpc) {
-                in_chunk -= kbs.bpc;
-                ci++;
-            }
-            if (kb >= kb1) break;
+    for (; kb < kb1; kb += W) {
+        step(fetch(kb));
+        in_chunk += over;
+        ci += past;
+        if (in_chunk >= kbs.bpc) {
+            in_chunk -= kbs.bpc;
+            ci++;
         }
     }
     // the wavefronts' (maximum, sum, weighted sums), merged as the split merge merges key ranges
@@ -2070,10 +2073,10 @@ KvImages kv_images_at(uint8_t *base, int rows, int chunk, int heads, int kv_form
 }
 
 // 4-bit tiles: which kernel, and into how many ranges the keys go. Both run in rounds of one workgroup a compute unit; a
-// range count is worth looking at where it fills a whole number of rounds. A round of k_attn_few4 takes 2.6 us a block of
+// range count is worth looking at where it fills a whole number of rounds. A round of k_attn_few4 takes 2.5 us a block of
 // its eight wavefronts' turns and one and a half more, the merge of ranges as much again; one of k_attn_split64 2 us a
-// block and eight and a half more (queries x rows, 8 heads, by the one and the other: 512 x 10,000 33 and 42 us, 600 x 2,000
-// 15 and 21, 1,024 x 10,000 55 and 56, 1,536 x 10,000 106 and 77, 2,048 x 2,000 30 and 34, 2,048 x 10,000 107 and 95).
+// block and eight and a half more (queries x rows, 8 heads, by the one and the other: 512 x 10,000 32 and 42 us, 600 x 2,000
+// 15 and 21, 1,024 x 10,000 52 and 56, 1,536 x 10,000 106 and 76, 2,048 x 2,000 29 and 34, 2,048 x 10,000 107 and 95).
 static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
     auto ranges = [&](int per, int least_blocks, auto cost_of, float &cost) {
         int best = 1;
@@ -2097,7 +2100,7 @@ static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
     // one range while a wavefront has no more than two blocks: a second one's merge takes longer
     int splits = ranges(a.heads * p.groups, FEW4_WAVES,
                         [](int rounds, int blocks, bool merge) {
-                            return 2.6f * (rounds * ((blocks + FEW4_WAVES - 1) / FEW4_WAVES + 1.5f) + (merge ? 1.5f : 0.0f));
+                            return 2.5f * (rounds * ((blocks + FEW4_WAVES - 1) / FEW4_WAVES + 1.5f) + (merge ? 1.5f : 0.0f));
                         },
                         few_cost);
     if (a.nq > 128) {
