@@ -9,7 +9,7 @@
 // (Soft::merge, src/nn.rs:261-276) and divided through (Soft::finish).
 //
 // The kernels:
-//  * k_attn_split64: head width 64 over tile images (below; any cache format) from 17 queries, 32 queries a
+//  * k_attn_split64: head width 64 over tile images (below; f32, i16 and i8) from 17 queries, 32 queries a
 //    wavefront. Every f32
 //    product runs on the fp16 matrix cores as three products of fp16 halves (device_math.hpp): the error is that
 //    of an f32 dot product, at v_mfma_f32_32x32x16_f16's rate (2 PFLOP/s sustained, 16x that of the f32 matrix
@@ -19,8 +19,9 @@
 //  * k_attn_few: head width 64, 1 to 16 queries over f32 images and i8 code images (2 to 16 over i16 code tiles):
 //    the four wavefronts of a workgroup split each key block, with the queries as the 16 columns of 16 x 16
 //    products, and merge their softmax states at the end.
-//  * k_attn_few4: head width 64 over i4 code tiles, up to where k_attn_split64's larger query tiles are quicker (plan4):
-//    eight wavefronts with key blocks of their own, tiles straight into registers, 16 or 32 queries a workgroup.
+//  * k_attn_few4: head width 64 over i4 code tiles, up to where k_attn_many4 is quicker (plan4): eight wavefronts with key
+//    blocks of their own, tiles straight into registers, 16 or 32 queries a workgroup.
+//  * k_attn_many4: the same from there: 256 queries a workgroup over operands widened into LDS.
 //  * k_attn_decode_w: head width 64 and few queries (or no images), from the records: 256 threads per (six key
 //    blocks, head, 8 queries), each wavefront streaming a key block at a time with no barrier (lane = key for the
 //    scores, lane = coordinate for the weighted sum), integer codes scaled through the query and the sums.
@@ -778,6 +779,13 @@ __device__ __forceinline__ void half_image_to_lds(const uint8_t *src, uint8_t *d
     }
 }
 
+// i16 staging (k_attn_split64 with STAGED): half a code tile (8 KB of codes and its 256 bytes of factors, keys or
+// values) into a staging slot's half by DMA: 528 copies of 16 bytes, the last 16 by wavefront 0.
+template <int WAVES>
+__device__ __forceinline__ void stage_half16(const uint8_t *src, uint8_t *dst, int tid) {
+    half_image_to_lds<WAVES, HALF16>(src, dst, tid);
+}
+
 // A staging slot's key codes into the split image kdst (K hi, K lo) and its value codes into vdst (V hi, V lo), either
 // null for none: the dequantised values (code times its coordinate's factor, in f32) split into fp16 halves, written
 // swizzled as the images are; each thread takes 16 bytes (8 codes) of a 128-byte row at a time.
@@ -808,31 +816,6 @@ __device__ __forceinline__ void convert16(const uint8_t *st, uint8_t *kdst, uint
     }
 }
 
-// The same for a 4-bit code tile (a halves' layout above k_kv_tiles4): the numbers as fp16, one plane each.
-template <int WAVES>
-__device__ __forceinline__ void convert4(const uint8_t *st, uint8_t *kdst, uint8_t *vdst, int tid) {
-#pragma unroll
-    for (int i = 0; i < 512 / (64 * WAVES); i++) {
-        const int u = tid + 64 * WAVES * i, r = u >> 3, c = u & 7;
-        const int off = r * 128 + swz(r, c) * 16;
-        if (kdst) {
-            // key r, coordinates 8 c .. 8 c + 7, each with its own step and offset
-            const halfx8 s = *reinterpret_cast<const halfx8 *>(st + 2048 + 16 * c);
-            const halfx8 z = *reinterpret_cast<const halfx8 *>(st + 2176 + 16 * c);
-            *reinterpret_cast<halfx8 *>(kdst + off) = values4(*reinterpret_cast<const uint32_t *>(st + key_at4(r, c)), s, z);
-        }
-        if (vdst) {
-            // coordinate r, keys 8 c .. 8 c + 7, one step and offset
-            const uint8_t *sv = st + HALF4;
-            const halfx2 f = *reinterpret_cast<const halfx2 *>(sv + 2048 + 16 * (r & 15) + 4 * (r >> 4));
-            const _Float16 s = f[0], z = f[1];
-            *reinterpret_cast<halfx8 *>(vdst + off) =
-                values4(*reinterpret_cast<const uint32_t *>(sv + value_at4(r, c)), halfx8{s, s, s, s, s, s, s, s},
-                        halfx8{z, z, z, z, z, z, z, z});
-        }
-    }
-}
-
 template <bool B>
 struct Flag {
     static constexpr bool value = B;
@@ -851,11 +834,6 @@ struct Flag {
 // in f32) and writes them split into the same LDS images as an f32 layer's, which the rest of the kernel reads
 // unchanged. In step kb the staging slot of its parity holds keys kb + 2 and values kb + 1 (converted then), and the
 // copies bring keys kb + 3 and values kb + 2 into the other.
-//
-// An i4 cache's code tiles (FOUR) go the same way, but what they stand for is exact in fp16: the LDS images have one
-// plane, as the i8 code images, and the products are two a term, with neither scales to follow nor a query to split again.
-// 2,048 queries over 10,000 rows 95 us: 883 TFLOP/s of fp16 products. The matrix units are busy 38% of the time; the widening
-// and the weights' exponentials and splits take the issue slots beside them.
 template <int WAVES, int FMT>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows, int chunk, int d, int heads,
                                                                const float *__restrict__ q,
@@ -865,12 +843,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
                                                                int qtiles, int splits, float *__restrict__ part_o,
                                                                float *__restrict__ part_ml, float *__restrict__ out) {
     constexpr bool CODES = FMT == TAH_KV_I8;    // fp16 code images, scales applied in the kernel
-    constexpr bool FOUR = FMT == TAH_KV_I4;     // 4-bit code tiles dequantised into fp16 images in the kernel
-    constexpr bool STAGED = FMT == TAH_KV_I16 || FOUR;  // code tiles dequantised into images in the kernel
-    constexpr bool SINGLE = CODES || FOUR;          // keys and values are one fp16 plane
-    constexpr int HB = SINGLE ? IMG8 / 2 : IMG / 2;  // bytes of an LDS image's keys (or values)
+    constexpr bool STAGED = FMT == TAH_KV_I16;  // int16 code tiles dequantised into split images in the kernel
+    constexpr int HB = CODES ? IMG8 / 2 : IMG / 2;  // bytes of an LDS image's keys (or values)
     constexpr int IS = img_bytes(FMT);              // bytes of a tile in memory
-    constexpr int SG = IS, SH = IS / 2;             // STAGED: a staging slot, a whole code tile; half of it
+    constexpr int SG = IMG16;                       // STAGED: a staging slot, a whole code tile
     __shared__ __align__(16) uint8_t kt[2][HB], vt[2][HB];
     __shared__ __align__(16) float sb[CODES ? 4 : 1][192];  // CODES: scale ring, [chunk % 4][key, value, ratio]
     // CODES: each lane's 32 query coordinates, kept for the per-chunk splits: [wavefront][8 chunks of 4][lane][4];
@@ -897,17 +873,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
                                              reinterpret_cast<uint8_t *>(&sb[ci & 3][0]), 16, 0, 0);
     };
     // STAGED: block kb's key codes and key factors into staging slot sl; its value codes and value factors
-    auto stage_keys = [&](int kb, int sl) {
-        half_image_to_lds<WAVES, SH>(head_images + kb * kb_stride, side + sl * SG, tid);
-    };
+    auto stage_keys = [&](int kb, int sl) { stage_half16<WAVES>(head_images + kb * kb_stride, side + sl * SG, tid); };
     auto stage_values = [&](int kb, int sl) {
-        half_image_to_lds<WAVES, SH>(head_images + kb * kb_stride + SH, side + sl * SG + SH, tid);
+        stage_half16<WAVES>(head_images + kb * kb_stride + HALF16, side + sl * SG + HALF16, tid);
     };
     auto convert = [&](int sl, int kdst, int vdst) {
-        const uint8_t *st = side + sl * SG;
-        uint8_t *kd = kdst >= 0 ? kt[kdst] : nullptr, *vd = vdst >= 0 ? vt[vdst] : nullptr;
-        if constexpr (FOUR) convert4<WAVES>(st, kd, vd, tid);
-        else convert16<WAVES>(st, kd, vd, tid);
+        convert16<WAVES>(side + sl * SG, kdst >= 0 ? kt[kdst] : nullptr, vdst >= 0 ? vt[vdst] : nullptr, tid);
     };
     if (kb0 < kb1) {
         if constexpr (STAGED) {
@@ -1074,7 +1045,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
                 const int r = 32 * kh + krow;
                 const int off = r * 128 + swz(r, 2 * dc + g) * 16;
                 khi[dc][kh] = *reinterpret_cast<const halfx8 *>(tile + off);
-                if constexpr (!SINGLE) klo[dc][kh] = *reinterpret_cast<const halfx8 *>(tile + 8192 + off);
+                if constexpr (!CODES) klo[dc][kh] = *reinterpret_cast<const halfx8 *>(tile + 8192 + off);
             }
 #pragma unroll
         for (int dc = 0; dc < 4; dc++)
@@ -1082,7 +1053,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
             for (int kh = 0; kh < 2; kh++) {
                 sc[kh] = mfma16(khi[dc][kh], qh[dc], dc == 0 ? zero : sc[kh]);
                 sc[kh] = mfma16(khi[dc][kh], ql[dc], sc[kh]);
-                if constexpr (!SINGLE) sc[kh] = mfma16(klo[dc][kh], qh[dc], sc[kh]);
+                if constexpr (!CODES) sc[kh] = mfma16(klo[dc][kh], qh[dc], sc[kh]);
             }
         return tl_q;
     };
@@ -1152,7 +1123,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
                     const int r = 32 * db + r32;
                     const int voff = r * 128 + swz(r, 4 * kh + 2 * hh + g) * 16;
                     const halfx8 vhi = *reinterpret_cast<const halfx8 *>(vtile + voff);
-                    if constexpr (SINGLE) {
+                    if constexpr (CODES) {
                         acc_o[db] = mfma16(vhi, ph[kh][hh], acc_o[db]);
                         acc_o[db] = mfma16(vhi, pl[kh][hh], acc_o[db]);
                     } else {
@@ -1163,7 +1134,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_split64(int nq, int rows
                     }
                 }
         l += ps;
-        if constexpr (NEXT && SINGLE) {
+        if constexpr (NEXT && CODES) {
             // one region: 8 key and 8 value operand reads, 16 + 16 products and the weights' VALU work
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
             __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
@@ -1834,7 +1805,7 @@ __global__ __launch_bounds__(64 * FEW4_WAVES, G == 1 ? 4 : 2) void k_attn_few4(i
     }
     if (splits == 1) {
         const float fo = unscale / L;
-        *reinterpret_cast<float4 *>(out + (size_t)oq * d + h * 64 + oc) = make_float4(o[0] * fo, o[1] * fo, o[2] * fo, o[3] * fo);
+    __shared__ __align__(16) uint8_t img[2][16384];  // the operands of a block's keys, then values; this and the next block's
     } else {
         const size_t at = ((size_t)split * nq + oq) * heads + h;
         *reinterpret_cast<float4 *>(part_o + at * 64 + oc) =
@@ -1843,6 +1814,184 @@ __global__ __launch_bounds__(64 * FEW4_WAVES, G == 1 ? 4 : 2) void k_attn_few4(i
             part_ml[at * 2] = m;
             part_ml[at * 2 + 1] = L;
         }
+    }
+}
+
+// ---- 4-bit code tiles, many queries: head width 64 ------------------------------------------------------------------------
+// A flat grid of heads x query tiles x key ranges (workgroup i: head i % heads, so that with 8 heads an XCD reads one head's
+// tiles); 1,024 threads: 16 wavefronts of 16 queries each over the same key blocks. Each wavefront widens one of a block's 16
+// operands (half of the wavefronts the keys', half the values', a word of eight codes a lane) into LDS in the order in which
+// the products read them, 1 KB each, no bank twice; the block after next is on its way in registers. One barrier a block.
+// The products and the softmax are k_attn_few4's.
+//
+// 2,048 queries over 10,000 rows 92 us, 912 TFLOP/s of fp16 products (a term is two), where a large fp16 matrix product of
+// the library reaches 1,100. Without the operands' LDS reads it would take 66 us, without the exponentials 86, the low halves'
+// products 74, the widening 82: none alone bounds it, their sum does, though four wavefronts share a SIMD. So the halves of
+// the wavefronts widen at different times (all together 93 us). Tried and slower: 32 queries a wavefront, half the LDS reads
+// and two wavefronts a SIMD (98); the next block's scores among this one's exponentials (98 to 101); a barrier every two or
+// four blocks (93 to 94); the sums of the weights as products with ones (95).
+constexpr int MANY4_WAVES = 16;
+__global__ __launch_bounds__(64 * MANY4_WAVES) void k_attn_many4(int nq, KeyBlocks kbs, int chunk, int heads,
+                                                                 const float *__restrict__ q,
+                                                                 const uint8_t *__restrict__ tiles,
+                                                                 const uint32_t *__restrict__ kvmax, int kb_per_split,
+                                                                 int qtiles, int splits, float *__restrict__ part_o,
+                                                                 float *__restrict__ part_ml, float *__restrict__ out) {
+    __shared__ __align__(16) uint8_t img[2][16384];  // a block's keys and its values as operands, this block's and the next's
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int qi = lane & 15, lg = lane >> 4, d = 64 * heads;
+    const int h = blockIdx.x % heads, rest = blockIdx.x / heads, split = rest / qtiles;
+    const int at = (rest % qtiles) * (16 * MANY4_WAVES) + 16 * wave + qi;
+    const int kb0 = split * kb_per_split, kb1 = min(kbs.n_kb, kb0 + kb_per_split);
+    const size_t kb_stride = (size_t)heads * IMG4;
+    const bool keys = wave < 8;
+    const int o = wave & 7;
+    const uint8_t *src = tiles + (size_t)h * IMG4 + (keys ? 0 : HALF4);
+    const int word_at = 1024 * (o >> 2) + 16 * lane + 4 * (o & 3);
+    const int factor_at = keys ? 2048 + 64 * (o & 1) + 16 * lg : 2048 + 16 * qi;
+    const int factor2_at = factor_at + (keys ? 128 : 0);
+    uint32_t word;
+    u32x4 fa, fb;  // keys: the steps and the offsets of the word's coordinates; values: (step, offset) of four coordinates
+    auto fetch = [&](int kb) {
+        const uint8_t *t = src + (size_t)kb * kb_stride;
+        word = *reinterpret_cast<const uint32_t *>(t + word_at);
+        fa = *reinterpret_cast<const u32x4 *>(t + factor_at);
+        fb = *reinterpret_cast<const u32x4 *>(t + factor2_at);
+    };
+    const int to = (keys ? 0 : 8192) + 1024 * o + 16 * lane;
+    auto widen = [&](int buf) {
+        halfx8 s, z;
+        if (keys) {
+            s = __builtin_bit_cast(halfx8, fa);
+            z = __builtin_bit_cast(halfx8, fb);
+        } else {
+            const uint32_t f01 = o & 1 ? fa[1] : fa[0], f23 = o & 1 ? fa[3] : fa[2], f = o & 2 ? f23 : f01;
+            const halfx2 sz = __builtin_bit_cast(halfx2, f);
+            const _Float16 s1 = sz[0], z1 = sz[1];
+            s = halfx8{s1, s1, s1, s1, s1, s1, s1, s1};
+            z = halfx8{z1, z1, z1, z1, z1, z1, z1, z1};
+        }
+        *reinterpret_cast<halfx8 *>(img[buf] + to) = values4(word, s, z);
+    };
+    fetch(kb0);
+    halfx8 qh[2], ql[2];
+    float to_log2;
+    {
+        const float *from = q + (size_t)min(at, nq - 1) * d + h * 64 + 8 * lg;
+        float qv[2][8], qmax = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            load8(from + 32 * ks, qv[ks]);
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+                qv[ks][t] = at < nq ? qv[ks][t] : 0.0f;
+                qmax = fmaxf(qmax, fabsf(qv[ks][t]));
+            }
+        }
+        qmax = max32(max16(qmax));
+        const int eq = shift_for_max(qmax);
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) split8(qv[ks], ldexpf(1.0f, eq), qh[ks], ql[ks]);
+        to_log2 = ldexpf(LOG2E, -(shift_for(kvmax[h * 2]) + eq));
+    }
+    widen(0);
+    if (kb0 + 1 < kb1) fetch(kb0 + 1);
+    int in_chunk = kb0 % kbs.bpc, ci = kb0 / kbs.bpc, buf = 0;
+    // the next block's operand, and the loads of the one after
+    auto ahead = [&](int kb) {
+        if (kb + 1 >= kb1) return;
+        widen(buf ^ 1);
+        if (kb + 2 < kb1) fetch(kb + 2);
+    };
+    float ref = -INFINITY, l = 0.0f;
+    const floatx4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+    floatx4 acc[4] = {none, none, none, none};
+    for (int kb = kb0; kb < kb1; kb++) {
+        __syncthreads();
+        if (keys) ahead(kb);
+        const uint8_t *im = img[buf] + 16 * lane;
+        const int nk = min(KB, (ci == kbs.n_chunks - 1 ? kbs.last_rc : chunk) - in_chunk * KB);
+        floatx4 a[4];
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            halfx8 kv[4];
+#pragma unroll
+            for (int sp = 0; sp < 4; sp++) {
+                kv[sp] = *reinterpret_cast<const halfx8 *>(im + 1024 * (2 * sp + ks));
+                a[sp] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[sp], qh[ks], ks ? a[sp] : none, 0, 0, 0);
+            }
+#pragma unroll
+            for (int sp = 0; sp < 4; sp++) a[sp] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv[sp], ql[ks], a[sp], 0, 0, 0);
+        }
+        if (!keys) ahead(kb);
+        float sc[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) sc[j] = a[j >> 2][j & 3];
+        if (nk < KB) {
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (32 * (j >> 3) + 8 * lg + (j & 7) >= nk) sc[j] = -INFINITY;
+        }
+        float mb = sc[0];
+#pragma unroll
+        for (int j = 1; j < 16; j++) mb = fmaxf(mb, sc[j]);
+        mb = max32(max16(mb)) * to_log2;
+        const bool grow = mb > ref + 3.0f;
+        if (__any(grow)) {
+            const float nref = grow ? mb : ref;
+            const float alpha = exp2_hw(ref - nref);
+            l *= alpha;
+#pragma unroll
+            for (int m = 0; m < 4; m++) acc[m] *= alpha;
+            ref = nref;
+        }
+        const float off = 12.0f - ref;
+        halfx8 ph[2], pl[2];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            u32x4 hw, lw;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const float p0 = exp2_hw(fmaf(sc[8 * s + 2 * t], to_log2, off));
+                const float p1 = exp2_hw(fmaf(sc[8 * s + 2 * t + 1], to_log2, off));
+                l += p0 + p1;
+                uint32_t hi, lo;
+                split2(p0, p1, hi, lo);
+                hw[t] = hi;
+                lw[t] = lo;
+            }
+            ph[s] = __builtin_bit_cast(halfx8, hw);
+            pl[s] = __builtin_bit_cast(halfx8, lw);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            halfx8 v[4];
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                v[m] = *reinterpret_cast<const halfx8 *>(im + 8192 + 1024 * (4 * s + m));
+                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[m], ph[s], acc[m], 0, 0, 0);
+            }
+#pragma unroll
+            for (int m = 0; m < 4; m++) acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[m], pl[s], acc[m], 0, 0, 0);
+        }
+        buf ^= 1;
+        if (++in_chunk == kbs.bpc) {
+            in_chunk = 0;
+            ci++;
+        }
+    }
+    l = sum32(sum16(l));
+    if (at >= nq) return;
+    const float unscale = ldexpf(1.0f, -shift_for(kvmax[h * 2 + 1]));
+    const float f = splits == 1 ? unscale / l : unscale;
+    const size_t pair = splits == 1 ? (size_t)at * heads + h : ((size_t)split * nq + at) * heads + h;
+    float *dst = (splits == 1 ? out : part_o) + pair * 64 + 4 * lg;
+#pragma unroll
+    for (int m = 0; m < 4; m++)
+        *reinterpret_cast<float4 *>(dst + 16 * m) = make_float4(acc[m][0] * f, acc[m][1] * f, acc[m][2] * f, acc[m][3] * f);
+    if (splits > 1 && lg == 0) {
+        part_ml[pair * 2] = ref;
+        part_ml[pair * 2 + 1] = l;
     }
 }
 
@@ -2074,9 +2223,9 @@ KvImages kv_images_at(uint8_t *base, int rows, int chunk, int heads, int kv_form
 
 // 4-bit tiles: which kernel, and into how many ranges the keys go. Both run in rounds of one workgroup a compute unit; a
 // range count is worth looking at where it fills a whole number of rounds. A round of k_attn_few4 takes 2.5 us a block of
-// its eight wavefronts' turns and one and a half more, the merge of ranges as much again; one of k_attn_split64 2 us a
-// block and eight and a half more (queries x rows, 8 heads, by the one and the other: 512 x 10,000 32 and 42 us, 600 x 2,000
-// 15 and 21, 1,024 x 10,000 52 and 56, 1,536 x 10,000 106 and 76, 2,048 x 2,000 29 and 34, 2,048 x 10,000 107 and 95).
+// its eight wavefronts' turns and one and a half more, the merge of ranges as much again; one of k_attn_many4 1.83 us a block
+// and eight and a half more (queries x rows, 8 heads, by the one and the other: 512 x 10,000 32 and 35 us, 600 x 10,000 48 and
+// 43, 800 x 10,000 52 and 50, 1,300 x 10,000 88 and 71, 2,048 x 2,000 29 and 32, 2,048 x 10,000 105 and 92).
 static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
     auto ranges = [&](int per, int least_blocks, auto cost_of, float &cost) {
         int best = 1;
@@ -2105,7 +2254,8 @@ static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
                         few_cost);
     if (a.nq > 128) {
         const int tiles = (a.nq + 255) / 256;
-        const int s = ranges(a.heads * tiles, 2, [](int rounds, int blocks, bool) { return 2.0f * rounds * (blocks + 8.5f); }, many_cost);
+        const int s = ranges(a.heads * tiles, 2,
+                             [](int rounds, int blocks, bool) { return 1.83f * rounds * (blocks + 8.5f); }, many_cost);
         if (many_cost < few_cost) {
             p.few = false;
             p.split16 = true;
@@ -2212,8 +2362,8 @@ static void launch_split(hipStream_t s, const AttnShape &a, const AttnPlan &p, c
 }
 
 // ---- launch probe ---------------------------------------------------------------------------------------------------
-// While armed for a stream, each launch of the many-query kernel (k_attn_split64) on it is bracketed by a pair of HIP
-// events, up to the armed number of launches; probe_read sums their elapsed times. One probe per process.
+// While armed for a stream, each launch of the many-query kernels (k_attn_split64, k_attn_many4) on it is bracketed by a
+// pair of HIP events, up to the armed number of launches; probe_read sums their elapsed times. One probe per process.
 namespace {
 std::mutex probe_mu;
 std::atomic<bool> probe_on{false};
@@ -2323,7 +2473,10 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
                 else launch_split<4, TAH_KV_I16>(s, a, p, q, *img, out, part_o, part_ml);
                 break;
             case TAH_KV_I4:
-                launch_split<8, TAH_KV_I4>(s, a, p, q, *img, out, part_o, part_ml);
+                hipLaunchKernelGGL(k_attn_many4, dim3(p.groups * a.heads * p.splits), dim3(64 * MANY4_WAVES), 0, s, a.nq,
+                                   key_blocks(a.rows, a.chunk), a.chunk, a.heads, q, img->images, img->kvmax, p.kb_per_split,
+                                   p.groups, p.splits, part_o, part_ml, out);
+                TAH_LAUNCHED();
                 break;
             default:
                 if (p.waves == 8) launch_split<8, TAH_KV_I8>(s, a, p, q, *img, out, part_o, part_ml);
