@@ -1805,7 +1805,7 @@ __global__ __launch_bounds__(64 * FEW4_WAVES, G == 1 ? 4 : 2) void k_attn_few4(i
     }
     if (splits == 1) {
         const float fo = unscale / L;
-    __shared__ __align__(16) uint8_t img[2][16384];  // the operands of a block's keys, then values; this and the next block's
+        *reinterpret_cast<float4 *>(out + (size_t)oq * d + h * 64 + oc) = make_float4(o[0] * fo, o[1] * fo, o[2] * fo, o[3] * fo);
     } else {
         const size_t at = ((size_t)split * nq + oq) * heads + h;
         *reinterpret_cast<float4 *>(part_o + at * 64 + oc) =
@@ -1837,7 +1837,7 @@ __global__ __launch_bounds__(64 * MANY4_WAVES) void k_attn_many4(int nq, KeyBloc
                                                                  const uint32_t *__restrict__ kvmax, int kb_per_split,
                                                                  int qtiles, int splits, float *__restrict__ part_o,
                                                                  float *__restrict__ part_ml, float *__restrict__ out) {
-    __shared__ __align__(16) uint8_t img[2][16384];  // a block's keys and its values as operands, this block's and the next's
+    __shared__ __align__(16) uint8_t img[2][16384];  // the operands of a block's keys, then values; this and the next block's
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qi = lane & 15, lg = lane >> 4, d = 64 * heads;
     const int h = blockIdx.x % heads, rest = blockIdx.x / heads, split = rest / qtiles;
