@@ -318,8 +318,8 @@ int tah_quantile_stats_dev(tah_dev *dev, const float *q_dev, int32_t rows, int32
  * with TAH_E_ARG. No counterpart in the reference, which stops at the probabilities. */
 int tah_class_stats(tah_dev *dev, const float *scores, int32_t rows, int32_t n, float temperature,
                     const int32_t *given, int32_t n_given, int32_t top, float *stats, int32_t *ids);
-/* The same with every array in device memory, and rows of scores ld floats apart (0: n); queued on the handle's stream.
- * The given ids are not looked at beforehand: one outside [0, n) gives NaN. */
+/* The same with every array in device memory (4-byte aligned), and rows of scores ld floats apart (0: n); queued on the
+ * handle's stream. The given ids are not looked at beforehand: one outside [0, n) gives NaN. */
 int tah_class_stats_dev(tah_dev *dev, const float *scores_dev, int32_t rows, int32_t n, int64_t ld, float temperature,
                         const int32_t *given_dev, int32_t n_given, int32_t top, float *stats_dev, int32_t *ids_dev);
 

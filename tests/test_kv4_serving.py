@@ -120,6 +120,9 @@ def test_a_held_problem(gpu):
     assert np.array_equal(a, gpu.predict(w, vm, xt, 3)) and np.all(np.isfinite(a))
     sizes = [hip.VramModel.model_bytes(w, fmt, 500, 100) for fmt in (abi.KV_F32, abi.KV_I16, abi.KV_I8, abi.KV_I4)]
     assert sizes == sorted(sizes, reverse=True)
+    up = lambda n: -(-n // 256) * 256
+    blocks = 5 * 2  # of 64 keys, chunks of 100 rows
+    assert sizes[-1] == 2 * (up(blocks * 8 * 4608) + 256) + up(2 * m.d * 4)  # a layer's tiles and its heads' maxima; the scales
     vm.free()
     w.free()
 
