@@ -492,10 +492,11 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
     if (segs > 1 && tid >= end - base && tid < o.top) reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[tid] = 0;
 }
 
-// grid rows; 512 threads: the segments of a row joined; segs (at most 64) lists of top falling keys, in LDS. With j =
-// ceil(top / segs), the ceil(top / j)-th largest of the lists' j-th entries is a bound that top keys reach; what reaches it
-// is placed by counting (all of it, 960 keys of one row, took 25 us of LDS reads).
-constexpr int JOIN_LIST = 512;
+// grid rows; 512 threads: the segments of a row joined; segs (at most 64) lists of top falling keys, in LDS, placed by
+// counting the larger ones: up to 192 all of them (64 x 30,000 with 20 best 13.1 us, 14.6 by a bound), else those that reach a
+// bound: with j = ceil(top / segs), the ceil(top / j)-th largest of the lists' j-th entries, which top keys reach (all 960 keys
+// of one row took 25 us of LDS reads).
+constexpr int JOIN_LIST = 512, JOIN_ALL = 192;
 __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, const float *__restrict__ x, float inv, int segs,
                                                           const uint8_t *__restrict__ state, ClassOut o) {
     extern __shared__ uint64_t all[];
@@ -516,28 +517,31 @@ __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, cons
     write_row(says, o, row, n, x + row * ld, inv, tid);
     if (o.top == 0) return;
     __syncthreads();
-    const int j = (o.top + segs - 1) / segs, need = (o.top + j - 1) / j;
-    // lanes past the lists count as reaching any bound
-    const uint32_t entry = lane < segs ? (uint32_t)(all[lane * o.top + j - 1] >> 32) : 0xFFFFFFFFu;
-    const uint32_t bound = bound_of(entry, 0xFFFFFFFFu, wave_max_u32(lane < segs ? entry : 0u), need + 64 + 64 - segs);
-    for (int i = tid; i < total; i += 512) {
-        const uint64_t key = all[i];
-        if (key && (uint32_t)(key >> 32) >= bound) {
-            const int at = atomicAdd(&listed, 1);
-            if (at < JOIN_LIST) list[at] = key;
+    const bool all_of_them = total <= JOIN_ALL;
+    if (!all_of_them) {
+        const int j = (o.top + segs - 1) / segs, need = (o.top + j - 1) / j;
+        // lanes past the lists count as reaching any bound
+        const uint32_t entry = lane < segs ? (uint32_t)(all[lane * o.top + j - 1] >> 32) : 0xFFFFFFFFu;
+        const uint32_t bound = bound_of(entry, 0xFFFFFFFFu, wave_max_u32(lane < segs ? entry : 0u), need + 64 + 64 - segs);
+        for (int i = tid; i < total; i += 512) {
+            const uint64_t key = all[i];
+            if (key && (uint32_t)(key >> 32) >= bound) {
+                const int at = atomicAdd(&listed, 1);
+                if (at < JOIN_LIST) list[at] = key;
+            }
         }
+        __syncthreads();
     }
-    __syncthreads();
-    const int got = listed;
-    const bool few = got <= JOIN_LIST;  // else equal scores without end
-    const uint64_t *keys = few ? list : all;
+    const int got = all_of_them ? total : listed;
+    const bool few = all_of_them || got <= JOIN_LIST;  // else equal scores without end
+    const uint64_t *keys = few && !all_of_them ? list : all;
     for (int i = tid; i < (few ? got : total); i += 512) {
         const uint64_t key = keys[i];
         if (!key) continue;
         int place = 0;
         if (few) {
 #pragma unroll 8
-            for (int u = 0; u < got; u++) place += list[u] > key;
+            for (int u = 0; u < got; u++) place += keys[u] > key;
         } else {
             place = place_of(key, all, segs, o.top);
         }
