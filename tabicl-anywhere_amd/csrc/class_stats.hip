@@ -254,11 +254,12 @@ __device__ __forceinline__ uint64_t wave_top_each(const float (&v)[E], int live,
     return got;
 }
 
-// The largest key that at least top of the lanes' keys (two a lane) reach, or a little less: halved between the least and
-// the largest of them (hi).
+// The largest key that at least top of the lanes' keys (two a lane) reach, or a little less: halved ten times between the
+// least and the largest of them (hi). 14 times are a finer bound and take longer (3,000 x 1,001 with ten best 7.9 us for 7.6,
+// 1,000 x 5,000 with five 14.2 for 13.5), eight let too many past where the keys span zero (8.7 and 13.1).
 __device__ __forceinline__ uint32_t bound_of(uint32_t key, uint32_t other, uint32_t hi, int top) {
     uint32_t lo = ~wave_max_u32(~min(key, other));
-    for (int i = 0; i < 14 && lo < hi; i++) {
+    for (int i = 0; i < 10 && lo < hi; i++) {
         const uint32_t mid = hi - (hi - lo) / 2;
         if (__popcll(__ballot(key >= mid)) + __popcll(__ballot(other >= mid)) >= top) lo = mid;
         else hi = mid - 1;
@@ -269,7 +270,7 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t key, uint32_t other, uint3
 // The same sooner. A bound that top lanes' own largest scores reach, and few more (bound_of): top scores reach it, so nothing
 // below it is among the top. What reaches it goes into a list in LDS, whose entries are placed by counting the larger ones.
 // Where that does not serve (too many equal scores, or rising ones in few lanes; a bound of -inf; NaN among the top) the keys
-// are taken one by one (3,000 x 1,001 with ten best: 15.2 us for all rows so, 7.9 by the bound).
+// are taken one by one (3,000 x 1,001 with ten best: 15.2 us for all rows so, 7.6 by the bound).
 constexpr int LIST = 256;
 template <int E, class Id>
 __device__ __forceinline__ uint64_t wave_top(const float (&v)[E], const ClassDist &c, int live, int top, int lane,
@@ -493,7 +494,7 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
 }
 
 // grid rows; 512 threads: the segments of a row joined; segs (at most 64) lists of top falling keys, in LDS, placed by
-// counting the larger ones: up to 192 all of them (64 x 30,000 with 20 best 13.1 us, 14.6 by a bound), else those that reach a
+// counting the larger ones: up to 192 all of them (64 x 30,000 with 20 best 12.8 us, 14.1 by a bound), else those that reach a
 // bound: with j = ceil(top / segs), the ceil(top / j)-th largest of the lists' j-th entries, which top keys reach (all 960 keys
 // of one row took 25 us of LDS reads).
 constexpr int JOIN_LIST = 512, JOIN_ALL = 192;
