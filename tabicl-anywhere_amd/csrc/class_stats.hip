@@ -494,7 +494,7 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
 }
 
 // grid rows; 512 threads: the segments of a row joined; segs (at most 64) lists of top falling keys, in LDS, placed by
-// counting the larger ones: up to 192 all of them (64 x 30,000 with 20 best 12.8 us, 14.1 by a bound), else those that reach a
+// counting the larger ones: up to 192 all of them (64 x 30,000 with 20 best 14.6 us by a bound, 13.1 so), else those that reach a
 // bound: with j = ceil(top / segs), the ceil(top / j)-th largest of the lists' j-th entries, which top keys reach (all 960 keys
 // of one row took 25 us of LDS reads).
 constexpr int JOIN_LIST = 512, JOIN_ALL = 192;

@@ -57,7 +57,8 @@ def class_report(sums: np.ndarray, members: int, temperature: float, labels=None
     """What `finish_proba`'s distributions say, in logarithms: per row of the summed scores the entropy (nats), the log
     probability of the row's label (`labels`, class ids or -1 for none: NaN) and the `top` most probable classes with
     theirs. Returns a dict of float64 "entropy" [n], "log_p" [n] (with labels), "top_log_p" [n][top] and int32 "top"
-    [n][top]. With a card (`hip.Gpu`) the rows are read there, the sums as float32 (`tah_class_stats`)."""
+    [n][top]. With a card (`hip.Gpu`) the rows are read there, the sums as float32 (`tah_class_stats`: up to 2^20 classes,
+    64 of the most probable)."""
     sums = np.asarray(sums, np.float64)
     n, classes = sums.shape
     if not 0 <= top <= classes:
