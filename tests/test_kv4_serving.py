@@ -127,6 +127,31 @@ def test_a_held_problem(gpu):
     w.free()
 
 
+def test_a_class_tree(gpu):
+    """More classes than the network tells apart: every problem of the tree in 4 bits, each its f32 self of the values that
+    its records stand for."""
+    m = network(2)
+    w = gpu.weights(m)
+    rng = np.random.default_rng(6)
+    x = rng.standard_normal((900, 4)).astype(np.float32)
+    y = (np.arange(900) % 25).astype(np.float32)
+    f = fit.fit_raw(gpu, w, x, y, 25, chunk=101, kv_format=abi.KV_I4)
+    c = C.Cache.open(B.Bundle(f.write()))
+    vms = c.load(gpu, w)
+    assert len(vms) > 1
+    h = (rng.standard_normal((30, m.d)) * 0.5).astype(np.float32)
+    for i, vm in enumerate(vms):
+        plain = [gpu.unpack(r, m.d, vm.rows, vm.chunk, abi.KV_I4).view(np.uint8) for r in c.layers(i, m.icl_layers)]
+        vp = gpu.load(w, abi.KV_F32, vm.rows, vm.chunk, plain, c.scales(i))
+        for n in (1, 30):
+            a, b = gpu.in_context(w, vm, h[:n], 10), gpu.in_context(w, vp, h[:n], 10)
+            say(f"  problem {i}, {vm.rows} rows, {n} queries: worst {np.abs(a - b).max():.2e}")
+            assert np.all(np.isfinite(a)) and np.abs(a - b).max() < 5e-5
+        vp.free()
+        vm.free()
+    w.free()
+
+
 @pytest.mark.parametrize("rows,chunk,calls", [(2000, 256, (256, 4)), (2000, 256, (3, 1)), (40000, 256, (256, 16)), (333, 100, (200, 17))])
 def test_stage_without_allocating(gpu, rows, chunk, calls):
     say(f"stage without allocating over i4: {rows} rows, calls of {calls}")
