@@ -82,7 +82,8 @@ def class_report(sums: np.ndarray, members: int, temperature: float, labels=None
     logp = u - np.log(np.where(total > 0, total, 1.0))
     logp[~(peak[:, 0] < np.inf)] = np.nan
     ent = -np.sum(np.where(e > 0, e * np.where(e > 0, logp, 0.0), 0.0), axis=1) / np.maximum(total[:, 0], 1.0)
-    ids = np.argsort(np.where(np.isnan(sums), np.inf, -sums), axis=1, kind="stable")[:, :top].astype(np.int32)
+    nan = np.isnan(sums)  # after every number, -inf too
+    ids = np.lexsort((np.where(nan, 0.0, -sums), nan), axis=1)[:, :top].astype(np.int32)
     out = {"entropy": np.where(peak[:, 0] < np.inf, ent, np.nan), "top": ids,
            "top_log_p": np.take_along_axis(logp, ids.astype(np.int64), 1)}
     if labels is not None:

@@ -1,0 +1,50 @@
+"""Class scores read as distributions where rows are unusual: a NaN beside classes ruled out, classes all but certain."""
+import numpy as np
+import pytest
+
+from conftest import pkg
+
+hip, T = pkg("hip"), pkg("table")
+
+
+def order(row):
+    """Class ids in order: larger scores first, the lower id among equals, NaN after every number."""
+    return sorted(range(len(row)), key=lambda i: (np.isnan(row[i]), 0.0 if np.isnan(row[i]) else -row[i], i))
+
+
+def unusual_rows(rng, rows, n):
+    """Scores with both a NaN and a class ruled out, at different places: numbers beside them, or nothing else."""
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    x[rng.random((rows, n)) < 0.4] = -np.inf
+    x[rng.random((rows, n)) < 0.3] = np.nan
+    x[0, ::2], x[0, 1::2] = np.nan, -np.inf
+    x[1, ::2], x[1, 1::2] = -np.inf, np.nan
+    return x
+
+
+# ---- without a card ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n", [2, 3, 11])
+def test_the_host_orders_nan_after_every_number(n):
+    assert T.class_report([[np.nan, -np.inf, 1.0]], 1, 1.0, top=3)["top"].tolist() == [[2, 1, 0]]
+    x = unusual_rows(np.random.default_rng(n), 40, n)
+    assert T.class_report(x, 1, 1.0, top=n)["top"].tolist() == [order(row) for row in x]
+
+
+# ---- the card ------------------------------------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def gpu():
+    g = hip.Gpu(0)
+    yield g
+    g.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,top", [(3, 3), (10, 10), (50, 50), (100, 8), (200, 64), (1000, 64), (2000, 64), (20000, 64)])
+def test_the_card_orders_nan_after_every_number(gpu, n, top):
+    print(f"order of rows with NaN and -inf: {n} classes, {top} best", flush=True)
+    x = unusual_rows(np.random.default_rng(n), 9, n)
+    x[2, : n - top // 2 - 1] = np.nan  # fewer numbers than are wanted
+    x[3] = np.nan
+    st, ids = gpu.class_stats(x, None, top)
+    assert np.all(np.isnan(st[np.isnan(x).any(1)]))
+    assert ids.tolist() == [order(row)[:top] for row in x]
