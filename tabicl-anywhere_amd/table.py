@@ -78,10 +78,12 @@ def class_report(sums: np.ndarray, members: int, temperature: float, labels=None
     with np.errstate(invalid="ignore"):  # inf - inf: a row that has no distribution
         u = (sums - np.where(peak == -np.inf, 0.0, peak)) / (members * temperature)
     e = np.exp(u)
-    total = e.sum(axis=1, keepdims=True)
-    logp = u - np.log(np.where(total > 0, total, 1.0))
+    # the sum without the largest score's own 1, so that a certain row's logarithms keep their precision
+    rest = np.where(np.arange(classes) == sums.argmax(axis=1)[:, None], 0.0, e).sum(axis=1, keepdims=True)
+    logs = np.log1p(rest)
+    logp = u - logs
     logp[~(peak[:, 0] < np.inf)] = np.nan
-    ent = -np.sum(np.where(e > 0, e * np.where(e > 0, logp, 0.0), 0.0), axis=1) / np.maximum(total[:, 0], 1.0)
+    ent = (logs + np.sum(np.where(e > 0, e * np.where(e > 0, -u, 0.0), 0.0), axis=1, keepdims=True) / (1.0 + rest))[:, 0]
     nan = np.isnan(sums)  # after every number, -inf too
     ids = np.lexsort((np.where(nan, 0.0, -sums), nan), axis=1)[:, :top].astype(np.int32)
     out = {"entropy": np.where(peak[:, 0] < np.inf, ent, np.nan), "top": ids,

@@ -30,6 +30,20 @@ def test_the_host_orders_nan_after_every_number(n):
     assert T.class_report(x, 1, 1.0, top=n)["top"].tolist() == [order(row) for row in x]
 
 
+def test_the_host_keeps_a_certain_rows_precision():
+    """One class far ahead: log p of it is minus the others' weight, although 1 and that weight round to 1. float64's
+    roundings are 2^-53 each: the exponents' (of at most 80, so 2^-53 * 80 of a weight) and a few more."""
+    x = np.zeros((41, 10))
+    x[:, 3] = np.arange(41) * 2.0
+    rep = T.class_report(x, 1, 1.0, np.full(41, 3), 2)
+    rest = 9 * np.exp(-x[:, 3])
+    log_p, entropy = -np.log1p(rest), np.log1p(rest) + rest * x[:, 3] / (1 + rest)
+    for got, want in ((rep["log_p"], log_p), (rep["top_log_p"][1:, 0], log_p[1:]), (rep["entropy"], entropy)):
+        assert np.all(np.abs(got - want) <= 100 * 2.0 ** -53 * np.abs(want))
+    pair = T.class_report([[0.0, 50.0]], 1, 1.0, [1])
+    assert abs(pair["log_p"][0] + np.exp(-50.0)) <= 60 * 2.0 ** -53 * np.exp(-50.0)
+
+
 # ---- the card ------------------------------------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def gpu():
