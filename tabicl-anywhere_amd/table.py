@@ -61,6 +61,8 @@ def class_report(sums: np.ndarray, members: int, temperature: float, labels=None
     64 of the most probable)."""
     sums = np.asarray(sums, np.float64)
     n, classes = sums.shape
+    if not 0.0 < members * temperature < np.inf:
+        raise ValueError("class_report: members times temperature has to be positive")
     if not 0 <= top <= classes:
         raise ValueError(f"class_report: top must be from 0 to {classes}")
     if labels is not None:

@@ -44,6 +44,12 @@ def test_the_host_keeps_a_certain_rows_precision():
     assert abs(pair["log_p"][0] + np.exp(-50.0)) <= 60 * 2.0 ** -53 * np.exp(-50.0)
 
 
+@pytest.mark.parametrize("members,temperature", [(1, 0.0), (0, 0.9), (2, -1.0), (1, np.nan), (1, np.inf)])
+def test_the_host_refuses_what_is_no_temperature(members, temperature):
+    with pytest.raises(ValueError):
+        T.class_report(np.zeros((2, 3)), members, temperature, [0, 1], 1)
+
+
 # ---- the card ------------------------------------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def gpu():
