@@ -152,7 +152,7 @@ namespace tah {
 
 // ---- stored chunk records (include/tah.h) -------------------------------------------------------------------------
 constexpr int GROUP4 = 64;  // i4: rows that share a step and an offset
-__host__ __device__ inline int groups4(int rc) { return (rc + GROUP4 - 1) / GROUP4; }
+__host__ __device__ inline int groups4(int rc) { return (int)(((unsigned)rc + GROUP4 - 1) / GROUP4); }  // rc up to 2^31 - 1
 
 // bytes of one chunk of rc rows
 __host__ __device__ inline size_t record_bytes(int fmt, int d, int rc) {
