@@ -58,10 +58,11 @@ struct KeyBlocks {
 
 __host__ __device__ inline KeyBlocks key_blocks(int rows, int chunk) {
     KeyBlocks k;
-    k.bpc = (chunk + KB - 1) / KB;
-    k.n_chunks = (rows + chunk - 1) / chunk;
+    // rows and chunk from 1 to 2^31 - 1: no sum of the two
+    k.bpc = (chunk - 1) / KB + 1;
+    k.n_chunks = (rows - 1) / chunk + 1;
     k.last_rc = rows - (k.n_chunks - 1) * chunk;
-    k.n_kb = (k.n_chunks - 1) * k.bpc + (k.last_rc + KB - 1) / KB;
+    k.n_kb = (k.n_chunks - 1) * k.bpc + (k.last_rc - 1) / KB + 1;
     return k;
 }
 

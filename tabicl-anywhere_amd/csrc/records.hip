@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void k_to_records(int rows, int d2, int chunk,
         tile[i][tx] = (m < rows && n < d2) ? kv[(size_t)m * d2 + n] : 0.0f;
     }
     __syncthreads();
-    const int n_chunks = (rows + chunk - 1) / chunk;
+    const int n_chunks = (rows - 1) / chunk + 1;
     const int last_rc = rows - (n_chunks - 1) * chunk;
     for (int j = ty; j < 64; j += 4) {
         const int n = n0 + j, m = m0 + tx;
