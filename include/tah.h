@@ -200,7 +200,8 @@ int tah_predict_rows_dev(tah_dev *dev, const tah_weights *w, const tah_model *mo
 /* ---- fitting: the fit::Attend hooks (src/fit.rs:45-74) ---------------------------------------------------------
  *
  * tah_pack: one stored chunk from its f32 keys and values c ([2d][rc]: the d key rows then the d value rows) to the
- * record of format kv_format, quantised on the card exactly as the reference's pack (src/fit.rs:549-576). */
+ * record of format kv_format, quantised on the card exactly as the reference's pack (src/fit.rs:549-576). Here and in
+ * the calls below a chunk has at most 2^31 - 1024 rows (a chunk longer than the table counts as the table). */
 int tah_pack(tah_dev *dev, const float *c, int32_t d, int32_t rc, int32_t kv_format, uint8_t *out);
 /* A whole layer's records from its f32 keys and values in chunk layout (2 * rows * d floats), both on the card, as the
  * fit forms them; the pointers 4-byte aligned. */

@@ -835,10 +835,16 @@ extern "C" int tah_stage_dev_noalloc(tah_dev *dev, const tah_weights *w, const t
 }
 
 // ---- fitting ---------------------------------------------------------------------------------------------------
+// The kernels number a chunk's rows in an int, up to a workgroup's stride past the last.
+static void check_chunk_rows(const char *what, int rc) {
+    if (rc > 0x7FFFFFFF - 1023) throw ArgError{std::string(what) + ": at most 2^31 - 1024 rows a chunk"};
+}
+
 extern "C" int tah_pack(tah_dev *dev, const float *c, int32_t d, int32_t rc, int32_t kv_format, uint8_t *out) {
     if (!c || !out) return TAH_E_ARG;
     return guarded(dev, [&] {
         if (d <= 0 || rc <= 0 || !kv_known(kv_format)) throw ArgError{"pack: bad size or format"};
+        check_chunk_rows("pack", rc);
         Loans loans(dev);
         const size_t n = 2 * (size_t)d * rc, bytes = tah_kv_record(kv_format, d, rc);
         float *cd = loans.take<float>(n);
@@ -856,6 +862,7 @@ extern "C" int tah_pack(tah_dev *dev, const float *c, int32_t d, int32_t rc, int
 
 static void check_layer(const char *what, int d, int rows, int chunk, int kv_format, const void *a, const void *b) {
     if (d <= 0 || rows < 0 || chunk <= 0 || !kv_known(kv_format)) throw ArgError{std::string(what) + ": bad size or format"};
+    check_chunk_rows(what, std::min(chunk, rows));
     // the kernels number a chunk's fours of rows, and i16 and i8 packing its coordinates in a grid's second dimension
     if ((std::min(chunk, std::max(rows, 1)) + 3L) / 4 * 2 * d > 0x7FFFFFFF - 1024 || d > 131070)
         throw ArgError{std::string(what) + ": a chunk of more numbers than a call takes"};
