@@ -139,7 +139,8 @@ void tah_weights_free(tah_weights *w);
  * layer_records[l] points at layer l's bytes (tah_kv_record summed over its chunks); scales is n{j}_scale,
  * [layers][d]. A layer of head width 64 is held once, as the tiles the card makes of its records (f32: split-fp16
  * images; i16: the codes with their dequantisation factors; i8: the codes as fp16 with the scales; i4: the codes with
- * their steps and offsets as fp16), which every attention kernel reads; other head widths keep the records.
+ * their steps and offsets as fp16), which every attention kernel reads; other head widths keep the records. i4 records may
+ * be another's than tah_pack's: any finite steps and offsets (one that is not makes no number of its head).
  * tah_model_bytes (like Gpu::model_bytes, from the weights' shape) counts what the layers are held as, and the scales; 0
  * without weights. */
 size_t tah_model_bytes(const tah_weights *w, int32_t kv_format, int32_t rows, int32_t chunk);

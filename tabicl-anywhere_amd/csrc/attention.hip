@@ -168,7 +168,8 @@ constexpr int IMG16 = 2 * HALF16;
 
 // i4 caches: code tiles, 4.5 KB per (key block, head): the codes of the block's keys (2 KB) and their 64 steps and 64
 // offsets, then the same of its values, the steps and offsets as fp16 times the head's power of two (2^sk, 2^sv: from the
-// largest |K| and |V| the records stand for, kvmax, as for f32 images; exact down to 2^-28 of it). value = offset + step
+// largest |K| and |V| the records stand for, kvmax, as for f32 images; exact down to 2^-28 of it; records whose steps and
+// offsets are far larger than what they stand for: k_kv_absmax, k_kv_tiles4). value = offset + step
 // code in fp16 is then one fused multiply-add with one rounding to eleven bits, what the record stands for.
 // The codes are in the order in which a wavefront reads them as operands of 16 x 16 x 32 products (k_attn_few4): two
 // kilobytes for 32 keys each, 16 bytes a lane, a word of eight codes an operand:
@@ -545,6 +546,19 @@ __global__ __launch_bounds__(256) void k_kv_absmax(int rows, int chunk, int d, i
         mk = fmaxf(mk, fabsf(tk[i]));
         mv = fmaxf(mv, fabsf(tv[i]));
     }
+    if constexpr (FMT == TAH_KV_I4) {
+        // half an offset counts too, so that offsets fit the tiles' fp16 as values do (of packing's own none is larger: they lie
+        // among their group's values). Not where the step is over twice the group's largest value: all its codes are then
+        // the same, and k_kv_tiles4 can hold that one value
+        auto with_offset = [&](float m, int j) {
+            m = fmaxf(m, dpp<0xb1>(m));  // the coordinate's four lanes
+            m = fmaxf(m, dpp<0x4e>(m));
+            const Step4 st = step_at4(w.rec, w.rc, j, w.o / KB);
+            return fabsf(st.s) > 2.0f * m ? m : fmaxf(m, 0.5f * fabsf(st.z));
+        };
+        mk = with_offset(mk, h * 64 + lc);
+        mv = with_offset(mv, d + h * 64 + lc);
+    }
     mk = wave_max(mk);
     mv = wave_max(mv);
     if ((tid & 63) == 0) {
@@ -715,8 +729,15 @@ __global__ __launch_bounds__(256) void k_kv_tiles4(int rows, int chunk, int d, i
     }
     if (tid < 128) {
         const int c = tid & 63, which = tid >> 6, e = shift_for(kvmax[h * 2 + which]);
-        const Step4 st = step_at4(w.rec, w.rc, which * d + h * 64 + c, w.o / KB);
-        const _Float16 s = (_Float16)ldexpf(st.s, e), z = (_Float16)ldexpf(st.z, e);
+        const int j = which * d + h * 64 + c;
+        const Step4 st = step_at4(w.rec, w.rc, j, w.o / KB);
+        float sf = ldexpf(st.s, e), zf = ldexpf(st.z, e);
+        if (fmaxf(fabsf(sf), fabsf(zf)) >= 0x1p15f) {
+            // a group of one code (k_kv_absmax): its value, without a step
+            sf = 0.0f;
+            zf = ldexpf(record_value4(w.rec, d, w.rc, j, w.o), e);
+        }
+        const _Float16 s = (_Float16)sf, z = (_Float16)zf;
         _Float16 *f = reinterpret_cast<_Float16 *>(tile + which * HALF4 + 2048);
         if (which == 0) {
             f[c] = s;
