@@ -316,7 +316,8 @@ int tah_quantile_stats_dev(tah_dev *dev, const float *q_dev, int32_t rows, int32
  * then NULL). Writes stats [rows][1 + n_given + top]: the entropy in nats, log p of each given class, log p of the top
  * most probable ones, falling; and ids [rows][top], those classes (the lower id first among equal scores, NaN after
  * every number). A score of -inf is a class ruled out; a row of nothing else has entropy 0 and every log p -inf. A row
- * with a NaN or +inf has NaN for all of them. A given id of -1 means none: its log p is NaN. Ids outside [-1, n) fail
+ * with a NaN or +inf has NaN for all of them. Scores may be as far apart as floats are; a log p past float's range is
+ * -inf. A given id of -1 means none: its log p is NaN. Ids outside [-1, n) fail
  * with TAH_E_ARG. No counterpart in the reference, which stops at the probabilities. */
 int tah_class_stats(tah_dev *dev, const float *scores, int32_t rows, int32_t n, float temperature,
                     const int32_t *given, int32_t n_given, int32_t top, float *stats, int32_t *ids);

@@ -27,19 +27,35 @@ struct ClassDist {
 // e^x for x <= 0 on the hardware's exp2 (1 ulp; x log2 e rounded: 2^-24 of it in the exponent)
 __device__ __forceinline__ float exp_below(float x) { return exp2_hw(x * LOG2E); }
 
-__device__ __forceinline__ ClassDist join(ClassDist a, ClassDist b, float inv) {
+// (x - m) / T as (part x - part m) inv: at temperatures over 1 the halves' difference, which is finite for all finite scores
+// (elsewhere a difference past float's largest has a quotient past it too). Scaling by 2 is exact: no result changes.
+struct ClassScale {
+    float part, inv;
+    explicit ClassScale(float temperature) : part(temperature > 1.0f ? 0.5f : 1.0f), inv(1.0f / temperature / part) {}
+    __device__ __forceinline__ float below(float x, float m) const { return fmaf(part, x, -(part * m)) * inv; }
+    // a row's scores, where that is the kernel's time: f(part, inv), in halves only where m is large enough for them to matter
+    // (below 2^100, float's least less m rounds to float's least; in halves always 64 x 100,000 18.8 -> 19.2 us; up to 256
+    // classes the choice itself takes longer, 200,000 x 7 5.76 -> 5.83)
+    template <class F>
+    __device__ __forceinline__ void over(float m, F &&f) const {
+        if (m < 0x1p100f) f(1.0f, part * inv);
+        else f(part, inv);
+    }
+};
+
+__device__ __forceinline__ ClassDist join(ClassDist a, ClassDist b, ClassScale by) {
     const bool swap = b.m > a.m;
     const float m = swap ? b.m : a.m, m2 = swap ? a.m : b.m;
     const float s1 = swap ? b.s : a.s, t1 = swap ? b.t : a.t, s2 = (swap ? a.s : b.s) + 1.0f, t2 = swap ? a.t : b.t;
-    const float g = (m - m2) * inv, f = exp_below(-g);
+    const float g = by.below(m, m2), f = exp_below(-g);
     // nothing but -inf in the lesser part, or too far below to count (g times 0 would be NaN where g is infinite)
     const bool none = m2 == -INFINITY || f == 0.0f;
     return {m, none ? s1 : fmaf(f, s2, s1), none ? t1 : fmaf(f, fmaf(g, s2, t2), t1), a.bad || b.bad};
 }
 
-__device__ __forceinline__ ClassDist join_lane(ClassDist a, int mask, float inv) {
+__device__ __forceinline__ ClassDist join_lane(ClassDist a, int mask, ClassScale by) {
     const ClassDist b{__shfl_xor(a.m, mask), __shfl_xor(a.s, mask), __shfl_xor(a.t, mask), (bool)__shfl_xor((int)a.bad, mask)};
-    return join(a, b, inv);
+    return join(a, b, by);
 }
 
 // a score as a number that orders as the scores do: a NaN 1, and 0 is left for none
@@ -75,7 +91,7 @@ struct ClassLogs {
         }
         if (c.bad || !(c.m < INFINITY)) entropy = logs = NAN;
     }
-    __device__ __forceinline__ float log_p(float x, float inv) const { return (x - from) * inv - logs; }
+    __device__ __forceinline__ float log_p(float x, ClassScale by) const { return by.below(x, from) - logs; }
 };
 
 // ---- up to 256 classes: one to 32 lanes a row ----------------------------------------------------------------------------
@@ -105,8 +121,8 @@ __device__ __forceinline__ T row_lanes(T v, F &&f) {
 // a wavefront or a workgroup a row spent most of its own on reductions (200,000 x 7: 664 us a workgroup a row). The most
 // probable classes by one scan of the keys each. Instructions bound it: 100,000 x 50 with five best 14.6 us, 1.4 TB/s.
 template <int N, int L>
-__global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t ld, const float *__restrict__ x, float inv,
-                                                         ClassOut o) {
+__global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t ld, const float *__restrict__ x,
+                                                         ClassScale by, ClassOut o) {
     constexpr int R = 64 / L, E = N / L;
     const int part = threadIdx.x % L;
     const size_t row = (size_t)blockIdx.x * R + threadIdx.x / L;
@@ -132,11 +148,11 @@ __global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t
     c.m = row_lanes<L>(c.m, [](float a, float b) { return fmaxf(a, b); });
     c.bad = row_lanes<L>(bad, [](int a, int b) { return a | b; }) != 0;
     // in units of log 2; the largest scores' terms are exactly 1 and are counted apart. From 2^-200 down a term is 0
-    const float inv2 = inv * LOG2E;
+    const float inv2 = by.inv * LOG2E, pm = by.part * c.m;
     int tops = 0;
 #pragma unroll
     for (int i = 0; i < E; i++) {
-        const float u = fmaxf((v[i] - c.m) * inv2, -200.0f);
+        const float u = fmaxf(fmaf(by.part, v[i], -pm) * inv2, -200.0f);
         const bool is_top = v[i] == c.m;
         const float w = is_top ? 0.0f : exp2_hw(u);
         tops += is_top;
@@ -151,7 +167,7 @@ __global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t
     if (part == 0) st[0] = says.entropy;
     for (int i = part; i < o.n_given; i += L) {
         const int id = o.given[row * o.n_given + i];
-        st[1 + i] = id >= 0 && id < n ? says.log_p(mine[id], inv) : NAN;
+        st[1 + i] = id >= 0 && id < n ? says.log_p(mine[id], by) : NAN;
     }
     for (int r = 0; r < o.top; r++) {
         uint32_t best = 0;
@@ -167,7 +183,7 @@ __global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t
 #pragma unroll
         for (int i = 0; i < E; i++) k[i] = L * i + part == id ? 0u : k[i];
         if (r % L == part) {
-            st[1 + o.n_given + r] = says.log_p(score_of(most), inv);
+            st[1 + o.n_given + r] = says.log_p(score_of(most), by);
             o.ids[row * o.top + r] = id;
         }
     }
@@ -195,7 +211,7 @@ __device__ __forceinline__ uint64_t wave_best(uint64_t key) {
 
 // The distribution of a wavefront's scores v (E a lane, -inf past the last), in every lane.
 template <int E>
-__device__ __forceinline__ ClassDist wave_dist(const float (&v)[E], float inv) {
+__device__ __forceinline__ ClassDist wave_dist(const float (&v)[E], ClassScale by) {
     float own = -INFINITY;
     bool bad = false;
 #pragma unroll
@@ -206,18 +222,20 @@ __device__ __forceinline__ ClassDist wave_dist(const float (&v)[E], float inv) {
     ClassDist c{wave_max(own), 0.0f, 0.0f, __any(bad) != 0};
     if (c.m == -INFINITY) return c;
     // in units of log 2; the terms of the largest score are exactly 1 and are counted apart. From 2^-200 down a term is 0
-    const float inv2 = inv * LOG2E;
     int tops = 0;
     float s = 0.0f, t = 0.0f;
+    by.over(c.m, [&](float part, float inv) {
+        const float inv2 = inv * LOG2E, pm = part * c.m;
 #pragma unroll
-    for (int r = 0; r < E; r++) {
-        const float u = fmaxf((v[r] - c.m) * inv2, -200.0f), e = exp2_hw(u);
-        const bool is_top = v[r] == c.m;
-        tops += __popcll(__ballot(is_top));
-        const float w = is_top ? 0.0f : e;
-        s += w;
-        t = fmaf(-w, u, t);
-    }
+        for (int r = 0; r < E; r++) {
+            const float u = fmaxf(fmaf(part, v[r], -pm) * inv2, -200.0f), e = exp2_hw(u);
+            const bool is_top = v[r] == c.m;
+            tops += __popcll(__ballot(is_top));
+            const float w = is_top ? 0.0f : e;
+            s += w;
+            t = fmaf(-w, u, t);
+        }
+    });
     c.s = wave_sum(s) + (float)(tops - 1);
     c.t = wave_sum(t) * LN2;
     return c;
@@ -323,8 +341,8 @@ __device__ __forceinline__ uint64_t wave_top(const float (&v)[E], const ClassDis
 // ---- up to 1,024 classes, many of them wanted: a wavefront a row ------------------------------------------------------------------------------
 // grid ceil(rows / 4); 256 threads. Entry r of a lane is class 64 r + lane: the row is read once, in whole lines, and kept.
 template <int E>
-__global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_t ld, const float *__restrict__ x, float inv,
-                                                          ClassOut o) {
+__global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_t ld, const float *__restrict__ x,
+                                                          ClassScale by, ClassOut o) {
     __shared__ uint64_t list[4][LIST];
     const int lane = threadIdx.x & 63;
     const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -333,19 +351,19 @@ __global__ __launch_bounds__(256) void k_class_stats_wave(int rows, int n, size_
     float v[E];
 #pragma unroll
     for (int r = 0; r < E; r++) v[r] = 64 * r + lane < n ? src[64 * r + lane] : -INFINITY;
-    const ClassDist c = wave_dist(v, inv);
+    const ClassDist c = wave_dist(v, by);
     float *st = o.stats + row * (1 + o.n_given + o.top);
     const ClassLogs says(c);
     if (lane == 0) st[0] = says.entropy;
     if (lane < o.n_given) {
         const int id = o.given[row * o.n_given + lane];
-        st[1 + lane] = id >= 0 && id < n ? says.log_p(src[id], inv) : NAN;
+        st[1 + lane] = id >= 0 && id < n ? says.log_p(src[id], by) : NAN;
     }
     if (o.top == 0) return;
     const uint64_t key = wave_top(v, c, (n - lane + 63) / 64, o.top, lane, list[threadIdx.x >> 6],
                                   [&](int r) { return 64 * r + lane; });
     if (lane < o.top) {
-        st[1 + o.n_given + lane] = says.log_p(score_of((uint32_t)(key >> 32)), inv);
+        st[1 + o.n_given + lane] = says.log_p(score_of((uint32_t)(key >> 32)), by);
         o.ids[row * o.top + lane] = class_of(key);
     }
 }
@@ -360,12 +378,12 @@ constexpr int SEG_T = 512, SEG = 32 * SEG_T, SEG_LIST = 1024;
 __host__ __device__ inline size_t seg_bytes(int top) { return sizeof(SegState) + 8 * (size_t)top; }
 
 __device__ __forceinline__ void write_row(const ClassLogs &says, const ClassOut &o, size_t row, int n, const float *src,
-                                          float inv, int tid) {
+                                          ClassScale by, int tid) {
     float *st = o.stats + row * (1 + o.n_given + o.top);
     if (tid == 0) st[0] = says.entropy;
     if (tid < o.n_given) {
         const int id = o.given[row * o.n_given + tid];
-        st[1 + tid] = id >= 0 && id < n ? says.log_p(src[id], inv) : NAN;
+        st[1 + tid] = id >= 0 && id < n ? says.log_p(src[id], by) : NAN;
     }
 }
 
@@ -391,7 +409,7 @@ __device__ __forceinline__ int place_of(uint64_t key, const uint64_t *keys, int 
 // 22 us for 18). Loads and arithmetic hardly overlap, since all workgroups start together.
 template <int E>
 __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_t ld, const float *__restrict__ x,
-                                                           float inv, uint8_t *__restrict__ state, ClassOut o) {
+                                                           ClassScale by, uint8_t *__restrict__ state, ClassOut o) {
     constexpr int W = SEG_T / 64;
     __shared__ ClassDist part[W];
     __shared__ float group[SEG_T / 4];
@@ -428,20 +446,20 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
         own = fmaxf(own, dpp<0x4e>(own));   // 2 apart
         if ((lane & 3) == 0) group[tid >> 2] = own;
     }
-    const ClassDist w = wave_dist(v, inv);
+    const ClassDist w = wave_dist(v, by);
     if (lane == 0) part[wave] = w;
     __syncthreads();
     ClassDist c = part[0];
 #pragma unroll
-    for (int i = 1; i < W; i++) c = join(c, part[i], inv);
+    for (int i = 1; i < W; i++) c = join(c, part[i], by);
     uint8_t *mine = state + (row * segs + seg) * seg_bytes(o.top);
     const ClassLogs says(c);
-    if (segs == 1) write_row(says, o, row, n, src, inv, tid);
+    if (segs == 1) write_row(says, o, row, n, src, by, tid);
     else if (tid == 0) reinterpret_cast<SegState *>(mine)->c = c;
     if (o.top == 0) return;
     auto put = [&](uint64_t key, int place) {
         if (segs == 1) {
-            o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = says.log_p(score_of((uint32_t)(key >> 32)), inv);
+            o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = says.log_p(score_of((uint32_t)(key >> 32)), by);
             o.ids[row * o.top + place] = class_of(key);
         } else {
             reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[place] = key;
@@ -498,8 +516,8 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
 // bound: with j = ceil(top / segs), the ceil(top / j)-th largest of the lists' j-th entries, which top keys reach (all 960 keys
 // of one row took 25 us of LDS reads).
 constexpr int JOIN_LIST = 512, JOIN_ALL = 192;
-__global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, const float *__restrict__ x, float inv, int segs,
-                                                          const uint8_t *__restrict__ state, ClassOut o) {
+__global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, const float *__restrict__ x, ClassScale by,
+                                                          int segs, const uint8_t *__restrict__ state, ClassOut o) {
     extern __shared__ uint64_t all[];
     __shared__ uint64_t list[JOIN_LIST];
     __shared__ int listed;
@@ -513,9 +531,9 @@ __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, cons
     }
     ClassDist c{-INFINITY, 0.0f, 0.0f, false};
     if (lane < segs) c = reinterpret_cast<const SegState *>(rows_state + lane * seg_bytes(o.top))->c;
-    for (int mask = 1; mask < 64; mask <<= 1) c = join_lane(c, mask, inv);
+    for (int mask = 1; mask < 64; mask <<= 1) c = join_lane(c, mask, by);
     const ClassLogs says(c);
-    write_row(says, o, row, n, x + row * ld, inv, tid);
+    write_row(says, o, row, n, x + row * ld, by, tid);
     if (o.top == 0) return;
     __syncthreads();
     const bool all_of_them = total <= JOIN_ALL;
@@ -547,7 +565,7 @@ __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, cons
             place = place_of(key, all, segs, o.top);
         }
         if (place < o.top) {
-            o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = says.log_p(score_of((uint32_t)(key >> 32)), inv);
+            o.stats[row * (1 + o.n_given + o.top) + 1 + o.n_given + place] = says.log_p(score_of((uint32_t)(key >> 32)), by);
             o.ids[row * o.top + place] = class_of(key);
         }
     }
@@ -576,54 +594,54 @@ size_t class_stats_work_bytes(int rows, int n, int top) {
 }
 
 template <int N, int L>
-static void launch_rows(hipStream_t s, int rows, int n, size_t ld, const float *x, float inv, const ClassOut &o) {
+static void launch_rows(hipStream_t s, int rows, int n, size_t ld, const float *x, ClassScale by, const ClassOut &o) {
     constexpr int R = 64 / L, MOST = 1 << 26;  // rows a launch: a grid holds fewer than 2^32 threads
     for (int r0 = 0; r0 < rows; r0 += std::min(MOST, rows - r0)) {
         const int here = std::min(MOST, rows - r0);
         hipLaunchKernelGGL(HIP_KERNEL_NAME(k_class_stats_rows<N, L>), dim3((here + R - 1) / R), dim3(64), 0, s, here, n, ld,
-                           x + r0 * ld, inv, o.from(r0));
+                           x + r0 * ld, by, o.from(r0));
     }
 }
 template <int E>
-static void launch_wave(hipStream_t s, int rows, int n, size_t ld, const float *x, float inv, const ClassOut &o) {
+static void launch_wave(hipStream_t s, int rows, int n, size_t ld, const float *x, ClassScale by, const ClassOut &o) {
     constexpr int MOST = 1 << 24;  // rows a launch: a grid holds fewer than 2^32 threads
     for (int r0 = 0; r0 < rows; r0 += std::min(MOST, rows - r0)) {
         const int here = std::min(MOST, rows - r0);
-        hipLaunchKernelGGL(k_class_stats_wave<E>, dim3((here + 3) / 4), dim3(256), 0, s, here, n, ld, x + r0 * ld, inv,
+        hipLaunchKernelGGL(k_class_stats_wave<E>, dim3((here + 3) / 4), dim3(256), 0, s, here, n, ld, x + r0 * ld, by,
                            o.from(r0));
     }
 }
 
 // the fewest scores a thread that hold a segment (1,000 x 2,000 by 32 a thread 17.8 us, by 8 10.8;
 // 1,000 x 5,000 by 32 18.7, by 16 14.1)
-static void launch_seg(hipStream_t s, int segs, int rows, int n, int len, size_t ld, const float *x, float inv, uint8_t *state,
-                       const ClassOut &o) {
+static void launch_seg(hipStream_t s, int segs, int rows, int n, int len, size_t ld, const float *x, ClassScale by,
+                       uint8_t *state, const ClassOut &o) {
     const dim3 grid(segs, rows), block(SEG_T);
-    if (len <= 8 * SEG_T) hipLaunchKernelGGL(k_class_stats_seg<8>, grid, block, 0, s, n, len, ld, x, inv, state, o);
-    else if (len <= 16 * SEG_T) hipLaunchKernelGGL(k_class_stats_seg<16>, grid, block, 0, s, n, len, ld, x, inv, state, o);
-    else hipLaunchKernelGGL(k_class_stats_seg<32>, grid, block, 0, s, n, len, ld, x, inv, state, o);
+    if (len <= 8 * SEG_T) hipLaunchKernelGGL(k_class_stats_seg<8>, grid, block, 0, s, n, len, ld, x, by, state, o);
+    else if (len <= 16 * SEG_T) hipLaunchKernelGGL(k_class_stats_seg<16>, grid, block, 0, s, n, len, ld, x, by, state, o);
+    else hipLaunchKernelGGL(k_class_stats_seg<32>, grid, block, 0, s, n, len, ld, x, by, state, o);
 }
 
 // work: class_stats_work_bytes(rows, n, top) bytes.
 void class_stats(hipStream_t s, int rows, int n, size_t ld, const float *x, float temperature, const int32_t *given,
                  int n_given, int top, float *stats, int32_t *ids, void *work) {
     if (rows <= 0) return;
-    const float inv = 1.0f / temperature;
+    const ClassScale by(temperature);
     ClassOut o{given, n_given, top, stats, ids};
     // Eight scores a lane (sixteen: 1,000 x 50 4.0 -> 5.1 us, 100,000 x 50 14.6 -> 15.0; four: 200,000 x 7 5.8 -> 6.7, 100,000 x
     // 20 8.9 -> 11.3), up to 256 classes while few of them are wanted one by one (20,000 x 100, a wavefront a row against this:
     // five best 15.5 -> 7.7 us, 20 best 16.9 and 16.1; 20,000 x 200: 17.2 -> 12.9, 18.7 and 29.2; 200 x 100, 20 best 4.7 and
     // 7.2). Else a wavefront a row, the fewest entries a lane that hold it.
-    if (n <= 8) launch_rows<8, 1>(s, rows, n, ld, x, inv, o);
-    else if (n <= 16) launch_rows<16, 2>(s, rows, n, ld, x, inv, o);
-    else if (n <= 32) launch_rows<32, 4>(s, rows, n, ld, x, inv, o);
-    else if (n <= 64) launch_rows<64, 8>(s, rows, n, ld, x, inv, o);
-    else if (n <= 128 && top <= 8) launch_rows<128, 16>(s, rows, n, ld, x, inv, o);
-    else if (n <= 256 && top <= 8) launch_rows<256, 32>(s, rows, n, ld, x, inv, o);
-    else if (n <= 128) launch_wave<2>(s, rows, n, ld, x, inv, o);
-    else if (n <= 256) launch_wave<4>(s, rows, n, ld, x, inv, o);
-    else if (n <= 512) launch_wave<8>(s, rows, n, ld, x, inv, o);
-    else if (n <= 1024) launch_wave<16>(s, rows, n, ld, x, inv, o);
+    if (n <= 8) launch_rows<8, 1>(s, rows, n, ld, x, by, o);
+    else if (n <= 16) launch_rows<16, 2>(s, rows, n, ld, x, by, o);
+    else if (n <= 32) launch_rows<32, 4>(s, rows, n, ld, x, by, o);
+    else if (n <= 64) launch_rows<64, 8>(s, rows, n, ld, x, by, o);
+    else if (n <= 128 && top <= 8) launch_rows<128, 16>(s, rows, n, ld, x, by, o);
+    else if (n <= 256 && top <= 8) launch_rows<256, 32>(s, rows, n, ld, x, by, o);
+    else if (n <= 128) launch_wave<2>(s, rows, n, ld, x, by, o);
+    else if (n <= 256) launch_wave<4>(s, rows, n, ld, x, by, o);
+    else if (n <= 512) launch_wave<8>(s, rows, n, ld, x, by, o);
+    else if (n <= 1024) launch_wave<16>(s, rows, n, ld, x, by, o);
     else {
         const ClassCut c = cut(n, top);
         const int segs = c.segs;
@@ -631,9 +649,9 @@ void class_stats(hipStream_t s, int rows, int n, size_t ld, const float *x, floa
             const int here = std::min(c.rows, rows - r0);
             const float *xr = x + r0 * ld;
             const ClassOut at = o.from(r0);
-            launch_seg(s, segs, here, n, c.len, ld, xr, inv, static_cast<uint8_t *>(work), at);
+            launch_seg(s, segs, here, n, c.len, ld, xr, by, static_cast<uint8_t *>(work), at);
             if (segs > 1)
-                hipLaunchKernelGGL(k_class_stats_join, dim3(here), dim3(512), (size_t)segs * top * 8, s, n, ld, xr, inv, segs,
+                hipLaunchKernelGGL(k_class_stats_join, dim3(here), dim3(512), (size_t)segs * top * 8, s, n, ld, xr, by, segs,
                                    static_cast<const uint8_t *>(work), at);
         }
     }

@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+import test_class_stats as S
 from conftest import pkg
 
 hip, T = pkg("hip"), pkg("table")
@@ -68,3 +69,28 @@ def test_the_card_orders_nan_after_every_number(gpu, n, top):
     st, ids = gpu.class_stats(x, None, top)
     assert np.all(np.isnan(st[np.isnan(x).any(1)]))
     assert ids.tolist() == [order(row)[:top] for row in x]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [0.9, 1.0, 2.5, 100.0, 1e38])
+@pytest.mark.parametrize("n,top", [(2, 2), (7, 3), (50, 5), (100, 8), (200, 20), (1000, 10), (2000, 10), (40000, 10)])
+def test_scores_further_apart_than_a_float_holds(gpu, n, top, temperature):
+    """Finite scores whose difference passes float32's largest: at a high temperature the quotient does not. What does is
+    -inf, as it rounds."""
+    print(f"scores far apart: {n} classes, temperature {temperature}", flush=True)
+    rng = np.random.default_rng(n)
+    x = (rng.uniform(-1, 1, (6, n)) * 3.4e38).astype(np.float32)
+    x[0, 0], x[0, 1] = 3.4e38, -3.4e38
+    x[1] = -np.finfo(np.float32).max  # masks of the lowest value, one row of nothing else
+    x[2, ::2] = -np.finfo(np.float32).max
+    x[2, 1::2] = rng.standard_normal(n // 2)
+    given = np.stack([np.zeros(6, int), np.full(6, n - 1), rng.integers(0, n, 6)], 1)
+    st, ids = gpu.class_stats(x, given, top, temperature)
+    inv = np.float64(np.float32(1.0) / np.float32(temperature))
+    want, wids = S.plain(x, given, top, 1.0 / inv)
+    with np.errstate(over="ignore"):
+        beyond = np.isinf(want.astype(np.float32))
+    assert np.array_equal(ids, wids)
+    assert np.array_equal(np.isinf(st), beyond) and np.all(st[beyond] < 0)
+    ok = ~beyond
+    assert np.all(np.abs(st[ok] - want[ok]) <= S.bound(want[ok], x, temperature))
