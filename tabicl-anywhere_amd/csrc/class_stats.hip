@@ -507,8 +507,6 @@ __global__ __launch_bounds__(SEG_T) void k_class_stats_seg(int n, int len, size_
         const int place = k ? place_of(k, list, W, o.top) : o.top;
         if (place < o.top) put(k, place);
     }
-    // a last segment of fewer classes than top: nothing in the places past them
-    if (segs > 1 && tid >= end - base && tid < o.top) reinterpret_cast<uint64_t *>(mine + sizeof(SegState))[tid] = 0;
 }
 
 // grid rows; 512 threads: the segments of a row joined; segs (at most 64) lists of top falling keys, in LDS, placed by
@@ -544,7 +542,7 @@ __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, cons
         const uint32_t bound = bound_of(entry, 0xFFFFFFFFu, wave_max_u32(lane < segs ? entry : 0u), need + 64 + 64 - segs);
         for (int i = tid; i < total; i += 512) {
             const uint64_t key = all[i];
-            if (key && (uint32_t)(key >> 32) >= bound) {
+            if ((uint32_t)(key >> 32) >= bound) {
                 const int at = atomicAdd(&listed, 1);
                 if (at < JOIN_LIST) list[at] = key;
             }
@@ -556,7 +554,6 @@ __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, cons
     const uint64_t *keys = few && !all_of_them ? list : all;
     for (int i = tid; i < (few ? got : total); i += 512) {
         const uint64_t key = keys[i];
-        if (!key) continue;
         int place = 0;
         if (few) {
 #pragma unroll 8
@@ -574,7 +571,9 @@ __global__ __launch_bounds__(512) void k_class_stats_join(int n, size_t ld, cons
 // Rows of more than 1,024 classes: how they are cut. As few segments as registers hold them in: more of them, to fill whole
 // rounds of the compute units, gave the join more to do than they saved (1 x 100,000 with 20 best in 7 and in 48 segments 14.0
 // and 14.8 us, 64 x 16,384 in 1 and in 4 8.9 and 14.9, 64 x 100,000 in 7 and in 8 alike). Rows at a time whose segments'
-// states fit 32 MB (and a launch's grid).
+// states fit 32 MB (and a launch's grid). Every segment has the top classes that it hands over: the last one has n / segs
+// less 4 (segs - 1) of them or more.
+static_assert(SEG / 2 - 4 * ((1 << 20) / SEG - 1) >= 64, "a last segment of 2^20 classes or fewer has 64");
 struct ClassCut {
     int segs, len, rows;
 };
