@@ -1618,17 +1618,20 @@ __global__ __launch_bounds__(256, 1) void k_attn_few(int nq, int rows, int chunk
 // ---- 4-bit code tiles straight into registers: head width 64 -------------------------------------------------------------
 // grid (heads, key ranges, groups of 16 G queries); 512 threads. Each wavefront takes key blocks of its own (kb0 + w,
 // kb0 + w + 8, ..): a tile is 4.5 KB in the order of its operands, so a block is nine 16-byte loads a lane straight into
-// registers, and there is no LDS and no barrier until the eight softmax states are merged. The products are 16 x 16 x 32 with
+// registers (as compiled the keys' six, and the values' three once the scores' products are under way), and there is no LDS and
+// no barrier until the eight softmax states are merged. The products are 16 x 16 x 32 with
 // the queries as columns: S = K Q^T (two for each of four sets of 16 keys and two halves of the coordinates, a group), O^T +=
 // V^T P^T by as many, the four accumulators in turn so that none waits for its own last product. The order of the keys within
 // a tile leaves a lane's eight scores of each 32 keys as the operand that the values' product takes. What fp16 holds of a key
 // or value is exact, so a term is two products (query or weight high and low), for f32's error.
 //
-// Few queries: one over 100,000 rows of 8 heads (57.6 MB of tiles) takes 17.8 us with the merge, 3.2 TB/s, where a wavefront's
-// turn of one block (350 vector instructions, 208 of them widening codes, and 32 products) is twice its loads' time; the next
-// block's loads issued ahead of it change nothing there and hold registers (16 over 50,000 rows 13.6 -> 12.9 us without). Over
-// 1,000 rows 6.8 us, one range. Many: widening is repeated by every workgroup, so two groups share it (G 2 from 17 queries:
-// 100 over 5,003 rows of 4 heads 11.0 us), until a tile of 256 queries wins.
+// Few queries: one over 100,000 rows of 8 heads (57.6 MB of tiles) takes 17.8 us with the merge. Of the kernel's 16.2 us the
+// bytes are 10.5 at a large copy's rate and the vector instructions 9.2 (350 a block, 208 of them widening codes, and 32
+// products): two wavefronts a SIMD overlap the two only in part, a wavefront at waits 45% of its time. The next block's loads
+// issued ahead of it hold registers and made it no shorter (16 over 50,000 rows 12.9 -> 13.6 us with them). Over 1,000 rows
+// 6.7 us, one range: two turns a wavefront, each waiting for the queries, the keys, the values and the maxima in turn. Many:
+// widening is repeated by every workgroup, so two sets of 16 queries share it (G 2 from 17 queries: 100 over 5,003 rows of 4
+// heads 10.9 us), until a tile of 256 queries wins.
 constexpr int FEW4_WAVES = 8;
 template <int G>
 __global__ __launch_bounds__(64 * FEW4_WAVES, G == 1 ? 4 : 2) void k_attn_few4(int nq, KeyBlocks kbs, int chunk,
@@ -1847,11 +1850,14 @@ __global__ __launch_bounds__(64 * FEW4_WAVES, G == 1 ? 4 : 2) void k_attn_few4(i
 // The products and the softmax are k_attn_few4's.
 //
 // 2,048 queries over 10,000 rows 92 us, 912 TFLOP/s of fp16 products (a term is two), where a large fp16 matrix product of
-// the library reaches 1,100. Without the operands' LDS reads it would take 66 us, without the exponentials 86, the low halves'
+// the library reaches 1,100 and the matrix units alone 1,650 on such operands: they are busy 39% of the cycles, vector
+// instructions issue in 58%. Without the operands' LDS reads it would take 66 us, without the exponentials 86, the low halves'
 // products 74, the widening 82: none alone bounds it, their sum does, though four wavefronts share a SIMD. So the halves of
 // the wavefronts widen at different times (all together 93 us). Tried and slower: 32 queries a wavefront, half the LDS reads
 // and two wavefronts a SIMD (98); the next block's scores among this one's exponentials (98 to 101); a barrier every two or
-// four blocks (93 to 94); the sums of the weights as products with ones (95).
+// four blocks (93 to 94); the sums of the weights as products with ones (95); k_attn_split64 over codes widened as they are
+// staged (95 to 97); a block's scores, the last one's weights and the values of the one before in one step (104 to 122, most of
+// them spilling); two halves of the wavefronts half a step apart, one multiplying while the other widens (105).
 constexpr int MANY4_WAVES = 16;
 __global__ __launch_bounds__(64 * MANY4_WAVES) void k_attn_many4(int nq, KeyBlocks kbs, int chunk, int heads,
                                                                  const float *__restrict__ q,
@@ -2178,8 +2184,9 @@ __global__ __launch_bounds__(256) void k_attn_merge_few(int items, int splits, c
 
 // ---- planning and launch --------------------------------------------------------------------------------------
 struct AttnPlan {
-    bool split16, few;  // few: k_attn_few (any tiles, at most FEW_Q queries; i16 from FEW16_FROM), i4: k_attn_few4<waves>
+    bool split16, few;  // few: k_attn_few (any tiles, at most FEW_Q queries; i16 from FEW16_FROM), i4: k_attn_few4<sets>
     int splits, kb_per_split, groups, waves;
+    int sets;  // i4: sets of 16 queries a workgroup of k_attn_few4
 };
 
 bool kv_images_apply(int kv_format, int d, int heads) {
@@ -2246,8 +2253,12 @@ KvImages kv_images_at(uint8_t *base, int rows, int chunk, int heads, int kv_form
 // 4-bit tiles: which kernel, and into how many ranges the keys go. Both run in rounds of one workgroup a compute unit; a
 // range count is worth looking at where it fills a whole number of rounds. A round of k_attn_few4 takes 2.5 us a block of
 // its eight wavefronts' turns and one and a half more, the merge of ranges as much again; one of k_attn_many4 1.83 us a block
-// and eight and a half more (queries x rows, 8 heads, by the one and the other: 512 x 10,000 32 and 35 us, 600 x 10,000 48 and
-// 43, 800 x 10,000 52 and 50, 1,300 x 10,000 88 and 71, 2,048 x 2,000 29 and 32, 2,048 x 10,000 105 and 92).
+// and eight and a half more. Which is quicker changes back and forth as rounds fill (us by the one and the other, each in its
+// own best ranges, heads x rows x queries; < and > say which is taken, of 36 shapes one wrongly, by 2%):
+//     8 x 1,000: 256 10 < 14, 2,048 21 < 26              8 x 3,000: 769 21 < 27, 1,025 37 > 30, 2,048 40 < 39
+//     8 x 10,000: 256 21 < 27, 512 33 < 35, 513 46 > 42, 800 52 > 50          8 x 20,001: 193 32 < 33, 300 40 < 48
+//     8 x 40,000: 160 42 < 48, 193 56 > 50, 300 70 < 84, 512 103 > 91         8 x 100,000: 150 96 < 106, 200 129 > 110
+//     4 x 10,000: 512 23 < 29, 673 34 > 33, 1,024 33 < 36                     16 x 10,000: 320 49 < 52, 321 54 > 50
 static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
     auto ranges = [&](int per, int least_blocks, auto cost_of, float &cost) {
         int best = 1;
@@ -2265,8 +2276,8 @@ static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
     };
     AttnPlan p{};
     p.few = true;
-    p.waves = a.nq <= 16 ? 1 : 2;  // groups of 16 queries a workgroup
-    p.groups = std::max(1, (a.nq + 16 * p.waves - 1) / (16 * p.waves));
+    p.sets = a.nq <= 16 ? 1 : 2;
+    p.groups = std::max(1, (a.nq + 16 * p.sets - 1) / (16 * p.sets));
     float few_cost, many_cost;
     // one range while a wavefront has no more than two blocks: a second one's merge takes longer
     int splits = ranges(a.heads * p.groups, FEW4_WAVES,
@@ -2281,7 +2292,6 @@ static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
         if (many_cost < few_cost) {
             p.few = false;
             p.split16 = true;
-            p.waves = 8;
             p.groups = tiles;
             splits = s;
         }
@@ -2292,7 +2302,7 @@ static AttnPlan plan4(const AttnShape &a, const KeyBlocks &k) {
 }
 
 static AttnPlan plan(const AttnShape &a, bool images) {
-    AttnPlan p;
+    AttnPlan p{};
     const KeyBlocks k = key_blocks(a.rows, a.chunk);
     const int hd = a.d / a.heads;
     const bool tiles = hd == 64 && images && kv_images_apply(a.kv_format, a.d, a.heads);
@@ -2463,7 +2473,7 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
     if (p.few) {
         const dim3 grid(a.heads * p.splits);
         const dim3 grid4(a.heads, p.splits, p.groups);
-        if (a.kv_format == TAH_KV_I4 && p.waves == 1)
+        if (a.kv_format == TAH_KV_I4 && p.sets == 1)
             hipLaunchKernelGGL(k_attn_few4<1>, grid4, dim3(64 * FEW4_WAVES), 0, s, a.nq, key_blocks(a.rows, a.chunk),
                                a.chunk, q, img->images, img->kvmax, p.kb_per_split, part_o, part_ml, out);
         else if (a.kv_format == TAH_KV_I4)

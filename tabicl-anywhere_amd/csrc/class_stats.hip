@@ -117,9 +117,10 @@ __device__ __forceinline__ T row_lanes(T v, F &&f) {
 
 // grid ceil(rows / (64 / L)); 64 threads. Each of a row's L lanes keeps N / L of its N >= n scores in registers, read where
 // they lie: a wavefront's loads meet the same few lines again and again, in L1 (turned in LDS first, whole lines at a time:
-// 200,000 x 7 6.9 us for 5.8, 100,000 x 20 10.9 for 8.9). A row of ten classes takes two lanes about 150 instructions, where
-// a wavefront or a workgroup a row spent most of its own on reductions (200,000 x 7: 664 us a workgroup a row). The most
-// probable classes by one scan of the keys each. Instructions bound it: 100,000 x 50 with five best 14.6 us, 1.4 TB/s.
+// 200,000 x 7 6.9 us for 5.8, 100,000 x 20 10.9 for 8.9). A wavefront or a workgroup a row spent most of its instructions on
+// reductions (200,000 x 7: 664 us a workgroup a row). The most probable classes by one scan of the keys each. 200,000 x 7 with
+// three best takes 460 instructions a wavefront of 64 rows, 2.7 us of issue; its wavefronts wait for memory 56% of their time.
+// 100,000 x 50 with five best, 14.6 us, 1.4 TB/s, is bound by its instructions (724 for eight rows).
 template <int N, int L>
 __global__ __launch_bounds__(64) void k_class_stats_rows(int rows, int n, size_t ld, const float *__restrict__ x,
                                                          ClassScale by, ClassOut o) {

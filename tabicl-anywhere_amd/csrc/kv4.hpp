@@ -55,7 +55,7 @@ __device__ __forceinline__ int code4(Step4 st, float v) {
 }
 
 // The same of four values, eight more than each in four bits, with one reciprocal: it is off by 2^-22 of the quotient at
-// most, so that away from a tie the nearest level is the same; where a lane of the wavefront is near one (one in 2^16
+// most, so that away from a tie the nearest level is the same; where a lane of the wavefront is near one (one in 2^15
 // values), by the division.
 __device__ __forceinline__ uint32_t codes4(Step4 st, const float (&v)[4]) {
     const float inv = st.s > 0.0f ? __builtin_amdgcn_rcpf(st.s) : 0.0f;
@@ -89,9 +89,10 @@ __device__ __forceinline__ float record_value4(const uint8_t *rec, int d, int rc
 }
 
 // A tile word's eight codes (code t at bits 4 (t / 2) + 16 (t % 2), 8 more than it is) as the fp16 numbers z + s c, each
-// rounded once. Four bits or'ed into the significand of 1024 are 1024 + n, or 1024 + 16 n from the next four, so that a
-// pair of codes is a half each in two instructions (three for all four pairs' shifts), exact; then one packed
-// multiply-add.
+// rounded once. The conversion is the published one by exponent: bits or'ed into the significand of a power of two are that
+// power and their number (for 4-bit weights in fp16: Kim, Henry, Fahim and Awadalla, "Who Says Elephants Can't Run", 2022).
+// Four bits in 1024 are 1024 + n, or 1024 + 16 n from the next four, so that a pair of codes is a half each in two
+// instructions (one shift for the second two pairs), exact; then one packed multiply-add.
 __device__ __forceinline__ halfx8 values4(uint32_t word, halfx8 s, halfx8 z) {
     const halfx2 down = {(_Float16)-1032.0f, (_Float16)-1032.0f}, down16 = {(_Float16)-72.0f, (_Float16)-72.0f};
     const halfx2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
