@@ -326,6 +326,59 @@ int tah_class_stats(tah_dev *dev, const float *scores, int32_t rows, int32_t n, 
 int tah_class_stats_dev(tah_dev *dev, const float *scores_dev, int32_t rows, int32_t n, int64_t ld, float temperature,
                         const int32_t *given_dev, int32_t n_given, int32_t top, float *stats_dev, int32_t *ids_dev);
 
+/* ---- many tables at once: keys and values in pages ---------------------------------------------------------
+ *
+ * No counterpart in the reference, whose layers are held whole, a table each. A pool holds one layer's keys and values of any
+ * number of tables in pages of page_rows rows; a table's pages are listed in order, so tables grow a row at a time, and may
+ * share pages. Stored chunk records have a scale per coordinate over a chunk's rows, so a chunk has to be whole before it is
+ * packed; a page has a step per row and head, so a row is written when it is there and changes no other.
+ *
+ * A page, for each of kv_heads heads one after the other: the rows' keys [page_rows][hd], their values [hd][page_rows], both
+ * f32, int16 or int8, then (int16, int8) the rows' key steps and their value steps, [page_rows] f32 each.
+ *     value = int * step; step = the row's largest finite magnitude over 32767 or 127 in f32, 0 (and every int 0) where that
+ *     is below 2^-126; int = the number over its step rounded to the nearest, ties to even; a NaN 0, an infinity the last int
+ *     of its sign. f32 pages hold every number as it is.
+ * kv_format is TAH_KV_F32, TAH_KV_I16 or TAH_KV_I8 (four bits need each coordinate's mean over many rows: TAH_E_ARG); hd a
+ * multiple of 16 up to 128; page_rows 16, 32, 64, 128 or 256; tables, ld and pages at least 1. tah_page_bytes: 0 for sizes
+ * outside these. */
+typedef struct tah_pages {
+    uint8_t *pool;        /* device memory, pages * tah_page_bytes bytes, 16-byte aligned */
+    const int32_t *table; /* [tables][ld]: each table's pages in order; an id outside [0, pages) is no page */
+    int32_t kv_format, kv_heads, hd, page_rows;
+    int32_t pages, tables, ld;
+} tah_pages;
+size_t tah_page_bytes(int32_t kv_format, int32_t kv_heads, int32_t hd, int32_t page_rows);
+
+/* Rows into pages, and what pages stand for. k and v hold rows rows of kv_heads * hd floats, row_ld floats apart (0:
+ * kv_heads * hd); rows offsets[t] .. offsets[t + 1] - 1 are table t's (offsets [tables + 1], from 0 up) and go to, or come
+ * from, its rows starts[t], starts[t] + 1, ... (starts [tables]). Rows from offsets[tables] on are left alone.
+ * The _dev forms take every array in device memory (4-byte aligned; the table too), are queued on the handle's stream, and
+ * look at nothing beforehand: a row that falls on no page, or outside its table's, is not written, and is read as zeros. The
+ * others take the arrays (the table too, not the pool) in host memory and refuse such rows with TAH_E_ARG. Two rows written to
+ * the same place in one call: tah_pages_write refuses them, tah_pages_write_dev leaves numbers of either. */
+int tah_pages_write(tah_dev *dev, const tah_pages *p, const int32_t *starts, const int32_t *offsets, const float *k,
+                    const float *v, int32_t rows, int64_t row_ld);
+int tah_pages_write_dev(tah_dev *dev, const tah_pages *p, const int32_t *starts, const int32_t *offsets, const float *k,
+                        const float *v, int32_t rows, int64_t row_ld);
+int tah_pages_read(tah_dev *dev, const tah_pages *p, const int32_t *starts, const int32_t *offsets, float *k, float *v,
+                   int32_t rows, int64_t row_ld);
+int tah_pages_read_dev(tah_dev *dev, const tah_pages *p, const int32_t *starts, const int32_t *offsets, float *k, float *v,
+                       int32_t rows, int64_t row_ld);
+
+/* Attention of queries of many tables, each over its own table's pages: q [nq][heads * hd] (already scaled), rows q_ld floats
+ * apart (0: heads * hd); queries offsets[t] .. offsets[t + 1] - 1 are table t's and see its first lengths[t] rows. With causal
+ * they are its last rows: of n queries query i sees all but the last n - 1 - i rows. Head h reads key/value head
+ * h / (heads / kv_heads); kv_heads divides heads. out [nq][heads * hd], before the output projection; queries from
+ * offsets[tables] on are left as they were. Rows on no page are not seen (a length counts as no more than ld * page_rows);
+ * a query that sees none gives zeros. A number that is not finite makes NaN of the outputs that see it, and of no others: a key
+ * of its head's, a value of its own coordinate's. The _dev form takes every array in device memory as above (lengths and
+ * offsets may change between replays of a captured call); the other takes them in host memory, but for the pool, and refuses
+ * lengths over ld * page_rows or of rows on no page with TAH_E_ARG. */
+int tah_pages_attend(tah_dev *dev, const tah_pages *p, const int32_t *lengths, const float *q, const int32_t *offsets,
+                     int32_t nq, int32_t heads, int32_t causal, int64_t q_ld, float *out);
+int tah_pages_attend_dev(tah_dev *dev, const tah_pages *p, const int32_t *lengths, const float *q, const int32_t *offsets,
+                         int32_t nq, int32_t heads, int32_t causal, int64_t q_ld, float *out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,6 +37,13 @@ class ModelDesc(ctypes.Structure):
         ("dec2b", F32P)]
 
 
+class Pages(ctypes.Structure):
+    """A pool of pages and its tables (`tah_pages`): `pool` and, for the calls on device memory, `table` are device
+    addresses."""
+    _fields_ = [("pool", ctypes.c_void_p), ("table", ctypes.c_void_p)] + [
+        (n, ctypes.c_int32) for n in ("kv_format", "kv_heads", "hd", "page_rows", "pages", "tables", "ld")]
+
+
 # int (*tah_layer_sink)(void *ctx, int32_t layer, const uint8_t *records, size_t bytes)
 LAYER_SINK = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int32, U8P, ctypes.c_size_t)
 
@@ -47,6 +54,12 @@ def kv_record(kv_format: int, d: int, rc: int) -> int:
         return 2 * d * (4 * ((rc + 63) // 64) + (rc + 1) // 2)
     w = {KV_F32: 4, KV_I16: 2, KV_I8: 1}[kv_format]
     return 2 * d * rc * w + (0 if kv_format == KV_F32 else 8 * d)
+
+
+def page_bytes(kv_format: int, kv_heads: int, hd: int, page_rows: int) -> int:
+    """Bytes of a page of `page_rows` rows (`tah_page_bytes`)."""
+    w = {KV_F32: 4, KV_I16: 2, KV_I8: 1}[kv_format]
+    return kv_heads * page_rows * (2 * hd * w + (0 if kv_format == KV_F32 else 8))
 
 
 def layer_bytes(kv_format: int, rows: int, chunk: int, d: int) -> int:
@@ -142,6 +155,11 @@ SIGNATURES = {
     "tah_class_stats_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
                                            ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_int32,
                                            ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),
+    "tah_page_bytes": (ctypes.c_size_t, [ctypes.c_int32] * 4),
+    **{name: (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Pages)] + [ctypes.c_void_p] * 4 + [ctypes.c_int32, ctypes.c_int64])
+       for name in ("tah_pages_write", "tah_pages_write_dev", "tah_pages_read", "tah_pages_read_dev")},
+    **{name: (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Pages)] + [ctypes.c_void_p] * 3 + [ctypes.c_int32] * 3 +
+              [ctypes.c_int64, ctypes.c_void_p]) for name in ("tah_pages_attend", "tah_pages_attend_dev")},
     "tah_quantile_stats_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, F32P,
                                               ctypes.c_int32, ctypes.c_void_p]),
 }

@@ -10,6 +10,7 @@
 
 #include "common.hpp"
 #include "host_copy.hpp"
+#include "pages.hpp"
 
 using namespace tah;
 
@@ -1021,6 +1022,188 @@ extern "C" int tah_class_stats(tah_dev *dev, const float *scores, int32_t rows, 
                     work ? loans.take<uint8_t>(work) : nullptr);
         TAH_HIP(hipMemcpyAsync(stats, sd, sizeof(float) * nout, hipMemcpyDeviceToHost, dev->stream));
         if (nt) TAH_HIP(hipMemcpyAsync(ids, id, sizeof(int32_t) * nt, hipMemcpyDeviceToHost, dev->stream));
+        TAH_HIP(hipStreamSynchronize(dev->stream));
+        return TAH_OK;
+    });
+}
+
+// ---- many tables at once: keys and values in pages --------------------------------------------------------------
+static bool page_shape_ok(int kv_format, int kv_heads, int hd, int page_rows) {
+    return kv_format >= TAH_KV_F32 && kv_format <= TAH_KV_I8 && kv_heads > 0 && kv_heads <= 65535 && hd > 0 && hd <= 128 &&
+           hd % 16 == 0 && page_rows >= 16 && page_rows <= 256 && (page_rows & (page_rows - 1)) == 0;
+}
+
+static size_t page_head_bytes(int kv_format, int hd, int page_rows) {
+    return (size_t)page_rows * (2 * (size_t)hd * page_width(kv_format) + (kv_format == TAH_KV_F32 ? 0 : 8));
+}
+
+extern "C" size_t tah_page_bytes(int32_t kv_format, int32_t kv_heads, int32_t hd, int32_t page_rows) {
+    return page_shape_ok(kv_format, kv_heads, hd, page_rows) ? kv_heads * page_head_bytes(kv_format, hd, page_rows) : 0;
+}
+
+static bool aligned4(std::initializer_list<const void *> ps) {
+    uintptr_t bits = 0;
+    for (const void *q : ps) bits |= reinterpret_cast<uintptr_t>(q);
+    return bits % 4 == 0;
+}
+
+// The pool as the kernels take it, with `table` (device memory) in place of the caller's.
+static PageSet page_set(const char *what, const tah_pages *p, const int32_t *table) {
+    const std::string w = what;
+    if (!page_shape_ok(p->kv_format, p->kv_heads, p->hd, p->page_rows))
+        throw ArgError{w + ": pages of 16 to 256 rows (a power of two) in f32, i16 or i8, heads of 16 to 128 (in sixteens)"};
+    if (!p->pool || !p->table || p->pages <= 0 || p->tables <= 0 || p->ld <= 0) throw ArgError{w + ": no pool, pages or tables"};
+    if (reinterpret_cast<uintptr_t>(p->pool) % 16) throw ArgError{w + ": the pool has to be 16-byte aligned"};
+    int log_rows = 4;
+    while (1 << log_rows < p->page_rows) log_rows++;
+    const size_t head = page_head_bytes(p->kv_format, p->hd, p->page_rows);
+    return PageSet{p->pool, table, p->kv_heads, p->hd, p->page_rows, log_rows, p->pages, p->tables, p->ld, head, head * p->kv_heads};
+}
+
+// Rows of `width` floats, ld apart (0: width).
+static size_t row_stride(const std::string &what, int rows, int64_t ld, size_t width) {
+    if (ld == 0) ld = (int64_t)width;
+    if (rows < 0 || rows > 0x7FFFFFFF - 1024) throw ArgError{what + ": at most 2^31 - 1024 rows"};
+    if (ld < (int64_t)width) throw ArgError{what + ": rows nearer to each other than they are long"};
+    return (size_t)ld;
+}
+
+static void check_offsets(const std::string &what, const int32_t *offsets, int tables, int rows) {
+    if (offsets[0] != 0) throw ArgError{what + ": the offsets have to begin at 0"};
+    for (int t = 0; t < tables; t++)
+        if (offsets[t + 1] < offsets[t]) throw ArgError{what + ": offsets that fall"};
+    if (offsets[tables] > rows) throw ArgError{what + ": offsets past the rows there are"};
+}
+
+// Rows at .. at + n - 1 of table t on the host: all on pages.
+static void check_on_pages(const std::string &what, const tah_pages *p, int t, int64_t at, int64_t n) {
+    if (n <= 0) return;
+    if (at < 0 || (at + n - 1) / p->page_rows >= p->ld) throw ArgError{what + ": rows outside their table's pages"};
+    for (int64_t i = at / p->page_rows; i <= (at + n - 1) / p->page_rows; i++) {
+        const int id = p->table[(size_t)t * p->ld + i];
+        if (id < 0 || id >= p->pages) throw ArgError{what + ": rows on no page of the pool"};
+    }
+}
+
+static int pages_rows_dev(const char *what, tah_dev *dev, const tah_pages *p, const int32_t *starts, const int32_t *offsets,
+                          float *k, float *v, int32_t rows, int64_t row_ld, bool write) {
+    if (!p || !starts || !offsets || !k || !v) return TAH_E_ARG;
+    return guarded(dev, [&] {
+        const PageSet set = page_set(what, p, p->table);
+        const size_t ld = row_stride(what, rows, row_ld, (size_t)set.heads * set.hd);
+        if (!aligned4({p->table, starts, offsets, k, v})) throw ArgError{std::string(what) + ": the pointers have to be 4-byte aligned"};
+        pages_rows(dev->stream, p->kv_format, set, starts, offsets, k, v, rows, ld, write);
+        return TAH_OK;
+    });
+}
+
+static int pages_rows_host(const char *what, tah_dev *dev, const tah_pages *p, const int32_t *starts, const int32_t *offsets,
+                           float *k, float *v, int32_t rows, int64_t row_ld, bool write) {
+    if (!p || !starts || !offsets || !k || !v) return TAH_E_ARG;
+    return guarded(dev, [&] {
+        PageSet set = page_set(what, p, nullptr);
+        const size_t width = (size_t)set.heads * set.hd, ld = row_stride(what, rows, row_ld, width);
+        check_offsets(what, offsets, p->tables, rows);
+        std::vector<int64_t> places;
+        for (int t = 0; t < p->tables; t++) {
+            const int64_t n = offsets[t + 1] - offsets[t];
+            check_on_pages(what, p, t, starts[t], n);
+            if (write)
+                for (int64_t at = starts[t]; at < starts[t] + n; at++)
+                    places.push_back((int64_t)p->table[(size_t)t * p->ld + at / p->page_rows] * p->page_rows + at % p->page_rows);
+        }
+        std::sort(places.begin(), places.end());
+        if (std::adjacent_find(places.begin(), places.end()) != places.end())
+            throw ArgError{std::string(what) + ": two rows to the same place"};
+        const int n = offsets[p->tables];  // the rows from here on are left alone
+        if (n == 0) return TAH_OK;
+        Loans loans(dev);
+        const size_t cells = (size_t)p->tables * p->ld;
+        float *kd = loans.take<float>(n * width), *vd = loans.take<float>(n * width);
+        int32_t *td = loans.take<int32_t>(cells), *sd = loans.take<int32_t>(p->tables), *od = loans.take<int32_t>(p->tables + 1);
+        set.table = td;
+        TAH_HIP(hipMemcpyAsync(td, p->table, cells * sizeof(int32_t), hipMemcpyHostToDevice, dev->stream));
+        TAH_HIP(hipMemcpyAsync(sd, starts, p->tables * sizeof(int32_t), hipMemcpyHostToDevice, dev->stream));
+        TAH_HIP(hipMemcpyAsync(od, offsets, (p->tables + 1) * sizeof(int32_t), hipMemcpyHostToDevice, dev->stream));
+        const size_t wide = width * sizeof(float), far = ld * sizeof(float);
+        if (write) {
+            TAH_HIP(hipMemcpy2DAsync(kd, wide, k, far, wide, n, hipMemcpyHostToDevice, dev->stream));
+            TAH_HIP(hipMemcpy2DAsync(vd, wide, v, far, wide, n, hipMemcpyHostToDevice, dev->stream));
+        }
+        pages_rows(dev->stream, p->kv_format, set, sd, od, kd, vd, n, width, write);
+        if (!write) {
+            TAH_HIP(hipMemcpy2DAsync(k, far, kd, wide, wide, n, hipMemcpyDeviceToHost, dev->stream));
+            TAH_HIP(hipMemcpy2DAsync(v, far, vd, wide, wide, n, hipMemcpyDeviceToHost, dev->stream));
+        }
+        TAH_HIP(hipStreamSynchronize(dev->stream));
+        return TAH_OK;
+    });
+}
+
+extern "C" int tah_pages_write_dev(tah_dev *dev, const tah_pages *p, const int32_t *starts, const int32_t *offsets, const float *k,
+                                   const float *v, int32_t rows, int64_t row_ld) {
+    return pages_rows_dev("pages_write", dev, p, starts, offsets, const_cast<float *>(k), const_cast<float *>(v), rows, row_ld, true);
+}
+extern "C" int tah_pages_read_dev(tah_dev *dev, const tah_pages *p, const int32_t *starts, const int32_t *offsets, float *k,
+                                  float *v, int32_t rows, int64_t row_ld) {
+    return pages_rows_dev("pages_read", dev, p, starts, offsets, k, v, rows, row_ld, false);
+}
+extern "C" int tah_pages_write(tah_dev *dev, const tah_pages *p, const int32_t *starts, const int32_t *offsets, const float *k,
+                               const float *v, int32_t rows, int64_t row_ld) {
+    return pages_rows_host("pages_write", dev, p, starts, offsets, const_cast<float *>(k), const_cast<float *>(v), rows, row_ld, true);
+}
+extern "C" int tah_pages_read(tah_dev *dev, const tah_pages *p, const int32_t *starts, const int32_t *offsets, float *k, float *v,
+                              int32_t rows, int64_t row_ld) {
+    return pages_rows_host("pages_read", dev, p, starts, offsets, k, v, rows, row_ld, false);
+}
+
+static void check_heads(const std::string &what, int nq, int heads, int kv_heads) {
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads) throw ArgError{what + ": the key/value heads have to divide the heads"};
+    if (nq < 0 || (int64_t)nq * heads > 0x7FFFFFFF - 1024) throw ArgError{what + ": at most 2^31 - 1024 queries and heads"};
+}
+
+extern "C" int tah_pages_attend_dev(tah_dev *dev, const tah_pages *p, const int32_t *lengths, const float *q, const int32_t *offsets,
+                                    int32_t nq, int32_t heads, int32_t causal, int64_t q_ld, float *out) {
+    if (!p || !lengths || !q || !offsets || !out) return TAH_E_ARG;
+    return guarded(dev, [&] {
+        const PageSet set = page_set("pages_attend", p, p->table);
+        check_heads("pages_attend", nq, heads, set.heads);
+        const size_t ld = row_stride("pages_attend", nq, q_ld, (size_t)heads * set.hd);
+        if (!aligned4({p->table, lengths, q, offsets, out})) throw ArgError{"pages_attend: the pointers have to be 4-byte aligned"};
+        if (nq == 0) return TAH_OK;
+        Loans loans(dev);
+        void *work = loans.take<uint8_t>(pages_attend_work_bytes(set, nq, heads));
+        pages_attend(dev->stream, p->kv_format, set, lengths, q, offsets, nq, heads, causal != 0, ld, out, work);
+        return TAH_OK;
+    });
+}
+
+extern "C" int tah_pages_attend(tah_dev *dev, const tah_pages *p, const int32_t *lengths, const float *q, const int32_t *offsets,
+                                int32_t nq, int32_t heads, int32_t causal, int64_t q_ld, float *out) {
+    if (!p || !lengths || !q || !offsets || !out) return TAH_E_ARG;
+    return guarded(dev, [&] {
+        PageSet set = page_set("pages_attend", p, nullptr);
+        check_heads("pages_attend", nq, heads, set.heads);
+        const size_t width = (size_t)heads * set.hd, ld = row_stride("pages_attend", nq, q_ld, width);
+        check_offsets("pages_attend", offsets, p->tables, nq);
+        for (int t = 0; t < p->tables; t++) {
+            if (lengths[t] < 0) throw ArgError{"pages_attend: a length below 0"};
+            check_on_pages("pages_attend", p, t, 0, lengths[t]);
+        }
+        const int n = offsets[p->tables];  // the queries from here on are left alone
+        if (n == 0) return TAH_OK;
+        Loans loans(dev);
+        const size_t cells = (size_t)p->tables * p->ld, wide = width * sizeof(float);
+        float *qd = loans.take<float>(n * width), *od = loans.take<float>(n * width);
+        int32_t *td = loans.take<int32_t>(cells), *ld_ = loans.take<int32_t>(p->tables), *fd = loans.take<int32_t>(p->tables + 1);
+        void *work = loans.take<uint8_t>(pages_attend_work_bytes(set, n, heads));
+        set.table = td;
+        TAH_HIP(hipMemcpyAsync(td, p->table, cells * sizeof(int32_t), hipMemcpyHostToDevice, dev->stream));
+        TAH_HIP(hipMemcpyAsync(ld_, lengths, p->tables * sizeof(int32_t), hipMemcpyHostToDevice, dev->stream));
+        TAH_HIP(hipMemcpyAsync(fd, offsets, (p->tables + 1) * sizeof(int32_t), hipMemcpyHostToDevice, dev->stream));
+        TAH_HIP(hipMemcpy2DAsync(qd, wide, q, ld * sizeof(float), wide, n, hipMemcpyHostToDevice, dev->stream));
+        pages_attend(dev->stream, p->kv_format, set, ld_, qd, fd, n, heads, causal != 0, width, od, work);
+        TAH_HIP(hipMemcpyAsync(out, od, n * wide, hipMemcpyDeviceToHost, dev->stream));
         TAH_HIP(hipStreamSynchronize(dev->stream));
         return TAH_OK;
     });

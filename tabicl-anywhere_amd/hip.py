@@ -346,6 +346,75 @@ class Gpu:
         """`unpack` with the records and the values in device memory."""
         self._check(self._l.tah_unpack_dev(self._h, records_ptr, d, rows, chunk, kv_format, kv_ptr))
 
+    # ---- many tables at once: keys and values in pages ------------------------------------------------------------
+    # `pages` is an abi.Pages; the calls on host arrays take its pool on the card and `table` [tables][ld] as an array
+    def _pages_of(self, pages: abi.Pages, table, what: str) -> tuple:
+        table = np.ascontiguousarray(table, np.int32)
+        if table.shape != (pages.tables, pages.ld):
+            raise ValueError(f"{what}: expected a table of [{pages.tables}][{pages.ld}] pages, got shape {table.shape}")
+        p = abi.Pages.from_buffer_copy(pages)
+        p.table = table.ctypes.data
+        return p, table
+
+    @staticmethod
+    def _counts(a, n: int, what: str) -> np.ndarray:
+        a = np.asarray(a)
+        if a.shape != (n,) or a.dtype.kind not in "iu" or (a.size and (a.min() < -2**31 or a.max() >= 2**31)):
+            raise ValueError(f"{what}: expected {n} whole numbers of 32 bits")
+        return np.ascontiguousarray(a, np.int32)
+
+    def pages_write(self, pages: abi.Pages, table, starts, offsets, k, v) -> None:
+        """New rows' keys and values [rows][kv_heads * hd] into their tables' pages, quantised on the card as they are
+        written: rows offsets[t] .. offsets[t + 1] - 1 become rows starts[t], .. of table t."""
+        p, table = self._pages_of(pages, table, "pages_write")
+        k, v = (_rows_of(a, p.kv_heads * p.hd, "pages_write") for a in (k, v))
+        if k.shape != v.shape:
+            raise ValueError("pages_write: keys and values must have the same shape")
+        starts, offsets = self._counts(starts, p.tables, "pages_write"), self._counts(offsets, p.tables + 1, "pages_write")
+        self._check(self._l.tah_pages_write(self._h, ctypes.byref(p), starts.ctypes.data, offsets.ctypes.data, k.ctypes.data,
+                                            v.ctypes.data, k.shape[0], 0))
+
+    def pages_read(self, pages: abi.Pages, table, starts, offsets) -> tuple:
+        """What rows of tables' pages stand for: keys and values [rows][kv_heads * hd], offsets[t + 1] - offsets[t] rows of
+        table t from its row starts[t] on."""
+        p, table = self._pages_of(pages, table, "pages_read")
+        starts, offsets = self._counts(starts, p.tables, "pages_read"), self._counts(offsets, p.tables + 1, "pages_read")
+        shape = (max(0, int(offsets[-1])), p.kv_heads * p.hd)
+        k, v = np.empty(shape, np.float32), np.empty(shape, np.float32)
+        self._check(self._l.tah_pages_read(self._h, ctypes.byref(p), starts.ctypes.data, offsets.ctypes.data, k.ctypes.data,
+                                           v.ctypes.data, shape[0], 0))
+        return k, v
+
+    def pages_attend(self, pages: abi.Pages, table, lengths, q, offsets, heads: int, causal: bool = False) -> np.ndarray:
+        """Attention outputs [nq][heads * hd] of scaled queries of many tables over their pages: queries offsets[t] ..
+        offsets[t + 1] - 1 over the first lengths[t] rows of table t (causal: they are its last rows, and see those before
+        them). Queries past the last table's give zeros."""
+        p, table = self._pages_of(pages, table, "pages_attend")
+        q = _rows_of(q, int(heads) * p.hd, "pages_attend")
+        lengths, offsets = self._counts(lengths, p.tables, "pages_attend"), self._counts(offsets, p.tables + 1, "pages_attend")
+        out = np.zeros(q.shape, np.float32)
+        self._check(self._l.tah_pages_attend(self._h, ctypes.byref(p), lengths.ctypes.data, q.ctypes.data, offsets.ctypes.data,
+                                             q.shape[0], int(heads), int(bool(causal)), 0, out.ctypes.data))
+        return out
+
+    def pages_write_dev(self, pages: abi.Pages, starts_ptr: int, offsets_ptr: int, k_ptr: int, v_ptr: int, rows: int,
+                        row_ld: int = 0) -> None:
+        """`pages_write` with every array in device memory, queued on the handle's stream; rows `row_ld` floats apart (0:
+        kv_heads * hd). Rows on no page are not written."""
+        self._check(self._l.tah_pages_write_dev(self._h, pages, starts_ptr, offsets_ptr, k_ptr, v_ptr, rows, row_ld))
+
+    def pages_read_dev(self, pages: abi.Pages, starts_ptr: int, offsets_ptr: int, k_ptr: int, v_ptr: int, rows: int,
+                       row_ld: int = 0) -> None:
+        """`pages_read` with every array in device memory; rows on no page are zeros."""
+        self._check(self._l.tah_pages_read_dev(self._h, pages, starts_ptr, offsets_ptr, k_ptr, v_ptr, rows, row_ld))
+
+    def pages_attend_dev(self, pages: abi.Pages, lengths_ptr: int, q_ptr: int, offsets_ptr: int, nq: int, heads: int,
+                         out_ptr: int, causal: bool = False, q_ld: int = 0) -> None:
+        """`pages_attend` with every array in device memory; queries `q_ld` floats apart (0: heads * hd). Queries past the
+        last table's are left as they were."""
+        self._check(self._l.tah_pages_attend_dev(self._h, pages, lengths_ptr, q_ptr, offsets_ptr, nq, heads, causal, q_ld,
+                                                 out_ptr))
+
     def attend(self, q, kv, rows: int, chunk: int, d: int, heads: int) -> np.ndarray:
         """`Attend::attend`: all rows' attention over the layer's exact f32 keys and values (chunk layout)."""
         q, kv = _f32(q), _f32(kv).reshape(-1)
