@@ -160,6 +160,8 @@ SIGNATURES = {
        for name in ("tah_pages_write", "tah_pages_write_dev", "tah_pages_read", "tah_pages_read_dev")},
     **{name: (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Pages)] + [ctypes.c_void_p] * 3 + [ctypes.c_int32] * 3 +
               [ctypes.c_int64, ctypes.c_void_p]) for name in ("tah_pages_attend", "tah_pages_attend_dev")},
+    **{name: (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_int32] * 7 + [ctypes.c_int64] * 2 + [ctypes.c_void_p])
+       for name in ("tah_attend_packed", "tah_attend_packed_dev")},
     "tah_quantile_stats_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, F32P,
                                               ctypes.c_int32, ctypes.c_void_p]),
 }

@@ -37,10 +37,10 @@
 #include "common.hpp"
 #include "device_math.hpp"
 #include "kv4.hpp"
+#include "tiles.hpp"
 
 namespace tah {
 
-constexpr int KB = 64;   // keys per block
 constexpr int QG = 8;    // queries per decode workgroup
 // Queries from which a layer's tiles are read by the matrix kernel rather than the decode kernel. Over f32 images and
 // i8 code images from one query: the matrix kernel reads a tile with whole-row DMA copies, where the decode kernel's
@@ -194,10 +194,6 @@ __host__ __device__ constexpr int img_bytes(int fmt) {
 __host__ __device__ inline size_t image_bytes_of(int rows, int chunk, int heads, int fmt) {
     return (size_t)key_blocks(rows, chunk).n_kb * heads * img_bytes(fmt);
 }
-
-// rows r and r + 1 already sit in different bank halves (128-byte rows); rows of one parity among 16 consecutive ones
-// get eight different chunks
-__device__ __forceinline__ int swz(int r, int c) { return c ^ ((r >> 1) & 7); }
 
 // ---- decode kernel: any head width <= 64, few queries --------------------------------------------------------
 // grid (splits, heads, query groups of QG); 64 threads.
@@ -783,24 +779,6 @@ __global__ __launch_bounds__(256) void k_kv_tiles4(int rows, int chunk, int d, i
 // more than 3 (then the sums are rescaled): weights exp2(t - ref + 12) stay below 2^15, inside fp16, and most blocks
 // skip the rescaling.
 
-// Half an image (its keys or its values: BYTES, 16 KB of split values or 8 KB of codes) into an LDS buffer, 16 bytes
-// a lane: in copy i, wavefront w fills the 1 KB at chunk 64 (WAVES i + w) (a wavefront-uniform LDS base; the lanes'
-// offsets are implicit).
-template <int WAVES, int BYTES>
-__device__ __forceinline__ void half_image_to_lds(const uint8_t *src, uint8_t *dst, int tid) {
-    constexpr int T = 64 * WAVES, CHUNKS = BYTES / 16;
-    static_assert(BYTES % 16 == 0, "whole 16-byte copies");
-    const int w = tid >> 6;
-#pragma unroll
-    for (int i = 0; i < (CHUNKS + T - 1) / T; i++) {
-        const int base = i * T + 64 * w;
-        // lanes past the last copy stay idle (a copy a lane: each writes its own 16 bytes at dst + 16 (base + lane))
-        if (CHUNKS % T == 0 || base + (tid & 63) < CHUNKS)
-            __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint4 *>(src) + base + (tid & 63), dst + 16 * base, 16,
-                                             0, 0);
-    }
-}
-
 // i16 staging (k_attn_split64 with STAGED): half a code tile (8 KB of codes and its 256 bytes of factors, keys or
 // values) into a staging slot's half by DMA: 528 copies of 16 bytes, the last 16 by wavefront 0.
 template <int WAVES>
@@ -837,11 +815,6 @@ __device__ __forceinline__ void convert16(const uint8_t *st, uint8_t *kdst, uint
         }
     }
 }
-
-template <bool B>
-struct Flag {
-    static constexpr bool value = B;
-};
 
 // With CODES (i8 caches) the images hold the codes and `scl` the scales (k_kv_codes): the scores are two products of
 // the query, multiplied by the chunk's key scales and split again whenever a block starts a new chunk (the raw query

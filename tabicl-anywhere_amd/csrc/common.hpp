@@ -303,6 +303,15 @@ int probe_read(hipStream_t s, double *ms);
 void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t *records, float *out, void *work,
                const KvImages *img = nullptr);
 
+// Attention of packed tables (packed.hip): q [nq][heads * hd] over k, v [nkv][kv_heads * hd], rows q_ld and kv_ld floats apart;
+// work of packed_work_bytes (which refuses calls that are too large).
+struct PackedShape {
+    int tables, nq, nkv, heads, kv_heads, hd;
+};
+size_t packed_work_bytes(const PackedShape &a);
+void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const float *k, const float *v, const int32_t *q_offsets,
+                      const int32_t *kv_offsets, bool causal, size_t q_ld, size_t kv_ld, float *out, void *work);
+
 // The regression head (quantiles.hip): per row of q [rows][n], mean, variance, median and icdf at alphas [na]
 // (device) into stats [rows][3 + na].
 void quantile_stats(hipStream_t s, int rows, int n, const float *q, int na, const float *alphas, float *stats);

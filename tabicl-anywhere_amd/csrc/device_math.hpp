@@ -223,6 +223,30 @@ __device__ __forceinline__ void dequant_split8(uint4 codes, const float (&f)[8],
     lo = __builtin_bit_cast(halfx8, lw);
 }
 
+// 2^e, e cut to what f32 holds
+__device__ __forceinline__ float pow2(int e) { return ldexpf(1.0f, min(max(e, -149), 127)); }
+
+// the bits of a float's magnitude, 0 if it is not finite
+__device__ __forceinline__ uint32_t finite_bits(uint32_t w) {
+    const uint32_t u = w & 0x7fffffffu;
+    return u < 0x7f800000u ? u : 0u;
+}
+
+// the sum over a lane and the lanes before it
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const T o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+// four floats of which only 4-byte alignment is known
+typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));
+
 // Row i of a 32-row MFMA A operand holding row sigma(i) (bits 3 and 2 swapped): the accumulators v = 8 hh .. 8 hh + 7
 // of lane l of a 32 x 32 v_mfma_f32_32x32x16 result then hold rows 16 hh + 8 (l / 32) + 0..7 -- eight consecutive
 // rows, which is how a B operand of a following product over those rows wants them.

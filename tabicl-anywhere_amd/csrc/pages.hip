@@ -78,10 +78,7 @@ __device__ void find_places(const PageSet &p, const int32_t *starts, const int32
     __syncthreads();
 }
 
-__device__ __forceinline__ float finite_abs(float x) {
-    const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
-    return u < 0x7f800000u ? __uint_as_float(u) : 0.0f;
-}
+__device__ __forceinline__ float finite_abs(float x) { return __uint_as_float(finite_bits(__float_as_uint(x))); }
 
 // x / s rounded to the nearest int, ties to even, within the top; inv is about 1 / s. The product's rounding may miss by one
 // where x / s is next to a tie: its residual x - c s is exact in f32 (a multiple of half an ulp of s, below 2^24 of them), and

@@ -47,7 +47,4 @@ size_t pages_attend_work_bytes(const PageSet &p, int nq, int heads);
 void pages_attend(hipStream_t s, int fmt, const PageSet &p, const int32_t *lengths, const float *q, const int32_t *offsets, int nq,
                   int heads, bool causal, size_t q_ld, float *out, void *work);
 
-// four floats of which only 4-byte alignment is known
-typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));
-
 }  // namespace tah

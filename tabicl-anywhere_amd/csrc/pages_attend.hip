@@ -41,16 +41,6 @@ __device__ __forceinline__ TableWork table_work(const PageSet &p, const int32_t 
     return w;
 }
 
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {  // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-
 // sixteen stored numbers of a lane as halves: eight for either half of 16, exact in hi (i8) or hi + lo
 template <int FMT>
 struct Raw;
@@ -114,14 +104,6 @@ __device__ __forceinline__ void to_halves(const Raw<FMT> &r, int s, float f, hal
     }
 }
 
-__device__ __forceinline__ uint32_t finite_bits(uint32_t w) {
-    const uint32_t u = w & 0x7fffffffu;
-    return u < 0x7f800000u ? u : 0u;
-}
-
-// a power of two that is a float: 2^e, e cut to what f32 holds
-__device__ __forceinline__ float pow2(int e) { return ldexpf(1.0f, min(max(e, -149), 127)); }
-
 __device__ __forceinline__ floatx4 mfma(halfx8 a, halfx8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -142,7 +124,7 @@ template <int FMT, int C, int CT>
 __global__ __launch_bounds__(64 * WAVES) void k_pages_attend(PageSet p, const int32_t *__restrict__ lengths,
                                                              const float *__restrict__ q, const int32_t *__restrict__ offsets,
                                                              int nq, int heads, int causal, size_t q_ld,
-                                                             float *__restrict__ out, Parts parts) {
+                                                             float *__restrict__ out, Parts parts, uint64_t most_blocks) {
     constexpr int W = page_width(FMT), COLS = 16 * CT, HD = 64 * C, M = 4 * C;
     constexpr bool INTS = FMT != TAH_KV_F32, LO = FMT != TAH_KV_I8;
     __shared__ float mref[WAVES][COLS], msum[WAVES][COLS], macc[WAVES][HD][17];
@@ -151,14 +133,16 @@ __global__ __launch_bounds__(64 * WAVES) void k_pages_attend(PageSet p, const in
     const uint32_t waves = gridDim.x * WAVES, me = blockIdx.x * WAVES + wave;
 
     // the plan: every wavefront adds up all tables' blocks and finds its own
-    uint32_t total = 0;
+    uint64_t all = 0;
     for (int t0 = 0; t0 < p.tables; t0 += 64) {
         const int t = t0 + lane;
-        const uint32_t c = t < p.tables ? table_work(p, lengths, offsets, nq, group, COLS, t).cost : 0;
-        const uint32_t sum = wave_scan(c);
-        if (me == 0 && t < p.tables) parts.plan[1 + t] = total + sum - c;
-        total += __builtin_amdgcn_readlane(sum, 63);
+        const uint64_t c = t < p.tables ? table_work(p, lengths, offsets, nq, group, COLS, t).cost : 0;
+        const uint64_t sum = wave_scan(c);
+        if (me == 0 && t < p.tables) parts.plan[1 + t] = (uint32_t)(all + sum - c);
+        all += __shfl(sum, 63);
     }
+    // offsets that fall may make more of the queries than there are: nothing is done then
+    const uint32_t total = all <= most_blocks ? __builtin_amdgcn_readfirstlane((uint32_t)all) : 0;
     const uint32_t per = max(1u, (total + waves - 1) / waves);
     if (me == 0 && lane == 0) {
         parts.plan[0] = per;
@@ -585,14 +569,15 @@ __global__ __launch_bounds__(256) void k_pages_join(PageSet p, const int32_t *__
     for (int t0 = 0; t0 < p.tables - 1; t0 += 64) t += __popcll(__ballot(t0 + lane < p.tables - 1 && offsets[t0 + lane + 1] <= r));
     const TableWork tw = table_work(p, lengths, offsets, nq, group, COLS, t);
     if (r < tw.first || r >= tw.first + tw.n) return;
-    const uint32_t per = parts.plan[0];
+    const uint32_t per = parts.plan[0], total = parts.plan[1 + p.tables];
+    if (total == 0) return;
     const int h = head / group, c = (r - tw.first) * group + head - h * group, tile = c / COLS, col = c - tile * COLS;
     const uint32_t u0 = parts.plan[1 + t] + ((uint32_t)tile * p.heads + h) * tw.nb, u1 = u0 + tw.nb;
     const uint32_t w0 = u0 / per, w1 = (u1 - 1) / per;
     if (w0 == w1) return;
     if (u0 % per == 0 && w0 % WAVES == 0 && u1 <= (w0 + WAVES) * per) {
         // one workgroup may have held it whole, with its wavefronts in turn
-        const uint32_t wg0 = w0 * per, wg1 = min(parts.plan[1 + p.tables], wg0 + WAVES * per);
+        const uint32_t wg0 = w0 * per, wg1 = min(total, wg0 + WAVES * per);
         if (wg1 == u1) return;
     }
     float M = -INFINITY, L = 0.0f, o[2] = {0.0f, 0.0f};
@@ -644,26 +629,6 @@ __global__ __launch_bounds__(256) void k_pages_join(PageSet p, const int32_t *__
     if (64 + lane < hd) dst[64 + lane] = o[1] * inv;
 }
 
-template <int FMT, int C, int CT>
-void launch(hipStream_t s, const PageSet &p, const int32_t *lengths, const float *q, const int32_t *offsets, int nq, int heads,
-            bool causal, size_t q_ld, float *out, const Parts &parts, int wgs) {
-    hipLaunchKernelGGL((k_pages_attend<FMT, C, CT>), dim3(wgs), dim3(64 * WAVES), 0, s, p, lengths, q, offsets, nq, heads,
-                       causal ? 1 : 0, q_ld, out, parts);
-    TAH_LAUNCHED();
-    hipLaunchKernelGGL(k_pages_join<CT>, dim3((unsigned)nq * heads), dim3(256), 0, s, p, lengths, offsets, nq, heads,
-                       (uint32_t)wgs * WAVES, out, parts);
-    TAH_LAUNCHED();
-}
-
-template <int FMT, int C>
-void launch_sets(int sets, hipStream_t s, const PageSet &p, const int32_t *lengths, const float *q, const int32_t *offsets, int nq,
-                 int heads, bool causal, size_t q_ld, float *out, const Parts &parts, int wgs) {
-    if (sets == 1)
-        launch<FMT, C, 1>(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, wgs);
-    else
-        launch<FMT, C, 2>(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, wgs);
-}
-
 // Sets of 16 columns that share what a wavefront reads, and the workgroups: one a compute unit, fewer where there may not be a
 // block for each of their wavefronts.
 struct Shape {
@@ -685,6 +650,26 @@ Shape shape(const PageSet &p, int nq, int heads) {
     s.o_floats = slots * 16 * s.sets * p.hd;
     s.ml_count = slots * 16 * s.sets;
     return s;
+}
+
+template <int FMT, int C, int CT>
+void launch(hipStream_t s, const PageSet &p, const int32_t *lengths, const float *q, const int32_t *offsets, int nq, int heads,
+            bool causal, size_t q_ld, float *out, const Parts &parts, const Shape &sh) {
+    hipLaunchKernelGGL((k_pages_attend<FMT, C, CT>), dim3(sh.wgs), dim3(64 * WAVES), 0, s, p, lengths, q, offsets, nq,
+                       heads, causal ? 1 : 0, q_ld, out, parts, sh.blocks);
+    TAH_LAUNCHED();
+    hipLaunchKernelGGL(k_pages_join<CT>, dim3((unsigned)nq * heads), dim3(256), 0, s, p, lengths, offsets, nq, heads,
+                       (uint32_t)sh.wgs * WAVES, out, parts);
+    TAH_LAUNCHED();
+}
+
+template <int FMT, int C>
+void launch_sets(hipStream_t s, const PageSet &p, const int32_t *lengths, const float *q, const int32_t *offsets, int nq,
+                 int heads, bool causal, size_t q_ld, float *out, const Parts &parts, const Shape &sh) {
+    if (sh.sets == 1)
+        launch<FMT, C, 1>(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh);
+    else
+        launch<FMT, C, 2>(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -709,9 +694,9 @@ void pages_attend(hipStream_t s, int fmt, const PageSet &p, const int32_t *lengt
     auto with = [&](auto f) {
         constexpr int FMT = decltype(f)::value;
         if (p.hd <= 64)
-            launch_sets<FMT, 1>(sh.sets, s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh.wgs);
+            launch_sets<FMT, 1>(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh);
         else
-            launch_sets<FMT, 2>(sh.sets, s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh.wgs);
+            launch_sets<FMT, 2>(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh);
     };
     if (fmt == TAH_KV_F32)
         with(std::integral_constant<int, TAH_KV_F32>{});

@@ -346,7 +346,7 @@ class Gpu:
         """`unpack` with the records and the values in device memory."""
         self._check(self._l.tah_unpack_dev(self._h, records_ptr, d, rows, chunk, kv_format, kv_ptr))
 
-    # ---- many tables at once: keys and values in pages ------------------------------------------------------------
+    # ---- many tables at once: keys and values in pages, packed tables ---------------------------------------------
     # `pages` is an abi.Pages; the calls on host arrays take its pool on the card and `table` [tables][ld] as an array
     def _pages_of(self, pages: abi.Pages, table, what: str) -> tuple:
         table = np.ascontiguousarray(table, np.int32)
@@ -414,6 +414,35 @@ class Gpu:
         last table's are left as they were."""
         self._check(self._l.tah_pages_attend_dev(self._h, pages, lengths_ptr, q_ptr, offsets_ptr, nq, heads, causal, q_ld,
                                                  out_ptr))
+
+    def attend_packed(self, q, k, v, q_offsets, heads: int, kv_heads: int, causal: bool = False, kv_offsets=None) -> np.ndarray:
+        """Attention outputs [nq][heads * hd] of several tables at once in full precision: scaled queries q_offsets[t] ..
+        q_offsets[t + 1] - 1 over rows kv_offsets[t] .. kv_offsets[t + 1] - 1 of k and v [rows][kv_heads * hd] (None: the same
+        offsets); causal: a table's last query sees all its rows, each one before it one less. Queries past the last table's
+        give zeros."""
+        k = _f32(k)
+        if heads <= 0 or kv_heads <= 0 or k.ndim != 2 or k.shape[1] % kv_heads:
+            raise ValueError("attend_packed: expected keys [rows][kv_heads * hd]")
+        hd = k.shape[1] // kv_heads
+        q, v = _rows_of(q, int(heads) * hd, "attend_packed"), _rows_of(v, k.shape[1], "attend_packed")
+        if k.shape != v.shape:
+            raise ValueError("attend_packed: keys and values must have the same shape")
+        tables = len(q_offsets) - 1
+        qo = self._counts(q_offsets, tables + 1, "attend_packed")
+        ko = qo if kv_offsets is None else self._counts(kv_offsets, tables + 1, "attend_packed")
+        out = np.zeros(q.shape, np.float32)
+        self._check(self._l.tah_attend_packed(self._h, q.ctypes.data, k.ctypes.data, v.ctypes.data, qo.ctypes.data, ko.ctypes.data,
+                                              tables, q.shape[0], k.shape[0], int(heads), int(kv_heads), hd, int(bool(causal)), 0, 0,
+                                              out.ctypes.data))
+        return out
+
+    def attend_packed_dev(self, q_ptr: int, k_ptr: int, v_ptr: int, q_offsets_ptr: int, kv_offsets_ptr: int, tables: int, nq: int,
+                          nkv: int, heads: int, kv_heads: int, hd: int, out_ptr: int, causal: bool = False, q_ld: int = 0,
+                          kv_ld: int = 0) -> None:
+        """`attend_packed` with every array in device memory, queued on the handle's stream; rows `q_ld` and `kv_ld` floats
+        apart (0: heads * hd, kv_heads * hd). Queries past the last table's are left as they were."""
+        self._check(self._l.tah_attend_packed_dev(self._h, q_ptr, k_ptr, v_ptr, q_offsets_ptr, kv_offsets_ptr, tables, nq, nkv, heads,
+                                                  kv_heads, hd, causal, q_ld, kv_ld, out_ptr))
 
     def attend(self, q, kv, rows: int, chunk: int, d: int, heads: int) -> np.ndarray:
         """`Attend::attend`: all rows' attention over the layer's exact f32 keys and values (chunk layout)."""
