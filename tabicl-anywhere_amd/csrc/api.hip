@@ -1172,7 +1172,7 @@ extern "C" int tah_pages_attend_dev(tah_dev *dev, const tah_pages *p, const int3
         if (!aligned4({p->table, lengths, q, offsets, out})) throw ArgError{"pages_attend: the pointers have to be 4-byte aligned"};
         if (nq == 0) return TAH_OK;
         Loans loans(dev);
-        void *work = loans.take<uint8_t>(pages_attend_work_bytes(set, nq, heads));
+        void *work = loans.take<uint8_t>(pages_attend_work_bytes(p->kv_format, set, nq, heads));
         pages_attend(dev->stream, p->kv_format, set, lengths, q, offsets, nq, heads, causal != 0, ld, out, work);
         return TAH_OK;
     });
@@ -1196,7 +1196,7 @@ extern "C" int tah_pages_attend(tah_dev *dev, const tah_pages *p, const int32_t 
         const size_t cells = (size_t)p->tables * p->ld, wide = width * sizeof(float);
         float *qd = loans.take<float>(n * width), *od = loans.take<float>(n * width);
         int32_t *td = loans.take<int32_t>(cells), *ld_ = loans.take<int32_t>(p->tables), *fd = loans.take<int32_t>(p->tables + 1);
-        void *work = loans.take<uint8_t>(pages_attend_work_bytes(set, n, heads));
+        void *work = loans.take<uint8_t>(pages_attend_work_bytes(p->kv_format, set, n, heads));
         set.table = td;
         TAH_HIP(hipMemcpyAsync(td, p->table, cells * sizeof(int32_t), hipMemcpyHostToDevice, dev->stream));
         TAH_HIP(hipMemcpyAsync(ld_, lengths, p->tables * sizeof(int32_t), hipMemcpyHostToDevice, dev->stream));

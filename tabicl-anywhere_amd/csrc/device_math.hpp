@@ -232,16 +232,18 @@ __device__ __forceinline__ uint32_t finite_bits(uint32_t w) {
     return u < 0x7f800000u ? u : 0u;
 }
 
-// the sum over a lane and the lanes before it
-template <class T>
-__device__ __forceinline__ T wave_scan(T v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const T o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
+// the sum over a lane and the lanes before it: within rows of sixteen lanes, then the rows' last lanes to the rows after
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_zero(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += dpp_or_zero<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_or_zero<0x112, 0xf>(v);
+    v += dpp_or_zero<0x114, 0xf>(v);
+    v += dpp_or_zero<0x118, 0xf>(v);
+    v += dpp_or_zero<0x142, 0xa>(v);     // row_bcast 15 into rows 1 and 3
+    return v + dpp_or_zero<0x143, 0xc>(v);  // row_bcast 31 into rows 2 and 3
 }
 
 // four floats of which only 4-byte alignment is known

@@ -43,7 +43,7 @@ void pages_rows(hipStream_t s, int fmt, const PageSet &p, const int32_t *starts,
                 int rows, size_t row_ld, bool write);
 
 // The queries' attention (pages_attend.hip), work of pages_attend_work_bytes (which refuses calls that are too large).
-size_t pages_attend_work_bytes(const PageSet &p, int nq, int heads);
+size_t pages_attend_work_bytes(int fmt, const PageSet &p, int nq, int heads);
 void pages_attend(hipStream_t s, int fmt, const PageSet &p, const int32_t *lengths, const float *q, const int32_t *offsets, int nq,
                   int heads, bool causal, size_t q_ld, float *out, void *work);
 

@@ -11,57 +11,65 @@ namespace tah {
 
 namespace {
 
-constexpr int WAVES = 8;
+constexpr int WAVES = 4;
+// What beginning and ending a unit costs, in blocks: a unit counts as so many more than it has, so that wavefronts with several
+// units get fewer of them.
+constexpr int BEGIN = 2;
 
-// What a run of blocks leaves behind for the join, per slot: [columns][hd] outputs and [columns] (maximum, sum). A wavefront has
-// at most two units that are not whole, its first and its last: slots 2 w and 2 w + 1.
+// What runs of blocks leave behind for the join: per slot [columns][hd] outputs and [columns] (maximum, sum); a wavefront has at
+// most two units that are not whole, its first and its last: slots 2 w and 2 w + 1. Per query and head the unit's first block and
+// the one behind its last, the blocks a wavefront, and the column (blocks a wavefront 0: the output is there).
 struct Parts {
     float *o;
     float2 *ml;
-    uint32_t *plan;  // blocks a wavefront; each table's first block; the blocks in all
+    uint4 *units;
+    uint32_t *plan;  // blocks a wavefront, blocks in all
 };
 
-// queries of table t (from `first`), its rows, and its blocks
+// A table's queries (from `first`), rows, and blocks: in the chunk of 64 tables that a wavefront holds, one a lane
 struct TableWork {
-    int first, n, len, tiles, nb;
-    uint32_t cost;
+    int first, n, len;
+    uint32_t nb, cost;
 };
 
 __device__ __forceinline__ TableWork table_work(const PageSet &p, const int32_t *lengths, const int32_t *offsets, int nq, int group,
-                                                int columns, int t) {
-    TableWork w;
-    const int a = min(max(offsets[t], 0), nq), b = min(max(offsets[t + 1], a), nq);
-    w.first = a;
-    w.n = b - a;
+                                                int columns, int keys, int t) {
+    const int i = min(t, p.tables - 1), from = offsets[i], to = offsets[i + 1], told = lengths[i];
+    const int a = min(max(from, 0), nq), b = min(max(to, a), nq);
     const long most = min((long)p.ld << p.log_rows, (long)0x7fffffff - 64);
-    w.len = (int)min((long)max(lengths[t], 0), most);
-    w.tiles = (w.n * group + columns - 1) / columns;
-    w.nb = max(1, (w.len + 63) >> 6);
-    w.cost = (uint32_t)w.tiles * p.heads * w.nb;
+    TableWork w;
+    w.first = a;
+    w.n = t < p.tables ? b - a : 0;
+    w.len = (int)min((long)max(told, 0), most);
+    w.nb = (w.len + keys - 1) / keys + BEGIN;
+    w.cost = (uint32_t)((w.n * group + columns - 1) / columns) * p.heads * w.nb;
     return w;
 }
 
-// sixteen stored numbers of a lane as halves: eight for either half of 16, exact in hi (i8) or hi + lo
-template <int FMT>
-struct Raw;
-template <>
-struct Raw<TAH_KV_I8> {
-    u32x4 w[1];
-};
-template <>
-struct Raw<TAH_KV_I16> {
-    u32x4 w[2];
-};
-template <>
-struct Raw<TAH_KV_F32> {
-    u32x4 w[4];
+// 16 (N 2) or 8 (N 1) stored numbers of a lane
+template <int FMT, int N>
+struct Raw {
+    static constexpr int WORDS = 2 * N * page_width(FMT);
+    uint32_t w[WORDS];
 };
 
-template <int FMT>
-__device__ __forceinline__ Raw<FMT> load_raw(const uint8_t *at) {
-    Raw<FMT> r;
+template <int FMT, int N>
+__device__ __forceinline__ Raw<FMT, N> load_raw(const uint8_t *at) {
+    Raw<FMT, N> r;
+    if constexpr (Raw<FMT, N>::WORDS == 2) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(at);
+        r.w[0] = x.x;
+        r.w[1] = x.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(r) / 16); i++) r.w[i] = reinterpret_cast<const u32x4 *>(at)[i];
+        for (int i = 0; i < Raw<FMT, N>::WORDS / 4; i++) {
+            const uint4 x = reinterpret_cast<const uint4 *>(at)[i];
+            r.w[4 * i] = x.x;
+            r.w[4 * i + 1] = x.y;
+            r.w[4 * i + 2] = x.z;
+            r.w[4 * i + 3] = x.w;
+        }
+    }
     return r;
 }
 
@@ -70,13 +78,15 @@ __device__ __forceinline__ halfx2 half_bytes(uint32_t flipped, uint32_t sel) {
     return __builtin_bit_cast(halfx2, __builtin_amdgcn_perm(flipped, 0x64646464u, sel)) - halfx2{(_Float16)1152.0f, (_Float16)1152.0f};
 }
 
-template <int FMT>
-__device__ __forceinline__ void to_halves(const Raw<FMT> &r, int s, float f, halfx8 &hi, halfx8 &lo) {
+// numbers 8 s .. 8 s + 7 as halves: exact in hi (i8); i16 as 256 (hi + lo), hi the high byte, lo the low one over 256: five
+// instructions for two, where rounding to a half and the rest took eight; f32 times f in hi + lo
+template <int FMT, int N>
+__device__ __forceinline__ void to_halves(const Raw<FMT, N> &r, int s, float f, halfx8 &hi, halfx8 &lo) {
     if constexpr (FMT == TAH_KV_I8) {
         u32x4 o;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const uint32_t w = r.w[0][2 * s + i] ^ 0x80808080u;
+            const uint32_t w = r.w[2 * s + i] ^ 0x80808080u;
             o[2 * i] = __builtin_bit_cast(uint32_t, half_bytes(w, 0x00050004u));
             o[2 * i + 1] = __builtin_bit_cast(uint32_t, half_bytes(w, 0x00070006u));
         }
@@ -85,21 +95,18 @@ __device__ __forceinline__ void to_halves(const Raw<FMT> &r, int s, float f, hal
         u32x4 a, b;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const uint32_t w = r.w[s][i];
-            uint32_t x, y;
-            split2((float)(int16_t)(w & 0xffffu), (float)(int16_t)(w >> 16), x, y);
-            a[i] = x;
-            b[i] = y;
+            const uint32_t w = r.w[4 * s + i] ^ 0x80008000u;
+            a[i] = __builtin_bit_cast(uint32_t, half_bytes(w, 0x00070005u));
+            const halfx2 low = __builtin_bit_cast(halfx2, __builtin_amdgcn_perm(w, 0x64646464u, 0x00060004u));
+            const _Float16 part = (_Float16)0x1p-8f, back = (_Float16)-4.0f;
+            b[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(low, halfx2{part, part}, halfx2{back, back}));
         }
         hi = __builtin_bit_cast(halfx8, a);
         lo = __builtin_bit_cast(halfx8, b);
     } else {
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t w = r.w[2 * s + (i >> 2)][i & 3];
-            v[i] = __uint_as_float(w);
-        }
+        for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r.w[8 * s + i]);
         split8(v, f, hi, lo);
     }
 }
@@ -108,85 +115,112 @@ __device__ __forceinline__ floatx4 mfma(halfx8 a, halfx8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// grid: any number of workgroups of 8 wavefronts.
+// grid: any number of workgroups; WAVES wavefronts each.
 //
-// Products are 16 x 16 x 32 with the queries as columns: S = K Q^T for sets of 16 keys, then O^T += V^T P^T. A lane (lg = lane /
-// 16) has keys 16 lg .. 16 lg + 15 of a block: set (s, p)'s row r is key 16 (r / 4) + 8 s + 4 p + r % 4, so that the scores of
-// sets (s, 0) and (s, 1) are the operand of the values' product s in place, sixteen consecutive numbers of a coordinate are what
-// a lane reads of the values, and a page of 16 rows or more holds all that a lane reads at once. Coordinates go likewise: step
-// (c, ks) takes 64 c + 16 lg + 8 ks .. + 7.
+// Products are 16 x 16 x 32 with the queries as columns: S = K Q^T for sets of 16 keys, then O^T += V^T P^T. Of a block's 32 KS
+// keys a lane (lg = lane / 16) has N = 8 KS: keys N lg .. N lg + N - 1. Set (s, p)'s row r is key N (r / 4) + 8 s + 4 p + r % 4, so
+// that the scores of sets (s, 0) and (s, 1) are the operand of the values' product s in place, N consecutive numbers of a
+// coordinate are what a lane reads of the values, and a page of 16 rows or more holds all that a lane reads at once. Coordinates go
+// likewise: step (c, ks) takes 64 c + 16 lg + 8 ks .. + 7.
 //
-// Numbers: ints go in as they are (i8 exact in one half, i16 in two), the key's step multiplies its scores, the value's its
+// Numbers: ints go in as they are (i8 exact in one half, i16 in two bytes), the key's step multiplies its scores, the value's its
 // weights; f32 goes in as two halves times the block's power of two. Queries and weights are two halves. So a term is two
-// products (i8) or three, for f32's error. Weights are held below 2^15 (their maximum raised by blocks that pass it by more than
+// products (i8), three (f32) or four (i16: a low byte is 2^-8 of the largest number, so its product with a low half counts), for
+// f32's error. Weights are held below 2^15 (their maximum raised by blocks that pass it by more than
 // 2^3), times the value's step over a power of two that no step so far passes.
-template <int FMT, int C, int CT>
-__global__ __launch_bounds__(64 * WAVES) void k_pages_attend(PageSet p, const int32_t *__restrict__ lengths,
-                                                             const float *__restrict__ q, const int32_t *__restrict__ offsets,
-                                                             int nq, int heads, int causal, size_t q_ld,
-                                                             float *__restrict__ out, Parts parts, uint64_t most_blocks) {
-    constexpr int W = page_width(FMT), COLS = 16 * CT, HD = 64 * C, M = 4 * C;
-    constexpr bool INTS = FMT != TAH_KV_F32, LO = FMT != TAH_KV_I8;
-    __shared__ float mref[WAVES][COLS], msum[WAVES][COLS], macc[WAVES][HD][17];
+template <int FMT, int C, int CT, int KS>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const int32_t *__restrict__ lengths,
+                                                                const float *__restrict__ q, const int32_t *__restrict__ offsets,
+                                                                int nq, int heads, int causal, size_t q_ld,
+                                                                float *__restrict__ out, Parts parts, uint64_t most_blocks) {
+    constexpr int W = page_width(FMT), COLS = 16 * CT, HD = 64 * C, M = 4 * C, N = 8 * KS, KEYS = 32 * KS;
+    constexpr bool INTS = FMT != TAH_KV_F32, LO = FMT != TAH_KV_I8, BYTES = FMT == TAH_KV_I16;
+    // more queries than 16 columns of 64 coordinates wait in LDS, each wavefront's own; the join's sums take their place
+    constexpr bool WAIT = C * CT > 1;
+    constexpr int QS = WAIT ? CT * C * 2 * 2 * 64 : 0;  // 16-byte words of a wavefront's
+    __shared__ __align__(16) uint8_t store[WAVES * (QS * 16 > HD * 68 ? QS * 16 : HD * 68)];
+    __shared__ float mref[WAVES][COLS], msum[WAVES][COLS];
+    float (*macc)[HD][17] = reinterpret_cast<float (*)[HD][17]>(store);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qi = lane & 15, lg = lane >> 4, group = heads / p.heads, hd = p.hd, P = p.rows;
     const uint32_t waves = gridDim.x * WAVES, me = blockIdx.x * WAVES + wave;
 
-    // the plan: every wavefront adds up all tables' blocks and finds its own
+    // the plan: every wavefront adds up all tables' blocks and finds its own; a chunk of 64 tables, one a lane, is kept
+    TableWork mine_of{};
+    uint32_t sums = 0;          // blocks of the chunk's tables up to the lane's
+    uint32_t chunk_before = 0;  // blocks before the chunk
+    int chunk = 0;
     uint64_t all = 0;
     for (int t0 = 0; t0 < p.tables; t0 += 64) {
-        const int t = t0 + lane;
-        const uint64_t c = t < p.tables ? table_work(p, lengths, offsets, nq, group, COLS, t).cost : 0;
-        const uint64_t sum = wave_scan(c);
-        if (me == 0 && t < p.tables) parts.plan[1 + t] = (uint32_t)(all + sum - c);
-        all += __shfl(sum, 63);
+        mine_of = table_work(p, lengths, offsets, nq, group, COLS, KEYS, t0 + lane);
+        sums = wave_scan(mine_of.cost);
+        // in two halves of 16 bits, which 64 tables' sums do not overflow, whatever their offsets say
+        const uint32_t low = wave_scan(mine_of.cost & 0xffffu), high = wave_scan(mine_of.cost >> 16);
+        all += ((uint64_t)__builtin_amdgcn_readlane(high, 63) << 16) + __builtin_amdgcn_readlane(low, 63);
     }
     // offsets that fall may make more of the queries than there are: nothing is done then
-    const uint32_t total = all <= most_blocks ? __builtin_amdgcn_readfirstlane((uint32_t)all) : 0;
+    const uint32_t total = all <= most_blocks ? (uint32_t)all : 0;
     const uint32_t per = max(1u, (total + waves - 1) / waves);
     if (me == 0 && lane == 0) {
         parts.plan[0] = per;
-        parts.plan[1 + p.tables] = total;
+        parts.plan[1] = total;
     }
     const uint32_t wg0 = blockIdx.x * WAVES * per, wg1 = min(total, wg0 + WAVES * per);
     if (wg0 >= total) return;
-
-    // the table of block `at`, at or behind the one held
-    int t = -1;
+    if (p.tables > 64) {
+        mine_of = table_work(p, lengths, offsets, nq, group, COLS, KEYS, lane);
+        sums = wave_scan(mine_of.cost);
+    }
+    // the table of block `at`, which is at or behind the last one's
+    int t = 0;
     uint32_t before = 0;  // blocks before table t
     TableWork tw{};
     auto seek = [&](uint32_t at) {
-        if (t >= 0 && at < before + tw.cost) return;
-        uint32_t sums = t < 0 ? 0 : before + tw.cost;
-        for (int t0 = t + 1; t0 < p.tables; t0 += 64) {
-            const int i = t0 + lane;
-            const uint32_t c = i < p.tables ? table_work(p, lengths, offsets, nq, group, COLS, i).cost : 0;
-            const uint32_t sum = wave_scan(c);
-            const uint64_t past = __ballot(sums + sum > at);
-            if (past) {
-                const int l = __ffsll((unsigned long long)past) - 1;
-                t = __builtin_amdgcn_readfirstlane(t0 + l);
-                before = sums + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(c, l);
-                tw = table_work(p, lengths, offsets, nq, group, COLS, t);
-                return;
-            }
-            sums += __builtin_amdgcn_readlane(sum, 63);
+        uint64_t past;
+        while (!(past = __ballot(chunk_before + sums > at)) && chunk + 64 < p.tables) {
+            chunk_before += __builtin_amdgcn_readlane(sums, 63);
+            chunk += 64;
+            mine_of = table_work(p, lengths, offsets, nq, group, COLS, KEYS, chunk + lane);
+            sums = wave_scan(mine_of.cost);
         }
+        const int l = past ? __ffsll((unsigned long long)past) - 1 : 0;
+        t = chunk + l;
+        tw.first = __builtin_amdgcn_readlane(mine_of.first, l);
+        tw.n = __builtin_amdgcn_readlane(mine_of.n, l);
+        tw.len = __builtin_amdgcn_readlane(mine_of.len, l);
+        tw.nb = __builtin_amdgcn_readlane(mine_of.nb, l);
+        tw.cost = __builtin_amdgcn_readlane(mine_of.cost, l);
+        before = chunk_before + __builtin_amdgcn_readlane(sums, l) - tw.cost;
     };
 
-    // one unit: its columns' queries and limits, and the state that its blocks add to
-    int tile = 0, h = 0;
-    halfx8 qh[CT][C][2], ql[CT][C][2];
-    float to_log2[CT], ref[CT], l[CT];
-    int limit[CT], ev;
-    floatx4 acc[CT][M];
-    int lim_most = 0, lim_least = 0;
-    auto begin = [&](uint32_t unit) {
-        tile = unit / p.heads;
-        h = unit - tile * p.heads;
-        ev = INTS ? -1000 : 1000;
-        lim_most = 0;
-        lim_least = tw.len;
+    // a workgroup whose blocks are one unit's: its wavefronts take them in turn and join what they have
+    seek(wg0);
+    const bool together = wg1 - wg0 > 1 && wg1 <= before + ((wg0 - before) / tw.nb + 1) * tw.nb;
+    uint32_t at = together ? wg0 : wg0 + wave * per;
+    const uint32_t end = together ? wg1 : min(total, at + per), mine = at;
+    while (at < end) {
+        seek(at);
+        const uint32_t unit = (at - before) / tw.nb, b0 = at - before - unit * tw.nb, b1 = min(tw.nb, b0 + (end - at));
+        const bool done = b0 == 0 && b1 == tw.nb;
+        if (!together && b0 > 0 && b0 + BEGIN >= tw.nb) {  // behind the unit's blocks
+            if (lane < COLS) parts.ml[(2 * (size_t)me + (at == mine ? 0 : 1)) * COLS + lane] = make_float2(-INFINITY, 0.0f);
+            at += b1 - b0;
+            continue;
+        }
+        const int tile = unit / p.heads, h = unit - tile * p.heads;
+        const int step = together ? WAVES : 1;
+        int kb = (int)b0 + (together ? wave : 0);
+        // pages of the table, one a lane from `ids0` on
+        const int32_t *pages = p.table + (size_t)t * p.ld;
+        int ids0 = ((long)kb * KEYS) >> p.log_rows;
+        int ids = pages[min(ids0 + lane, p.ld - 1)];
+        // the columns' queries and limits
+        halfx8 qh[WAIT ? 1 : CT][C][2], ql[WAIT ? 1 : CT][C][2];
+        halfx8 *waiting = reinterpret_cast<halfx8 *>(store) + (size_t)wave * QS + lane;
+        float to_log2[CT], ref[CT], l[CT];
+        int limit[CT], ev = INTS ? -1000 : 1000;
+        floatx4 acc[CT][M];
+        int lim_most = 0, lim_least = tw.len;
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             const int col = tile * COLS + 16 * ct + qi, i = col / group;
@@ -201,11 +235,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_pages_attend(PageSet p, const in
                 const bool in = 64 * c + 16 * lg < hd;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const floatx4 x = in ? (floatx4) * reinterpret_cast<const floatx4u *>(src + 64 * c + 16 * lg + 4 * j)
-                                         : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                    const floatx4 x = *reinterpret_cast<const floatx4u *>(src + (in ? 64 * c + 16 * lg + 4 * j : 0));
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        qv[c][4 * j + e] = live ? x[e] : 0.0f;
+                        qv[c][4 * j + e] = live && in ? x[e] : 0.0f;
                         most = fmaxf(most, __uint_as_float(finite_bits(__float_as_uint(qv[c][4 * j + e]))));
                     }
                 }
@@ -216,12 +249,25 @@ __global__ __launch_bounds__(64 * WAVES) void k_pages_attend(PageSet p, const in
 #pragma unroll
             for (int c = 0; c < C; c++)
 #pragma unroll
-                for (int ks = 0; ks < 2; ks++) split8(qv[c] + 8 * ks, f, qh[ct][c][ks], ql[ct][c][ks]);
-            to_log2[ct] = LOG2E * pow2(-eq);
+                for (int ks = 0; ks < 2; ks++) {
+                    const int at = WAIT ? 0 : ct;
+                    split8(qv[c] + 8 * ks, f, qh[at][c][ks], ql[at][c][ks]);
+                    if constexpr (WAIT) {
+                        waiting[64 * (4 * (ct * C + c) + 2 * ks)] = qh[0][c][ks];
+                        waiting[64 * (4 * (ct * C + c) + 2 * ks + 1)] = ql[0][c][ks];
+                    }
+                }
+            to_log2[ct] = (BYTES ? 256.0f : 1.0f) * LOG2E * pow2(-eq);
             ref[ct] = -INFINITY;
             l[ct] = 0.0f;
 #pragma unroll
             for (int m = 0; m < M; m++) acc[ct][m] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            // where the join finds the unit
+            if (b0 == 0 && lg == 0 && live && (!together || wave == 0)) {
+                const uint32_t u0 = before + unit * tw.nb;
+                parts.units[(size_t)(tw.first + i) * heads + h * group + col - i * group] =
+                    make_uint4(u0, u0 + tw.nb, done ? 0 : per, 16 * ct + qi);
+            }
         }
 #pragma unroll
         for (int d = 1; d < 16; d *= 2) {
@@ -230,480 +276,492 @@ __global__ __launch_bounds__(64 * WAVES) void k_pages_attend(PageSet p, const in
         }
         lim_most = __builtin_amdgcn_readfirstlane(lim_most);
         lim_least = __builtin_amdgcn_readfirstlane(lim_least);
-    };
+        const int last = min((int)b1, (lim_most + KEYS - 1) / KEYS);  // blocks behind every column's limit are not looked at
 
-    // pages of the table, one a lane from `ids0` on
-    int ids = -1, ids0 = 0;
-    auto pages_from = [&](int i0) {
-        ids0 = i0;
-        ids = page_of(p, t, (long)(i0 + lane) << p.log_rows);
-    };
-    auto block = [&](int kb) {
-        const int first = kb * 64;
-        const int i0 = first >> p.log_rows, i1 = (first + 48) >> p.log_rows;
-        if (i0 < ids0 || i1 >= ids0 + 64) pages_from(i0);
-        const int kk = first + 16 * (qi >> 2), kv = first + 16 * lg;  // the first keys of what the lane reads
-        const int idk = __shfl(ids, (kk >> p.log_rows) - ids0), idv = __shfl(ids, (kv >> p.log_rows) - ids0);
-        const uint8_t *bk = p.pool + (size_t)max(idk, 0) * p.page_bytes + (size_t)h * p.head_bytes;
-        const uint8_t *bv = p.pool + (size_t)max(idv, 0) * p.page_bytes + (size_t)h * p.head_bytes;
-        const int slk = (kk & (P - 1)) + (qi & 3), slv = kv & (P - 1);
-        const bool whole = first + 64 <= tw.len && __all(idv >= 0);  // every key there is and on a page
-        // of the lane's sixteen keys (values), how many there are
-        const int here = whole ? 16 : (idv >= 0 ? min(max(tw.len - kv, 0), 16) : 0);
-        const bool all_seen = whole && first + 64 <= lim_least;
-        Raw<FMT> kr[4][C], vr[M];
-#pragma unroll
-        for (int sp = 0; sp < 4; sp++)
-#pragma unroll
-            for (int c = 0; c < C; c++) {
-                const bool in = 64 * c + 16 * lg < hd;
-                kr[sp][c] = load_raw<FMT>(bk + ((size_t)(slk + 4 * sp) * hd + (in ? 64 * c + 16 * lg : 0)) * W);
-                if (!in)
-#pragma unroll
-                    for (int i = 0; i < (int)(sizeof(Raw<FMT>) / 16); i++) kr[sp][c].w[i] = u32x4{0, 0, 0, 0};
+        // where the lane's parts of block kb are
+        const uint8_t *bk, *bv;
+        int slk, slv, idk, idv;
+        auto place = [&](int kb) {
+            const int first = kb * KEYS;
+            const int i0 = first >> p.log_rows, i1 = (first + KEYS - N) >> p.log_rows;
+            if (i0 < ids0 || i1 >= ids0 + 64) {
+                ids0 = i0;
+                ids = pages[min(i0 + lane, p.ld - 1)];
             }
-        floatx4 stk[INTS ? 4 : 1], stv[INTS ? 4 : 1];
-        if constexpr (INTS) {
-            const float *steps = reinterpret_cast<const float *>(bv + 2 * (size_t)P * hd * W) + slv;
+            const int kk = first + N * (qi >> 2), kv = first + N * lg;  // the first keys of what the lane reads
+            idk = __shfl(ids, (kk >> p.log_rows) - ids0);
+            idv = __shfl(ids, (kv >> p.log_rows) - ids0);
+            // not one of the pool's, or behind the table's last: -1, and page 0 read instead
+            if ((unsigned)idk >= (unsigned)p.pages || kk >> p.log_rows >= p.ld) idk = -1;
+            if ((unsigned)idv >= (unsigned)p.pages || kv >> p.log_rows >= p.ld) idv = -1;
+            bk = p.pool + (size_t)max(idk, 0) * p.page_bytes + (size_t)h * p.head_bytes;
+            bv = p.pool + (size_t)max(idv, 0) * p.page_bytes + (size_t)h * p.head_bytes;
+            slk = (kk & (P - 1)) + (qi & 3);
+            slv = kv & (P - 1);
+        };
+        Raw<FMT, 2> kr[2 * KS][C];
+        Raw<FMT, KS> vr[M];
+        floatx4 stk[INTS ? N / 4 : 1], stv[INTS ? N / 4 : 1];
+        auto load_keys = [&] {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                stk[j] = reinterpret_cast<const floatx4 *>(steps)[j];
-                stv[j] = reinterpret_cast<const floatx4 *>(steps + P)[j];
+            for (int sp = 0; sp < 2 * KS; sp++)
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    const bool in = 64 * c + 16 * lg < hd;
+                    kr[sp][c] = load_raw<FMT, 2>(bk + ((size_t)(slk + 4 * sp) * hd + (in ? 64 * c + 16 * lg : 0)) * W);
+                }
+        };
+        auto load_values = [&] {
+#pragma unroll
+            for (int m = 0; m < M; m++)
+                vr[m] = load_raw<FMT, KS>(bv + ((size_t)P * hd + (size_t)(16 * m < hd ? 16 * m + qi : qi) * P + slv) * W);
+            if constexpr (INTS) {
+                const float *steps = reinterpret_cast<const float *>(bv + 2 * (size_t)P * hd * W) + slv;
+#pragma unroll
+                for (int j = 0; j < N / 4; j++) {
+                    stk[j] = reinterpret_cast<const floatx4 *>(steps)[j];
+                    stv[j] = reinterpret_cast<const floatx4 *>(steps + P)[j];
+                }
             }
-        }
+        };
+        while (kb < last) {
+            place(kb);
+            load_keys();
+            if constexpr (C * CT <= 2) load_values();
+            const int first = kb * KEYS, kv = first + N * lg;
+            const bool whole = first + KEYS <= tw.len && __all(idv >= 0);  // every key there is and on a page
+            // of the lane's N keys (values), how many there are
+            const int here = whole ? N : (idv >= 0 ? min(max(tw.len - kv, 0), N) : 0);
+            const bool all_seen = whole && first + KEYS <= lim_least;
+            // coordinates past the head's width; f32: keys that are not there, and the block's keys' power of two
+            int ek = 0;
+            if (hd & 63) {
 #pragma unroll
-        for (int m = 0; m < M; m++) {
-            const int dim = 16 * m + qi;
-            vr[m] = load_raw<FMT>(bv + ((size_t)P * hd + (size_t)(16 * m < hd ? dim : qi) * P + slv) * W);
-        }
-        // f32: the block's keys' power of two, those that are not there left out
-        int ek = 0;
-        if constexpr (!INTS) {
-            if (!whole) {
-                const int there = idk >= 0 ? tw.len - kk - (qi & 3) : 0;  // row of set sp is there: 4 sp < there
+                for (int sp = 0; sp < 2 * KS; sp++)
 #pragma unroll
-                for (int sp = 0; sp < 4; sp++)
-                    if (4 * sp >= there)
+                    for (int c = 0; c < C; c++)
+                        if (64 * c + 16 * lg >= hd)
 #pragma unroll
-                        for (int c = 0; c < C; c++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) kr[sp][c].w[i] = u32x4{0, 0, 0, 0};
+                            for (int i = 0; i < Raw<FMT, 2>::WORDS; i++) kr[sp][c].w[i] = 0;
             }
-            uint32_t most = 0;
+            if constexpr (!INTS) {
+                if (!whole) {
+                    const int there = idk >= 0 ? tw.len - first - N * (qi >> 2) - (qi & 3) : 0;  // row of set sp is: 4 sp < there
 #pragma unroll
-            for (int sp = 0; sp < 4; sp++)
+                    for (int sp = 0; sp < 2 * KS; sp++)
+                        if (4 * sp >= there)
 #pragma unroll
-                for (int c = 0; c < C; c++)
+                            for (int c = 0; c < C; c++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                                for (int i = 0; i < Raw<FMT, 2>::WORDS; i++) kr[sp][c].w[i] = 0;
+                }
+                uint32_t most = 0;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) most = max(most, finite_bits(kr[sp][c].w[i][e]));
-            ek = min(shift_for_max(wave_max(__uint_as_float(most))), 126);
-        }
-        const float fk = INTS ? 1.0f : pow2(ek), unk = INTS ? 1.0f : pow2(-ek);
-        floatx4 sc[4][CT];  // set sp = 2 s + p
-        const floatx4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int sp = 0; sp < 2 * KS; sp++)
 #pragma unroll
-        for (int sp = 0; sp < 4; sp++)
+                    for (int c = 0; c < C; c++)
+#pragma unroll
+                        for (int i = 0; i < Raw<FMT, 2>::WORDS; i++) most = max(most, finite_bits(kr[sp][c].w[i]));
+                ek = min(shift_for_max(wave_max(__uint_as_float(most))), 126);
+            }
+            const float fk = INTS ? 1.0f : pow2(ek), unk = INTS ? 1.0f : pow2(-ek);
+            floatx4 sc[2 * KS][CT];  // set sp = 2 s + p
+            const floatx4 none = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < C; c++)
 #pragma unroll
-                for (int ks = 0; ks < 2; ks++) {
-                    halfx8 hi, lo;
-                    to_halves<FMT>(kr[sp][c], ks, fk, hi, lo);
+                for (int ks = 0; ks < 2; ks++)
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++) {
-                        sc[sp][ct] = mfma(hi, qh[ct][c][ks], c + ks ? sc[sp][ct] : none);
-                        sc[sp][ct] = mfma(hi, ql[ct][c][ks], sc[sp][ct]);
-                        if constexpr (LO) sc[sp][ct] = mfma(lo, qh[ct][c][ks], sc[sp][ct]);
+                    for (int sp = 0; sp < 2 * KS; sp++) {
+                        halfx8 hi, lo;
+                        to_halves<FMT, 2>(kr[sp][c], ks, fk, hi, lo);
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++) {
+                            halfx8 qhi, qlo;
+                            if constexpr (WAIT) {
+                                qhi = waiting[64 * (4 * (ct * C + c) + 2 * ks)];
+                                qlo = waiting[64 * (4 * (ct * C + c) + 2 * ks + 1)];
+                            } else {
+                                qhi = qh[ct][c][ks];
+                                qlo = ql[ct][c][ks];
+                            }
+                            sc[sp][ct] = mfma(hi, qhi, c + ks ? sc[sp][ct] : none);
+                            sc[sp][ct] = mfma(hi, qlo, sc[sp][ct]);
+                            if constexpr (LO) sc[sp][ct] = mfma(lo, qhi, sc[sp][ct]);
+                            if constexpr (BYTES) sc[sp][ct] = mfma(lo, qlo, sc[sp][ct]);
+                        }
                     }
+            if constexpr (C * CT > 2) {  // no registers for them before
+                __builtin_amdgcn_sched_barrier(0);
+                load_values();
+            }
+            // the values' scale: ints by a power of two that no step passes, f32 by one that brings every value below 2^14
+            float vs = 1.0f;
+            uint32_t odd = 0;  // f32: whether a value is not finite
+            if constexpr (INTS) {
+                float most = 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    if (!whole && j >= here) stv[j >> 2][j & 3] = 0.0f;
+                    most = fmaxf(most, stv[j >> 2][j & 3]);
                 }
-        // the values' scale: ints by a power of two that no step passes, f32 by one that brings every value below 2^14
-        float vs = 1.0f;
-        uint32_t odd = 0;  // f32: whether a value is not finite
-        if constexpr (INTS) {
-            float most = 0.0f;
+                most = half_max(row_max(most));
+                const int e = most > 0.0f ? __builtin_amdgcn_frexp_expf(most) : -1000;
+                if (e > ev) {
+                    const float f = ev > -1000 ? pow2(ev - e) : 0.0f;
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                if (!whole && j >= here) stv[j >> 2][j & 3] = 0.0f;
-                most = fmaxf(most, stv[j >> 2][j & 3]);
-            }
-            most = half_max(row_max(most));
-            const int e = most > 0.0f ? __builtin_amdgcn_frexp_expf(most) : -1000;
-            if (e > ev) {
-                const float f = ev > -1000 ? pow2(ev - e) : 0.0f;
+                    for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int m = 0; m < M; m++) acc[ct][m] *= f;
-                ev = e;
-            }
-            vs = pow2(-max(ev, -126));
-        } else {
-            uint32_t most = 0;
-#pragma unroll
-            for (int m = 0; m < M; m++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (!whole && 4 * i + e >= here) vr[m].w[i][e] = 0;
-                        odd = max(odd, vr[m].w[i][e] & 0x7fffffffu);
-                        most = max(most, finite_bits(vr[m].w[i][e]));
-                    }
-            const int e = min(shift_for_max(wave_max(__uint_as_float(most))), 126);
-            if (e < ev) {
-                const float f = ev < 1000 ? pow2(e - ev) : 0.0f;
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int m = 0; m < M; m++) acc[ct][m] *= f;
-                ev = e;
-            }
-            vs = pow2(ev);
-        }
-        halfx8 ph[CT][2], pl[CT][2];
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            float x[16];
-            const float f = INTS ? to_log2[ct] : fminf(fmaxf(to_log2[ct] * unk, 0x1p-126f), 0x1p126f);
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                x[j] = sc[j >> 2][ct][j & 3];
-                if constexpr (INTS) x[j] *= stk[j >> 2][j & 3];
-            }
-            if (!all_seen) {
-                const int seen = min(here, min(max(limit[ct] - kv, 0), 16));
-#pragma unroll
-                for (int j = 0; j < 16; j++)
-                    if (j >= seen) x[j] = -INFINITY;
-            }
-            float mb = x[0];
-#pragma unroll
-            for (int j = 1; j < 16; j++) mb = fmaxf(mb, x[j]);
-            mb = half_max(row_max(mb)) * f;
-            const bool grow = mb > ref[ct] + 3.0f;
-            if (__any(grow)) {
-                const float nref = grow ? mb : ref[ct];
-                const float alpha = grow ? exp2_hw(ref[ct] - nref) : 1.0f;
-                l[ct] *= alpha;
-#pragma unroll
-                for (int m = 0; m < M; m++) acc[ct][m] *= alpha;
-                ref[ct] = nref;
-            }
-            const float off = ref[ct] == -INFINITY ? 0.0f : 12.0f - ref[ct];
-#pragma unroll
-            for (int s = 0; s < 2; s++) {
-                u32x4 hw, lw;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int j = 8 * s + 2 * i;
-                    float p0 = exp2_hw(fmaf(x[j], f, off)), p1 = exp2_hw(fmaf(x[j + 1], f, off));
-                    l[ct] += p0 + p1;
-                    if constexpr (INTS) {
-                        p0 *= stv[j >> 2][j & 3] * vs;
-                        p1 *= stv[j >> 2][(j + 1) & 3] * vs;
-                    }
-                    uint32_t a, b;
-                    split2(p0, p1, a, b);
-                    hw[i] = a;
-                    lw[i] = b;
+                        for (int m = 0; m < M; m++) acc[ct][m] *= f;
+                    ev = e;
                 }
-                ph[ct][s] = __builtin_bit_cast(halfx8, hw);
-                pl[ct][s] = __builtin_bit_cast(halfx8, lw);
-            }
-        }
-        // values that are not finite: zeros in the products, and what sees one is no number
-        if constexpr (!INTS) {
-            if (__any(odd >= 0x7f800000u)) {
-                const _Float16 one = (_Float16)1.0f, zero = (_Float16)0.0f;
+                vs = pow2(-max(ev, -126));
+            } else {
+                uint32_t most = 0;
 #pragma unroll
                 for (int m = 0; m < M; m++)
 #pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        halfx8 bad;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const uint32_t w = vr[m].w[2 * s + (e >> 2)][e & 3];
-                            const bool b = (w & 0x7fffffffu) >= 0x7f800000u;
-                            bad[e] = b ? one : zero;
-                            vr[m].w[2 * s + (e >> 2)][e & 3] = b ? 0u : w;
-                        }
-#pragma unroll
-                        for (int ct = 0; ct < CT; ct++) {
-                            const int seen = min(here, min(max(limit[ct] - kv, 0), 16));
-                            halfx8 sees;
-#pragma unroll
-                            for (int e = 0; e < 8; e++) sees[e] = 8 * s + e < seen ? one : zero;
-                            const floatx4 n = mfma(bad, sees, none);
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                if (n[i] > 0.0f) acc[ct][m][i] = NAN;
-                        }
+                    for (int i = 0; i < N; i++) {
+                        if (!whole && i >= here) vr[m].w[i] = 0;
+                        odd = max(odd, vr[m].w[i] & 0x7fffffffu);
+                        most = max(most, finite_bits(vr[m].w[i]));
                     }
+                const int e = min(shift_for_max(wave_max(__uint_as_float(most))), 126);
+                if (e < ev) {
+                    const float f = ev < 1000 ? pow2(e - ev) : 0.0f;
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                        for (int m = 0; m < M; m++) acc[ct][m] *= f;
+                    ev = e;
+                }
+                vs = pow2(ev);
             }
-        }
+            halfx8 ph[CT][KS], pl[CT][KS];
 #pragma unroll
-        for (int m = 0; m < M; m++) {
-            if (16 * m >= hd) break;
+            for (int ct = 0; ct < CT; ct++) {
+                float x[N];
+                const float f = INTS ? to_log2[ct] : fminf(fmaxf(to_log2[ct] * unk, 0x1p-126f), 0x1p126f);
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
-                halfx8 hi, lo;
-                to_halves<FMT>(vr[m], s, vs, hi, lo);
+                for (int j = 0; j < N; j++) {
+                    x[j] = sc[j >> 2][ct][j & 3];
+                    if constexpr (INTS) x[j] *= stk[j >> 2][j & 3];
+                }
+                if (!all_seen) {
+                    const int seen = min(here, min(max(limit[ct] - kv, 0), N));
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) {
-                    acc[ct][m] = mfma(hi, ph[ct][s], acc[ct][m]);
-                    acc[ct][m] = mfma(hi, pl[ct][s], acc[ct][m]);
-                    if constexpr (LO) acc[ct][m] = mfma(lo, ph[ct][s], acc[ct][m]);
+                    for (int j = 0; j < N; j++)
+                        if (j >= seen) x[j] = -INFINITY;
+                }
+                float mb = x[0];
+#pragma unroll
+                for (int j = 1; j < N; j++) mb = fmaxf(mb, x[j]);
+                mb = half_max(row_max(mb)) * f;
+                const bool grow = mb > ref[ct] + 3.0f;
+                if (__any(grow)) {
+                    const float nref = grow ? mb : ref[ct];
+                    const float alpha = grow ? exp2_hw(ref[ct] - nref) : 1.0f;
+                    l[ct] *= alpha;
+#pragma unroll
+                    for (int m = 0; m < M; m++) acc[ct][m] *= alpha;
+                    ref[ct] = nref;
+                }
+                const float off = ref[ct] == -INFINITY ? 0.0f : 12.0f - ref[ct];
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    u32x4 hw, lw;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int j = 8 * s + 2 * i;
+                        float p0 = exp2_hw(fmaf(x[j], f, off)), p1 = exp2_hw(fmaf(x[j + 1], f, off));
+                        l[ct] += p0 + p1;
+                        if constexpr (INTS) {
+                            p0 *= stv[j >> 2][j & 3] * vs;
+                            p1 *= stv[j >> 2][(j + 1) & 3] * vs;
+                        }
+                        uint32_t a, b;
+                        split2(p0, p1, a, b);
+                        hw[i] = a;
+                        lw[i] = b;
+                    }
+                    ph[ct][s] = __builtin_bit_cast(halfx8, hw);
+                    pl[ct][s] = __builtin_bit_cast(halfx8, lw);
                 }
             }
+            // values that are not finite: zeros in the products, and what sees one is no number
+            if constexpr (!INTS) {
+                if (__any(odd >= 0x7f800000u)) {
+                    const _Float16 one = (_Float16)1.0f, zero = (_Float16)0.0f;
+#pragma unroll
+                    for (int m = 0; m < M; m++)
+#pragma unroll
+                        for (int s = 0; s < KS; s++) {
+                            halfx8 bad;
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                const uint32_t w = vr[m].w[8 * s + e];
+                                const bool b = (w & 0x7fffffffu) >= 0x7f800000u;
+                                bad[e] = b ? one : zero;
+                                vr[m].w[8 * s + e] = b ? 0u : w;
+                            }
+#pragma unroll
+                            for (int ct = 0; ct < CT; ct++) {
+                                const int seen = min(here, min(max(limit[ct] - kv, 0), N));
+                                halfx8 sees;
+#pragma unroll
+                                for (int e = 0; e < 8; e++) sees[e] = 8 * s + e < seen ? one : zero;
+                                const floatx4 n = mfma(bad, sees, none);
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    if (n[i] > 0.0f) acc[ct][m][i] = NAN;
+                            }
+                        }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+                if (16 * m >= hd) break;
+                __builtin_amdgcn_sched_barrier(0);  // a set's halves at a time: all at once they do not fit the registers
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    halfx8 hi, lo;
+                    to_halves<FMT, KS>(vr[m], s, vs, hi, lo);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) {
+                        acc[ct][m] = mfma(hi, ph[ct][s], acc[ct][m]);
+                        acc[ct][m] = mfma(hi, pl[ct][s], acc[ct][m]);
+                        if constexpr (LO) acc[ct][m] = mfma(lo, ph[ct][s], acc[ct][m]);
+                        if constexpr (BYTES) acc[ct][m] = mfma(lo, pl[ct][s], acc[ct][m]);
+                    }
+                }
+            }
+            kb += step;
         }
-    };
-    // blocks b0 <= kb < b1 of the unit, every `step`th; those behind every column's limit are not looked at
-    auto blocks = [&](int b0, int b1, int step) {
-        ids0 = -64;
-        b1 = min(b1, (lim_most + 63) >> 6);
-        for (int kb = b0; kb < b1; kb += step) block(kb);
-    };
-    // acc over l is in units of this
-    auto unit_value = [&] { return INTS ? (ev > -1000 ? pow2(ev) : 0.0f) : pow2(-min(ev, 149)); };
-
-    seek(wg0);
-    const uint32_t unit0 = (wg0 - before) / tw.nb, u0 = before + unit0 * tw.nb;
-    if (wg1 <= u0 + tw.nb && wg1 - wg0 > 1) {
-        // the workgroup's blocks are one unit's: its wavefronts take them in turn and join what they have
-        begin(unit0);
-        blocks((int)(wg0 - u0) + wave, (int)(wg1 - u0), WAVES);
-        const bool done = wg0 == u0 && wg1 == u0 + tw.nb;
-        const float unit = unit_value();
+        at += b1 - b0;
+        // the sums over the weights' sum, in their own units
+        const float uv = (BYTES ? 256.0f : 1.0f) * (INTS ? (ev > -1000 ? pow2(ev) : 0.0f) : pow2(-min(ev, 149)));
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             const float lw = half_sum(row_sum(l[ct]));
             const float inv = lw > 0.0f ? 1.0f / lw : lw;  // 0 and NaN stay
+            if (!together) {
+                const size_t own = 2 * (size_t)me + (at - (b1 - b0) == mine ? 0 : 1);
+                const int col = 16 * ct + qi, c = tile * COLS + col, i = c / group;
+                if (done && i >= tw.n) continue;
+                float *dst = done ? out + (size_t)(tw.first + i) * heads * hd + (size_t)(h * group + c - i * group) * hd
+                                  : parts.o + (own * COLS + col) * hd;
+#pragma unroll
+                for (int m = 0; m < M; m++)
+                    if (16 * m < hd) {
+                        const floatx4 o = acc[ct][m] * inv * uv;
+                        *reinterpret_cast<floatx4u *>(dst + 16 * m + 4 * lg) = o;
+                    }
+                if (!done && lg == 0) parts.ml[own * COLS + col] = make_float2(ref[ct], lw);
+                continue;
+            }
             if (lg == 0) {
                 mref[wave][16 * ct + qi] = ref[ct];
                 msum[wave][16 * ct + qi] = lw;
             }
-            if (ct) __syncthreads();
+            if (WAIT || ct) __syncthreads();
 #pragma unroll
             for (int m = 0; m < M; m++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) macc[wave][16 * m + 4 * lg + i][qi] = acc[ct][m][i] * inv * unit;
+                for (int i = 0; i < 4; i++) macc[wave][16 * m + 4 * lg + i][qi] = acc[ct][m][i] * inv * uv;
             __syncthreads();
-            // thread t: column t / 32, coordinates t % 32 + 32 ..
-            const int c16 = tid >> 5, col = 16 * ct + c16;
+            // 64 WAVES / 16 threads a column
+            constexpr int TH = 4 * WAVES;
+            const int c16 = tid / TH, col = 16 * ct + c16, c = tile * COLS + col, i = c / group;
             float m = -INFINITY, L = 0.0f, f[WAVES];
 #pragma unroll
             for (int w = 0; w < WAVES; w++)
                 if (msum[w][col] > 0.0f) m = fmaxf(m, mref[w][col]);
 #pragma unroll
             for (int w = 0; w < WAVES; w++) {
-                const float s = msum[w][col];
-                f[w] = s > 0.0f ? s * exp2_hw(mref[w][col] - m) : s;
+                const float sw = msum[w][col];
+                f[w] = sw > 0.0f ? sw * exp2_hw(mref[w][col] - m) : sw;
                 L += f[w];
             }
             const float Li = L > 0.0f ? 1.0f / L : L;
-            const int at = tile * COLS + col, i = at / group;
-            const size_t slot = 2 * (size_t)(blockIdx.x * WAVES);
-            for (int dim = tid & 31; dim < hd; dim += 32) {
+            const size_t own = 2 * (size_t)(blockIdx.x * WAVES);
+            for (int dim = tid % TH; dim < hd; dim += TH) {
                 float o = 0.0f;
 #pragma unroll
                 for (int w = 0; w < WAVES; w++)
                     if (msum[w][col] != 0.0f) o += f[w] * macc[w][dim][c16];
                 o *= Li;
-                if (done) {
-                    if (i < tw.n) out[(size_t)(tw.first + i) * heads * hd + (size_t)(h * group + at - i * group) * hd + dim] = o;
-                } else {
-                    parts.o[(slot * COLS + col) * hd + dim] = o;
-                }
+                if (!done)
+                    parts.o[(own * COLS + col) * hd + dim] = o;
+                else if (i < tw.n)
+                    out[(size_t)(tw.first + i) * heads * hd + (size_t)(h * group + c - i * group) * hd + dim] = o;
             }
-            if (!done && (tid & 31) < WAVES)
-                parts.ml[(slot + 2 * (tid & 31)) * COLS + col] = (tid & 31) ? make_float2(-INFINITY, 0.0f) : make_float2(m, L);
+            if (!done && tid % TH == 0) parts.ml[own * COLS + col] = make_float2(m, L);
         }
-        return;
-    }
-    // every wavefront its own blocks
-    uint32_t at = wg0 + wave * per;
-    const uint32_t end = min(total, at + per);
-    const uint32_t mine = at;
-    while (at < end) {
-        seek(at);
-        const uint32_t unit = (at - before) / tw.nb, b0 = at - before - unit * tw.nb;
-        const uint32_t b1 = min((uint32_t)tw.nb, b0 + (end - at));
-        begin(unit);
-        blocks((int)b0, (int)b1, 1);
-        const bool done = b0 == 0 && b1 == (uint32_t)tw.nb;
-        const float uv = unit_value();
-        const size_t slot = 2 * (size_t)me + (at == mine ? 0 : 1);
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            const float lw = half_sum(row_sum(l[ct]));
-            const float inv = lw > 0.0f ? 1.0f / lw : lw;
-            const int col = 16 * ct + qi, c = tile * COLS + col, i = c / group;
-            if (done && i >= tw.n) continue;
-            float *dst = done ? out + (size_t)(tw.first + i) * heads * hd + (size_t)(h * group + c - i * group) * hd
-                              : parts.o + (slot * COLS + col) * hd;
-#pragma unroll
-            for (int m = 0; m < M; m++)
-                if (16 * m < hd) {
-                    floatx4 o = acc[ct][m] * inv * uv;
-                    *reinterpret_cast<floatx4u *>(dst + 16 * m + 4 * lg) = o;
-                }
-            if (!done && lg == 0) parts.ml[slot * COLS + col] = make_float2(ref[ct], lw);
-        }
-        at += b1 - b0;
+        if (together) break;
     }
 }
 
-// grid (queries x heads); 256 threads: the states that wavefronts left of one query and head, together. A unit that one run held
-// whole has its output already.
-template <int CT>
-__global__ __launch_bounds__(256) void k_pages_join(PageSet p, const int32_t *__restrict__ lengths, const int32_t *__restrict__ offsets,
-                                                    int nq, int heads, uint32_t waves, float *__restrict__ out, Parts parts) {
-    constexpr int COLS = 16 * CT;
+// grid (queries x heads, over 4 / PER); 256 threads: the states that runs of blocks left of a query and head, together: PER
+// wavefronts for each query and head, every PER-th state each. Four where there are few (a state after the other takes longest),
+// one where there are many (their number does).
+template <int CT, int PER>
+__global__ __launch_bounds__(256) void k_pages_join(int tables, int hd, const int32_t *__restrict__ offsets, int items,
+                                                    int heads, float *__restrict__ out, Parts parts) {
+    constexpr int COLS = 16 * CT, AHEAD = 8;
     __shared__ float wm[4], wl[4], wo[4][128];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = heads / p.heads, hd = p.hd;
-    const int r = blockIdx.x / heads, head = blockIdx.x - r * heads;
-    // the table of the query: so many tables' queries end at or before it
-    int t = 0;
-    for (int t0 = 0; t0 < p.tables - 1; t0 += 64) t += __popcll(__ballot(t0 + lane < p.tables - 1 && offsets[t0 + lane + 1] <= r));
-    const TableWork tw = table_work(p, lengths, offsets, nq, group, COLS, t);
-    if (r < tw.first || r >= tw.first + tw.n) return;
-    const uint32_t per = parts.plan[0], total = parts.plan[1 + p.tables];
-    if (total == 0) return;
-    const int h = head / group, c = (r - tw.first) * group + head - h * group, tile = c / COLS, col = c - tile * COLS;
-    const uint32_t u0 = parts.plan[1 + t] + ((uint32_t)tile * p.heads + h) * tw.nb, u1 = u0 + tw.nb;
-    const uint32_t w0 = u0 / per, w1 = (u1 - 1) / per;
-    if (w0 == w1) return;
-    if (u0 % per == 0 && w0 % WAVES == 0 && u1 <= (w0 + WAVES) * per) {
-        // one workgroup may have held it whole, with its wavefronts in turn
-        const uint32_t wg0 = w0 * per, wg1 = min(total, wg0 + WAVES * per);
-        if (wg1 == u1) return;
-    }
-    float M = -INFINITY, L = 0.0f, o[2] = {0.0f, 0.0f};
-    for (uint32_t b = w0 + 64 * wave; b <= w1; b += 256) {
-        const uint32_t w = b + lane;
-        const size_t slot = 2 * (size_t)w + (w == w0 && u0 > w0 * per ? 1 : 0);
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        if (w <= w1) ml = parts.ml[slot * COLS + col];
-        const float m = wave_max(ml.y > 0.0f ? ml.x : -INFINITY);
-        const float top = fmaxf(M, m);
-        const float f = ml.y > 0.0f ? ml.y * exp2_hw(ml.x - top) : ml.y;
-        const float old = M == -INFINITY ? 0.0f : exp2_hw(M - top);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int item = PER == 4 ? blockIdx.x : blockIdx.x * 4 + wave, part = PER == 4 ? wave : 0;
+    if (item >= items) return;
+    const uint4 unit = parts.units[item];
+    const uint32_t per = parts.plan[0], total = parts.plan[1], u0 = unit.x, u1 = unit.y, col = unit.w;
+    // of no table (what its place holds is another call's); there already
+    if (item / heads >= offsets[tables] || unit.z != per || u1 > total || u0 >= u1 || col >= COLS) return;
+    const uint32_t w0 = u0 / per, w1 = (u1 - 1) / per, g0 = w0 / WAVES, g1 = w1 / WAVES;
+    // the states: the first workgroup's, a wavefront each or one for all, one of each workgroup between, the last one's
+    auto together = [&](uint32_t g) {
+        const uint32_t a = g * WAVES * per, b = min(total, a + WAVES * per);
+        return b - a > 1 && a >= u0 && b <= u1;
+    };
+    const uint32_t n0 = together(g0) ? 1 : min(w1, g0 * WAVES + WAVES - 1) - w0 + 1;
+    const uint32_t n1 = g1 > g0 ? g1 - g0 - 1 : 0, n2 = g1 > g0 ? (together(g1) ? 1 : w1 - g1 * WAVES + 1) : 0;
+    const uint32_t count = n0 + n1 + n2;
+    auto slot = [&](uint32_t e) {
+        const uint32_t w = e < n0 ? w0 + e : (e < n0 + n1 ? (g0 + 1 + e - n0) * WAVES : g1 * WAVES + e - n0 - n1);
+        return 2 * (size_t)w + (w == w0 && u0 > w0 * per ? 1 : 0);
+    };
+    float M = -INFINITY, L = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    const int d0 = min(lane, hd - 1), d1 = min(64 + lane, hd - 1);
+    for (uint32_t e = part; e < count; e += PER * AHEAD) {
+        float2 ml[AHEAD];
+        float x0[AHEAD], x1[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            // past the last: the last again, without weight
+            const size_t at = slot(min(e + PER * i, count - 1)) * COLS + col;
+            ml[i] = parts.ml[at];
+            x0[i] = parts.o[at * hd + d0];
+            x1[i] = hd > 64 ? parts.o[at * hd + d1] : 0.0f;
+            if (e + PER * i >= count) ml[i] = make_float2(-INFINITY, 0.0f);
+        }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (ml[i].y > 0.0f) top = fmaxf(top, ml[i].x);
+        const float old = M == -INFINITY ? 1.0f : exp2_hw(M - top);  // nothing yet, or NaN
         L *= old;
-        o[0] *= old;
-        o[1] *= old;
+        o0 *= old;
+        o1 *= old;
         M = top;
-        uint64_t live = __ballot(ml.y != 0.0f);
-        while (live) {
-            const int j = __ffsll((unsigned long long)live) - 1;
-            live &= live - 1;
-            const float fj = __shfl(f, j);
-            const size_t sj = 2 * (size_t)(b + j) + (b + j == w0 && u0 > w0 * per ? 1 : 0);
-            const float *src = parts.o + (sj * COLS + col) * hd;
-            L += fj;
-            if (lane < hd) o[0] += fj * src[lane];
-            if (64 + lane < hd) o[1] += fj * src[64 + lane];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            if (ml[i].y == 0.0f) continue;
+            const float f = ml[i].y > 0.0f ? ml[i].y * exp2_hw(ml[i].x - M) : ml[i].y;
+            L += f;
+            o0 += f * x0[i];
+            o1 += f * x1[i];
         }
     }
-    wo[wave][lane] = o[0];
-    wo[wave][64 + lane] = o[1];
-    if (lane == 0) {
-        wm[wave] = M;
-        wl[wave] = L;
-    }
-    __syncthreads();
-    if (wave > 0) return;
-    const float top = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-    L = o[0] = o[1] = 0.0f;
-    for (int w = 0; w < 4; w++) {
-        if (wl[w] == 0.0f) continue;
-        const float f = wm[w] == -INFINITY ? 1.0f : exp2_hw(wm[w] - top);
-        L += wl[w] * f;
-        o[0] += wo[w][lane] * f;
-        o[1] += wo[w][64 + lane] * f;
+    if constexpr (PER == 4) {
+        wo[wave][lane] = o0;
+        wo[wave][64 + lane] = o1;
+        if (lane == 0) {
+            wm[wave] = M;
+            wl[wave] = L;
+        }
+        __syncthreads();
+        if (wave > 0) return;
+        const float top = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+        L = o0 = o1 = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            if (wl[w] == 0.0f) continue;
+            const float f = wm[w] == -INFINITY ? 1.0f : exp2_hw(wm[w] - top);
+            L += wl[w] * f;
+            o0 += wo[w][lane] * f;
+            o1 += wo[w][64 + lane] * f;
+        }
     }
     const float inv = L > 0.0f ? 1.0f / L : L;
-    float *dst = out + (size_t)r * heads * hd + (size_t)head * hd;
-    if (lane < hd) dst[lane] = o[0] * inv;
-    if (64 + lane < hd) dst[64 + lane] = o[1] * inv;
+    float *dst = out + (size_t)item * hd;
+    if (lane < hd) dst[lane] = o0 * inv;
+    if (64 + lane < hd) dst[64 + lane] = o1 * inv;
 }
 
-// Sets of 16 columns that share what a wavefront reads, and the workgroups: one a compute unit, fewer where there may not be a
-// block for each of their wavefronts.
+// Keys of a block: 64, or 32 where a wavefront's registers do not hold more (C parts of 64 coordinates, CT sets of 16 columns).
+constexpr int block_keys(int fmt, int C, int CT) {
+    const int bytes = page_width(fmt) * C;
+    return bytes > 2 || (bytes == 2 && C * CT == 4) ? 32 : 64;
+}
+
+// Sets of 16 columns that share what a wavefront reads (f32 heads over 64 wide: no registers for two); workgroups, two a compute
+// unit, fewer where there may not be a block for each of their wavefronts.
 struct Shape {
     int sets, wgs;
-    size_t o_floats, ml_count;
+    size_t o_floats, ml_count, units;
     uint64_t blocks;  // at most
 };
 
-Shape shape(const PageSet &p, int nq, int heads) {
+Shape shape(int fmt, const PageSet &p, int nq, int heads) {
     Shape s;
     const int64_t group = heads / p.heads, columns = (int64_t)nq * group;
-    s.sets = columns > 16 * (int64_t)p.tables ? 2 : 1;
+    s.sets = columns > 16 * (int64_t)p.tables && (fmt != TAH_KV_F32 || p.hd <= 64) ? 2 : 1;
+    const int keys = block_keys(fmt, p.hd > 64 ? 2 : 1, s.sets);
     const uint64_t rows = std::min((uint64_t)p.ld << p.log_rows, (uint64_t)0x7fffffff - 64);
     const uint64_t units = ((uint64_t)std::min(p.tables, nq) + columns / (16 * s.sets)) * p.heads;
-    const uint64_t nb = std::max<uint64_t>(1, (rows + 63) / 64);
+    const uint64_t nb = (rows + keys - 1) / keys + BEGIN;
     s.blocks = units > (uint64_t(1) << 32) ? ~uint64_t(0) : units * nb;
-    s.wgs = (int)std::min<uint64_t>(256, (s.blocks + WAVES - 1) / WAVES);
+    s.wgs = (int)std::min<uint64_t>(512, (s.blocks + WAVES - 1) / WAVES);
     const size_t slots = 2 * (size_t)s.wgs * WAVES;
     s.o_floats = slots * 16 * s.sets * p.hd;
     s.ml_count = slots * 16 * s.sets;
+    s.units = (size_t)nq * heads;
     return s;
 }
 
 template <int FMT, int C, int CT>
 void launch(hipStream_t s, const PageSet &p, const int32_t *lengths, const float *q, const int32_t *offsets, int nq, int heads,
             bool causal, size_t q_ld, float *out, const Parts &parts, const Shape &sh) {
-    hipLaunchKernelGGL((k_pages_attend<FMT, C, CT>), dim3(sh.wgs), dim3(64 * WAVES), 0, s, p, lengths, q, offsets, nq,
-                       heads, causal ? 1 : 0, q_ld, out, parts, sh.blocks);
+    hipLaunchKernelGGL((k_pages_attend<FMT, C, CT, block_keys(FMT, C, CT) / 32>), dim3(sh.wgs), dim3(64 * WAVES), 0, s, p, lengths, q,
+                       offsets, nq, heads, causal ? 1 : 0, q_ld, out, parts, sh.blocks);
     TAH_LAUNCHED();
-    hipLaunchKernelGGL(k_pages_join<CT>, dim3((unsigned)nq * heads), dim3(256), 0, s, p, lengths, offsets, nq, heads,
-                       (uint32_t)sh.wgs * WAVES, out, parts);
-    TAH_LAUNCHED();
-}
-
-template <int FMT, int C>
-void launch_sets(hipStream_t s, const PageSet &p, const int32_t *lengths, const float *q, const int32_t *offsets, int nq,
-                 int heads, bool causal, size_t q_ld, float *out, const Parts &parts, const Shape &sh) {
-    if (sh.sets == 1)
-        launch<FMT, C, 1>(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh);
+    const int items = nq * heads;
+    if (items <= 1024)
+        hipLaunchKernelGGL((k_pages_join<CT, 4>), dim3(items), dim3(256), 0, s, p.tables, p.hd, offsets, items, heads, out, parts);
     else
-        launch<FMT, C, 2>(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh);
+        hipLaunchKernelGGL((k_pages_join<CT, 1>), dim3((items + 3) / 4), dim3(256), 0, s, p.tables, p.hd, offsets, items, heads, out, parts);
+    TAH_LAUNCHED();
 }
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 }  // namespace
 
-size_t pages_attend_work_bytes(const PageSet &p, int nq, int heads) {
-    const Shape s = shape(p, nq, heads);
+size_t pages_attend_work_bytes(int fmt, const PageSet &p, int nq, int heads) {
+    const Shape s = shape(fmt, p, nq, heads);
     // the kernels number all units' blocks in 32 bits
     if (s.blocks >= (uint64_t(1) << 31)) throw ArgError{"pages_attend: more rows than a call takes: fewer tables a call"};
-    return up256(s.o_floats * sizeof(float)) + up256(s.ml_count * sizeof(float2)) + up256(((size_t)p.tables + 2) * sizeof(uint32_t));
+    return up256(s.o_floats * sizeof(float)) + up256(s.ml_count * sizeof(float2)) + up256(s.units * sizeof(uint4)) + 256;
 }
 
 void pages_attend(hipStream_t s, int fmt, const PageSet &p, const int32_t *lengths, const float *q, const int32_t *offsets, int nq,
                   int heads, bool causal, size_t q_ld, float *out, void *work) {
-    const Shape sh = shape(p, nq, heads);
+    const Shape sh = shape(fmt, p, nq, heads);
     uint8_t *at = static_cast<uint8_t *>(work);
     Parts parts;
     parts.o = reinterpret_cast<float *>(at);
     parts.ml = reinterpret_cast<float2 *>(at += up256(sh.o_floats * sizeof(float)));
-    parts.plan = reinterpret_cast<uint32_t *>(at + up256(sh.ml_count * sizeof(float2)));
-    auto with = [&](auto f) {
-        constexpr int FMT = decltype(f)::value;
-        if (p.hd <= 64)
-            launch_sets<FMT, 1>(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh);
-        else
-            launch_sets<FMT, 2>(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh);
-    };
+    parts.units = reinterpret_cast<uint4 *>(at += up256(sh.ml_count * sizeof(float2)));
+    parts.plan = reinterpret_cast<uint32_t *>(at + up256(sh.units * sizeof(uint4)));
+    auto go = [&](auto kernel) { kernel(s, p, lengths, q, offsets, nq, heads, causal, q_ld, out, parts, sh); };
+    const bool wide = p.hd > 64, two = sh.sets == 2;
     if (fmt == TAH_KV_F32)
-        with(std::integral_constant<int, TAH_KV_F32>{});
+        wide ? go(launch<TAH_KV_F32, 2, 1>) : (two ? go(launch<TAH_KV_F32, 1, 2>) : go(launch<TAH_KV_F32, 1, 1>));
     else if (fmt == TAH_KV_I16)
-        with(std::integral_constant<int, TAH_KV_I16>{});
+        wide ? (two ? go(launch<TAH_KV_I16, 2, 2>) : go(launch<TAH_KV_I16, 2, 1>))
+             : (two ? go(launch<TAH_KV_I16, 1, 2>) : go(launch<TAH_KV_I16, 1, 1>));
     else
-        with(std::integral_constant<int, TAH_KV_I8>{});
+        wide ? (two ? go(launch<TAH_KV_I8, 2, 2>) : go(launch<TAH_KV_I8, 2, 1>))
+             : (two ? go(launch<TAH_KV_I8, 1, 2>) : go(launch<TAH_KV_I8, 1, 1>));
 }
 
 }  // namespace tah
