@@ -12,6 +12,19 @@ namespace tah {
 
 namespace {
 
+// What the attention's workgroups do (k_packed): of each head's units, `own` are a workgroup's each; the blocks of the others, `rest` of
+// a head from block own_blocks on, go in `runs` runs of `per`.
+struct PackedPlan {
+    uint32_t own, own_blocks, rest, per, runs;
+};
+
+// A unit that several runs have parts of, from the one it begins in (slot) to last_run: its queries from row on, `live` of them, and
+// its head. live 0: there is none.
+struct CutUnit {
+    uint32_t slot, last_run;
+    int row, live, head;
+};
+
 struct Packed {
     const float *q, *k, *v;
     const int32_t *qo, *ko;
@@ -19,15 +32,20 @@ struct Packed {
     size_t q_ld, kv_ld;
     float *out;
     // working memory: the tiles, per tile the keys' and the values' power of two (twice it, and 1 if a value is not finite), which
-    // keys of each coordinate hold values that are not, the tables' first blocks, the key ranges' states
+    // keys of each coordinate hold values that are not; the attention's plan, and per table its first block of rows, and for one head the
+    // tiles of queries of the tables before it and those tiles' blocks (tables + 1)
     int blocks;  // room for so many
     uint8_t *tiles;
     int *shifts;
     uint64_t *odd;
-    uint32_t *first;
-    int splits;
+    PackedPlan *plan;
+    uint32_t *first, *tile_sums, *block_sums;
+    // the attention's runs of blocks, and per slot (two a run) [queries][hd] outputs and [queries] (maximum, sum); per run the unit
+    // that begins in it and ends in a later one
+    int waves, runs;
     float *part_o;
     float2 *part_ml;
+    CutUnit *cut;
 };
 
 // rows [a, a + n) of table t, cut to what there are
@@ -56,6 +74,104 @@ __device__ __forceinline__ int table_with(const int32_t *offsets, int tables, in
     return -1;
 }
 
+// What beginning and ending a unit costs, in blocks; and a unit of so many blocks is not cut.
+constexpr int BEGIN = 1, WHOLE = 8;
+
+// A table's tiles of queries in the order in which they are taken (causal: the last first, which have the most to do), the blocks of
+// tile i and of all tiles before it (BEGIN more for each).
+template <int QT>
+struct Tiles {
+    int n_q, n_k, causal;
+    __device__ __forceinline__ int count() const { return (n_q + QT - 1) / QT; }
+    __device__ __forceinline__ int first_query(int i) const { return (causal ? count() - 1 - i : i) * QT; }
+    __device__ __forceinline__ int all() const { return (n_k + KB - 1) / KB; }
+    // causal, by place: tile j's last query sees the rows but those of the queries behind it, so its blocks are ahead() + (j + 1) QT /
+    // KB, none below 0, but for the last tile, which ends with the last query
+    __device__ __forceinline__ int ahead() const { return (n_k - n_q + KB - 1) >> 6; }
+    __device__ __forceinline__ int blocks(int i) const {
+        return !causal || i == 0 ? all() : max(0, ahead() + (count() - i) * (QT / KB));
+    }
+    __device__ __forceinline__ uint64_t before(int i) const {
+        if (!causal || i == 0) return (uint64_t)i * (all() + BEGIN);
+        // places count() - i .. count() - 2, and the last
+        const long a = ahead(), m = QT / KB, j1 = count() - 1, low = count() - i;
+        const long j0 = a >= 0 ? low : max(low, min(j1, -a / m));
+        const long sum = (j1 - j0) * a + m * ((j1 * (j1 + 1) - j0 * (j0 + 1)) / 2);
+        return (uint64_t)(sum + all() + (long)i * BEGIN);
+    }
+};
+
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {  // of numbers below 2^50
+    const uint32_t lo = wave_scan((uint32_t)v & 0x1ffffffu), hi = wave_scan((uint32_t)(v >> 25));
+    return ((uint64_t)hi << 25) + lo;
+}
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int l) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), l) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, l);
+}
+
+// One wavefront: the attention's plan for tiles of QT queries. As many units of each head as make whole rounds of p.runs workgroups are
+// a workgroup's each, one round less where they are of different lengths (there have to be enough blocks in runs to fill the places
+// that end first); all of them where units are short, or blocks too many for 32 bits.
+template <int QT>
+__device__ void make_plan(const Packed &p) {
+    const int lane = threadIdx.x & 63;
+    uint64_t rows = 0, units = 0, blocks = 0;
+    int longest = 0, shortest = 0x7fffff;
+    for (int t0 = 0; t0 < p.tables; t0 += 64) {
+        const int t = min(t0 + lane, p.tables - 1);
+        const bool in = t0 + lane < p.tables;
+        int qa = 0, ka = 0;
+        const int n_q = rows_of(p.qo, t, p.nq, qa), n_t = rows_of(p.ko, t, p.nkv, ka);
+        const uint32_t nb = in ? (n_t + KB - 1) / KB : 0;
+        const uint64_t before = rows + wave_scan(nb) - nb;  // of 64 tables: below 2^32
+        if (in) p.first[t] = (uint32_t)min(before, (uint64_t)0x7fffffff);
+        rows = lane64(before + nb, 63);
+        // a table past the room that the offsets' promise gives has no rows
+        const Tiles<QT> ts{n_q, before + nb <= (uint64_t)p.blocks ? n_t : 0, p.causal};
+        const uint64_t tiles = in ? ts.count() : 0, cost = in ? ts.before(ts.count()) : 0;
+        const uint64_t tile_sum = units + wave_scan64(tiles), block_sum = blocks + wave_scan64(cost);
+        if (in) {
+            p.tile_sums[t] = (uint32_t)(tile_sum - tiles);
+            p.block_sums[t] = (uint32_t)min(block_sum - cost, (uint64_t)0xffffffff);
+        }
+        units = lane64(tile_sum, 63);
+        blocks = lane64(block_sum, 63);
+        if (tiles) {
+            longest = max(longest, ts.all());
+            shortest = min(shortest, ts.all());
+        }
+    }
+    longest = (int)wave_max((float)longest);
+    shortest = (int)-wave_max(-(float)shortest);
+    const uint64_t rounds = units * p.heads / p.runs;
+    const bool even = !p.causal && shortest + 1 >= longest;
+    uint64_t own = rounds * p.runs / p.heads;
+    if (longest <= WHOLE || (!even && rounds >= 3) || blocks * p.heads >> 32) own = units;
+    uint64_t own_blocks = own < units ? 0 : blocks;
+    if (own > 0 && own < units)
+        for (int t0 = 0; t0 < p.tables; t0 += 64) {
+            const int t = min(t0 + lane, p.tables - 1);
+            int qa = 0, ka = 0;
+            const int n_q = rows_of(p.qo, t, p.nq, qa), n_t = rows_of(p.ko, t, p.nkv, ka);
+            const Tiles<QT> ts{n_q, (uint64_t)p.first[t] + (n_t + KB - 1) / KB <= (uint64_t)p.blocks ? n_t : 0, p.causal};
+            const uint64_t a = p.tile_sums[t];
+            const uint64_t here = __ballot(t0 + lane < p.tables && own >= a && own < a + ts.count());
+            if (here) {
+                const int l = __ffsll((unsigned long long)here) - 1;
+                own_blocks = lane64(p.block_sums[t] + ts.before((int)min(max(own, a) - a, (uint64_t)ts.count())), l);
+                break;
+            }
+        }
+    if (lane == 0) {
+        const uint64_t rest = blocks - own_blocks, total = rest * p.heads;
+        const uint64_t per = max((uint64_t)WHOLE, (total + p.runs - 1) / p.runs);
+        p.tile_sums[p.tables] = (uint32_t)units;
+        p.block_sums[p.tables] = (uint32_t)min(blocks, (uint64_t)0xffffffff);
+        *p.plan = PackedPlan{(uint32_t)own, (uint32_t)own_blocks, (uint32_t)rest, (uint32_t)per, (uint32_t)((total + per - 1) / per)};
+    }
+}
+
 // Bytes of a tile of C x 64 coordinates: keys by 64 coordinates, hi then lo [64 keys][64] each, then values, hi then lo [64 C][64
 // keys], rows of 128 bytes in swizzled chunks of 16 (swz).
 template <int C>
@@ -71,16 +187,7 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     __shared__ int some[4];
     const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.y;
     const bool values = blockIdx.z == 1;
-    if (blockIdx.x == 0 && h == 0 && !values && tid < 64) {  // the tables' first blocks, for the attention
-        uint64_t before = 0;
-        for (int t0 = 0; t0 < p.tables; t0 += 64) {
-            int a = 0;
-            const uint32_t c = t0 + lane < p.tables ? (uint32_t)((rows_of(p.ko, t0 + lane, p.nkv, a) + KB - 1) / KB) : 0;
-            const uint64_t sum = before + wave_scan(c);
-            if (t0 + lane < p.tables) p.first[t0 + lane] = (uint32_t)min(sum - c, (uint64_t)0x7fffffff);
-            before = __shfl(sum, 63);
-        }
-    }
+    if (blockIdx.x == 0 && h == 0 && !values && tid < 64) p.waves == 8 ? make_plan<256>(p) : make_plan<128>(p);
     uint32_t kb = 0;
     const int t = table_with(p.ko, p.tables, p.nkv, KB, blockIdx.x, kb);
     if (t < 0) return;
@@ -149,38 +256,89 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     }
 }
 
-// grid (query tiles x heads x key ranges); 64 WAVES threads, 32 queries of one table and head a wavefront.
+// grid: a workgroup for each unit, and p.runs; 64 WAVES threads, 32 queries of one table and head a wavefront.
+//
+// A unit is (head, table, tile of 32 WAVES queries); its blocks are the 64-row tiles that its queries see. p.runs workgroups are what
+// the card holds at once. As many units of each head as make whole rounds of them are a workgroup's each (all of them where units are
+// short); the blocks of the others, one unit after the other, are cut into equal runs, which end together, for tables of any lengths,
+// causal or not. A run that is not a whole unit leaves a state for k_packed_join. One table of 10,000 rows and 8 heads, 632 units on
+// 512 places: two rounds X us, everything in runs 840 us (workgroups of an XCD then read different keys at a time, more than its
+// cache holds; whole units read the same ones), as it is X us.
 //
 // S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_32x32x16_f16, three products of halves a term, the keys in sigma32 order so that
 // the weights of a block are the values' operand where they stand. Tiles come by DMA into two LDS buffers each for keys and
-// values. The softmax is in log2 units against a reference that is raised when a block passes it by more than 3; weights stay
+// values, a block ahead. The softmax is in log2 units against a reference that is raised when a block passes it by more than 3; weights stay
 // below 2^15. The sums are held in units of the least power of two that the values' tiles so far have; a block with a larger one
 // has its weights smaller by the difference (at most 2^60: what is cut off there is below 2^-60 of the largest value).
+//
 template <int C, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
     constexpr int QT = 32 * WAVES, HALF = C * 16384, HD = 64 * C;
     __shared__ __align__(16) uint8_t kt[2][HALF], vt[2][HALF];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r32 = lane & 31, g = lane >> 5;
-    const int per_tile = p.heads * p.splits, tile_at = blockIdx.x / per_tile, rest = blockIdx.x - tile_at * per_tile;
-    const int split = rest / p.heads, hpos = rest - split * p.heads;
-    // heads that share keys on the same XCD (workgroup i runs on XCD i % 8)
-    const int h = p.heads % 8 == 0 ? (hpos % 8) * (p.heads / 8) + hpos / 8 : hpos, hk = h / (p.heads / p.kv_heads);
-    uint32_t tile = 0;
-    const int t = table_with(p.qo, p.tables, p.nq, QT, tile_at, tile);
-    if (t < 0) return;
+
+    const PackedPlan plan = *p.plan;
+    // what follows each other on the same XCD (workgroup i runs on XCD i % 8): it reads the same head's keys and values
+    const uint32_t share = (plan.own * p.heads + 7) / 8, share_runs = (plan.runs + 7) / 8;
+    const bool whole = blockIdx.x < 8 * share;
+    const uint32_t idx = whole ? blockIdx.x : blockIdx.x - 8 * share, each = whole ? share : share_runs;
+    const uint32_t run = (idx & 7) * each + (idx >> 3), total = whole ? plan.own * p.heads : plan.rest * p.heads;
+    if ((idx >> 3) >= each || run >= (whole ? total : plan.runs)) return;
+    const uint32_t mine = whole ? run : run * plan.per, end = whole ? run + 1 : min(total, mine + plan.per);
+    const uint32_t a_head = whole ? plan.own : plan.rest;
+    const uint32_t *sums = whole ? p.tile_sums : p.block_sums;
+
+    for (uint32_t at = mine; at < end;) {
+    if (at != mine) __syncthreads();  // the unit before's buffers are no longer read
+    const int h = (int)(at / a_head), hk = h / (p.heads / p.kv_heads);
+    const uint32_t in_head = at - h * a_head + (whole ? 0 : plan.own_blocks);
+    // the table: so many end at or before here (those without queries among them)
+    int t = 0;
+    for (int t0 = 0; t0 < p.tables - 1; t0 += 64) {
+        const uint64_t past = __ballot(t0 + lane < p.tables - 1 && sums[t0 + lane + 1] <= in_head);
+        t += __popcll(past);
+        if (~past) break;
+    }
+    t = __builtin_amdgcn_readfirstlane(t);
     int qa = 0, ka = 0;
     const int n_q = rows_of(p.qo, t, p.nq, qa), n_t = rows_of(p.ko, t, p.nkv, ka);
-    const uint32_t first = p.first[t];
-    // a table past the room that the offsets' promise gives has no rows
+    const uint32_t first = p.first[t], local = in_head - sums[t];
     const int n_k = (uint64_t)first + (n_t + KB - 1) / KB <= (uint64_t)p.blocks ? n_t : 0;
-    // causal: a table's last tile first, which has the most to do
-    const int q0 = (p.causal ? (n_q + QT - 1) / QT - 1 - (int)tile : (int)tile) * QT, w0 = q0 + 32 * wave, qi = w0 + r32;
+    const Tiles<QT> ts{n_q, n_k, p.causal};
+    int tile = 0;
+    if (whole) {
+        tile = (int)local;
+    } else if (!p.causal) {
+        tile = (int)(local / (uint32_t)(ts.all() + BEGIN));
+    } else {
+        int hi = ts.count();
+        while (hi - tile > 1) {
+            const int mid = (tile + hi) >> 1;
+            if (ts.before(mid) <= local)
+                tile = mid;
+            else
+                hi = mid;
+        }
+    }
+    const int nb = ts.blocks(tile), b0 = whole ? 0 : (int)(local - (uint32_t)ts.before(tile));
+    const int b1 = whole ? nb + BEGIN : min(nb + BEGIN, b0 + (int)(end - at));
+    const bool done = b0 == 0 && b1 == nb + BEGIN;
+    const size_t slot = 2 * (size_t)run + (at == mine ? 0 : 1);
+    const uint32_t last_run = done ? run : (at - b0 + nb + BEGIN - 1) / plan.per;
+    at += whole ? 1 : b1 - b0;
+    const int w0 = ts.first_query(tile) + 32 * wave, qi = w0 + r32;
     auto limit_of = [&](int i) { return p.causal ? max(0, n_k - (n_q - 1 - i)) : n_k; };
     const bool live = qi < n_q;
+    if (!whole && at >= end && tid == 0)
+        p.cut[run] = b0 == 0 && !done ? CutUnit{(uint32_t)slot, last_run, qa + ts.first_query(tile), min(QT, n_q - ts.first_query(tile)), h}
+                                      : CutUnit{};
+    if (b0 > 0 && b0 >= nb) {  // behind the unit's blocks
+        if (g == 0) p.part_ml[slot * QT + 32 * wave + r32] = make_float2(-INFINITY, 0.0f);
+        continue;
+    }
     const int limit = live ? limit_of(qi) : n_k, least = w0 < n_q ? limit_of(w0) : n_k;
-    const int nb = (limit_of(min(n_q, q0 + QT) - 1) + KB - 1) / KB;
-    const int kb0 = (int)((long)nb * split / p.splits), kb1 = (int)((long)nb * (split + 1) / p.splits);
+    const int kb0 = b0, kb1 = min(b1, nb);
     const uint8_t *tiles = p.tiles + ((size_t)first * p.kv_heads + hk) * TILE_BYTES<C>;
     const int *shifts = p.shifts + 2 * ((size_t)first * p.kv_heads + hk);
     const size_t kb_bytes = (size_t)p.kv_heads * TILE_BYTES<C>;
@@ -217,7 +375,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
         for (int dc = 0; dc < 4 * C; dc++) split8(qv[dc], f, qh[dc], ql[dc]);
         to_log2 = LOG2E * pow2(-eq);
     }
+    // where a lane's operands begin in a buffer: key row sigma(r32), value row r32, and the four chunks of each; rows 32 further on are
+    // in the same chunks
     const int krow = sigma32(r32);
+    int kat[4], vat[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        kat[i] = krow * 128 + swz(krow, 2 * i + g) * 16;
+        vat[i] = r32 * 128 + swz(r32, 2 * i + g) * 16;
+    }
     float ref = -INFINITY, l = 0.0f;
     int ev = 1000;  // the sums are in units of 2^-ev
     floatx16 acc[2 * C];
@@ -229,32 +395,28 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
 #pragma unroll
     for (int v = 0; v < 16; v++) zero[v] = 0.0f;
 
-    auto scores = [&](const uint8_t *buf, floatx16 (&sc)[2]) {
-#pragma unroll
-        for (int dc = 0; dc < 4 * C; dc++)
-#pragma unroll
-            for (int kh = 0; kh < 2; kh++) {
-                const int r = 32 * kh + krow;
-                const uint8_t *at = buf + (dc >> 2) * 16384 + r * 128 + swz(r, 2 * (dc & 3) + g) * 16;
-                const halfx8 hi = *reinterpret_cast<const halfx8 *>(at), lo = *reinterpret_cast<const halfx8 *>(at + 8192);
-                sc[kh] = mfma16(hi, qh[dc], dc == 0 ? zero : sc[kh]);
-                sc[kh] = mfma16(hi, ql[dc], sc[kh]);
-                sc[kh] = mfma16(lo, qh[dc], sc[kh]);
-            }
-    };
-    auto step = [&](int kb) {
-        const int sl = (kb - kb0) & 1;
+    auto step = [&](auto odd_flag, int kb) {
+        constexpr int sl = decltype(odd_flag)::value;  // (kb - kb0) & 1
+        const int ek = shifts[2 * (size_t)kb * p.kv_heads], evo = shifts[2 * (size_t)kb * p.kv_heads + 1], eb = evo >> 1;
+        // here, before the next copies are on their way: waiting for these two would wait for them
+        const float f = fminf(fmaxf(to_log2 * pow2(-ek), 0x1p-126f), 0x1p126f);  // from raw scores to log2 units
         __builtin_amdgcn_s_waitcnt(0);  // this wavefront's copies of block kb have landed
         __syncthreads();                // everyone's have, and block kb - 1's buffers are no longer read
         if (kb + 1 < kb1) {
             keys_to(kb + 1, sl ^ 1);
             values_to(kb + 1, sl ^ 1);
         }
-        const int *sh = shifts + 2 * (size_t)kb * p.kv_heads;
-        const int ek = sh[0], evo = sh[1], eb = evo >> 1;
         floatx16 sc[2];
-        scores(kt[sl], sc);
-        const float f = fminf(fmaxf(to_log2 * pow2(-ek), 0x1p-126f), 0x1p126f);
+#pragma unroll
+        for (int dc = 0; dc < 4 * C; dc++)
+#pragma unroll
+            for (int kh = 0; kh < 2; kh++) {
+                const uint8_t *at = kt[sl] + (dc >> 2) * 16384 + kh * 4096 + kat[dc & 3];
+                const halfx8 hi = *reinterpret_cast<const halfx8 *>(at), lo = *reinterpret_cast<const halfx8 *>(at + 8192);
+                sc[kh] = mfma16(hi, qh[dc], dc == 0 ? zero : sc[kh]);
+                sc[kh] = mfma16(hi, ql[dc], sc[kh]);
+                sc[kh] = mfma16(lo, qh[dc], sc[kh]);
+            }
         if ((kb + 1) * KB > least) {
             const int lim = limit - kb * KB - 8 * g;  // accumulator v of half kh is seen while 32 kh + 16 (v / 8) + v % 8 < lim
 #pragma unroll
@@ -286,7 +448,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
         }
         const int less = max(ev - eb, -60);
         const float off = (ref == -INFINITY ? 0.0f : 12.0f - ref) + (float)less;
-        halfx8 ph[2][2], pl[2][2];
         float ps = 0.0f;
 #pragma unroll
         for (int kh = 0; kh < 2; kh++)
@@ -303,24 +464,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
                     hw[i] = hi;
                     lw[i] = lo;
                 }
-                ph[kh][hh] = __builtin_bit_cast(halfx8, hw);
-                pl[kh][hh] = __builtin_bit_cast(halfx8, lw);
-            }
-        l += ps * pow2(-less);
-        const uint8_t *vb = vt[sl];
-#pragma unroll
-        for (int kh = 0; kh < 2; kh++)
-#pragma unroll
-            for (int hh = 0; hh < 2; hh++)
+                const halfx8 ph = __builtin_bit_cast(halfx8, hw), pl = __builtin_bit_cast(halfx8, lw);
 #pragma unroll
                 for (int db = 0; db < 2 * C; db++) {
-                    const int r = 32 * db + r32;
-                    const uint8_t *at = vb + r * 128 + swz(r, 4 * kh + 2 * hh + g) * 16;
+                    const uint8_t *at = vt[sl] + db * 4096 + vat[2 * kh + hh];
                     const halfx8 hi = *reinterpret_cast<const halfx8 *>(at), lo = *reinterpret_cast<const halfx8 *>(at + C * 8192);
-                    acc[db] = mfma16(hi, ph[kh][hh], acc[db]);
-                    acc[db] = mfma16(hi, pl[kh][hh], acc[db]);
-                    acc[db] = mfma16(lo, ph[kh][hh], acc[db]);
+                    acc[db] = mfma16(hi, ph, acc[db]);
+                    acc[db] = mfma16(hi, pl, acc[db]);
+                    acc[db] = mfma16(lo, ph, acc[db]);
                 }
+            }
+        l = fmaf(ps, pow2(-less), l);
         if (evo & 1) {  // values that are not finite, zeros in the tile: what sees one is no number
             const int left = limit - kb * KB;
             const uint64_t sees = left >= 64 ? ~uint64_t(0) : (left > 0 ? (uint64_t(1) << left) - 1 : 0);
@@ -332,59 +486,91 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
                     if (odd[32 * db + 8 * (v >> 2) + 4 * g + (v & 3)] & sees) acc[db][v] = NAN;
         }
     };
-    for (int kb = kb0; kb < kb1; kb++) step(kb);
+    int kb = kb0;
+    for (; kb + 1 < kb1; kb += 2) {  // two steps a turn: the buffers' places are constants
+        step(Flag<false>{}, kb);
+        step(Flag<true>{}, kb + 1);
+    }
+    if (kb < kb1) step(Flag<false>{}, kb);
     l = half_sum(l);  // lanes l and l ^ 32 have the same queries' sums over different keys
-    if (!live) return;
     const float inv = l > 0.0f ? 1.0f / l : l, unit = pow2(-min(ev, 149));  // 0 and NaN stay
-    const size_t row = (size_t)(qa + qi) * p.heads + h;
-    float *dst = p.splits == 1 ? p.out + row * p.hd : p.part_o + ((size_t)split * p.nq * p.heads + row) * p.hd;
+    if (!done || live) {
+        float *dst = done ? p.out + ((size_t)(qa + qi) * p.heads + h) * p.hd : p.part_o + (slot * QT + 32 * wave + r32) * p.hd;
 #pragma unroll
-    for (int db = 0; db < 2 * C; db++)
+        for (int db = 0; db < 2 * C; db++)
 #pragma unroll
-        for (int v4 = 0; v4 < 4; v4++) {
-            const int dim = 32 * db + 8 * v4 + 4 * g;
-            if (dim < p.hd) {
-                floatx4 o;
+            for (int v4 = 0; v4 < 4; v4++) {
+                const int dim = 32 * db + 8 * v4 + 4 * g;
+                if (dim < p.hd) {
+                    floatx4 o;
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[e] = acc[db][4 * v4 + e] * inv * unit;
-                *reinterpret_cast<floatx4u *>(dst + dim) = o;
+                    for (int e = 0; e < 4; e++) o[e] = acc[db][4 * v4 + e] * inv * unit;
+                    *reinterpret_cast<floatx4u *>(dst + dim) = o;
+                }
             }
-        }
-    if (p.splits > 1 && g == 0) p.part_ml[(size_t)split * p.nq * p.heads + row] = make_float2(ref, l);
+        if (!done && g == 0) p.part_ml[slot * QT + 32 * wave + r32] = make_float2(ref, l);
+    }
+    }
 }
 
-// grid (queries x heads / 4); 256 threads: a wavefront joins the key ranges' states of one query and head.
-constexpr int MOST_SPLITS = 32;
+// grid (runs, tiles' queries / 16); 256 threads: the states that runs left of a unit's sixteen queries, together, a wavefront for four
+// of them one after the other.
+template <int QT>
 __global__ __launch_bounds__(256) void k_packed_join(Packed p) {
-    const int lane = threadIdx.x & 63, items = p.nq * p.heads, i = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= items) return;
-    if (i / p.heads >= p.qo[p.tables]) return;  // of no table
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (lane < p.splits) ml = p.part_ml[(size_t)lane * items + i];
-    const float top = wave_max(ml.y > 0.0f ? ml.x : -INFINITY);
-    const float f = ml.y > 0.0f ? ml.y * exp2_hw(ml.x - top) : ml.y;
-    const float sum = wave_sum(f);
-    float o[2] = {0.0f, 0.0f};
-    for (int s = 0; s < p.splits; s++) {
-        const float fs = __shfl(f, s), ls = __shfl(ml.y, s);
-        if (ls == 0.0f) continue;
-        const float *src = p.part_o + ((size_t)s * items + i) * p.hd;
-        if (lane < p.hd) o[0] += fs * src[lane];
-        if (64 + lane < p.hd) o[1] += fs * src[64 + lane];
+    constexpr int AHEAD = 4;
+    if (blockIdx.x >= p.plan->runs) return;
+    const CutUnit unit = p.cut[blockIdx.x];
+    const int lane = threadIdx.x & 63, r0 = 16 * blockIdx.y + 4 * (threadIdx.x >> 6);
+    const int d0 = min(lane, p.hd - 1), d1 = min(64 + lane, p.hd - 1);
+#pragma unroll 4
+    for (int r = r0; r < min(r0 + 4, unit.live); r++) {
+        float M = -INFINITY, L = 0.0f, o0 = 0.0f, o1 = 0.0f;
+        for (uint32_t e = blockIdx.x; e <= unit.last_run; e += AHEAD) {
+            float2 ml[AHEAD];
+            float x0[AHEAD], x1[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) {
+                // past the last: the last again, without weight
+                const uint32_t run = min(e + j, unit.last_run);
+                const size_t at = (size_t)(run == blockIdx.x ? unit.slot : 2 * run) * QT + r;
+                ml[j] = p.part_ml[at];
+                x0[j] = p.part_o[at * p.hd + d0];
+                x1[j] = p.hd > 64 ? p.part_o[at * p.hd + d1] : 0.0f;
+                if (e + j > unit.last_run) ml[j] = make_float2(-INFINITY, 0.0f);
+            }
+            float top = M;
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++)
+                if (ml[j].y > 0.0f) top = fmaxf(top, ml[j].x);
+            const float old = M == -INFINITY ? 1.0f : exp2_hw(M - top);  // nothing yet, or NaN
+            L *= old;
+            o0 *= old;
+            o1 *= old;
+            M = top;
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) {
+                if (ml[j].y == 0.0f) continue;
+                const float f = ml[j].y > 0.0f ? ml[j].y * exp2_hw(ml[j].x - M) : ml[j].y;
+                L += f;
+                o0 += f * x0[j];
+                o1 += f * x1[j];
+            }
+        }
+        const float inv = L > 0.0f ? 1.0f / L : L;
+        float *dst = p.out + ((size_t)(unit.row + r) * p.heads + unit.head) * p.hd;
+        if (lane < p.hd) dst[lane] = o0 * inv;
+        if (64 + lane < p.hd) dst[64 + lane] = o1 * inv;
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : sum;
-    if (lane < p.hd) p.out[(size_t)i * p.hd + lane] = o[0] * inv;
-    if (64 + lane < p.hd) p.out[(size_t)i * p.hd + 64 + lane] = o[1] * inv;
 }
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
-// Wavefronts a workgroup, key ranges, workgroups and the working memory's parts.
+// Wavefronts a workgroup, runs, workgroups and the working memory's parts.
 struct Plan {
-    int waves, splits, blocks, c;
+    int waves, runs, blocks, c;
     int64_t grid;
-    size_t tiles, shifts, odd, first, part_o, part_ml;
-    size_t bytes() const { return tiles + shifts + odd + first + part_o + part_ml; }
+    size_t tiles, shifts, odd, tables, part_o, part_ml, cut;
+    size_t bytes() const { return tiles + shifts + odd + 256 + 3 * tables + part_o + part_ml + cut; }
 };
 
 Plan plan(const PackedShape &a) {
@@ -392,36 +578,29 @@ Plan plan(const PackedShape &a) {
     r.c = a.hd <= 64 ? 1 : 2;
     r.waves = r.c == 2 ? 8 : 4;
     const int qt = 32 * r.waves;
-    const int64_t tiles = a.nq / qt + (int64_t)std::min(a.tables, a.nq);
+    r.runs = r.waves == 8 ? 256 : 512;  // what the card holds at once, eight wavefronts a compute unit
+    r.grid = (a.nq / qt + (int64_t)std::min(a.tables, a.nq)) * a.heads + r.runs + 16;
     const int64_t blocks = a.nkv / KB + (int64_t)std::min(a.tables, a.nkv);
     r.blocks = (int)blocks;
-    // few query tiles: several key ranges each, so that every compute unit has a workgroup
-    const int64_t each = std::max<int64_t>(1, blocks / std::max<int64_t>(1, std::min(a.tables, a.nkv)));
-    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>({MOST_SPLITS, 256 / std::max<int64_t>(1, tiles * a.heads), each / 2}));
-    r.grid = tiles * a.heads * r.splits;
-    const size_t halves = (size_t)blocks * a.kv_heads;
+    const size_t halves = (size_t)blocks * a.kv_heads, places = 2 * (size_t)r.runs * qt;
     r.tiles = up256(halves * r.c * 32768);
     r.shifts = up256(halves * 2 * sizeof(int));
     r.odd = up256(halves * 64 * r.c * sizeof(uint64_t));
-    r.first = up256((size_t)a.tables * sizeof(uint32_t));
-    const size_t items = r.splits > 1 ? (size_t)r.splits * a.nq * a.heads : 0;
-    r.part_o = up256(items * a.hd * sizeof(float));
-    r.part_ml = up256(items * sizeof(float2));
+    r.tables = up256(((size_t)a.tables + 1) * sizeof(uint32_t));
+    r.part_o = up256(places * a.hd * sizeof(float));
+    r.part_ml = up256(places * sizeof(float2));
+    r.cut = up256((size_t)r.runs * sizeof(CutUnit));
     return r;
 }
 
 template <int C, int WAVES>
 void launch(hipStream_t s, const Packed &p, const Plan &r) {
-    if (r.blocks > 0) {
-        hipLaunchKernelGGL(k_packed_tiles<C>, dim3(r.blocks, p.kv_heads, 2), dim3(256), 0, s, p);
-        TAH_LAUNCHED();
-    }
+    hipLaunchKernelGGL(k_packed_tiles<C>, dim3(std::max(r.blocks, 1), p.kv_heads, 2), dim3(256), 0, s, p);
+    TAH_LAUNCHED();
     hipLaunchKernelGGL((k_packed<C, WAVES>), dim3((unsigned)r.grid), dim3(64 * WAVES), 0, s, p);
     TAH_LAUNCHED();
-    if (r.splits > 1) {
-        hipLaunchKernelGGL(k_packed_join, dim3(((unsigned)p.nq * p.heads + 3) / 4), dim3(256), 0, s, p);
-        TAH_LAUNCHED();
-    }
+    hipLaunchKernelGGL(k_packed_join<32 * WAVES>, dim3(r.runs, 2 * WAVES), dim3(256), 0, s, p);
+    TAH_LAUNCHED();
 }
 
 }  // namespace
@@ -446,10 +625,15 @@ void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const
     p.tiles = carve(r.tiles);
     p.shifts = reinterpret_cast<int *>(carve(r.shifts));
     p.odd = reinterpret_cast<uint64_t *>(carve(r.odd));
-    p.first = reinterpret_cast<uint32_t *>(carve(r.first));
-    p.splits = r.splits;
+    p.plan = reinterpret_cast<PackedPlan *>(carve(256));
+    p.first = reinterpret_cast<uint32_t *>(carve(r.tables));
+    p.tile_sums = reinterpret_cast<uint32_t *>(carve(r.tables));
+    p.block_sums = reinterpret_cast<uint32_t *>(carve(r.tables));
+    p.waves = r.waves;
+    p.runs = r.runs;
     p.part_o = reinterpret_cast<float *>(carve(r.part_o));
     p.part_ml = reinterpret_cast<float2 *>(carve(r.part_ml));
+    p.cut = reinterpret_cast<CutUnit *>(carve(r.cut));
     if (r.c == 2)
         launch<2, 8>(s, p, r);
     else
