@@ -1210,14 +1210,15 @@ extern "C" int tah_pages_attend(tah_dev *dev, const tah_pages *p, const int32_t 
 }
 
 // ---- packed tables ----------------------------------------------------------------------------------------------
-static PackedShape packed_shape(int tables, int nq, int nkv, int heads, int kv_heads, int hd, int64_t &q_ld, int64_t &kv_ld) {
+static PackedShape packed_shape(int tables, int nq, int nkv, int heads, int kv_heads, int hd, bool causal, int64_t &q_ld,
+                                int64_t &kv_ld) {
     if (hd <= 0 || hd > 128 || hd % 16) throw ArgError{"attend_packed: heads of 16 to 128, in sixteens"};
     if (tables <= 0 || kv_heads > 65535) throw ArgError{"attend_packed: no tables, or more than 65535 key/value heads"};
     check_heads("attend_packed", nq, heads, kv_heads);
     check_heads("attend_packed", nkv, kv_heads, kv_heads);
     q_ld = (int64_t)row_stride("attend_packed", nq, q_ld, (size_t)heads * hd);
     kv_ld = (int64_t)row_stride("attend_packed", nkv, kv_ld, (size_t)kv_heads * hd);
-    return PackedShape{tables, nq, nkv, heads, kv_heads, hd};
+    return PackedShape{tables, nq, nkv, heads, kv_heads, hd, causal};
 }
 
 extern "C" int tah_attend_packed_dev(tah_dev *dev, const float *q, const float *k, const float *v, const int32_t *q_offsets,
@@ -1225,12 +1226,12 @@ extern "C" int tah_attend_packed_dev(tah_dev *dev, const float *q, const float *
                                      int32_t kv_heads, int32_t hd, int32_t causal, int64_t q_ld, int64_t kv_ld, float *out) {
     if (!q || !k || !v || !q_offsets || !kv_offsets || !out) return TAH_E_ARG;
     return guarded(dev, [&] {
-        const PackedShape a = packed_shape(tables, nq, nkv, heads, kv_heads, hd, q_ld, kv_ld);
+        const PackedShape a = packed_shape(tables, nq, nkv, heads, kv_heads, hd, causal != 0, q_ld, kv_ld);
         if (!aligned4({q, k, v, q_offsets, kv_offsets, out})) throw ArgError{"attend_packed: the pointers have to be 4-byte aligned"};
         if (nq == 0) return TAH_OK;
         Loans loans(dev);
         void *work = loans.take<uint8_t>(packed_work_bytes(a));
-        packed_attention(dev->stream, a, q, k, v, q_offsets, kv_offsets, causal != 0, (size_t)q_ld, (size_t)kv_ld, out, work);
+        packed_attention(dev->stream, a, q, k, v, q_offsets, kv_offsets, (size_t)q_ld, (size_t)kv_ld, out, work);
         return TAH_OK;
     });
 }
@@ -1240,7 +1241,7 @@ extern "C" int tah_attend_packed(tah_dev *dev, const float *q, const float *k, c
                                  int32_t kv_heads, int32_t hd, int32_t causal, int64_t q_ld, int64_t kv_ld, float *out) {
     if (!q || !k || !v || !q_offsets || !kv_offsets || !out) return TAH_E_ARG;
     return guarded(dev, [&] {
-        PackedShape a = packed_shape(tables, nq, nkv, heads, kv_heads, hd, q_ld, kv_ld);
+        PackedShape a = packed_shape(tables, nq, nkv, heads, kv_heads, hd, causal != 0, q_ld, kv_ld);
         check_offsets("attend_packed", q_offsets, tables, nq);
         check_offsets("attend_packed", kv_offsets, tables, nkv);
         a.nq = q_offsets[tables];  // the queries from here on are left alone
@@ -1261,7 +1262,7 @@ extern "C" int tah_attend_packed(tah_dev *dev, const float *q, const float *k, c
         rows_in(vd, v, a.nkv, kw, kv_ld);
         TAH_HIP(hipMemcpyAsync(qo, q_offsets, offsets, hipMemcpyHostToDevice, dev->stream));
         TAH_HIP(hipMemcpyAsync(ko, kv_offsets, offsets, hipMemcpyHostToDevice, dev->stream));
-        packed_attention(dev->stream, a, qd, kd, vd, qo, ko, causal != 0, qw, kw, od, work);
+        packed_attention(dev->stream, a, qd, kd, vd, qo, ko, qw, kw, od, work);
         TAH_HIP(hipMemcpyAsync(out, od, a.nq * qw * sizeof(float), hipMemcpyDeviceToHost, dev->stream));
         TAH_HIP(hipStreamSynchronize(dev->stream));
         return TAH_OK;

@@ -307,10 +307,11 @@ void attention(hipStream_t s, const AttnShape &a, const float *q, const uint8_t 
 // work of packed_work_bytes (which refuses calls that are too large).
 struct PackedShape {
     int tables, nq, nkv, heads, kv_heads, hd;
+    bool causal;
 };
 size_t packed_work_bytes(const PackedShape &a);
 void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const float *k, const float *v, const int32_t *q_offsets,
-                      const int32_t *kv_offsets, bool causal, size_t q_ld, size_t kv_ld, float *out, void *work);
+                      const int32_t *kv_offsets, size_t q_ld, size_t kv_ld, float *out, void *work);
 
 // The regression head (quantiles.hip): per row of q [rows][n], mean, variance, median and icdf at alphas [na]
 // (device) into stats [rows][3 + na].

@@ -406,6 +406,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
             keys_to(kb + 1, sl ^ 1);
             values_to(kb + 1, sl ^ 1);
         }
+        if (w0 >= n_q) return;  // a wavefront without queries: its part of the copies is all it does
         floatx16 sc[2];
 #pragma unroll
         for (int dc = 0; dc < 4 * C; dc++)
@@ -513,54 +514,56 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
     }
 }
 
-// grid (runs, tiles' queries / 16); 256 threads: the states that runs left of a unit's sixteen queries, together, a wavefront for four
-// of them one after the other.
-template <int QT>
+// grid (runs, tiles' queries / 16); 256 threads: the states that runs left of a unit's sixteen queries, together: sixteen lanes a
+// query, four of each 64 coordinates a lane.
+template <int C, int QT>
 __global__ __launch_bounds__(256) void k_packed_join(Packed p) {
     constexpr int AHEAD = 4;
     if (blockIdx.x >= p.plan->runs) return;
     const CutUnit unit = p.cut[blockIdx.x];
-    const int lane = threadIdx.x & 63, r0 = 16 * blockIdx.y + 4 * (threadIdx.x >> 6);
-    const int d0 = min(lane, p.hd - 1), d1 = min(64 + lane, p.hd - 1);
-#pragma unroll 4
-    for (int r = r0; r < min(r0 + 4, unit.live); r++) {
-        float M = -INFINITY, L = 0.0f, o0 = 0.0f, o1 = 0.0f;
-        for (uint32_t e = blockIdx.x; e <= unit.last_run; e += AHEAD) {
-            float2 ml[AHEAD];
-            float x0[AHEAD], x1[AHEAD];
+    const int r = 16 * blockIdx.y + (threadIdx.x >> 4), dim = 4 * (threadIdx.x & 15);
+    if (r >= unit.live) return;
+    float M = -INFINITY, L = 0.0f;
+    floatx4 o[C];
 #pragma unroll
-            for (int j = 0; j < AHEAD; j++) {
-                // past the last: the last again, without weight
-                const uint32_t run = min(e + j, unit.last_run);
-                const size_t at = (size_t)(run == blockIdx.x ? unit.slot : 2 * run) * QT + r;
-                ml[j] = p.part_ml[at];
-                x0[j] = p.part_o[at * p.hd + d0];
-                x1[j] = p.hd > 64 ? p.part_o[at * p.hd + d1] : 0.0f;
-                if (e + j > unit.last_run) ml[j] = make_float2(-INFINITY, 0.0f);
-            }
-            float top = M;
+    for (int c = 0; c < C; c++) o[c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t e = blockIdx.x; e <= unit.last_run; e += AHEAD) {
+        float2 ml[AHEAD];
+        floatx4 x[AHEAD][C];
 #pragma unroll
-            for (int j = 0; j < AHEAD; j++)
-                if (ml[j].y > 0.0f) top = fmaxf(top, ml[j].x);
-            const float old = M == -INFINITY ? 1.0f : exp2_hw(M - top);  // nothing yet, or NaN
-            L *= old;
-            o0 *= old;
-            o1 *= old;
-            M = top;
+        for (int j = 0; j < AHEAD; j++) {
+            // past the last: the last again, without weight
+            const uint32_t run = min(e + j, unit.last_run);
+            const size_t at = (size_t)(run == blockIdx.x ? unit.slot : 2 * run) * QT + r;
+            ml[j] = p.part_ml[at];
 #pragma unroll
-            for (int j = 0; j < AHEAD; j++) {
-                if (ml[j].y == 0.0f) continue;
-                const float f = ml[j].y > 0.0f ? ml[j].y * exp2_hw(ml[j].x - M) : ml[j].y;
-                L += f;
-                o0 += f * x0[j];
-                o1 += f * x1[j];
-            }
+            for (int c = 0; c < C; c++)
+                x[j][c] = *reinterpret_cast<const floatx4 *>(p.part_o + at * p.hd + (64 * c + dim < p.hd ? 64 * c + dim : 0));
+            if (e + j > unit.last_run) ml[j] = make_float2(-INFINITY, 0.0f);
         }
-        const float inv = L > 0.0f ? 1.0f / L : L;
-        float *dst = p.out + ((size_t)(unit.row + r) * p.heads + unit.head) * p.hd;
-        if (lane < p.hd) dst[lane] = o0 * inv;
-        if (64 + lane < p.hd) dst[64 + lane] = o1 * inv;
+        float top = M;
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++)
+            if (ml[j].y > 0.0f) top = fmaxf(top, ml[j].x);
+        const float old = M == -INFINITY ? 1.0f : exp2_hw(M - top);  // nothing yet, or NaN
+        L *= old;
+#pragma unroll
+        for (int c = 0; c < C; c++) o[c] *= old;
+        M = top;
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            if (ml[j].y == 0.0f) continue;
+            const float f = ml[j].y > 0.0f ? ml[j].y * exp2_hw(ml[j].x - M) : ml[j].y;
+            L += f;
+#pragma unroll
+            for (int c = 0; c < C; c++) o[c] += f * x[j][c];
+        }
     }
+    const float inv = L > 0.0f ? 1.0f / L : L;
+#pragma unroll
+    for (int c = 0; c < C; c++)
+        if (64 * c + dim < p.hd)
+            *reinterpret_cast<floatx4u *>(p.out + ((size_t)(unit.row + r) * p.heads + unit.head) * p.hd + 64 * c + dim) = o[c] * inv;
 }
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -576,7 +579,9 @@ struct Plan {
 Plan plan(const PackedShape &a) {
     Plan r;
     r.c = a.hd <= 64 ? 1 : 2;
-    r.waves = r.c == 2 ? 8 : 4;
+    // tiles of 256 queries where all of a long table's are full (10,000 rows 619 -> 598 us), else of 128 (five tables of up to 6,007 rows
+    // in order 513, with 256 534); heads over 64 wide leave room for one workgroup a compute unit
+    r.waves = r.c == 2 || (!a.causal && a.nq / 4096 >= a.tables) ? 8 : 4;
     const int qt = 32 * r.waves;
     r.runs = r.waves == 8 ? 256 : 512;  // what the card holds at once, eight wavefronts a compute unit
     r.grid = (a.nq / qt + (int64_t)std::min(a.tables, a.nq)) * a.heads + r.runs + 16;
@@ -599,7 +604,7 @@ void launch(hipStream_t s, const Packed &p, const Plan &r) {
     TAH_LAUNCHED();
     hipLaunchKernelGGL((k_packed<C, WAVES>), dim3((unsigned)r.grid), dim3(64 * WAVES), 0, s, p);
     TAH_LAUNCHED();
-    hipLaunchKernelGGL(k_packed_join<32 * WAVES>, dim3(r.runs, 2 * WAVES), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((k_packed_join<C, 32 * WAVES>), dim3(r.runs, 2 * WAVES), dim3(256), 0, s, p);
     TAH_LAUNCHED();
 }
 
@@ -612,7 +617,7 @@ size_t packed_work_bytes(const PackedShape &a) {
 }
 
 void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const float *k, const float *v, const int32_t *q_offsets,
-                      const int32_t *kv_offsets, bool causal, size_t q_ld, size_t kv_ld, float *out, void *work) {
+                      const int32_t *kv_offsets, size_t q_ld, size_t kv_ld, float *out, void *work) {
     const Plan r = plan(a);
     uint8_t *at = static_cast<uint8_t *>(work);
     auto carve = [&](size_t bytes) {
@@ -620,7 +625,7 @@ void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const
         at += bytes;
         return here;
     };
-    Packed p{q, k, v, q_offsets, kv_offsets, a.tables, a.nq, a.nkv, a.heads, a.kv_heads, a.hd, causal ? 1 : 0, q_ld, kv_ld, out};
+    Packed p{q, k, v, q_offsets, kv_offsets, a.tables, a.nq, a.nkv, a.heads, a.kv_heads, a.hd, a.causal ? 1 : 0, q_ld, kv_ld, out};
     p.blocks = r.blocks;
     p.tiles = carve(r.tiles);
     p.shifts = reinterpret_cast<int *>(carve(r.shifts));
@@ -636,6 +641,8 @@ void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const
     p.cut = reinterpret_cast<CutUnit *>(carve(r.cut));
     if (r.c == 2)
         launch<2, 8>(s, p, r);
+    else if (r.waves == 8)
+        launch<1, 8>(s, p, r);
     else
         launch<1, 4>(s, p, r);
 }
