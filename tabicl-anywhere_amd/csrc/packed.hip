@@ -274,10 +274,15 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
 template <int C, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
     constexpr int QT = 32 * WAVES, HALF = C * 16384, HD = 64 * C;
-    __shared__ __align__(16) uint8_t kt[2][HALF], vt[2][HALF];
+    __shared__ __align__(16) uint8_t kt0[HALF], kt1[HALF], vt0[HALF], vt1[HALF];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r32 = lane & 31, g = lane >> 5;
 
+    // the first 64 tables, one a lane, read beside the plan
+    const int t64 = min(lane, p.tables - 1);
+    uint32_t tiles64 = p.tile_sums[t64 + 1], blocks64 = p.block_sums[t64 + 1], first64 = p.first[t64];
+    int qa64 = 0, ka64 = 0;
+    const int q64 = rows_of(p.qo, t64, p.nq, qa64), k64 = rows_of(p.ko, t64, p.nkv, ka64);
     const PackedPlan plan = *p.plan;
     // what follows each other on the same XCD (workgroup i runs on XCD i % 8): it reads the same head's keys and values
     const uint32_t share = (plan.own * p.heads + 7) / 8, share_runs = (plan.runs + 7) / 8;
@@ -294,16 +299,25 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
     const int h = (int)(at / a_head), hk = h / (p.heads / p.kv_heads);
     const uint32_t in_head = at - h * a_head + (whole ? 0 : plan.own_blocks);
     // the table: so many end at or before here (those without queries among them)
-    int t = 0;
-    for (int t0 = 0; t0 < p.tables - 1; t0 += 64) {
-        const uint64_t past = __ballot(t0 + lane < p.tables - 1 && sums[t0 + lane + 1] <= in_head);
-        t += __popcll(past);
-        if (~past) break;
-    }
+    int t = __popcll(__ballot(lane < p.tables - 1 && (whole ? tiles64 : blocks64) <= in_head));
+    for (int t0 = 64; t == t0 && t0 < p.tables - 1; t0 += 64)
+        t += __popcll(__ballot(t0 + lane < p.tables - 1 && sums[t0 + lane + 1] <= in_head));
     t = __builtin_amdgcn_readfirstlane(t);
-    int qa = 0, ka = 0;
-    const int n_q = rows_of(p.qo, t, p.nq, qa), n_t = rows_of(p.ko, t, p.nkv, ka);
-    const uint32_t first = p.first[t], local = in_head - sums[t];
+    int qa, n_q, n_t;
+    uint32_t first, local;
+    if (t < 64) {
+        qa = __builtin_amdgcn_readlane(qa64, t);
+        n_q = __builtin_amdgcn_readlane(q64, t);
+        n_t = __builtin_amdgcn_readlane(k64, t);
+        first = __builtin_amdgcn_readlane(first64, t);
+        local = in_head - (t ? __builtin_amdgcn_readlane(whole ? tiles64 : blocks64, t - 1) : 0);
+    } else {
+        int ka = 0;
+        n_q = rows_of(p.qo, t, p.nq, qa);
+        n_t = rows_of(p.ko, t, p.nkv, ka);
+        first = p.first[t];
+        local = in_head - sums[t];
+    }
     const int n_k = (uint64_t)first + (n_t + KB - 1) / KB <= (uint64_t)p.blocks ? n_t : 0;
     const Tiles<QT> ts{n_q, n_k, p.causal};
     int tile = 0;
@@ -342,11 +356,25 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
     const uint8_t *tiles = p.tiles + ((size_t)first * p.kv_heads + hk) * TILE_BYTES<C>;
     const int *shifts = p.shifts + 2 * ((size_t)first * p.kv_heads + hk);
     const size_t kb_bytes = (size_t)p.kv_heads * TILE_BYTES<C>;
-    auto keys_to = [&](int kb, int s) { half_image_to_lds<WAVES, HALF>(tiles + kb * kb_bytes, kt[s], tid); };
-    auto values_to = [&](int kb, int s) { half_image_to_lds<WAVES, HALF>(tiles + kb * kb_bytes + HALF, vt[s], tid); };
+    // half a tile, 16 bytes a lane: in copy i wavefront w fills the 1 KB at 1024 (WAVES i + w), from a scalar address on
+    const uint32_t lane16 = 16 * lane;
+    auto copy = [&](const uint8_t *src, uint8_t *dst) {
+#pragma unroll
+        for (int i = 0; i < HALF / (1024 * WAVES); i++)
+            __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint4 *>(src + 1024 * (WAVES * i + wave) + lane16),
+                                             dst + 1024 * (WAVES * i + wave), 16, 0, 0);
+    };
+    // the powers of two of 64 blocks, one a lane
+    int shifts_at = kb0, key_shifts = 0, value_shifts = 0;
+    auto hold_shifts = [&] {
+        const int *at = shifts + 2 * (size_t)min(shifts_at + lane, kb1 - 1) * p.kv_heads;
+        key_shifts = at[0];
+        value_shifts = at[1];
+    };
     if (kb0 < kb1) {
-        keys_to(kb0, 0);
-        values_to(kb0, 0);
+        hold_shifts();
+        copy(tiles + kb0 * kb_bytes, kt0);
+        copy(tiles + kb0 * kb_bytes + HALF, vt0);
     }
     // this lane's query coordinates 16 dc + 8 g + t, at a maximum near 2^14, split
     halfx8 qh[4 * C], ql[4 * C];
@@ -395,16 +423,21 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
 #pragma unroll
     for (int v = 0; v < 16; v++) zero[v] = 0.0f;
 
-    auto step = [&](auto odd_flag, int kb) {
-        constexpr int sl = decltype(odd_flag)::value;  // (kb - kb0) & 1
-        const int ek = shifts[2 * (size_t)kb * p.kv_heads], evo = shifts[2 * (size_t)kb * p.kv_heads + 1], eb = evo >> 1;
-        // here, before the next copies are on their way: waiting for these two would wait for them
-        const float f = fminf(fmaxf(to_log2 * pow2(-ek), 0x1p-126f), 0x1p126f);  // from raw scores to log2 units
+    // Block kb from the buffers kc and vc, the next one on its way into kn and vn: four arrays, so that the compiler sees that it need
+    // not wait for the copies before it reads.
+    auto step = [&](const uint8_t *kc, const uint8_t *vc, uint8_t *kn, uint8_t *vn, int kb) __attribute__((always_inline)) {
+        if (kb >= shifts_at + 64) {
+            shifts_at += 64;
+            hold_shifts();
+        }
         __builtin_amdgcn_s_waitcnt(0);  // this wavefront's copies of block kb have landed
         __syncthreads();                // everyone's have, and block kb - 1's buffers are no longer read
+        const int evo = __builtin_amdgcn_readlane(value_shifts, kb - shifts_at), eb = evo >> 1;
+        const int ek = __builtin_amdgcn_readlane(key_shifts, kb - shifts_at);
+        const float f = fminf(fmaxf(to_log2 * pow2(-ek), 0x1p-126f), 0x1p126f);  // from raw scores to log2 units
         if (kb + 1 < kb1) {
-            keys_to(kb + 1, sl ^ 1);
-            values_to(kb + 1, sl ^ 1);
+            copy(tiles + (kb + 1) * kb_bytes, kn);
+            copy(tiles + (kb + 1) * kb_bytes + HALF, vn);
         }
         if (w0 >= n_q) return;  // a wavefront without queries: its part of the copies is all it does
         floatx16 sc[2];
@@ -412,7 +445,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
         for (int dc = 0; dc < 4 * C; dc++)
 #pragma unroll
             for (int kh = 0; kh < 2; kh++) {
-                const uint8_t *at = kt[sl] + (dc >> 2) * 16384 + kh * 4096 + kat[dc & 3];
+                const uint8_t *at = kc + (dc >> 2) * 16384 + kh * 4096 + kat[dc & 3];
                 const halfx8 hi = *reinterpret_cast<const halfx8 *>(at), lo = *reinterpret_cast<const halfx8 *>(at + 8192);
                 sc[kh] = mfma16(hi, qh[dc], dc == 0 ? zero : sc[kh]);
                 sc[kh] = mfma16(hi, ql[dc], sc[kh]);
@@ -468,7 +501,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
                 const halfx8 ph = __builtin_bit_cast(halfx8, hw), pl = __builtin_bit_cast(halfx8, lw);
 #pragma unroll
                 for (int db = 0; db < 2 * C; db++) {
-                    const uint8_t *at = vt[sl] + db * 4096 + vat[2 * kh + hh];
+                    const uint8_t *at = vc + db * 4096 + vat[2 * kh + hh];
                     const halfx8 hi = *reinterpret_cast<const halfx8 *>(at), lo = *reinterpret_cast<const halfx8 *>(at + C * 8192);
                     acc[db] = mfma16(hi, ph, acc[db]);
                     acc[db] = mfma16(hi, pl, acc[db]);
@@ -489,10 +522,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
     };
     int kb = kb0;
     for (; kb + 1 < kb1; kb += 2) {  // two steps a turn: the buffers' places are constants
-        step(Flag<false>{}, kb);
-        step(Flag<true>{}, kb + 1);
+        step(kt0, vt0, kt1, vt1, kb);
+        step(kt1, vt1, kt0, vt0, kb + 1);
     }
-    if (kb < kb1) step(Flag<false>{}, kb);
+    if (kb < kb1) step(kt0, vt0, kt1, vt1, kb);
     l = half_sum(l);  // lanes l and l ^ 32 have the same queries' sums over different keys
     const float inv = l > 0.0f ? 1.0f / l : l, unit = pow2(-min(ev, 149));  // 0 and NaN stay
     if (!done || live) {
