@@ -172,17 +172,16 @@ __device__ void make_plan(const Packed &p) {
     }
 }
 
-// Bytes of a tile of C x 64 coordinates: keys by 64 coordinates, hi then lo [64 keys][64] each, then values, hi then lo [64 C][64
-// keys], rows of 128 bytes in swizzled chunks of 16 (swz).
-template <int C>
-constexpr int TILE_BYTES = C * 32768;
+// Bytes of half a tile of D coordinates, keys or values: keys by 64 coordinates, hi then lo [64 keys][64] each (D 32: [64 keys], a
+// key's hi then its lo), values hi then lo [D][64 keys], rows of 128 bytes in swizzled chunks of 16 (swz).
+template <int D>
+constexpr int HALF_BYTES = D * 256;
 
 // grid (blocks, key/value heads, keys and values); 256 threads: one half tile. Scaled by the power of two that brings its own
 // largest finite number below 2^14. A value that is not finite is a zero in the tile, and its bit is set in `odd`.
-template <int C>
+template <int D>
 __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
-    constexpr int HD = 64 * C;
-    __shared__ float x[KB][HD + 1];
+    __shared__ float x[KB][D + 1];
     __shared__ float most[4];
     __shared__ int some[4];
     const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.y;
@@ -196,8 +195,8 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     const float *src = (values ? p.v : p.k) + (size_t)(a + (int)kb * KB) * p.kv_ld + (size_t)h * p.hd;
     uint32_t big = 0, raw = 0;
 #pragma unroll
-    for (int i = 0; i < KB * HD / 4 / 256; i++) {
-        const int u = tid + 256 * i, r = u / (HD / 4), dim = 4 * (u % (HD / 4));
+    for (int i = 0; i < KB * D / 4 / 256; i++) {
+        const int u = tid + 256 * i, r = u / (D / 4), dim = 4 * (u % (D / 4));
         const floatx4 w = r < n && dim < p.hd ? (floatx4) * reinterpret_cast<const floatx4u *>(src + (size_t)r * p.kv_ld + dim)
                                               : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -221,38 +220,41 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     const float f = pow2(shift);
     const size_t at = (size_t)blockIdx.x * p.kv_heads + h;
     if (tid == 0) p.shifts[2 * at + (values ? 1 : 0)] = values ? 2 * shift + (odd ? 1 : 0) : shift;
-    uint8_t *tile = p.tiles + at * TILE_BYTES<C>;
-    if (odd && tid < HD) {
+    uint8_t *tile = p.tiles + at * (2 * HALF_BYTES<D>);
+    if (odd && tid < D) {
         uint64_t bits = 0;
         for (int r = 0; r < KB; r++) {
             const bool b = (__float_as_uint(x[r][tid]) & 0x7fffffffu) >= 0x7f800000u;
             bits |= (uint64_t)b << r;
         }
-        p.odd[at * HD + tid] = bits;
+        p.odd[at * D + tid] = bits;
     }
 #pragma unroll
-    for (int i = 0; i < HD * 8 / 256; i++) {
-        const int u = tid + 256 * i, c = u & 7;
+    for (int i = 0; i < D * 8 / 256; i++) {
+        const int u = tid + 256 * i;
         float w[8];
-        uint8_t *hi;
+        uint8_t *hi, *lo;
         if (values) {
-            const int r = u >> 3;  // coordinate r, keys 8 c ..
+            const int c = u & 7, r = u >> 3;  // coordinate r, keys 8 c ..
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float y = x[8 * c + e][r];
                 w[e] = odd && (__float_as_uint(y) & 0x7fffffffu) >= 0x7f800000u ? 0.0f : y;
             }
-            hi = tile + C * 16384 + r * 128 + swz(r, c) * 16;
+            hi = tile + HALF_BYTES<D> + r * 128 + swz(r, c) * 16;
+            lo = hi + D * 128;
         } else {
-            const int part = u >> 9, r = (u >> 3) & 63;  // key r, coordinates 64 part + 8 c ..
+            constexpr int CHUNKS = D < 64 ? D / 8 : 8;
+            const int c = u % CHUNKS, r = (u / CHUNKS) & 63, part = u / (64 * CHUNKS);  // key r, coordinates 64 part + 8 c ..
 #pragma unroll
             for (int e = 0; e < 8; e++) w[e] = x[r][64 * part + 8 * c + e];
             hi = tile + part * 16384 + r * 128 + swz(r, c) * 16;
+            lo = D < 64 ? tile + r * 128 + swz(r, c + CHUNKS) * 16 : hi + 8192;
         }
         halfx8 wh, wl;
         split8(w, f, wh, wl);
         *reinterpret_cast<halfx8 *>(hi) = wh;
-        *reinterpret_cast<halfx8 *>(hi + (values ? C * 8192 : 8192)) = wl;
+        *reinterpret_cast<halfx8 *>(lo) = wl;
     }
 }
 
@@ -271,9 +273,9 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
 // below 2^15. The sums are held in units of the least power of two that the values' tiles so far have; a block with a larger one
 // has its weights smaller by the difference (at most 2^60: what is cut off there is below 2^-60 of the largest value).
 //
-template <int C, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
-    constexpr int QT = 32 * WAVES, HALF = C * 16384, HD = 64 * C;
+template <int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_packed(Packed p) {
+    constexpr int QT = 32 * WAVES, HALF = HALF_BYTES<D>, DC = D / 16, DB = D / 32;
     __shared__ __align__(16) uint8_t kt0[HALF], kt1[HALF], vt0[HALF], vt1[HALF];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r32 = lane & 31, g = lane >> 5;
@@ -353,9 +355,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
     }
     const int limit = live ? limit_of(qi) : n_k, least = w0 < n_q ? limit_of(w0) : n_k;
     const int kb0 = b0, kb1 = min(b1, nb);
-    const uint8_t *tiles = p.tiles + ((size_t)first * p.kv_heads + hk) * TILE_BYTES<C>;
+    const uint8_t *tiles = p.tiles + ((size_t)first * p.kv_heads + hk) * (2 * HALF);
     const int *shifts = p.shifts + 2 * ((size_t)first * p.kv_heads + hk);
-    const size_t kb_bytes = (size_t)p.kv_heads * TILE_BYTES<C>;
+    const size_t kb_bytes = (size_t)p.kv_heads * (2 * HALF);
     // half a tile, 16 bytes a lane: in copy i wavefront w fills the 1 KB at 1024 (WAVES i + w), from a scalar address on
     const uint32_t lane16 = 16 * lane;
     auto copy = [&](const uint8_t *src, uint8_t *dst) {
@@ -377,13 +379,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
         copy(tiles + kb0 * kb_bytes + HALF, vt0);
     }
     // this lane's query coordinates 16 dc + 8 g + t, at a maximum near 2^14, split
-    halfx8 qh[4 * C], ql[4 * C];
+    halfx8 qh[DC], ql[DC];
     float to_log2;
     {
-        float qv[4 * C][8], most = 0.0f;
+        float qv[DC][8], most = 0.0f;
         const float *src = p.q + (size_t)(qa + (live ? qi : 0)) * p.q_ld + (size_t)h * p.hd;
 #pragma unroll
-        for (int dc = 0; dc < 4 * C; dc++) {
+        for (int dc = 0; dc < DC; dc++) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const floatx4 w = live && 16 * dc < p.hd ? (floatx4) * reinterpret_cast<const floatx4u *>(src + 16 * dc + 8 * g + 4 * j)
@@ -400,7 +402,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
         const int eq = min(shift_for_max(most), 126);
         const float f = pow2(eq);
 #pragma unroll
-        for (int dc = 0; dc < 4 * C; dc++) split8(qv[dc], f, qh[dc], ql[dc]);
+        for (int dc = 0; dc < DC; dc++) split8(qv[dc], f, qh[dc], ql[dc]);
         to_log2 = LOG2E * pow2(-eq);
     }
     // where a lane's operands begin in a buffer: key row sigma(r32), value row r32, and the four chunks of each; rows 32 further on are
@@ -414,9 +416,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
     }
     float ref = -INFINITY, l = 0.0f;
     int ev = 1000;  // the sums are in units of 2^-ev
-    floatx16 acc[2 * C];
+    floatx16 acc[DB];
 #pragma unroll
-    for (int db = 0; db < 2 * C; db++)
+    for (int db = 0; db < DB; db++)
 #pragma unroll
         for (int v = 0; v < 16; v++) acc[db][v] = 0.0f;
     floatx16 zero;
@@ -442,11 +444,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
         if (w0 >= n_q) return;  // a wavefront without queries: its part of the copies is all it does
         floatx16 sc[2];
 #pragma unroll
-        for (int dc = 0; dc < 4 * C; dc++)
+        for (int dc = 0; dc < DC; dc++)
 #pragma unroll
             for (int kh = 0; kh < 2; kh++) {
                 const uint8_t *at = kc + (dc >> 2) * 16384 + kh * 4096 + kat[dc & 3];
-                const halfx8 hi = *reinterpret_cast<const halfx8 *>(at), lo = *reinterpret_cast<const halfx8 *>(at + 8192);
+                const halfx8 hi = *reinterpret_cast<const halfx8 *>(at);
+                const halfx8 lo = *reinterpret_cast<const halfx8 *>(D < 64 ? kc + kh * 4096 + kat[dc + 2] : at + 8192);
                 sc[kh] = mfma16(hi, qh[dc], dc == 0 ? zero : sc[kh]);
                 sc[kh] = mfma16(hi, ql[dc], sc[kh]);
                 sc[kh] = mfma16(lo, qh[dc], sc[kh]);
@@ -471,13 +474,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
             const float alpha = grow ? exp2_hw(ref - nref) : 1.0f;
             l *= alpha;
 #pragma unroll
-            for (int db = 0; db < 2 * C; db++) acc[db] *= alpha;
+            for (int db = 0; db < DB; db++) acc[db] *= alpha;
             ref = nref;
         }
         if (eb < ev) {
             const float beta = ev < 1000 ? pow2(eb - ev) : 0.0f;
 #pragma unroll
-            for (int db = 0; db < 2 * C; db++) acc[db] *= beta;
+            for (int db = 0; db < DB; db++) acc[db] *= beta;
             ev = eb;
         }
         const int less = max(ev - eb, -60);
@@ -500,9 +503,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
                 }
                 const halfx8 ph = __builtin_bit_cast(halfx8, hw), pl = __builtin_bit_cast(halfx8, lw);
 #pragma unroll
-                for (int db = 0; db < 2 * C; db++) {
+                for (int db = 0; db < DB; db++) {
                     const uint8_t *at = vc + db * 4096 + vat[2 * kh + hh];
-                    const halfx8 hi = *reinterpret_cast<const halfx8 *>(at), lo = *reinterpret_cast<const halfx8 *>(at + C * 8192);
+                    const halfx8 hi = *reinterpret_cast<const halfx8 *>(at), lo = *reinterpret_cast<const halfx8 *>(at + D * 128);
                     acc[db] = mfma16(hi, ph, acc[db]);
                     acc[db] = mfma16(hi, pl, acc[db]);
                     acc[db] = mfma16(lo, ph, acc[db]);
@@ -512,9 +515,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
         if (evo & 1) {  // values that are not finite, zeros in the tile: what sees one is no number
             const int left = limit - kb * KB;
             const uint64_t sees = left >= 64 ? ~uint64_t(0) : (left > 0 ? (uint64_t(1) << left) - 1 : 0);
-            const uint64_t *odd = p.odd + (((size_t)first + kb) * p.kv_heads + hk) * HD;
+            const uint64_t *odd = p.odd + (((size_t)first + kb) * p.kv_heads + hk) * D;
 #pragma unroll
-            for (int db = 0; db < 2 * C; db++)
+            for (int db = 0; db < DB; db++)
 #pragma unroll
                 for (int v = 0; v < 16; v++)
                     if (odd[32 * db + 8 * (v >> 2) + 4 * g + (v & 3)] & sees) acc[db][v] = NAN;
@@ -531,7 +534,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_packed(Packed p) {
     if (!done || live) {
         float *dst = done ? p.out + ((size_t)(qa + qi) * p.heads + h) * p.hd : p.part_o + (slot * QT + 32 * wave + r32) * p.hd;
 #pragma unroll
-        for (int db = 0; db < 2 * C; db++)
+        for (int db = 0; db < DB; db++)
 #pragma unroll
             for (int v4 = 0; v4 < 4; v4++) {
                 const int dim = 32 * db + 8 * v4 + 4 * g;
@@ -603,7 +606,7 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 // Wavefronts a workgroup, runs, workgroups and the working memory's parts.
 struct Plan {
-    int waves, runs, blocks, c;
+    int waves, runs, blocks, d;  // d: the heads' width, padded
     int64_t grid;
     size_t tiles, shifts, odd, tables, part_o, part_ml, cut;
     size_t bytes() const { return tiles + shifts + odd + 256 + 3 * tables + part_o + part_ml + cut; }
@@ -611,19 +614,19 @@ struct Plan {
 
 Plan plan(const PackedShape &a) {
     Plan r;
-    r.c = a.hd <= 64 ? 1 : 2;
+    r.d = a.hd <= 32 ? 32 : a.hd <= 64 ? 64 : 128;
     // tiles of 256 queries where all of a long table's are full (10,000 rows 619 -> 598 us), else of 128 (five tables of up to 6,007 rows
     // in order 513, with 256 534); heads over 64 wide leave room for one workgroup a compute unit
-    r.waves = r.c == 2 || (!a.causal && a.nq / 4096 >= a.tables) ? 8 : 4;
+    r.waves = r.d == 128 || (!a.causal && a.nq / 4096 >= a.tables) ? 8 : 4;
     const int qt = 32 * r.waves;
-    r.runs = r.waves == 8 ? 256 : 512;  // what the card holds at once, eight wavefronts a compute unit
+    r.runs = r.waves == 8 ? 256 : r.d == 32 ? 768 : 512;  // what the card holds at once
     r.grid = (a.nq / qt + (int64_t)std::min(a.tables, a.nq)) * a.heads + r.runs + 16;
     const int64_t blocks = a.nkv / KB + (int64_t)std::min(a.tables, a.nkv);
     r.blocks = (int)blocks;
     const size_t halves = (size_t)blocks * a.kv_heads, places = 2 * (size_t)r.runs * qt;
-    r.tiles = up256(halves * r.c * 32768);
+    r.tiles = up256(halves * r.d * 512);
     r.shifts = up256(halves * 2 * sizeof(int));
-    r.odd = up256(halves * 64 * r.c * sizeof(uint64_t));
+    r.odd = up256(halves * r.d * sizeof(uint64_t));
     r.tables = up256(((size_t)a.tables + 1) * sizeof(uint32_t));
     r.part_o = up256(places * a.hd * sizeof(float));
     r.part_ml = up256(places * sizeof(float2));
@@ -631,13 +634,13 @@ Plan plan(const PackedShape &a) {
     return r;
 }
 
-template <int C, int WAVES>
+template <int D, int WAVES>
 void launch(hipStream_t s, const Packed &p, const Plan &r) {
-    hipLaunchKernelGGL(k_packed_tiles<C>, dim3(std::max(r.blocks, 1), p.kv_heads, 2), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(k_packed_tiles<D>, dim3(std::max(r.blocks, 1), p.kv_heads, 2), dim3(256), 0, s, p);
     TAH_LAUNCHED();
-    hipLaunchKernelGGL((k_packed<C, WAVES>), dim3((unsigned)r.grid), dim3(64 * WAVES), 0, s, p);
+    hipLaunchKernelGGL((k_packed<D, WAVES>), dim3((unsigned)r.grid), dim3(64 * WAVES), 0, s, p);
     TAH_LAUNCHED();
-    hipLaunchKernelGGL((k_packed_join<C, 32 * WAVES>), dim3(r.runs, 2 * WAVES), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((k_packed_join<(D + 63) / 64, 32 * WAVES>), dim3(r.runs, 2 * WAVES), dim3(256), 0, s, p);
     TAH_LAUNCHED();
 }
 
@@ -672,12 +675,12 @@ void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const
     p.part_o = reinterpret_cast<float *>(carve(r.part_o));
     p.part_ml = reinterpret_cast<float2 *>(carve(r.part_ml));
     p.cut = reinterpret_cast<CutUnit *>(carve(r.cut));
-    if (r.c == 2)
-        launch<2, 8>(s, p, r);
-    else if (r.waves == 8)
-        launch<1, 8>(s, p, r);
+    if (r.d == 128)
+        launch<128, 8>(s, p, r);
+    else if (r.d == 64)
+        r.waves == 8 ? launch<64, 8>(s, p, r) : launch<64, 4>(s, p, r);
     else
-        launch<1, 4>(s, p, r);
+        r.waves == 8 ? launch<32, 8>(s, p, r) : launch<32, 4>(s, p, r);
 }
 
 }  // namespace tah
