@@ -2,8 +2,8 @@
 // precision on the fp16 matrix cores.
 //
 // Keys and values become split-fp16 tiles first, one per (block of 64 of a table's rows, key/value head), laid out as the LDS
-// images that the attention reads: tables begin at tiles of their own, short blocks are filled with zeros. The attention then
-// takes a tile of queries of one table and head a workgroup.
+// images that the attention reads: tables begin at tiles of their own, short blocks are filled with zeros. Tables that few workgroups
+// read get none: those make the images themselves. The attention then takes a tile of queries of one table and head a workgroup.
 #include "common.hpp"
 #include "device_math.hpp"
 #include "tiles.hpp"
@@ -43,6 +43,7 @@ struct Packed {
     // the attention's runs of blocks, and per slot (two a run) [queries][hd] outputs and [queries] (maximum, sum); per run the unit
     // that begins in it and ends in a later one
     int waves, runs;
+    int direct;  // tables that few workgroups read are read where they stand (few_readers)
     float *part_o;
     float2 *part_ml;
     CutUnit *cut;
@@ -100,6 +101,14 @@ struct Tiles {
         return (uint64_t)(sum + all() + (long)i * BEGIN);
     }
 };
+
+// Whether a table's blocks are split by the workgroups that read them, without tiles: where up to three do (200 tables of 50 to 100
+// rows 80 -> 56 us, 100 of 200 to 250, causal, 101 -> 87, 32 of 100 to 300 41 -> 39). More find the tiles as fast or faster (64 of 500
+// to 1,000, causal, 257, without 268; 8 of 1,000 to 2,000 150 and 171).
+constexpr int READERS = 3;
+__device__ __forceinline__ bool few_readers(const Packed &p, int n_q) {
+    return p.direct && (int64_t)((n_q + 127) / 128) * (p.heads / p.kv_heads) <= READERS;
+}
 
 __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {  // of numbers below 2^50
     const uint32_t lo = wave_scan((uint32_t)v & 0x1ffffffu), hi = wave_scan((uint32_t)(v >> 25));
@@ -191,6 +200,7 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     const int t = table_with(p.ko, p.tables, p.nkv, KB, blockIdx.x, kb);
     if (t < 0) return;
     int a = 0;
+    if (few_readers(p, rows_of(p.qo, t, p.nq, a))) return;
     const int n = min(rows_of(p.ko, t, p.nkv, a) - (int)kb * KB, KB);
     const float *src = (values ? p.v : p.k) + (size_t)(a + (int)kb * KB) * p.kv_ld + (size_t)h * p.hd;
     uint32_t big = 0, raw = 0;
@@ -258,33 +268,49 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     }
 }
 
+// what load instructions read from p on, zeros from its `bytes` on
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const float *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, bytes, 0x00027000);
+}
+
 // grid: a workgroup for each unit, and p.runs; 64 WAVES threads, 32 queries of one table and head a wavefront.
 //
 // A unit is (head, table, tile of 32 WAVES queries); its blocks are the 64-row tiles that its queries see. p.runs workgroups are what
 // the card holds at once. As many units of each head as make whole rounds of them are a workgroup's each (all of them where units are
 // short); the blocks of the others, one unit after the other, are cut into equal runs, which end together, for tables of any lengths,
 // causal or not. A run that is not a whole unit leaves a state for k_packed_join. One table of 10,000 rows and 8 heads, 632 units on
-// 512 places: two rounds X us, everything in runs 840 us (workgroups of an XCD then read different keys at a time, more than its
-// cache holds; whole units read the same ones), as it is X us.
+// 512 places: two rounds 720 us, everything in runs 840 (workgroups of an XCD then read different keys at a time, more than its
+// cache holds; whole units read the same ones), as it is 619 (557 with what follows).
 //
 // S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_32x32x16_f16, three products of halves a term, the keys in sigma32 order so that
 // the weights of a block are the values' operand where they stand. Tiles come by DMA into two LDS buffers each for keys and
-// values, a block ahead. The softmax is in log2 units against a reference that is raised when a block passes it by more than 3; weights stay
+// values, a block ahead, or are made here from rows read a block ahead (few_readers). The softmax is in log2 units against a reference that is raised when a block passes it by more than 3; weights stay
 // below 2^15. The sums are held in units of the least power of two that the values' tiles so far have; a block with a larger one
 // has its weights smaller by the difference (at most 2^60: what is cut off there is below 2^-60 of the largest value).
 //
+// In a long table the matrix pipes are busy 56% of the time and the vector pipes 46%, hardly ever at once:
+// 10,000 rows, 8 heads of 64, 557 us or 1,105 TFLOP/s of the three products, what a large fp16 product reaches here (1,109). Short
+// tables are bound by their start (plan, rows and queries on their way: about 9 us) and by memory.
 template <int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_packed(Packed p) {
     constexpr int QT = 32 * WAVES, HALF = HALF_BYTES<D>, DC = D / 16, DB = D / 32;
+    constexpr bool DIRECT = WAVES == 4 && D <= 64;
     __shared__ __align__(16) uint8_t kt0[HALF], kt1[HALF], vt0[HALF], vt1[HALF];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r32 = lane & 31, g = lane >> 5;
+    __shared__ int4 rows_here[64];
+    __shared__ uint32_t first_here[64];
+    __shared__ floatx4 most_here[4];
+    __shared__ __align__(8) uint8_t odd_here[64][8];
+    const int thread = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
 
     // the first 64 tables, one a lane, read beside the plan
-    const int t64 = min(lane, p.tables - 1);
-    uint32_t tiles64 = p.tile_sums[t64 + 1], blocks64 = p.block_sums[t64 + 1], first64 = p.first[t64];
-    int qa64 = 0, ka64 = 0;
-    const int q64 = rows_of(p.qo, t64, p.nq, qa64), k64 = rows_of(p.ko, t64, p.nkv, ka64);
+    const int t64 = min(thread & 63, p.tables - 1);
+    const uint32_t tiles64 = p.tile_sums[t64 + 1], blocks64 = p.block_sums[t64 + 1];
+    {
+        int qa = 0, ka = 0;
+        const int n_q = rows_of(p.qo, t64, p.nq, qa), n_t = rows_of(p.ko, t64, p.nkv, ka);
+        first_here[thread & 63] = p.first[t64];  // every wavefront writes the same and reads what it wrote
+        rows_here[thread & 63] = make_int4(qa, n_q, ka, n_t);
+    }
     const PackedPlan plan = *p.plan;
     // what follows each other on the same XCD (workgroup i runs on XCD i % 8): it reads the same head's keys and values
     const uint32_t share = (plan.own * p.heads + 7) / 8, share_runs = (plan.runs + 7) / 8;
@@ -295,26 +321,31 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
     const uint32_t mine = whole ? run : run * plan.per, end = whole ? run + 1 : min(total, mine + plan.per);
     const uint32_t a_head = whole ? plan.own : plan.rest;
     const uint32_t *sums = whole ? p.tile_sums : p.block_sums;
+    const uint32_t sum64 = whole ? tiles64 : blocks64;
 
     for (uint32_t at = mine; at < end;) {
     if (at != mine) __syncthreads();  // the unit before's buffers are no longer read
+    int tid = thread;
+    asm volatile("" : "+v"(tid));  // what follows from it is formed for each unit, not held for all
+    const int lane = tid & 63, r32 = lane & 31, g = lane >> 5;
     const int h = (int)(at / a_head), hk = h / (p.heads / p.kv_heads);
     const uint32_t in_head = at - h * a_head + (whole ? 0 : plan.own_blocks);
     // the table: so many end at or before here (those without queries among them)
-    int t = __popcll(__ballot(lane < p.tables - 1 && (whole ? tiles64 : blocks64) <= in_head));
+    int t = __popcll(__ballot(lane < p.tables - 1 && sum64 <= in_head));
     for (int t0 = 64; t == t0 && t0 < p.tables - 1; t0 += 64)
         t += __popcll(__ballot(t0 + lane < p.tables - 1 && sums[t0 + lane + 1] <= in_head));
     t = __builtin_amdgcn_readfirstlane(t);
-    int qa, n_q, n_t;
+    int qa, ka, n_q, n_t;
     uint32_t first, local;
     if (t < 64) {
-        qa = __builtin_amdgcn_readlane(qa64, t);
-        n_q = __builtin_amdgcn_readlane(q64, t);
-        n_t = __builtin_amdgcn_readlane(k64, t);
-        first = __builtin_amdgcn_readlane(first64, t);
-        local = in_head - (t ? __builtin_amdgcn_readlane(whole ? tiles64 : blocks64, t - 1) : 0);
+        const int4 rows = rows_here[t];
+        qa = __builtin_amdgcn_readfirstlane(rows.x);
+        n_q = __builtin_amdgcn_readfirstlane(rows.y);
+        ka = __builtin_amdgcn_readfirstlane(rows.z);
+        n_t = __builtin_amdgcn_readfirstlane(rows.w);
+        first = __builtin_amdgcn_readfirstlane(first_here[t]);
+        local = in_head - (t ? __builtin_amdgcn_readlane(sum64, t - 1) : 0);
     } else {
-        int ka = 0;
         n_q = rows_of(p.qo, t, p.nq, qa);
         n_t = rows_of(p.ko, t, p.nkv, ka);
         first = p.first[t];
@@ -353,7 +384,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
         if (g == 0) p.part_ml[slot * QT + 32 * wave + r32] = make_float2(-INFINITY, 0.0f);
         continue;
     }
+    // the rows that this lane's query sees, and those that all and any of the wavefront's see
     const int limit = live ? limit_of(qi) : n_k, least = w0 < n_q ? limit_of(w0) : n_k;
+    const int most_seen = w0 < n_q ? limit_of(min(w0 + 31, n_q - 1)) : 0;
     const int kb0 = b0, kb1 = min(b1, nb);
     const uint8_t *tiles = p.tiles + ((size_t)first * p.kv_heads + hk) * (2 * HALF);
     const int *shifts = p.shifts + 2 * ((size_t)first * p.kv_heads + hk);
@@ -373,10 +406,38 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
         key_shifts = at[0];
         value_shifts = at[1];
     };
+    const bool direct = DIRECT && few_readers(p, n_q);
+    // direct: a block's rows in registers, the next one's while a block is worked on: 8 coordinates of a key, 8 keys' value of a
+    // coordinate a lane
+    constexpr int HELD = DIRECT ? D / 32 : 1, CHUNKS = D < 64 ? D / 8 : 8;
+    u32x4 key_rows[HELD][2];
+    uint32_t value_rows[HELD][8];
+    const uint32_t ld4 = 4 * (uint32_t)p.kv_ld, past = 0x80000000u;  // past: behind all of a block's rows
+    const uint32_t key_at = 8 * (tid % CHUNKS) < p.hd ? (tid / CHUNKS) * ld4 + 32 * (tid % CHUNKS) : past;
+    const uint32_t value_at = tid % D < p.hd ? 8 * (tid / D) * ld4 + 4 * (tid % D) : past;
+    auto load_rows = [&](int kb) __attribute__((always_inline)) {
+        // rows behind the table's and coordinates behind the head's are zeros
+        const size_t at = (size_t)(ka + kb * KB) * p.kv_ld + (size_t)hk * p.hd;
+        const uint32_t bytes = (uint32_t)(min(n_k - kb * KB, KB) - 1) * ld4 + 4 * p.hd;
+        const auto ks = rows_from(p.k + at, bytes), vs = rows_from(p.v + at, bytes);
+#pragma unroll
+        for (int i = 0; i < HELD; i++) {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                key_rows[i][j] = __builtin_amdgcn_raw_buffer_load_b128(ks, key_at + i * (256 / CHUNKS) * ld4 + 16 * j, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                value_rows[i][e] = __builtin_amdgcn_raw_buffer_load_b32(vs, value_at + (i * 8 * (256 / D) + e) * ld4, 0, 0);
+        }
+    };
     if (kb0 < kb1) {
-        hold_shifts();
-        copy(tiles + kb0 * kb_bytes, kt0);
-        copy(tiles + kb0 * kb_bytes + HALF, vt0);
+        if (direct) {
+            load_rows(kb0);
+        } else {
+            hold_shifts();
+            copy(tiles + kb0 * kb_bytes, kt0);
+            copy(tiles + kb0 * kb_bytes + HALF, vt0);
+        }
     }
     // this lane's query coordinates 16 dc + 8 g + t, at a maximum near 2^14, split
     halfx8 qh[DC], ql[DC];
@@ -425,23 +486,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
 #pragma unroll
     for (int v = 0; v < 16; v++) zero[v] = 0.0f;
 
-    // Block kb from the buffers kc and vc, the next one on its way into kn and vn: four arrays, so that the compiler sees that it need
-    // not wait for the copies before it reads.
-    auto step = [&](const uint8_t *kc, const uint8_t *vc, uint8_t *kn, uint8_t *vn, int kb) __attribute__((always_inline)) {
-        if (kb >= shifts_at + 64) {
-            shifts_at += 64;
-            hold_shifts();
-        }
-        __builtin_amdgcn_s_waitcnt(0);  // this wavefront's copies of block kb have landed
-        __syncthreads();                // everyone's have, and block kb - 1's buffers are no longer read
-        const int evo = __builtin_amdgcn_readlane(value_shifts, kb - shifts_at), eb = evo >> 1;
-        const int ek = __builtin_amdgcn_readlane(key_shifts, kb - shifts_at);
+    // Block kb, scaled by 2^ek and 2^eb, in the buffers kc and vc.
+    auto block = [&](auto here, const uint8_t *kc, const uint8_t *vc, int kb, int ek, int evo) __attribute__((always_inline)) {
+        if (kb * KB >= most_seen) return;  // a wavefront whose queries see none of it: its part of the copies is all it does
+        const int eb = evo >> 1;
         const float f = fminf(fmaxf(to_log2 * pow2(-ek), 0x1p-126f), 0x1p126f);  // from raw scores to log2 units
-        if (kb + 1 < kb1) {
-            copy(tiles + (kb + 1) * kb_bytes, kn);
-            copy(tiles + (kb + 1) * kb_bytes + HALF, vn);
-        }
-        if (w0 >= n_q) return;  // a wavefront without queries: its part of the copies is all it does
         floatx16 sc[2];
 #pragma unroll
         for (int dc = 0; dc < DC; dc++)
@@ -515,7 +564,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
         if (evo & 1) {  // values that are not finite, zeros in the tile: what sees one is no number
             const int left = limit - kb * KB;
             const uint64_t sees = left >= 64 ? ~uint64_t(0) : (left > 0 ? (uint64_t(1) << left) - 1 : 0);
-            const uint64_t *odd = p.odd + (((size_t)first + kb) * p.kv_heads + hk) * D;
+            const uint64_t *odd;
+            if constexpr (decltype(here)::value)
+                odd = reinterpret_cast<const uint64_t *>(odd_here);
+            else
+                odd = p.odd + (((size_t)first + kb) * p.kv_heads + hk) * D;
 #pragma unroll
             for (int db = 0; db < DB; db++)
 #pragma unroll
@@ -523,12 +576,85 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
                     if (odd[32 * db + 8 * (v >> 2) + 4 * g + (v & 3)] & sees) acc[db][v] = NAN;
         }
     };
-    int kb = kb0;
-    for (; kb + 1 < kb1; kb += 2) {  // two steps a turn: the buffers' places are constants
-        step(kt0, vt0, kt1, vt1, kb);
-        step(kt1, vt1, kt0, vt0, kb + 1);
+    // Block kb from the buffers kc and vc, the next one on its way into kn and vn: four arrays, so that the compiler sees that it need
+    // not wait for the copies before it reads.
+    auto step = [&](const uint8_t *kc, const uint8_t *vc, uint8_t *kn, uint8_t *vn, int kb) __attribute__((always_inline)) {
+        if (kb >= shifts_at + 64) {
+            shifts_at += 64;
+            hold_shifts();
+        }
+        __builtin_amdgcn_s_waitcnt(0);  // this wavefront's copies of block kb have landed
+        __syncthreads();                // everyone's have, and block kb - 1's buffers are no longer read
+        const int evo = __builtin_amdgcn_readlane(value_shifts, kb - shifts_at);
+        const int ek = __builtin_amdgcn_readlane(key_shifts, kb - shifts_at);
+        if (kb + 1 < kb1) {
+            copy(tiles + (kb + 1) * kb_bytes, kn);
+            copy(tiles + (kb + 1) * kb_bytes + HALF, vn);
+        }
+        block(Flag<false>{}, kc, vc, kb, ek, evo);
+    };
+    if (direct) {
+        if constexpr (DIRECT)
+            for (int kb = kb0; kb < kb1; kb++) {
+                uint32_t big_k = 0, big_v = 0, raw_v = 0;
+#pragma unroll
+                for (int i = 0; i < HELD; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const uint32_t y = value_rows[i][e];
+                        big_k = max(big_k, finite_bits(key_rows[i][e >> 2][e & 3]));
+                        big_v = max(big_v, finite_bits(y));
+                        raw_v = max(raw_v, y & 0x7fffffffu);
+                    }
+                const float most_k = wave_max(__uint_as_float(big_k)), most_v = wave_max(__uint_as_float(big_v));
+                const bool any = __any(raw_v >= 0x7f800000u);
+                if (lane == 0) most_here[wave] = floatx4{most_k, most_v, any ? 1.0f : 0.0f, 0.0f};
+                __syncthreads();  // everyone's maxima are there, and block kb - 1's buffers are no longer read
+                floatx4 m = most_here[0];
+#pragma unroll
+                for (int w = 1; w < WAVES; w++)
+#pragma unroll
+                    for (int e = 0; e < 3; e++) m[e] = fmaxf(m[e], most_here[w][e]);
+                const int ek = __builtin_amdgcn_readfirstlane(min(shift_for_max(m[0]), 126));
+                const int ev = __builtin_amdgcn_readfirstlane(min(shift_for_max(m[1]), 126));
+                const bool odd = __builtin_amdgcn_readfirstlane(m[2] != 0.0f);
+                const float fk = pow2(ek), fv = pow2(ev);
+#pragma unroll
+                for (int i = 0; i < HELD; i++) {
+                    const int u = tid + 256 * i, c = u % CHUNKS, r = u / CHUNKS, dim = u % D, kc = u / D;
+                    float w[8];
+                    halfx8 wh, wl;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) w[e] = __uint_as_float(key_rows[i][e >> 2][e & 3]);
+                    split8(w, fk, wh, wl);
+                    *reinterpret_cast<halfx8 *>(kt0 + r * 128 + swz(r, c) * 16) = wh;
+                    *reinterpret_cast<halfx8 *>(D < 64 ? kt0 + r * 128 + swz(r, c + CHUNKS) * 16 : kt0 + 8192 + r * 128 + swz(r, c) * 16) = wl;
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        w[e] = __uint_as_float(value_rows[i][e]);
+                        if (odd && (value_rows[i][e] & 0x7fffffffu) >= 0x7f800000u) {
+                            bits |= 1u << e;
+                            w[e] = 0.0f;
+                        }
+                    }
+                    if (odd) odd_here[dim][kc] = (uint8_t)bits;
+                    split8(w, fv, wh, wl);
+                    *reinterpret_cast<halfx8 *>(vt0 + dim * 128 + swz(dim, kc) * 16) = wh;
+                    *reinterpret_cast<halfx8 *>(vt0 + D * 128 + dim * 128 + swz(dim, kc) * 16) = wl;
+                }
+                if (kb + 1 < kb1) load_rows(kb + 1);
+                __syncthreads();
+                block(Flag<true>{}, kt0, vt0, kb, ek, 2 * ev + (odd ? 1 : 0));
+            }
+    } else {
+        int kb = kb0;
+        for (; kb + 1 < kb1; kb += 2) {  // two steps a turn: the buffers' places are constants
+            step(kt0, vt0, kt1, vt1, kb);
+            step(kt1, vt1, kt0, vt0, kb + 1);
+        }
+        if (kb < kb1) step(kt0, vt0, kt1, vt1, kb);
     }
-    if (kb < kb1) step(kt0, vt0, kt1, vt1, kb);
     l = half_sum(l);  // lanes l and l ^ 32 have the same queries' sums over different keys
     const float inv = l > 0.0f ? 1.0f / l : l, unit = pow2(-min(ev, 149));  // 0 and NaN stay
     if (!done || live) {
@@ -672,6 +798,7 @@ void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const
     p.block_sums = reinterpret_cast<uint32_t *>(carve(r.tables));
     p.waves = r.waves;
     p.runs = r.runs;
+    p.direct = r.d <= 64 && r.waves == 4 && kv_ld < (size_t)1 << 22;  // a block's rows within 2^30 bytes
     p.part_o = reinterpret_cast<float *>(carve(r.part_o));
     p.part_ml = reinterpret_cast<float2 *>(carve(r.part_ml));
     p.cut = reinterpret_cast<CutUnit *>(carve(r.cut));

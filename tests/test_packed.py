@@ -130,6 +130,49 @@ def test_numbers_that_are_not_finite(gpu, hd, kind):
         assert np.all(np.isnan(got[sees])) and np.all(np.abs(got - out)[~sees] <= off[~sees])
 
 
+@pytest.mark.parametrize("hd", [16, 32, 64])
+@pytest.mark.parametrize("kind", ["value", "key", "query"])
+def test_numbers_that_are_not_finite_in_short_tables(gpu, hd, kind):
+    """The same for tables whose blocks only one or two tiles of queries read."""
+    rng = np.random.default_rng(hd + 1)
+    counts, heads = [128, 200, 90], 2
+    n = sum(counts)
+    for where, bad in ((128 + 3, np.nan), (128 + 133, np.inf), (128 + 199, -np.inf)):
+        q, k, v = inputs(rng, n, n, heads, heads, hd)
+        clean = [a.copy() for a in (q, k, v)]
+        dims = 7 if kind == "value" else slice(None)
+        {"query": q, "key": k, "value": v}[kind][where, 1, 7] = bad
+        got = gpu.attend_packed(flat(q), flat(k), flat(v), offsets_of(counts), heads, heads, True).reshape(q.shape)
+        sees = np.zeros(q.shape, bool)
+        sees[where:where + 1 if kind == "query" else 328, 1, dims] = True
+        out, off = wanted(*clean, counts, counts, True)
+        say(f"{kind} {bad} at row {where}: {int(sees.sum())} outputs see it")
+        assert np.all(np.isnan(got[sees])) and np.all(np.abs(got - out)[~sees] <= off[~sees])
+
+
+@pytest.mark.parametrize("beside", [np.nan, 1e30])
+@pytest.mark.parametrize("hd", [16, 48, 64, 80])
+def test_what_stands_beside_the_heads(gpu, dev, hd, beside):
+    """Rows of one head among columns, and between rows of no table, that hold anything: short tables, tables whose tiles are made
+    first, one long enough to be cut, and a table with rows but no queries."""
+    rng = np.random.default_rng(hd)
+    counts, ld = [100, 7, 250, 300, 64, 1100], hd + 11
+    n = sum(counts)
+    q, k, v = inputs(rng, n, n, 1, 1, hd)
+    around = np.full((2, n + 8, ld), beside, np.float32)
+    around[0, 4:-4, 5:5 + hd], around[1, 4:-4, 5:5 + hd] = flat(k), flat(v)
+    at, rows, skip = offsets_of(counts), dev.of(around), 4 * (4 * ld + 5)
+    asked = [c if i != 4 else 0 for i, c in enumerate(counts)]
+    keep = np.concatenate([np.arange(at[i], at[i] + a) for i, a in enumerate(asked)])
+    qd, qo, ko = dev.of(flat(q[keep])), dev.of(offsets_of(asked)), dev.of(at)
+    for causal in (False, True):
+        od = dev.of(np.full((len(keep), hd), 3.0, np.float32))
+        gpu.attend_packed_dev(qd.ptr, rows.ptr + skip, rows.ptr + 4 * (n + 8) * ld + skip, qo.ptr, ko.ptr, len(counts), len(keep), n, 1, 1,
+                              hd, od.ptr, causal, 0, ld)
+        gpu.sync()
+        check(od.download((len(keep), 1, hd)), *wanted(q[keep], k, v, asked, counts, causal), f"beside {beside}, causal {causal}")
+
+
 def test_strides_and_spare_rows_on_device_memory(gpu, dev):
     """Queries, keys and values as parts of wider rows at odd distances; queries past the last table's are left as they were, and
     rows past it, NaN here, are not read as any table's."""
