@@ -283,10 +283,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const float *p, uint
 // cache holds; whole units read the same ones), as it is 619 (557 with what follows).
 //
 // S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_32x32x16_f16, three products of halves a term, the keys in sigma32 order so that
-// the weights of a block are the values' operand where they stand. Tiles come by DMA into two LDS buffers each for keys and
-// values, a block ahead, or are made here from rows read a block ahead (few_readers). The softmax is in log2 units against a reference that is raised when a block passes it by more than 3; weights stay
-// below 2^15. The sums are held in units of the least power of two that the values' tiles so far have; a block with a larger one
-// has its weights smaller by the difference (at most 2^60: what is cut off there is below 2^-60 of the largest value).
+// the weights of a block are the values' operand where they stand. Tiles come by DMA into two LDS buffers each for keys and values,
+// a block ahead (one each where two would leave one workgroup of four wavefronts a compute unit), or are made here from rows read a
+// block ahead (few_readers). The softmax is in log2 units against a reference that is raised when a block passes it by more than 3;
+// weights stay below 2^15. The sums are held in units of the least power of two that the values' tiles so far have; a block with a
+// larger one has its weights smaller by the difference (at most 2^60: what is cut off there is below 2^-60 of the largest value).
 //
 // In a long table the matrix pipes are busy 56% of the time and the vector pipes 46%, hardly ever at once:
 // 10,000 rows, 8 heads of 64, 557 us or 1,105 TFLOP/s of the three products, what a large fp16 product reaches here (1,109). Short
@@ -294,8 +295,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const float *p, uint
 template <int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_packed(Packed p) {
     constexpr int QT = 32 * WAVES, HALF = HALF_BYTES<D>, DC = D / 16, DB = D / 32;
-    constexpr bool DIRECT = WAVES == 4 && D <= 64;
-    __shared__ __align__(16) uint8_t kt0[HALF], kt1[HALF], vt0[HALF], vt1[HALF];
+    constexpr bool DIRECT = WAVES == 4 && D <= 64, SINGLE = WAVES == 4 && D == 128;
+    __shared__ __align__(16) uint8_t kt0[HALF], kt1[SINGLE ? 16 : HALF], vt0[HALF], vt1[SINGLE ? 16 : HALF];
     __shared__ int4 rows_here[64];
     __shared__ uint32_t first_here[64];
     __shared__ floatx4 most_here[4];
@@ -628,7 +629,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
                     for (int e = 0; e < 8; e++) w[e] = __uint_as_float(key_rows[i][e >> 2][e & 3]);
                     split8(w, fk, wh, wl);
                     *reinterpret_cast<halfx8 *>(kt0 + r * 128 + swz(r, c) * 16) = wh;
-                    *reinterpret_cast<halfx8 *>(D < 64 ? kt0 + r * 128 + swz(r, c + CHUNKS) * 16 : kt0 + 8192 + r * 128 + swz(r, c) * 16) = wl;
+                    *reinterpret_cast<halfx8 *>(kt0 + r * 128 + (D < 64 ? swz(r, c + CHUNKS) * 16 : 8192 + swz(r, c) * 16)) = wl;
                     uint32_t bits = 0;
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
@@ -647,6 +648,22 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
                 __syncthreads();
                 block(Flag<true>{}, kt0, vt0, kb, ek, 2 * ev + (odd ? 1 : 0));
             }
+    } else if constexpr (SINGLE) {
+        for (int kb = kb0; kb < kb1; kb++) {
+            if (kb >= shifts_at + 64) {
+                shifts_at += 64;
+                hold_shifts();
+            }
+            __builtin_amdgcn_s_waitcnt(0);  // as in step
+            __syncthreads();
+            block(Flag<false>{}, kt0, vt0, kb, __builtin_amdgcn_readlane(key_shifts, kb - shifts_at),
+                  __builtin_amdgcn_readlane(value_shifts, kb - shifts_at));
+            if (kb + 1 < kb1) {
+                __syncthreads();  // the buffers are no longer read; the compute unit's other workgroup works meanwhile
+                copy(tiles + (kb + 1) * kb_bytes, kt0);
+                copy(tiles + (kb + 1) * kb_bytes + HALF, vt0);
+            }
+        }
     } else {
         int kb = kb0;
         for (; kb + 1 < kb1; kb += 2) {  // two steps a turn: the buffers' places are constants
@@ -742,8 +759,10 @@ Plan plan(const PackedShape &a) {
     Plan r;
     r.d = a.hd <= 32 ? 32 : a.hd <= 64 ? 64 : 128;
     // tiles of 256 queries where all of a long table's are full (10,000 rows 619 -> 598 us), else of 128 (five tables of up to 6,007 rows
-    // in order 513, with 256 534); heads over 64 wide leave room for one workgroup a compute unit
-    r.waves = r.d == 128 || (!a.causal && a.nq / 4096 >= a.tables) ? 8 : 4;
+    // in order 513, with 256 534). Heads over 64 wide: 256 at one workgroup a compute unit or, where tables are short, 128 at two,
+    // with one buffer each for keys and values (100 of up to 300 rows, in order, 155 -> 139 us, 32 of up to 300 66 -> 54; 8,000 rows 357
+    // and 373).
+    r.waves = (r.d == 128 ? a.nq / 2048 >= a.tables : !a.causal && a.nq / 4096 >= a.tables) ? 8 : 4;
     const int qt = 32 * r.waves;
     r.runs = r.waves == 8 ? 256 : r.d == 32 ? 768 : 512;  // what the card holds at once
     r.grid = (a.nq / qt + (int64_t)std::min(a.tables, a.nq)) * a.heads + r.runs + 16;
@@ -803,7 +822,7 @@ void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const
     p.part_ml = reinterpret_cast<float2 *>(carve(r.part_ml));
     p.cut = reinterpret_cast<CutUnit *>(carve(r.cut));
     if (r.d == 128)
-        launch<128, 8>(s, p, r);
+        r.waves == 8 ? launch<128, 8>(s, p, r) : launch<128, 4>(s, p, r);
     else if (r.d == 64)
         r.waves == 8 ? launch<64, 8>(s, p, r) : launch<64, 4>(s, p, r);
     else

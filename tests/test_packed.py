@@ -64,6 +64,17 @@ def test_long_tables(gpu, hd, causal):
     check(got, *wanted(q, k, v, counts, counts, causal), f"heads of {hd}, causal {causal}")
 
 
+@pytest.mark.parametrize("hd,rows,causal", [(32, 4300, False), (64, 4300, False), (128, 2300, False), (128, 2300, True)])
+def test_one_long_table(gpu, hd, rows, causal):
+    """Long enough alone for the larger tiles of queries, not long enough with another."""
+    rng = np.random.default_rng(rows)
+    for counts in ([rows], [3, rows - 40]):
+        n = sum(counts)
+        q, k, v = inputs(rng, n, n, 2, 1, hd)
+        got = gpu.attend_packed(flat(q), flat(k), flat(v), offsets_of(counts), 2, 1, causal).reshape(q.shape)
+        check(got, *wanted(q, k, v, counts, counts, causal), f"{counts} rows, heads of {hd}, causal {causal}")
+
+
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("q_counts,kv_counts", [
     ([1], [5000]), ([3, 0, 2], [0, 100, 4000]), ([10, 20, 1], [4, 20, 0]), ([40, 300], [1000, 299]), ([1, 1, 1, 1], [64, 128, 1, 63])])
@@ -151,7 +162,7 @@ def test_numbers_that_are_not_finite_in_short_tables(gpu, hd, kind):
 
 
 @pytest.mark.parametrize("beside", [np.nan, 1e30])
-@pytest.mark.parametrize("hd", [16, 48, 64, 80])
+@pytest.mark.parametrize("hd", [16, 48, 64, 80, 112])
 def test_what_stands_beside_the_heads(gpu, dev, hd, beside):
     """Rows of one head among columns, and between rows of no table, that hold anything: short tables, tables whose tiles are made
     first, one long enough to be cut, and a table with rows but no queries."""
