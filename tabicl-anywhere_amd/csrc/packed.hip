@@ -289,7 +289,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const float *p, uint
 // weights stay below 2^15. The sums are held in units of the least power of two that the values' tiles so far have; a block with a
 // larger one has its weights smaller by the difference (at most 2^60: what is cut off there is below 2^-60 of the largest value).
 //
-// In a long table the matrix pipes are busy 56% of the time and the vector pipes 46%, hardly ever at once:
+// In a long table the matrix pipes are busy 61% of the time and the vector pipes 48%, hardly ever at once:
 // 10,000 rows, 8 heads of 64, 557 us or 1,105 TFLOP/s of the three products, what a large fp16 product reaches here (1,109). Short
 // tables are bound by their start (plan, rows and queries on their way: about 9 us) and by memory.
 template <int D, int WAVES>

@@ -13,7 +13,7 @@ namespace {
 
 constexpr int WAVES = 4;
 // What beginning and ending a unit costs, in blocks: a unit counts as so many more than it has, so that wavefronts with several
-// units get fewer of them.
+// units get fewer of them. 24 tables of up to 6,001 rows 69, 62.5 and 62.4 us for 1, 2 and 4, 64 of up to 20,000 139.5, 140.8, 141.8.
 constexpr int BEGIN = 2;
 
 // What runs of blocks leave behind for the join: per slot [columns][hd] outputs and [columns] (maximum, sum); a wavefront has at
@@ -128,6 +128,13 @@ __device__ __forceinline__ floatx4 mfma(halfx8 a, halfx8 b, floatx4 c) {
 // products (i8), three (f32) or four (i16: a low byte is 2^-8 of the largest number, so its product with a low half counts), for
 // f32's error. Weights are held below 2^15 (their maximum raised by blocks that pass it by more than
 // 2^3), times the value's step over a power of two that no step so far passes.
+//
+// Bound by bytes where tables are long: 64 of up to 20,000 rows, 8 heads of 64 in i8, one query each, 133 us of kernel for 702 MB, 5.3
+// TB/s, what a large copy reaches (vector instructions issue in 55% of the cycles, matrix instructions in 14%). One table of 100,000
+// rows, 28 us, has 3.1 blocks a wavefront: the start (lengths, plan, queries, the first keys and their steps, one after the other)
+// is 8 us of it, all that 1,000 rows take. i16's four products of 16 columns twice and f32's splitting cost more than their bytes.
+// Tried and slower: a block's keys and values read while the one before is worked on (141 -> 153 us, the compiler has no registers
+// for both), three wavefronts a SIMD (176, spilling). Two sets of columns that share what is read: registers allow no third.
 template <int FMT, int C, int CT, int KS>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const int32_t *__restrict__ lengths,
                                                                 const float *__restrict__ q, const int32_t *__restrict__ offsets,
@@ -602,8 +609,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
 }
 
 // grid (queries x heads, over 4 / PER); 256 threads: the states that runs of blocks left of a query and head, together: PER
-// wavefronts for each query and head, every PER-th state each. Four where there are few (a state after the other takes longest),
-// one where there are many (their number does).
+// wavefronts for each query and head, every PER-th state each. Four where there are few (a state after the other takes longest:
+// the call of one query of 8 heads over 100,000 rows 33 us, with one 42; 7 tables of up to 9,000 23.6 and 27.5), one where there
+// are many (their number does: 24 tables, up to 9 queries each, of 16 heads 62.4 us, with four 65.6). The launch is most of it.
 template <int CT, int PER>
 __global__ __launch_bounds__(256) void k_pages_join(int tables, int hd, const int32_t *__restrict__ offsets, int items,
                                                     int heads, float *__restrict__ out, Parts parts) {
