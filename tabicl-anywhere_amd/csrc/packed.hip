@@ -12,14 +12,14 @@ namespace tah {
 
 namespace {
 
-// What the attention's workgroups do (k_packed): of each head's units, `own` are a workgroup's each; the blocks of the others, `rest` of
-// a head from block own_blocks on, go in `runs` runs of `per`.
+// What the attention's workgroups do (k_packed): of each head's units (of each 2^log_share heads'), `own` are a workgroup's each; the
+// blocks of the others, `rest` of a head from block own_blocks on, go in `runs` runs of `per`.
 struct PackedPlan {
     uint32_t own, own_blocks, rest, per, runs;
 };
 
-// A unit that several runs have parts of, from the one it begins in (slot) to last_run: its queries from row on, `live` of them, and
-// its head. live 0: there is none.
+// A unit that several runs have parts of, from the one it begins in (slot) to last_run: `live` columns, queries from row on and heads
+// from head on. live 0: there is none.
 struct CutUnit {
     uint32_t slot, last_run;
     int row, live, head;
@@ -31,6 +31,7 @@ struct Packed {
     int tables, nq, nkv, heads, kv_heads, hd, causal;
     size_t q_ld, kv_ld;
     float *out;
+    int log_share;  // a tile's columns are its queries' 2^log_share heads that share their keys
     // working memory: the tiles, per tile the keys' and the values' power of two (twice it, and 1 if a value is not finite), which
     // keys of each coordinate hold values that are not; the attention's plan, and per table its first block of rows, and for one head the
     // tiles of queries of the tables before it and those tiles' blocks (tables + 1)
@@ -75,29 +76,43 @@ __device__ __forceinline__ int table_with(const int32_t *offsets, int tables, in
     return -1;
 }
 
-// What beginning and ending a unit costs, in blocks; and a unit of so many blocks is not cut.
-constexpr int BEGIN = 1, WHOLE = 8;
+// What beginning and ending a unit costs, in blocks of heads padded to D (8,000 rows in order, 8 heads of 64 that share their keys, 260,
+// 237 and 225 us with 1, 2 and 3; three tables of up to 2,500, heads of 128, 99, 91 and 94). A unit of WHOLE blocks is not cut.
+template <int D>
+constexpr int BEGIN_OF = D == 128 ? 2 : 3;
+constexpr int WHOLE = 8;
 
 // A table's tiles of queries in the order in which they are taken (causal: the last first, which have the most to do), the blocks of
-// tile i and of all tiles before it (BEGIN more for each).
-template <int QT>
+// tile i and of all tiles before it (BEGIN more for each). A tile has 2^log_queries queries.
+template <int BEGIN>
 struct Tiles {
-    int n_q, n_k, causal;
-    __device__ __forceinline__ int count() const { return (n_q + QT - 1) / QT; }
-    __device__ __forceinline__ int first_query(int i) const { return (causal ? count() - 1 - i : i) * QT; }
+    int n_q, n_k, causal, log_queries;
+    __device__ __forceinline__ int count() const { return (n_q + (1 << log_queries) - 1) >> log_queries; }
+    __device__ __forceinline__ int first_query(int i) const { return (causal ? count() - 1 - i : i) << log_queries; }
     __device__ __forceinline__ int all() const { return (n_k + KB - 1) / KB; }
-    // causal, by place: tile j's last query sees the rows but those of the queries behind it, so its blocks are ahead() + (j + 1) QT /
-    // KB, none below 0, but for the last tile, which ends with the last query
-    __device__ __forceinline__ int ahead() const { return (n_k - n_q + KB - 1) >> 6; }
+    // causal, by place: tile j's last query sees the rows but those of the queries behind it, so its blocks are (seen() + j
+    // 2^log_queries) / 64, none below 0, but for the last tile, which ends with the last query
+    __device__ __forceinline__ int seen() const { return n_k - n_q + KB - 1 + (1 << log_queries); }
     __device__ __forceinline__ int blocks(int i) const {
-        return !causal || i == 0 ? all() : max(0, ahead() + (count() - i) * (QT / KB));
+        return !causal || i == 0 ? all() : max(0, (seen() + ((count() - 1 - i) << log_queries)) >> 6);
+    }
+    // sum of k >> log from 0 to n - 1
+    __device__ __forceinline__ static long quotients(long n, int log) {
+        const long q = n >> log;
+        return ((q * (q - 1) / 2) << log) + q * (n - (q << log));
     }
     __device__ __forceinline__ uint64_t before(int i) const {
         if (!causal || i == 0) return (uint64_t)i * (all() + BEGIN);
-        // places count() - i .. count() - 2, and the last
-        const long a = ahead(), m = QT / KB, j1 = count() - 1, low = count() - i;
-        const long j0 = a >= 0 ? low : max(low, min(j1, -a / m));
-        const long sum = (j1 - j0) * a + m * ((j1 * (j1 + 1) - j0 * (j0 + 1)) / 2);
+        // places count() - i .. count() - 2, from the first that has blocks on, and the last
+        const long c = seen(), j1 = count() - 1, low = count() - i;
+        const long j0 = c >= KB ? low : max(low, min(j1, (KB - c + (1 << log_queries) - 1) >> log_queries));
+        long sum;
+        if (log_queries >= 6) {
+            sum = (j1 - j0) * (c >> 6) + (((j1 * (j1 - 1) - j0 * (j0 - 1)) / 2) << (log_queries - 6));
+        } else {
+            const long f = c >> log_queries;
+            sum = j0 < j1 ? quotients(f + j1, 6 - log_queries) - quotients(f + j0, 6 - log_queries) : 0;
+        }
         return (uint64_t)(sum + all() + (long)i * BEGIN);
     }
 };
@@ -107,7 +122,8 @@ struct Tiles {
 // to 1,000, causal, 257, without 268; 8 of 1,000 to 2,000 150 and 171).
 constexpr int READERS = 3;
 __device__ __forceinline__ bool few_readers(const Packed &p, int n_q) {
-    return p.direct && (int64_t)((n_q + 127) / 128) * (p.heads / p.kv_heads) <= READERS;
+    const int log = 7 - p.log_share;  // of a tile's queries
+    return p.direct && (int64_t)((n_q + (1 << log) - 1) >> log) * ((p.heads / p.kv_heads) >> p.log_share) <= READERS;
 }
 
 __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {  // of numbers below 2^50
@@ -119,12 +135,13 @@ __device__ __forceinline__ uint64_t lane64(uint64_t v, int l) {
            (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, l);
 }
 
-// One wavefront: the attention's plan for tiles of QT queries. As many units of each head as make whole rounds of p.runs workgroups are
-// a workgroup's each, one round less where they are of different lengths (there have to be enough blocks in runs to fill the places
-// that end first); all of them where units are short, or blocks too many for 32 bits.
-template <int QT>
+// One wavefront: the attention's plan for tiles of QT columns. As many units of each head as make whole rounds of p.runs workgroups are
+// a workgroup's each. All of them where units are short, where they are of different lengths in two rounds or more (their ends
+// overlap by themselves: ten tables of 1,000 to 5,000 rows 675 us, with runs 710; four of up to 8,000, in order, 452 and 460), or
+// where blocks are too many for 32 bits.
+template <int QT, int BEGIN>
 __device__ void make_plan(const Packed &p) {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, heads = p.heads >> p.log_share, log_queries = (QT == 256 ? 8 : 7) - p.log_share;
     uint64_t rows = 0, units = 0, blocks = 0;
     int longest = 0, shortest = 0x7fffff;
     for (int t0 = 0; t0 < p.tables; t0 += 64) {
@@ -137,7 +154,7 @@ __device__ void make_plan(const Packed &p) {
         if (in) p.first[t] = (uint32_t)min(before, (uint64_t)0x7fffffff);
         rows = lane64(before + nb, 63);
         // a table past the room that the offsets' promise gives has no rows
-        const Tiles<QT> ts{n_q, before + nb <= (uint64_t)p.blocks ? n_t : 0, p.causal};
+        const Tiles<BEGIN> ts{n_q, before + nb <= (uint64_t)p.blocks ? n_t : 0, p.causal, log_queries};
         const uint64_t tiles = in ? ts.count() : 0, cost = in ? ts.before(ts.count()) : 0;
         const uint64_t tile_sum = units + wave_scan64(tiles), block_sum = blocks + wave_scan64(cost);
         if (in) {
@@ -153,17 +170,17 @@ __device__ void make_plan(const Packed &p) {
     }
     longest = (int)wave_max((float)longest);
     shortest = (int)-wave_max(-(float)shortest);
-    const uint64_t rounds = units * p.heads / p.runs;
+    const uint64_t rounds = units * heads / p.runs;
     const bool even = !p.causal && shortest + 1 >= longest;
-    uint64_t own = rounds * p.runs / p.heads;
-    if (longest <= WHOLE || (!even && rounds >= 3) || blocks * p.heads >> 32) own = units;
+    uint64_t own = rounds * p.runs / heads;
+    if (longest <= WHOLE || (!even && rounds >= 2) || blocks * heads >> 32) own = units;
     uint64_t own_blocks = own < units ? 0 : blocks;
     if (own > 0 && own < units)
         for (int t0 = 0; t0 < p.tables; t0 += 64) {
             const int t = min(t0 + lane, p.tables - 1);
             int qa = 0, ka = 0;
             const int n_q = rows_of(p.qo, t, p.nq, qa), n_t = rows_of(p.ko, t, p.nkv, ka);
-            const Tiles<QT> ts{n_q, (uint64_t)p.first[t] + (n_t + KB - 1) / KB <= (uint64_t)p.blocks ? n_t : 0, p.causal};
+            const Tiles<BEGIN> ts{n_q, (uint64_t)p.first[t] + (n_t + KB - 1) / KB <= (uint64_t)p.blocks ? n_t : 0, p.causal, log_queries};
             const uint64_t a = p.tile_sums[t];
             const uint64_t here = __ballot(t0 + lane < p.tables && own >= a && own < a + ts.count());
             if (here) {
@@ -173,7 +190,7 @@ __device__ void make_plan(const Packed &p) {
             }
         }
     if (lane == 0) {
-        const uint64_t rest = blocks - own_blocks, total = rest * p.heads;
+        const uint64_t rest = blocks - own_blocks, total = rest * heads;
         const uint64_t per = max((uint64_t)WHOLE, (total + p.runs - 1) / p.runs);
         p.tile_sums[p.tables] = (uint32_t)units;
         p.block_sums[p.tables] = (uint32_t)min(blocks, (uint64_t)0xffffffff);
@@ -195,7 +212,7 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     __shared__ int some[4];
     const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.y;
     const bool values = blockIdx.z == 1;
-    if (blockIdx.x == 0 && h == 0 && !values && tid < 64) p.waves == 8 ? make_plan<256>(p) : make_plan<128>(p);
+    if (blockIdx.x == 0 && h == 0 && !values && tid < 64) p.waves == 8 ? make_plan<256, BEGIN_OF<D>>(p) : make_plan<128, BEGIN_OF<D>>(p);
     uint32_t kb = 0;
     const int t = table_with(p.ko, p.tables, p.nkv, KB, blockIdx.x, kb);
     if (t < 0) return;
@@ -273,14 +290,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const float *p, uint
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, bytes, 0x00027000);
 }
 
-// grid: a workgroup for each unit, and p.runs; 64 WAVES threads, 32 queries of one table and head a wavefront.
+// grid: a workgroup for each unit, and p.runs; 64 WAVES threads, 32 columns a wavefront.
 //
-// A unit is (head, table, tile of 32 WAVES queries); its blocks are the 64-row tiles that its queries see. p.runs workgroups are what
-// the card holds at once. As many units of each head as make whole rounds of them are a workgroup's each (all of them where units are
-// short); the blocks of the others, one unit after the other, are cut into equal runs, which end together, for tables of any lengths,
-// causal or not. A run that is not a whole unit leaves a state for k_packed_join. One table of 10,000 rows and 8 heads, 632 units on
-// 512 places: two rounds 720 us, everything in runs 840 (workgroups of an XCD then read different keys at a time, more than its
-// cache holds; whole units read the same ones), as it is 619 (557 with what follows).
+// A unit is (heads that share keys, table, tile of 32 WAVES columns, each a query and one of those heads); its blocks are the 64-row
+// tiles that its queries see. 50 tables of 250 to 500 rows, in order, 16 heads of 32 over 4: 63 us, with a head a unit 70; 95 of 11
+// rows, 8 heads of 128 over one, 20 and 35. p.runs workgroups are what the card holds at once. As many units of each head as make whole
+// rounds of them are a workgroup's each (all of them where units are short); the blocks of the others, one unit after the other, are
+// cut into equal runs, which end together, for tables of any lengths, causal or not. A run that is not a whole unit leaves a state for
+// k_packed_join. One table of 10,000 rows and 8 heads, 632 units on 512 places: two rounds 720 us, everything in runs 840 (workgroups
+// of an XCD then read different keys at a time, more than its cache holds; whole units read the same ones), as it is 619 (557 with what
+// follows).
 //
 // S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_32x32x16_f16, three products of halves a term, the keys in sigma32 order so that
 // the weights of a block are the values' operand where they stand. Tiles come by DMA into two LDS buffers each for keys and values,
@@ -294,7 +313,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const float *p, uint
 // tables are bound by their start (plan, rows and queries on their way: about 9 us) and by memory.
 template <int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_packed(Packed p) {
-    constexpr int QT = 32 * WAVES, HALF = HALF_BYTES<D>, DC = D / 16, DB = D / 32;
+    constexpr int QT = 32 * WAVES, HALF = HALF_BYTES<D>, DC = D / 16, DB = D / 32, BEGIN = BEGIN_OF<D>;
     constexpr bool DIRECT = WAVES == 4 && D <= 64, SINGLE = WAVES == 4 && D == 128;
     __shared__ __align__(16) uint8_t kt0[HALF], kt1[SINGLE ? 16 : HALF], vt0[HALF], vt1[SINGLE ? 16 : HALF];
     __shared__ int4 rows_here[64];
@@ -313,12 +332,17 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
         rows_here[thread & 63] = make_int4(qa, n_q, ka, n_t);
     }
     const PackedPlan plan = *p.plan;
-    // what follows each other on the same XCD (workgroup i runs on XCD i % 8): it reads the same head's keys and values
-    const uint32_t share = (plan.own * p.heads + 7) / 8, share_runs = (plan.runs + 7) / 8;
+    const int heads = p.heads >> p.log_share, log_queries = (WAVES == 8 ? 8 : 7) - p.log_share;
+    // Workgroup i runs on XCD i % 8. So many XCDs as a head has, where there are fewer heads than XCDs, take turns at its units or runs
+    // (else an XCD has whole heads): an XCD reads few heads' keys, and all have long and short units alike.
+    const int log_turns = 3 - min(3, __builtin_ctz(heads)), turns = 1 << log_turns, sets = 8 >> log_turns;
+    const uint32_t set_units = plan.own * (uint32_t)(heads / sets), set_runs = (plan.runs + sets - 1) / sets;
+    const uint32_t share = (set_units + turns - 1) >> log_turns;
     const bool whole = blockIdx.x < 8 * share;
-    const uint32_t idx = whole ? blockIdx.x : blockIdx.x - 8 * share, each = whole ? share : share_runs;
-    const uint32_t run = (idx & 7) * each + (idx >> 3), total = whole ? plan.own * p.heads : plan.rest * p.heads;
-    if ((idx >> 3) >= each || run >= (whole ? total : plan.runs)) return;
+    const uint32_t idx = whole ? blockIdx.x : blockIdx.x - 8 * share, xcd = idx & 7, size = whole ? set_units : set_runs;
+    const uint32_t in_set = (idx >> 3 << log_turns) + (xcd & (turns - 1)), run = (xcd >> log_turns) * size + in_set;
+    const uint32_t total = plan.rest * heads;
+    if (in_set >= size || (!whole && run >= plan.runs)) return;
     const uint32_t mine = whole ? run : run * plan.per, end = whole ? run + 1 : min(total, mine + plan.per);
     const uint32_t a_head = whole ? plan.own : plan.rest;
     const uint32_t *sums = whole ? p.tile_sums : p.block_sums;
@@ -329,8 +353,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
     int tid = thread;
     asm volatile("" : "+v"(tid));  // what follows from it is formed for each unit, not held for all
     const int lane = tid & 63, r32 = lane & 31, g = lane >> 5;
-    const int h = (int)(at / a_head), hk = h / (p.heads / p.kv_heads);
-    const uint32_t in_head = at - h * a_head + (whole ? 0 : plan.own_blocks);
+    const uint32_t shared = at / a_head, in_head = at - shared * a_head + (whole ? 0 : plan.own_blocks);
+    const int h0 = (int)(shared << p.log_share), hk = h0 / (p.heads / p.kv_heads);
     // the table: so many end at or before here (those without queries among them)
     int t = __popcll(__ballot(lane < p.tables - 1 && sum64 <= in_head));
     for (int t0 = 64; t == t0 && t0 < p.tables - 1; t0 += 64)
@@ -353,7 +377,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
         local = in_head - sums[t];
     }
     const int n_k = (uint64_t)first + (n_t + KB - 1) / KB <= (uint64_t)p.blocks ? n_t : 0;
-    const Tiles<QT> ts{n_q, n_k, p.causal};
+    const Tiles<BEGIN> ts{n_q, n_k, p.causal, log_queries};
     int tile = 0;
     if (whole) {
         tile = (int)local;
@@ -375,11 +399,13 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
     const size_t slot = 2 * (size_t)run + (at == mine ? 0 : 1);
     const uint32_t last_run = done ? run : (at - b0 + nb + BEGIN - 1) / plan.per;
     at += whole ? 1 : b1 - b0;
-    const int w0 = ts.first_query(tile) + 32 * wave, qi = w0 + r32;
+    // a column is a query and one of the heads that share its keys; w0, w1 the wavefront's first and last query
+    const int row0 = ts.first_query(tile), w0 = row0 + ((32 * wave) >> p.log_share), w1 = row0 + ((32 * wave + 31) >> p.log_share);
+    const int qi = row0 + ((32 * wave + r32) >> p.log_share), h = h0 + ((32 * wave + r32) & ((1 << p.log_share) - 1));
     auto limit_of = [&](int i) { return p.causal ? max(0, n_k - (n_q - 1 - i)) : n_k; };
     const bool live = qi < n_q;
     if (!whole && at >= end && tid == 0)
-        p.cut[run] = b0 == 0 && !done ? CutUnit{(uint32_t)slot, last_run, qa + ts.first_query(tile), min(QT, n_q - ts.first_query(tile)), h}
+        p.cut[run] = b0 == 0 && !done ? CutUnit{(uint32_t)slot, last_run, qa + row0, min(QT >> p.log_share, n_q - row0) << p.log_share, h0}
                                       : CutUnit{};
     if (b0 > 0 && b0 >= nb) {  // behind the unit's blocks
         if (g == 0) p.part_ml[slot * QT + 32 * wave + r32] = make_float2(-INFINITY, 0.0f);
@@ -387,7 +413,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
     }
     // the rows that this lane's query sees, and those that all and any of the wavefront's see
     const int limit = live ? limit_of(qi) : n_k, least = w0 < n_q ? limit_of(w0) : n_k;
-    const int most_seen = w0 < n_q ? limit_of(min(w0 + 31, n_q - 1)) : 0;
+    const int most_seen = w0 < n_q ? limit_of(min(w1, n_q - 1)) : 0;
     const int kb0 = b0, kb1 = min(b1, nb);
     const uint8_t *tiles = p.tiles + ((size_t)first * p.kv_heads + hk) * (2 * HALF);
     const int *shifts = p.shifts + 2 * ((size_t)first * p.kv_heads + hk);
@@ -693,8 +719,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
     }
 }
 
-// grid (runs, tiles' queries / 16); 256 threads: the states that runs left of a unit's sixteen queries, together: sixteen lanes a
-// query, four of each 64 coordinates a lane.
+// grid (runs, tiles' queries / 16); 256 threads: the states that runs left of a unit's sixteen columns, together: sixteen lanes a
+// column, four of each 64 coordinates a lane.
 template <int C, int QT>
 __global__ __launch_bounds__(256) void k_packed_join(Packed p) {
     constexpr int AHEAD = 4;
@@ -742,14 +768,15 @@ __global__ __launch_bounds__(256) void k_packed_join(Packed p) {
 #pragma unroll
     for (int c = 0; c < C; c++)
         if (64 * c + dim < p.hd)
-            *reinterpret_cast<floatx4u *>(p.out + ((size_t)(unit.row + r) * p.heads + unit.head) * p.hd + 64 * c + dim) = o[c] * inv;
+            *reinterpret_cast<floatx4u *>(p.out + ((size_t)(unit.row + (r >> p.log_share)) * p.heads + unit.head +
+                                                   (r & ((1 << p.log_share) - 1))) * p.hd + 64 * c + dim) = o[c] * inv;
 }
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 // Wavefronts a workgroup, runs, workgroups and the working memory's parts.
 struct Plan {
-    int waves, runs, blocks, d;  // d: the heads' width, padded
+    int waves, runs, blocks, d, log_share;  // d: the heads' width, padded
     int64_t grid;
     size_t tiles, shifts, odd, tables, part_o, part_ml, cut;
     size_t bytes() const { return tiles + shifts + odd + 256 + 3 * tables + part_o + part_ml + cut; }
@@ -764,8 +791,11 @@ Plan plan(const PackedShape &a) {
     // and 373).
     r.waves = (r.d == 128 ? a.nq / 2048 >= a.tables : !a.causal && a.nq / 4096 >= a.tables) ? 8 : 4;
     const int qt = 32 * r.waves;
+    // heads that share their keys share tiles too, by powers of two up to a wavefront's columns
+    r.log_share = 0;
+    while (r.log_share < 5 && (a.heads / a.kv_heads) % (2 << r.log_share) == 0) r.log_share++;
     r.runs = r.waves == 8 ? 256 : r.d == 32 ? 768 : 512;  // what the card holds at once
-    r.grid = (a.nq / qt + (int64_t)std::min(a.tables, a.nq)) * a.heads + r.runs + 16;
+    r.grid = (a.nq / (qt >> r.log_share) + (int64_t)std::min(a.tables, a.nq)) * (a.heads >> r.log_share) + r.runs + 32;
     const int64_t blocks = a.nkv / KB + (int64_t)std::min(a.tables, a.nkv);
     r.blocks = (int)blocks;
     const size_t halves = (size_t)blocks * a.kv_heads, places = 2 * (size_t)r.runs * qt;
@@ -793,7 +823,7 @@ void launch(hipStream_t s, const Packed &p, const Plan &r) {
 
 size_t packed_work_bytes(const PackedShape &a) {
     const Plan r = plan(a);
-    if (r.grid > 0x7FFFFFFF || r.blocks > 0x7FFFFF) throw ArgError{"attend_packed: more rows than a call takes: fewer tables a call"};
+    if (r.grid > 0x7FFFFFFF || r.blocks > 0x7FFFFF || a.nq > 0x7FFFFF00) throw ArgError{"attend_packed: more rows than a call takes: fewer tables a call"};
     return r.bytes();
 }
 
@@ -817,6 +847,7 @@ void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const
     p.block_sums = reinterpret_cast<uint32_t *>(carve(r.tables));
     p.waves = r.waves;
     p.runs = r.runs;
+    p.log_share = r.log_share;
     p.direct = r.d <= 64 && r.waves == 4 && kv_ld < (size_t)1 << 22;  // a block's rows within 2^30 bytes
     p.part_o = reinterpret_cast<float *>(carve(r.part_o));
     p.part_ml = reinterpret_cast<float2 *>(carve(r.part_ml));

@@ -64,6 +64,18 @@ def test_long_tables(gpu, hd, causal):
     check(got, *wanted(q, k, v, counts, counts, causal), f"heads of {hd}, causal {causal}")
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(6, 1, 32), (12, 2, 64), (16, 1, 64), (32, 1, 16), (64, 1, 32), (24, 3, 128), (7, 1, 48)])
+def test_heads_that_share_keys(gpu, heads, kv_heads, hd, causal):
+    """Groups of every kind (odd, even, more than a wavefront's columns), tables short and long enough to be cut, more queries than
+    rows and fewer."""
+    rng = np.random.default_rng(heads)
+    q_counts, kv_counts = [900, 3, 0, 41, 130, 17], [900, 3, 5, 700, 60, 17]
+    q, k, v = inputs(rng, sum(q_counts), sum(kv_counts), heads, kv_heads, hd)
+    got = gpu.attend_packed(flat(q), flat(k), flat(v), offsets_of(q_counts), heads, kv_heads, causal, offsets_of(kv_counts)).reshape(q.shape)
+    check(got, *wanted(q, k, v, q_counts, kv_counts, causal), f"{heads}/{kv_heads} heads of {hd}, causal {causal}")
+
+
 @pytest.mark.parametrize("hd,rows,causal", [(32, 4300, False), (64, 4300, False), (128, 2300, False), (128, 2300, True)])
 def test_one_long_table(gpu, hd, rows, causal):
     """Long enough alone for the larger tiles of queries, not long enough with another."""
