@@ -3,6 +3,7 @@ HBM and time work on the library's own stream: `DeviceBuffer` (hipMalloc / hipMe
 (hipEventRecord on a given stream, hipEventElapsedTime)."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import ctypes.util
 
@@ -31,19 +32,45 @@ def rt():
             "hipMemset": [vp, ctypes.c_int, sz], "hipEventCreate": [ctypes.POINTER(vp)], "hipEventDestroy": [vp],
             "hipEventRecord": [vp, vp], "hipEventSynchronize": [vp],
             "hipEventElapsedTime": [ctypes.POINTER(ctypes.c_float), vp, vp], "hipDeviceSynchronize": [],
-            "hipStreamSynchronize": [vp],
+            "hipStreamSynchronize": [vp], "hipGetDevice": [ctypes.POINTER(ctypes.c_int)], "hipSetDevice": [ctypes.c_int],
         }.items():
             f = getattr(_rt, fn)
             f.restype, f.argtypes = ctypes.c_int, args
     return _rt
 
 
+OUT_OF_MEMORY = 2  # hipErrorOutOfMemory
+
+
+class HipError(RuntimeError):
+    def __init__(self, what: str, status: int):
+        super().__init__(f"graphics card: {what} failed with HIP status {status}")
+        self.status = status
+
+
 def _ok(rc: int, what: str) -> None:
     if rc != 0:
-        raise RuntimeError(f"graphics card: {what} failed with HIP status {rc}")
+        raise HipError(what, rc)
+
+
+@contextlib.contextmanager
+def on_card(ordinal):
+    """The calling thread's current card is `ordinal` (None: the one that it is) meanwhile."""
+    if ordinal is None:
+        yield
+        return
+    before = ctypes.c_int()
+    _ok(rt().hipGetDevice(ctypes.byref(before)), "hipGetDevice")
+    _ok(rt().hipSetDevice(int(ordinal)), "hipSetDevice")
+    try:
+        yield
+    finally:
+        _ok(rt().hipSetDevice(before.value), "hipSetDevice")
 
 
 class DeviceBuffer:
+    """Memory on the calling thread's current card (`on_card`)."""
+
     def __init__(self, nbytes: int):
         self.nbytes = int(nbytes)
         p = ctypes.c_void_p()

@@ -65,6 +65,7 @@ class Gpu:
         if rc != abi.OK:
             raise CardError(f"graphics card: none found at ordinal {ordinal} (status {rc})")
         self._h = h
+        self.ordinal = int(ordinal)
         buf = ctypes.create_string_buffer(256)
         self._l.tah_device_name(self._h, buf, 256)
         self.name = buf.value.decode()

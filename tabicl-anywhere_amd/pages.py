@@ -22,7 +22,12 @@ class PagePool:
         self.gpu, self.layers, self.heads, self.hd, self.pages = gpu, int(layers), int(heads), int(hd), int(pages)
         self.kv_format, self.page_rows = int(kv_format), int(page_rows)
         self.layer_bytes = pages * abi.page_bytes(kv_format, heads, hd, page_rows)
-        self._memory = devmem.DeviceBuffer(self.layers * self.layer_bytes)
+        # on the handle's card, whichever the calling thread's current one is
+        try:
+            with devmem.on_card(getattr(gpu, "ordinal", None)):
+                self._memory = devmem.DeviceBuffer(self.layers * self.layer_bytes)
+        except devmem.HipError as e:
+            raise (hip.BudgetError if e.status == devmem.OUT_OF_MEMORY else hip.CardError)(str(e)) from e
         self._free = list(range(self.pages - 1, -1, -1))
         self._held: dict = {}  # (prefix, node): [rows, pages]
         self._lock = threading.RLock()
