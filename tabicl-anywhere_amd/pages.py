@@ -4,7 +4,8 @@
 problem is held by `(prefix, node)` as `hip.CardAttend` holds models, from exact keys and values or from a bundle's stored
 records; `attend` has the form of `predict::AttendCached::attend` (`src/predict.rs:63-79`) and returns `None` for a problem the
 pool does not hold; `attend_many` answers rows of many problems in one call a layer. A problem's layers lie in the same pages of
-the layers' pools, and what a problem gives up the next one takes: no memory is asked for after the pool is made.
+the layers' pools, and what a problem gives up the next one takes: the pool never grows. Calls take arrays in host memory, and
+borrow room for them on the card from the handle's working memory, whose budget they can exceed (`hip.BudgetError`).
 """
 from __future__ import annotations
 
@@ -58,20 +59,21 @@ class PagePool:
     # ---- what is held ---------------------------------------------------------------------------------------------
     def hold(self, prefix: str, node: int, layers) -> None:
         """Hold a problem: `layers` its layers' keys and values, (k, v) of [rows][heads * hd] each. In place of what was held by
-        that name; if there are too few pages (`hip.BudgetError`) nothing changes."""
+        that name; if there are too few pages (`hip.BudgetError`) nothing changes. The rows are written into free pages, and
+        what was held is given up when they are there; only where that leaves too few pages are its own taken, and it is gone
+        if the writing then fails."""
         with self._lock:
             layers, rows = self._checked(layers)
             old = self._held.get((prefix, node), [0, []])
             need = -(-rows // self.page_rows)
             if need > len(self._free) + len(old[1]):
                 raise hip.BudgetError(f"graphics card: {need} pages wanted, {len(self._free) + len(old[1])} free")
-            self.drop(prefix, node)
-            self._held[(prefix, node)] = [0, []]
-            try:
-                self._append(prefix, node, layers, rows)
-            except BaseException:
+            if need > len(self._free):
                 self.drop(prefix, node)
-                raise
+            new = [0, []]
+            self._append(new, layers, rows)
+            self.drop(prefix, node)
+            self._held[(prefix, node)] = new
 
     def hold_records(self, prefix: str, node: int, kv_format: int, rows: int, chunk: int, records) -> None:
         """`hold` from a bundle's stored records (`n{j}_kv{l}`), what they stand for."""
@@ -88,7 +90,8 @@ class PagePool:
         with self._lock:
             if (prefix, node) not in self._held:
                 raise LookupError(f"no problem {prefix!r}, {node} in the pool")
-            self._append(prefix, node, *self._checked(layers))
+            held = self._held[(prefix, node)]
+            self._append(held, *self._checked(layers, held[0]))
 
     def drop(self, prefix: str, node: int) -> bool:
         """Give a problem's pages back; whether it was held."""
@@ -98,20 +101,22 @@ class PagePool:
                 self._free.extend(reversed(rows_pages[1]))
             return rows_pages is not None
 
-    def _checked(self, layers):
+    def _checked(self, layers, have: int = 0):
         layers = [tuple(hip._rows_of(a, self.d, "PagePool") for a in kv) for kv in layers]
         if len(layers) != self.layers or any(len(kv) != 2 or kv[0].shape != layers[0][0].shape or kv[1].shape != layers[0][0].shape
                                              for kv in layers):
             raise ValueError(f"PagePool: expected keys and values of {self.layers} layers, all of as many rows")
-        return layers, layers[0][0].shape[0]
+        rows = layers[0][0].shape[0]
+        if have + rows > 2**31 - 1024:
+            raise ValueError("PagePool: at most 2^31 - 1024 rows")
+        return layers, rows
 
-    def _append(self, prefix: str, node: int, layers, rows: int) -> None:
-        have, pages = self._held[(prefix, node)]
+    def _append(self, held: list, layers, rows: int) -> None:
+        """Rows behind those of `held` ([rows, pages]), which stays as it was if that fails."""
+        have, pages = held
         need = -(-(have + rows) // self.page_rows) - len(pages)
         if need > len(self._free):
             raise hip.BudgetError(f"graphics card: {need} pages wanted, {len(self._free)} free")
-        if have + rows > 2**31 - 1024:
-            raise ValueError("PagePool: at most 2^31 - 1024 rows")
         if rows == 0:
             return
         taken = [self._free.pop() for _ in range(need)]
@@ -123,7 +128,7 @@ class PagePool:
             self._free.extend(reversed(taken))  # the rows it has are as they were
             raise
         pages.extend(taken)
-        self._held[(prefix, node)][0] = have + rows
+        held[0] = have + rows
 
     def _pages(self, layer: int, table: np.ndarray) -> abi.Pages:
         return abi.Pages(pool=self._memory.ptr + layer * self.layer_bytes, kv_format=self.kv_format, kv_heads=self.heads, hd=self.hd,

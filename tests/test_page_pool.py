@@ -245,3 +245,29 @@ def test_two_threads_share_a_pool():
     assert np.array_equal(gk, k) and np.array_equal(gv, v)
     pool.free()
     gpu.close()
+
+
+@pytest.mark.parametrize("error", [hip.CardError, hip.BudgetError])
+def test_a_replacement_that_fails_leaves_what_was_held(pool, error):
+    """Where enough pages are free for the new rows beside the old ones; else the old ones' pages are taken first."""
+    a = kv(40, 1)
+    pool.hold("a", 0, a)
+    write, layer = pool.gpu.pages_write, []
+
+    def fails_at_the_second_layer(p, *args):
+        layer.append(p.pool)
+        if p.pool != pool._memory.ptr:
+            raise error("graphics card: gone")
+        write(p, *args)
+
+    pool.gpu.pages_write = fails_at_the_second_layer
+    with pytest.raises(error):
+        pool.hold("a", 0, kv(112, 2))  # seven pages, as many as are free
+    assert len(layer) == 2 and pool.rows("a", 0) == 40 and pool.free_pages == 7
+    same(pool, ("a", 0), a)
+    with pytest.raises(error):
+        pool.hold("a", 0, kv(113, 2))
+    assert pool.rows("a", 0) == 0 and pool.free_pages == 10
+    pool.gpu.pages_write = write
+    pool.hold("a", 0, kv(160, 3))
+    same(pool, ("a", 0), kv(160, 3))
