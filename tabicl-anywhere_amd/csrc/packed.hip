@@ -826,7 +826,8 @@ void launch(hipStream_t s, const Packed &p, const Plan &r) {
 
 size_t packed_work_bytes(const PackedShape &a) {
     const Plan r = plan(a);
-    if (r.grid > 0x7FFFFFFF || r.blocks > 0x7FFFFF || a.nq > 0x7FFFFF00)
+    // a launch takes fewer than 2^32 threads; the tiles' has 256 a block of rows
+    if ((uint64_t)r.grid * (64 * r.waves) >> 32 || r.blocks > 0x7FFFFF || a.nq > 0x7FFFFF00)
         throw ArgError{"attend_packed: more rows than a call takes: fewer tables a call"};
     return r.bytes();
 }
