@@ -9,6 +9,7 @@ namespace {
 
 constexpr int TILE = 64;      // rows a workgroup
 constexpr int IN_LDS = 256;   // tables whose offsets a workgroup looks through in LDS
+constexpr int MOST_TILES = (1 << 24) - 1;  // workgroups of 256 threads in a dimension of a launch
 
 template <int FMT>
 struct Number;
@@ -173,6 +174,10 @@ struct Words {
     static constexpr int N = page_width(FMT), ROW = TILE * N / 4 + (N == 4 ? 4 : N);
 };
 
+// the first row of a workgroup: grid (rows / 64 of a part, heads, keys and values of each part), parts where rows are too many for
+// one dimension
+__device__ __forceinline__ int first_row() { return (int)(((blockIdx.z >> 1) * gridDim.x + blockIdx.x) * TILE); }
+
 // grid (rows / 64, heads, keys and values); 256 threads: four rows and four of each 64 coordinates a lane, sixteen lanes a row.
 // Bound by bytes: 40 tables of up to 1,500 rows, 4 heads of 128 to i16 (180 MB) take 44 us, at the rate of a large copy 35;
 // without its stores the kernel takes 25 us (the reads at 4.7 TB/s), without its arithmetic 2 to 4 less. Values are turned in LDS, so
@@ -187,8 +192,9 @@ __global__ __launch_bounds__(256) void k_pages_write(PageSet p, const int32_t *_
     __shared__ uint32_t tile[64 * C][ROW];
     __shared__ Places pl;
     const int tid = threadIdx.x, l16 = tid & 15, quad = tid >> 4, h = blockIdx.y;
-    const bool values = blockIdx.z == 1;
-    const int r0 = blockIdx.x * TILE, hd = p.hd, P = p.rows;
+    const bool values = blockIdx.z & 1;
+    const int r0 = first_row(), hd = p.hd, P = p.rows;
+    if (r0 >= rows) return;
     const float *src = (values ? v : k) + (size_t)h * hd;
     floatx4 x[4][C];
 #pragma unroll
@@ -280,8 +286,9 @@ __global__ __launch_bounds__(256) void k_pages_read(PageSet p, const int32_t *__
     __shared__ uint32_t tile[64 * C][ROW];
     __shared__ Places pl;
     const int tid = threadIdx.x, l16 = tid & 15, quad = tid >> 4, h = blockIdx.y;
-    const bool values = blockIdx.z == 1;
-    const int r0 = blockIdx.x * TILE, hd = p.hd, P = p.rows;
+    const bool values = blockIdx.z & 1;
+    const int r0 = first_row(), hd = p.hd, P = p.rows;
+    if (r0 >= rows) return;
     find_places(p, starts, offsets, r0, rows, pl);
     const uint8_t *head = p.pool + (size_t)h * p.head_bytes;
     if (values) {
@@ -354,7 +361,9 @@ __global__ __launch_bounds__(256) void k_pages_read(PageSet p, const int32_t *__
 template <int FMT, int C>
 void launch_rows(hipStream_t s, const PageSet &p, const int32_t *starts, const int32_t *offsets, float *k, float *v, int rows,
                  size_t row_ld, bool write) {
-    const dim3 grid((rows + TILE - 1) / TILE, p.heads, 2);
+    // fewer than 2^32 threads in a dimension
+    const int tiles = (rows + TILE - 1) / TILE, parts = tiles / MOST_TILES + 1;
+    const dim3 grid((tiles + parts - 1) / parts, p.heads, 2 * parts);
     if (write)
         hipLaunchKernelGGL((k_pages_write<FMT, C>), grid, dim3(256), 0, s, p, starts, offsets, k, v, rows, row_ld);
     else

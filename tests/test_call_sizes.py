@@ -35,6 +35,36 @@ class Far:
         return a
 
 
+def test_rows_past_two_to_the_thirty(gpu):
+    """2^30 + 100 rows of one head of 16 (64 GiB; keys and values the same), of which the last 40 and some before fall on pages."""
+    rows, hd, page = 2**30 + 100, 16, 16
+    far = Far(rows * hd * 4)
+    try:
+        rng = np.random.default_rng(1)
+        first, last = rng.standard_normal((page, hd)).astype(np.float32), rng.standard_normal((40, hd)).astype(np.float32)
+        far.put(0, first)
+        far.put((rows - 40) * hd * 4, last)
+        pool = dm.DeviceBuffer(4 * abi.page_bytes(abi.KV_F32, 1, hd, page))
+        # table 0: the first 16 rows; table 1: all others, of which the last 40 are its rows 0 .. 39; rows before them are on no page
+        table = dm.DeviceBuffer.of(np.array([[2, -1, -1], [1, 3, 0]], np.int32))
+        starts, offsets = dm.DeviceBuffer.of(np.array([0, -(rows - page - 40)], np.int32)), dm.DeviceBuffer.of(np.array([0, page, rows], np.int32))
+        d = abi.Pages(pool=pool.ptr, table=table.ptr, kv_format=abi.KV_F32, kv_heads=1, hd=hd, page_rows=page, pages=4, tables=2, ld=3)
+        print("write", flush=True)
+        gpu.pages_write_dev(d, starts.ptr, offsets.ptr, far.b.ptr, far.b.ptr, rows)
+        gpu.sync()
+        # back into the same place: all other rows zeros, which they were
+        far.put(0, np.full((page, hd), 9.0, np.float32))
+        far.put((rows - 45) * hd * 4, np.full((45, hd), 9.0, np.float32))
+        print("read", flush=True)
+        gpu.pages_read_dev(d, starts.ptr, offsets.ptr, far.b.ptr, far.b.ptr, rows)
+        gpu.sync()
+        assert np.array_equal(far.take(0, (page, hd)), first)
+        assert np.array_equal(far.take((rows - 40) * hd * 4, (40, hd)), last)
+        assert not np.any(far.take((rows - 45) * hd * 4, (5, hd)))
+    finally:
+        far.b.free()
+
+
 def test_more_tiles_than_a_launch_takes_are_refused(gpu):
     """2^22 tables of a query each, 8 heads: 2^25 workgroups. Nothing is read: the arrays are as long as the sizes say all the same."""
     tables, hd = 2**22, 16
