@@ -12,6 +12,7 @@ namespace tah {
 namespace {
 
 constexpr int WAVES = 4;
+constexpr int MOST_WGS = (1 << 24) - 1;  // of 256 threads in a dimension of a launch, which takes fewer than 2^32 threads
 // What beginning and ending a unit costs, in blocks: a unit counts as so many more than it has, so that wavefronts with several
 // units get fewer of them. 24 tables of up to 6,001 rows 69, 62.5 and 62.4 us for 1, 2 and 4, 64 of up to 20,000 139.5, 140.8, 141.8.
 constexpr int BEGIN = 2;
@@ -608,7 +609,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
     }
 }
 
-// grid (queries x heads, over 4 / PER); 256 threads: the states that runs of blocks left of a query and head, together: PER
+// grid (queries x heads, over 4 / PER; in rows of MOST_WGS where there are more); 256 threads: the states that runs of blocks left of a query and head, together: PER
 // wavefronts for each query and head, every PER-th state each. Four where there are few (a state after the other takes longest:
 // the call of one query of 8 heads over 100,000 rows 33 us, with one 42; 7 tables of up to 9,000 23.6 and 27.5), one where there
 // are many (their number does: 24 tables, up to 9 queries each, of 16 heads 62.4 us, with four 65.6). The launch is most of it.
@@ -618,8 +619,9 @@ __global__ __launch_bounds__(256) void k_pages_join(int tables, int hd, const in
     constexpr int COLS = 16 * CT, AHEAD = 8;
     __shared__ float wm[4], wl[4], wo[4][128];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int item = PER == 4 ? blockIdx.x : blockIdx.x * 4 + wave, part = PER == 4 ? wave : 0;
-    if (item >= items) return;
+    const uint32_t nth = PER == 4 ? blockIdx.x : (blockIdx.y * gridDim.x + blockIdx.x) * 4 + wave;
+    if (nth >= (uint32_t)items) return;
+    const int item = (int)nth, part = PER == 4 ? wave : 0;
     const uint4 unit = parts.units[item];
     const uint32_t per = parts.plan[0], total = parts.plan[1], u0 = unit.x, u1 = unit.y, col = unit.w;
     // of no table (what its place holds is another call's); there already
@@ -733,10 +735,13 @@ void launch(hipStream_t s, const PageSet &p, const int32_t *lengths, const float
                        offsets, nq, heads, causal ? 1 : 0, q_ld, out, parts, sh.blocks);
     TAH_LAUNCHED();
     const int items = nq * heads;
-    if (items <= 1024)
+    if (items <= 1024) {
         hipLaunchKernelGGL((k_pages_join<CT, 4>), dim3(items), dim3(256), 0, s, p.tables, p.hd, offsets, items, heads, out, parts);
-    else
-        hipLaunchKernelGGL((k_pages_join<CT, 1>), dim3((items + 3) / 4), dim3(256), 0, s, p.tables, p.hd, offsets, items, heads, out, parts);
+    } else {
+        const int wgs = (items + 3) / 4, rows = (wgs + MOST_WGS - 1) / MOST_WGS;
+        hipLaunchKernelGGL((k_pages_join<CT, 1>), dim3((wgs + rows - 1) / rows, rows), dim3(256), 0, s, p.tables, p.hd, offsets, items,
+                           heads, out, parts);
+    }
     TAH_LAUNCHED();
 }
 

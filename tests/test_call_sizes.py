@@ -65,6 +65,29 @@ def test_rows_past_two_to_the_thirty(gpu):
         far.b.free()
 
 
+def test_queries_past_two_to_the_twenty_six(gpu):
+    """2^26 + 5 queries of a head of 16 over a table of two rows, a third of which the join puts together where their units are cut."""
+    nq, hd, page = 2**26 + 5, 16, 16
+    q, out = Far(nq * hd * 4), Far(nq * hd * 4)
+    try:
+        pool = dm.DeviceBuffer.of(np.zeros(abi.page_bytes(abi.KV_F32, 1, hd, page), np.uint8))
+        kv = np.arange(2 * hd, dtype=np.float32).reshape(2, hd)
+        d = abi.Pages(pool=pool.ptr, kv_format=abi.KV_F32, kv_heads=1, hd=hd, page_rows=page, pages=1, tables=1, ld=1)
+        gpu.pages_write(d, [[0]], [0], [0, 2], np.zeros((2, hd), np.float32), kv)
+        table, lengths = dm.DeviceBuffer.of(np.zeros((1, 1), np.int32)), dm.DeviceBuffer.of(np.array([2], np.int32))
+        offsets = dm.DeviceBuffer.of(np.array([0, nq], np.int32))
+        d.table = table.ptr
+        gpu.pages_attend_dev(d, lengths.ptr, q.b.ptr, offsets.ptr, nq, 1, out.b.ptr)
+        gpu.sync()
+        want = kv.mean(0)  # scores of 0: both rows alike
+        for a in (0, 2**24, 2**26 - 2000, nq - 2000):
+            got = out.take(a * hd * 4, (2000, hd))
+            assert np.all(np.abs(got - want) <= 2.0**-20 * 32), a
+    finally:
+        q.b.free()
+        out.b.free()
+
+
 def test_more_tiles_than_a_launch_takes_are_refused(gpu):
     """2^22 tables of a query each, 8 heads: 2^25 workgroups. Nothing is read: the arrays are as long as the sizes say all the same."""
     tables, hd = 2**22, 16
