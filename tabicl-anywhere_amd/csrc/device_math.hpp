@@ -232,6 +232,10 @@ __device__ __forceinline__ uint32_t finite_bits(uint32_t w) {
     return u < 0x7f800000u ? u : 0u;
 }
 
+// the power of two that brings numbers of this largest magnitude below 2^14 (2^126 at most). Zeros put no bound on it: taken as
+// if their largest were 1, a block of them would have set the units that tiny numbers of other blocks are then held in.
+__device__ __forceinline__ int shift_below(float max_abs) { return max_abs > 0.0f ? min(shift_for_max(max_abs), 126) : 126; }
+
 // the sum over a lane and the lanes before it: within rows of sixteen lanes, then the rows' last lanes to the rows after
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t dpp_or_zero(uint32_t v) {

@@ -244,7 +244,7 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
         some[tid >> 6] = any;
     }
     __syncthreads();
-    const int shift = min(shift_for_max(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))), 126);
+    const int shift = shift_below(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
     const bool odd = values && (some[0] | some[1] | some[2] | some[3]);
     const float f = pow2(shift);
     const size_t at = (size_t)blockIdx.x * p.kv_heads + h;
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
             }
         }
         most = half_max(most);
-        const int eq = min(shift_for_max(most), 126);
+        const int eq = shift_below(most);
         const float f = pow2(eq);
 #pragma unroll
         for (int dc = 0; dc < DC; dc++) split8(qv[dc], f, qh[dc], ql[dc]);
@@ -644,8 +644,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
                 for (int w = 1; w < WAVES; w++)
 #pragma unroll
                     for (int e = 0; e < 3; e++) m[e] = fmaxf(m[e], most_here[w][e]);
-                const int ek = __builtin_amdgcn_readfirstlane(min(shift_for_max(m[0]), 126));
-                const int ev = __builtin_amdgcn_readfirstlane(min(shift_for_max(m[1]), 126));
+                const int ek = __builtin_amdgcn_readfirstlane(shift_below(m[0]));
+                const int ev = __builtin_amdgcn_readfirstlane(shift_below(m[1]));
                 const bool odd = __builtin_amdgcn_readfirstlane(m[2] != 0.0f);
                 const float fk = pow2(ek), fv = pow2(ev);
 #pragma unroll

@@ -252,7 +252,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                 }
             }
             most = half_max(row_max(most));
-            const int eq = min(shift_for_max(most), 126);
+            const int eq = shift_below(most);
             const float f = pow2(eq);
 #pragma unroll
             for (int c = 0; c < C; c++)
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                     for (int c = 0; c < C; c++)
 #pragma unroll
                         for (int i = 0; i < Raw<FMT, 2>::WORDS; i++) most = max(most, finite_bits(kr[sp][c].w[i]));
-                ek = min(shift_for_max(wave_max(__uint_as_float(most))), 126);
+                ek = shift_below(wave_max(__uint_as_float(most)));
             }
             const float fk = INTS ? 1.0f : pow2(ek), unk = INTS ? 1.0f : pow2(-ek);
             floatx4 sc[2 * KS][CT];  // set sp = 2 s + p
@@ -434,7 +434,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                         odd = max(odd, vr[m].w[i] & 0x7fffffffu);
                         most = max(most, finite_bits(vr[m].w[i]));
                     }
-                const int e = min(shift_for_max(wave_max(__uint_as_float(most))), 126);
+                const int e = shift_below(wave_max(__uint_as_float(most)));
                 if (e < ev) {
                     const float f = ev < 1000 ? pow2(e - ev) : 0.0f;
 #pragma unroll

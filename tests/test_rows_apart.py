@@ -1,0 +1,73 @@
+"""Attention of packed tables and over pages where rows of one table are of very different sizes: blocks of zeros and of missing
+rows beside tiny values, against 64 bits within the sum of the worst roundings of what a query sees (`pages_plain.attention`)."""
+import numpy as np
+import pytest
+
+import pages_plain as P
+from conftest import pkg
+from test_packed import flat, inputs, wanted
+from test_pages import FORMATS, check, described, dev, gpu, offsets_of, values  # noqa: F401 (fixtures)
+
+abi = pkg("abi")
+pytestmark = pytest.mark.gpu
+
+# counts of rows: all read by few tiles of queries; made into tiles first (more readers, or heads over 64 wide); long, cut into runs
+SHAPES = [([130, 200], 2, 2, 32), ([130, 200], 2, 2, 64), ([700, 90], 2, 1, 64), ([130, 200], 2, 1, 128), ([200, 130], 8, 1, 64),
+          ([1500], 1, 1, 64), ([1500], 2, 2, 32)]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("tiny", [1e-8, 1e-12, 1e-25, 1e-36])
+@pytest.mark.parametrize("counts,heads,kv_heads,hd", SHAPES)
+def test_packed_blocks_of_zeros(gpu, counts, heads, kv_heads, hd, tiny, causal):
+    """64 rows whose values are all zeros, before or behind rows of tiny ones."""
+    for zeros in (0, 1, 3):
+        rng = np.random.default_rng(hd + zeros)
+        n = sum(counts)
+        q, k, v = inputs(rng, n, n, heads, kv_heads, hd)
+        v *= np.float32(tiny)
+        at = 0
+        for c in counts:
+            for b in range(zeros % 2, -(-c // 64), 2) if zeros < 3 else [0]:
+                v[at + 64 * b:min(at + 64 * b + 64, at + c)] = 0.0
+            at += c
+        got = gpu.attend_packed(flat(q), flat(k), flat(v), offsets_of(counts), heads, kv_heads, causal).reshape(q.shape)
+        got = got.astype(np.float64) / tiny
+        out, off = (a / tiny for a in wanted(q, k, v, counts, counts, causal))
+        at = 0
+        for c in counts:
+            check(got[at:at + c], out[at:at + c], off[at:at + c], f"zeros {zeros}, {c} rows, heads of {hd}, {tiny}, causal {causal}")
+            at += c
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tiny", [1e-8, 1e-12, 1e-25])
+@pytest.mark.parametrize("hd,group", [(64, 1), (64, 20), (128, 2)])
+def test_pages_of_zeros_and_missing_pages(gpu, dev, fmt, tiny, hd, group):
+    """Tables with 64 rows of zeros or on no page, before or behind rows of tiny values; each asked 250 times at once, so that
+    a wavefront has several of their blocks."""
+    rng = np.random.default_rng(hd + group)
+    rows, T, length, copies = 32, 4, 200, 250
+    pool = P.Pool(fmt, 1, hd, rows, T * 7, fill=0)
+    table = rng.permutation(T * 7).astype(np.int32).reshape(T, 7)
+    k, v = values(rng, T * length, 1, hd).reshape(T, length, 1, hd), (values(rng, T * length, 1, hd) * np.float32(tiny)).reshape(T, length, 1, hd)
+    v[0, :64], v[1, 64:128], v[1, 192:] = 0.0, 0.0, 0.0
+    there = np.ones((T, length), bool)
+    there[2, :64] = there[3, 64:128] = False
+    for t in range(T):
+        for i in range(length):
+            pool.write(table[t, i // rows], i % rows, k[t, i], v[t, i])
+    told = table.copy()
+    told[2, :2] = told[3, 2:4] = -1
+    told, n = np.repeat(told, copies, 0), T * copies
+    q = (rng.standard_normal((n, group, hd)) * 0.4).astype(np.float32)
+    card, tb, ln, of = dev.of(pool.bytes), dev.of(told), dev.of(np.full(n, length, np.int32)), dev.of(offsets_of([1] * n))
+    qd, od = dev.of(q), dev.of(np.zeros(q.shape, np.float32))
+    gpu.pages_attend_dev(described(pool, n, 7, card.ptr, tb.ptr), ln.ptr, qd.ptr, of.ptr, n, group, od.ptr)
+    gpu.sync()
+    got = od.download(q.shape).astype(np.float64) / tiny
+    for t in range(T):
+        kt, vt = pool.rows_of(table[t], length)
+        asked = slice(copies * t, copies * (t + 1))
+        out, off = P.attention(q[asked], kt[there[t]], vt[there[t]], [int(there[t].sum())] * copies)
+        check(got[asked], out / tiny, off / tiny, f"format {fmt}, table {t}, {tiny}")
