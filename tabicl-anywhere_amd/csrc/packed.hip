@@ -753,26 +753,31 @@ __global__ __launch_bounds__(256) void k_packed_join(Packed p) {
 #pragma unroll
         for (int j = 0; j < AHEAD; j++)
             if (ml[j].y > 0.0f) top = fmaxf(top, ml[j].x);
-        const float old = M == -INFINITY ? 1.0f : exp2_hw(M - top);  // nothing yet, or NaN
-        L *= old;
-#pragma unroll
-        for (int c = 0; c < C; c++) o[c] *= old;
+        // shares of the sum so far, so that no value is multiplied by more than 1
+        const float old = M == -INFINITY ? L : L * exp2_hw(M - top);  // nothing yet, or NaN
+        float f[AHEAD];
+        L = old;
         M = top;
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) {
-            if (ml[j].y == 0.0f) continue;
-            const float f = ml[j].y > 0.0f ? ml[j].y * exp2_hw(ml[j].x - M) : ml[j].y;
-            L += f;
+            f[j] = ml[j].y > 0.0f ? ml[j].y * exp2_hw(ml[j].x - M) : ml[j].y;
+            L += f[j];
+        }
+        const float inv = L > 0.0f ? 1.0f / L : L;
 #pragma unroll
-            for (int c = 0; c < C; c++) o[c] += f * x[j][c];
+        for (int c = 0; c < C; c++) o[c] *= old * inv;
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            if (ml[j].y == 0.0f) continue;
+#pragma unroll
+            for (int c = 0; c < C; c++) o[c] += f[j] * inv * x[j][c];
         }
     }
-    const float inv = L > 0.0f ? 1.0f / L : L;
 #pragma unroll
     for (int c = 0; c < C; c++)
         if (64 * c + dim < p.hd)
             *reinterpret_cast<floatx4u *>(p.out + ((size_t)(unit.row + (r >> p.log_share)) * p.heads + unit.head +
-                                                   (r & ((1 << p.log_share) - 1))) * p.hd + 64 * c + dim) = o[c] * inv;
+                                                   (r & ((1 << p.log_share) - 1))) * p.hd + 64 * c + dim) = o[c];
 }
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }

@@ -596,8 +596,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                 float o = 0.0f;
 #pragma unroll
                 for (int w = 0; w < WAVES; w++)
-                    if (msum[w][col] != 0.0f) o += f[w] * macc[w][dim][c16];
-                o *= Li;
+                    if (msum[w][col] != 0.0f) o += f[w] * Li * macc[w][dim][c16];
                 if (!done)
                     parts.o[(own * COLS + col) * hd + dim] = o;
                 else if (i < tw.n)
@@ -657,18 +656,24 @@ __global__ __launch_bounds__(256) void k_pages_join(int tables, int hd, const in
 #pragma unroll
         for (int i = 0; i < AHEAD; i++)
             if (ml[i].y > 0.0f) top = fmaxf(top, ml[i].x);
-        const float old = M == -INFINITY ? 1.0f : exp2_hw(M - top);  // nothing yet, or NaN
-        L *= old;
-        o0 *= old;
-        o1 *= old;
+        // shares of the sum so far, so that no value is multiplied by more than 1
+        const float old = M == -INFINITY ? L : L * exp2_hw(M - top);  // nothing yet, or NaN
+        float f[AHEAD];
+        L = old;
         M = top;
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
+            f[i] = ml[i].y > 0.0f ? ml[i].y * exp2_hw(ml[i].x - M) : ml[i].y;
+            L += f[i];
+        }
+        const float inv = L > 0.0f ? 1.0f / L : L;
+        o0 *= old * inv;
+        o1 *= old * inv;
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
             if (ml[i].y == 0.0f) continue;
-            const float f = ml[i].y > 0.0f ? ml[i].y * exp2_hw(ml[i].x - M) : ml[i].y;
-            L += f;
-            o0 += f * x0[i];
-            o1 += f * x1[i];
+            o0 += f[i] * inv * x0[i];
+            o1 += f[i] * inv * x1[i];
         }
     }
     if constexpr (PER == 4) {
@@ -682,19 +687,23 @@ __global__ __launch_bounds__(256) void k_pages_join(int tables, int hd, const in
         if (wave > 0) return;
         const float top = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
         L = o0 = o1 = 0.0f;
+        float f[4];
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            f[w] = wm[w] == -INFINITY ? wl[w] : wl[w] * exp2_hw(wm[w] - top);
+            L += f[w];
+        }
+        const float inv = L > 0.0f ? 1.0f / L : L;
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             if (wl[w] == 0.0f) continue;
-            const float f = wm[w] == -INFINITY ? 1.0f : exp2_hw(wm[w] - top);
-            L += wl[w] * f;
-            o0 += wo[w][lane] * f;
-            o1 += wo[w][64 + lane] * f;
+            o0 += f[w] * inv * wo[w][lane];
+            o1 += f[w] * inv * wo[w][64 + lane];
         }
     }
-    const float inv = L > 0.0f ? 1.0f / L : L;
     float *dst = out + (size_t)item * hd;
-    if (lane < hd) dst[lane] = o0 * inv;
-    if (64 + lane < hd) dst[64 + lane] = o1 * inv;
+    if (lane < hd) dst[lane] = o0;
+    if (64 + lane < hd) dst[64 + lane] = o1;
 }
 
 // Keys of a block: 64, or 32 where a wavefront's registers do not hold more (C parts of 64 coordinates, CT sets of 16 columns).

@@ -71,3 +71,44 @@ def test_pages_of_zeros_and_missing_pages(gpu, dev, fmt, tiny, hd, group):
         asked = slice(copies * t, copies * (t + 1))
         out, off = P.attention(q[asked], kt[there[t]], vt[there[t]], [int(there[t].sum())] * copies)
         check(got[asked], out / tiny, off / tiny, f"format {fmt}, table {t}, {tiny}")
+
+
+LARGE = 1e37
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("counts,heads,kv_heads,hd", SHAPES + [([2300], 2, 1, 128), ([4300], 1, 1, 64)])
+def test_packed_values_near_the_largest_float(gpu, counts, heads, kv_heads, hd, causal):
+    """Outputs are means of values: finite where those are, also where several states are put together."""
+    rng = np.random.default_rng(hd)
+    n = sum(counts)
+    q, k, v = inputs(rng, n, n, heads, kv_heads, hd)
+    got = gpu.attend_packed(flat(q), flat(k), flat(v * np.float32(LARGE)), offsets_of(counts), heads, kv_heads, causal).reshape(q.shape)
+    check(got.astype(np.float64) / LARGE, *wanted(q, k, v, counts, counts, causal), f"{counts} rows, heads of {hd}, causal {causal}")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hd,lengths,counts,causal", [(64, [9000], [2], False), (64, [3000, 2500], [9, 8], True), (128, [5000], [3], True),
+                                                      (64, [300] * 40, [40] * 40, True)])
+def test_pages_values_near_the_largest_float(gpu, dev, fmt, hd, lengths, counts, causal):
+    """One query's parts joined by four wavefronts, many queries' by one, a workgroup's parts joined in it, and none."""
+    rng = np.random.default_rng(hd + len(lengths))
+    rows, ld = 64, -(-max(lengths) // 64)
+    table = np.arange(len(lengths) * ld, dtype=np.int32).reshape(len(lengths), ld)
+    pool = P.Pool(fmt, 1, hd, rows, table.size)
+    for t, n in enumerate(lengths):
+        for i in range(n):
+            pool.write(table[t, i // rows], i % rows, *(values(rng, 1, 1, hd)[0] * np.float32(f) for f in (1.0, LARGE)))
+    q = (rng.standard_normal((sum(counts), 2, hd)) * 0.4).astype(np.float32)
+    card = dev.of(pool.bytes)
+    got = gpu.pages_attend(described(pool, len(lengths), ld, card.ptr), table, lengths, flat(q), offsets_of(counts), 2, causal).reshape(q.shape)
+    at = 0
+    for t, n in enumerate(counts):
+        k, v = pool.rows_of(table[t], lengths[t])
+        out, off = P.attention(q[at:at + n], k, v / LARGE, P.limits_of(lengths[t], n, causal))
+        # Values without a mean: the outputs are their weights' chance, 1 / sqrt(rows) of a value, and so are the weights' errors'. A
+        # weight's: a score of 128 products of 0.5 by 0.4 (a sum of about 2) added in f32, 2^-24 sqrt(132 / 3) 2 = 8e-7, its products'
+        # halves 2^-22 0.2 sqrt(128) 1.7 = 9e-7, the exponent's argument below 16 2^-21 0.69 / sqrt(3) = 2e-7, exp2 1e-7: 1.3e-6
+        # together, of which a head's outputs have three times as much at most.
+        check(got[at:at + n].astype(np.float64) / LARGE, out, off, f"format {fmt}, table {t}", 3 * 1.3e-6)
+        at += n
