@@ -32,12 +32,14 @@ struct Packed {
     size_t q_ld, kv_ld;
     float *out;
     int log_share;  // a tile's columns are its queries' 2^log_share heads that share their keys
-    // working memory: the tiles, per tile the keys' and the values' power of two (twice it, and 1 if a value is not finite), which
-    // keys of each coordinate hold values that are not; the attention's plan, and per table its first block of rows, and for one head the
-    // tiles of queries of the tables before it and those tiles' blocks (tables + 1)
+    // working memory: the tiles, per tile the keys' and the values' power of two (four times it, 2 if each row has one of its own, 1
+    // if a value is not finite), the rows' own (64 of the keys, 64 of the values), which keys of each coordinate hold values that are
+    // not finite; the attention's plan, and per table its first block of rows, and for one head the tiles of queries of the tables
+    // before it and those tiles' blocks (tables + 1)
     int blocks;  // room for so many
     uint8_t *tiles;
     int *shifts;
+    int8_t *row_shifts;
     uint64_t *odd;
     PackedPlan *plan;
     uint32_t *first, *tile_sums, *block_sums;
@@ -204,15 +206,43 @@ __device__ void make_plan(const Packed &p) {
 template <int D>
 constexpr int HALF_BYTES = D * 256;
 
+// Where rows of a block lie further apart than this, each row takes a power of two of its own. One for all would cost a
+// row 2^-39 of the block's largest number, so less than 2^-26 of its own within this; and rows that a query does not see would
+// count, in order, for the rows before them. Layer norms leave rows within a few powers of two of each other.
+constexpr float APART = 0x1p-12f;
+__device__ __forceinline__ bool rows_apart(float least, float most) { return least < most * APART; }  // least: not of zeros
+
+// the largest of LANES lanes next to each other, in each
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
+    v = fmaxf(v, dpp<0xb1>(v));
+    v = fmaxf(v, dpp<0x4e>(v));
+    if constexpr (LANES >= 8) v = fmaxf(v, dpp<0x141>(v));
+    if constexpr (LANES >= 16) v = fmaxf(v, dpp<0x140>(v));
+    return v;
+}
+
+// the same of floats' bits, which NaN pass
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_most(uint32_t v) {
+    auto step = [](uint32_t a, int b) { return max(a, (uint32_t)b); };
+    v = step(v, __builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, false));
+    v = step(v, __builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, false));
+    if constexpr (LANES >= 8) v = step(v, __builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, false));
+    if constexpr (LANES >= 16) v = step(v, __builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, false));
+    return v;
+}
+
 // grid (blocks, key/value heads, keys and values); 256 threads: one half tile. Scaled by the power of two that brings its own
-// largest finite number below 2^14. A value that is not finite is a zero in the tile, and its bit is set in `odd`. Bound by bytes: 10,000
-// rows of 8 heads of 64, 41 MB read and 41 written, 15.6 us, 5.2 TB/s.
+// largest finite number below 2^14, or each row by one of its own (APART). A value that is not finite is a zero in the tile, and its
+// bit is set in `odd`. Bound by bytes: 10,000 rows of 8 heads of 64, 41 MB read and 41 written, 15.6 us, 5.2 TB/s.
 template <int D>
 __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     __shared__ float x[KB][D + 1];
-    __shared__ float most[4];
-    __shared__ int some[4];
-    const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.y;
+    constexpr int LANES = D / 4 < 16 ? D / 4 : 16, PARTS = D / 4 / LANES;  // of a row
+    __shared__ uint32_t rows_most[KB][PARTS];
+    __shared__ float scale_here[4][KB];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = blockIdx.y;
     const bool values = blockIdx.z == 1;
     if (blockIdx.x == 0 && h == 0 && !values && tid < 64) p.waves == 8 ? make_plan<256, BEGIN_OF<D>>(p) : make_plan<128, BEGIN_OF<D>>(p);
     uint32_t kb = 0;
@@ -222,33 +252,39 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     if (few_readers(p, rows_of(p.qo, t, p.nq, a))) return;
     const int n = min(rows_of(p.ko, t, p.nkv, a) - (int)kb * KB, KB);
     const float *src = (values ? p.v : p.k) + (size_t)(a + (int)kb * KB) * p.kv_ld + (size_t)h * p.hd;
-    uint32_t big = 0, raw = 0;
 #pragma unroll
     for (int i = 0; i < KB * D / 4 / 256; i++) {
         const int u = tid + 256 * i, r = u / (D / 4), dim = 4 * (u % (D / 4));
         const floatx4 w = r < n && dim < p.hd ? (floatx4) * reinterpret_cast<const floatx4u *>(src + (size_t)r * p.kv_ld + dim)
                                               : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t raw = 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const float f = w[j];
-            const uint32_t b = __float_as_uint(f);
-            big = max(big, finite_bits(b));
-            raw = max(raw, b & 0x7fffffffu);
+            raw = max(raw, __float_as_uint(f) & 0x7fffffffu);
             x[r][dim + j] = f;
         }
-    }
-    const float m = wave_max(__uint_as_float(big));
-    const bool any = __any(raw >= 0x7f800000u);
-    if (lane == 0) {
-        most[tid >> 6] = m;
-        some[tid >> 6] = any;
+        raw = lanes_most<LANES>(raw);
+        if (dim % (4 * LANES) == 0) rows_most[r][dim / (4 * LANES)] = raw;
     }
     __syncthreads();
-    const int shift = shift_below(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
-    const bool odd = values && (some[0] | some[1] | some[2] | some[3]);
-    const float f = pow2(shift);
+    // a row a lane
+    uint32_t raw = rows_most[lane][0];
+#pragma unroll
+    for (int i = 1; i < PARTS; i++) raw = max(raw, rows_most[lane][i]);
+    const bool any = __any(raw >= 0x7f800000u), odd = values && any;
+    if (any) {
+        raw = 0;
+        for (int j = 0; j < D; j++) raw = max(raw, finite_bits(__float_as_uint(x[lane][j])));
+    }
+    const float mine = __uint_as_float(raw), most = wave_max(mine), least = -wave_max(raw ? -mine : -INFINITY);
+    const bool apart = rows_apart(least, most);
+    const int shift = shift_below(most), own = apart ? shift_below(mine) : shift;
+    scale_here[wave][lane] = pow2(own);  // each wavefront reads what it wrote
+    const float *scale = scale_here[wave];
     const size_t at = (size_t)blockIdx.x * p.kv_heads + h;
-    if (tid == 0) p.shifts[2 * at + (values ? 1 : 0)] = values ? 2 * shift + (odd ? 1 : 0) : shift;
+    if (tid == 0) p.shifts[2 * at + (values ? 1 : 0)] = 4 * shift + (apart ? 2 : 0) + (odd ? 1 : 0);
+    if (tid < KB) p.row_shifts[(2 * at + (values ? 1 : 0)) * KB + tid] = (int8_t)own;
     uint8_t *tile = p.tiles + at * (2 * HALF_BYTES<D>);
     if (odd && tid < D) {
         uint64_t bits = 0;
@@ -268,20 +304,21 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float y = x[8 * c + e][r];
-                w[e] = odd && (__float_as_uint(y) & 0x7fffffffu) >= 0x7f800000u ? 0.0f : y;
+                w[e] = (odd && (__float_as_uint(y) & 0x7fffffffu) >= 0x7f800000u ? 0.0f : y) * scale[8 * c + e];
             }
             hi = tile + HALF_BYTES<D> + r * 128 + swz(r, c) * 16;
             lo = hi + D * 128;
         } else {
             constexpr int CHUNKS = D < 64 ? D / 8 : 8;
             const int c = u % CHUNKS, r = (u / CHUNKS) & 63, part = u / (64 * CHUNKS);  // key r, coordinates 64 part + 8 c ..
+            const float f = scale[r];
 #pragma unroll
-            for (int e = 0; e < 8; e++) w[e] = x[r][64 * part + 8 * c + e];
+            for (int e = 0; e < 8; e++) w[e] = x[r][64 * part + 8 * c + e] * f;
             hi = tile + part * 16384 + r * 128 + swz(r, c) * 16;
             lo = D < 64 ? tile + r * 128 + swz(r, c + CHUNKS) * 16 : hi + 8192;
         }
         halfx8 wh, wl;
-        split8(w, f, wh, wl);
+        split8(w, 1.0f, wh, wl);
         *reinterpret_cast<halfx8 *>(hi) = wh;
         *reinterpret_cast<halfx8 *>(lo) = wl;
     }
@@ -307,14 +344,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const float *p, uint
 // the weights of a block are the values' operand where they stand. Tiles come by DMA into two LDS buffers each for keys and values,
 // a block ahead (one each where two would leave one workgroup of four wavefronts a compute unit), or are made here from rows read a
 // block ahead (few_readers). The softmax is in log2 units against a reference that is raised when a block passes it by more than 3;
-// weights stay below 2^15. The sums are held in units of the least power of two that the values' tiles so far have; a block with a
-// larger one has its weights smaller by the difference (at most 2^60: what is cut off there is below 2^-60 of the largest value).
+// weights stay below 2^15. A column's sums of values are held in units of their own, 2^(12 - unit): the unit is raised, as the reference is, when a
+// block's largest weight times its values' power of two passes it by more than 3, so that what a column does not see, or gives no
+// weight, takes none of its precision; the block's weights are taken smaller or larger by the difference.
 //
 // In a long table the matrix pipes are busy 61% of the time and the vector pipes 48%, hardly ever at once:
 // 10,000 rows, 8 heads of 64, 557 us or 1,103 TFLOP/s of the three products, what a large fp16 product reaches here (1,109). Short
 // tables are bound by their start (plan, rows and queries on their way: about 9 us) and by memory.
 template <int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_packed(Packed p) {
+__global__ __launch_bounds__(64 * WAVES, D == 32 ? (WAVES == 4 ? 3 : 4) : 2) void k_packed(Packed p) {
     constexpr int QT = 32 * WAVES, HALF = HALF_BYTES<D>, DC = D / 16, DB = D / 32, BEGIN = BEGIN_OF<D>;
     constexpr bool DIRECT = WAVES == 4 && D <= 64, SINGLE = WAVES == 4 && D == 128;
     __shared__ __align__(16) uint8_t kt0[HALF], kt1[SINGLE ? 16 : HALF], vt0[HALF], vt1[SINGLE ? 16 : HALF];
@@ -322,6 +360,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
     __shared__ uint32_t first_here[64];
     __shared__ floatx4 most_here[4];
     __shared__ __align__(8) uint8_t odd_here[64][8];
+    __shared__ uint32_t rows_most[DIRECT ? KB : 1];  // values'
+    __shared__ __align__(8) int8_t shifts_here[2][DIRECT ? KB : 8];  // the rows' own powers of two, keys' and values'
     const int thread = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
 
     // the first 64 tables, one a lane, read beside the plan
@@ -504,8 +544,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
         kat[i] = krow * 128 + swz(krow, 2 * i + g) * 16;
         vat[i] = r32 * 128 + swz(r32, 2 * i + g) * 16;
     }
-    float ref = -INFINITY, l = 0.0f;
-    int ev = 1000;  // the sums are in units of 2^-ev
+    // whole numbers: the weights' sum is in units of 2^(ref - 12), the values' sums in 2^(unit - 12)
+    float ref = -INFINITY, unit = -INFINITY, l = 0.0f;
     floatx16 acc[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++)
@@ -515,11 +555,15 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
 #pragma unroll
     for (int v = 0; v < 16; v++) zero[v] = 0.0f;
 
-    // Block kb, scaled by 2^ek and 2^eb, in the buffers kc and vc.
-    auto block = [&](auto here, const uint8_t *kc, const uint8_t *vc, int kb, int ek, int evo) __attribute__((always_inline)) {
+    // Block kb in the buffers kc and vc, with its powers of two as k_packed_tiles leaves them.
+    // With is_apart rows may have powers of two of their own.
+    auto block_of = [&](auto here, auto is_apart, const uint8_t *kc, const uint8_t *vc, int kb, int eko,
+                        int evo) __attribute__((always_inline)) {
+        constexpr bool apart = decltype(is_apart)::value;
         if (kb * KB >= most_seen) return;  // a wavefront whose queries see none of it: its part of the copies is all it does
-        const int eb = evo >> 1;
-        const float f = fminf(fmaxf(to_log2 * pow2(-ek), 0x1p-126f), 0x1p126f);  // from raw scores to log2 units
+        const int eb = evo >> 2;
+        auto in_log2 = [&](int shift) { return fminf(fmaxf(to_log2 * pow2(-shift), 0x1p-126f), 0x1p126f); };
+        const float f = in_log2(eko >> 2);  // from raw scores to log2 units
         floatx16 sc[2];
 #pragma unroll
         for (int dc = 0; dc < DC; dc++)
@@ -546,34 +590,66 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
 #pragma unroll
             for (int v = 0; v < 16; v++) mb = fmaxf(mb, sc[kh][v]);
         mb = half_max(mb) * f;
-        const bool grow = mb > ref + 3.0f;
-        if (__any(grow)) {
-            const float nref = grow ? mb : ref;
-            const float alpha = grow ? exp2_hw(ref - nref) : 1.0f;
-            l *= alpha;
+        float top = mb - (float)eb;  // of weights times values, in log2
+        // eight rows' own powers of two, keys' or values', from row 32 kh + 16 hh + 8 g on
+        auto rows_shifts = [&](int which, int kh, int hh) {
+            const int8_t *at = decltype(here)::value ? shifts_here[which]
+                                                     : p.row_shifts + (2 * (((size_t)first + kb) * p.kv_heads + hk) + which) * KB;
+            return *reinterpret_cast<const uint2 *>(at + 32 * kh + 16 * hh + 8 * g);
+        };
+        auto byte_of = [](uint2 w, int e) { return (int)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3))); };
+        if constexpr (apart) {  // scores in log2, and what they come to with their values
+            mb = top = -INFINITY;
 #pragma unroll
-            for (int db = 0; db < DB; db++) acc[db] *= alpha;
-            ref = nref;
+            for (int kh = 0; kh < 2; kh++)
+#pragma unroll
+                for (int hh = 0; hh < 2; hh++) {
+                    __builtin_amdgcn_sched_barrier(0);  // eight rows at a time: there are no registers for more
+                    const uint2 ks = rows_shifts(0, kh, hh), vs = rows_shifts(1, kh, hh);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float x = sc[kh][8 * hh + e] * in_log2(byte_of(ks, e));
+                        sc[kh][8 * hh + e] = x;
+                        mb = fmaxf(mb, x);
+                        top = fmaxf(top, x - (float)byte_of(vs, e));
+                    }
+                }
+            mb = half_max(mb);
+            top = half_max(top);
         }
-        if (eb < ev) {
-            const float beta = ev < 1000 ? pow2(eb - ev) : 0.0f;
+        const bool grow = mb > ref + 3.0f, grow_unit = top > unit + 3.0f;
+        if (__any(grow || grow_unit)) {
+            const float nref = grow ? floorf(mb) : ref, nunit = grow_unit ? floorf(top) : unit;
+            l *= grow ? pow2((int)fmaxf(ref - nref, -200.0f)) : 1.0f;
+            const float beta = grow_unit ? pow2((int)fmaxf(unit - nunit, -200.0f)) : 1.0f;
 #pragma unroll
             for (int db = 0; db < DB; db++) acc[db] *= beta;
-            ev = eb;
+            ref = nref;
+            unit = nunit;
         }
-        const int less = max(ev - eb, -60);
-        const float off = (ref == -INFINITY ? 0.0f : 12.0f - ref) + (float)less;
+        // what the block's weights are taken larger by (below 2^-60 they are zeros as halves; their sum is taken of them)
+        const float less = ref == -INFINITY ? 0.0f : apart ? ref - unit : fmaxf(ref - unit - (float)eb, -60.0f);
+        const float off_sum = ref == -INFINITY ? 0.0f : 12.0f - ref, off = off_sum + less;
         float ps = 0.0f;
 #pragma unroll
         for (int kh = 0; kh < 2; kh++)
 #pragma unroll
             for (int hh = 0; hh < 2; hh++) {
                 u32x4 hw, lw;
+                const uint2 vs = apart ? rows_shifts(1, kh, hh) : make_uint2(0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float p0 = exp2_hw(fmaf(sc[kh][8 * hh + 2 * i], f, off));
-                    const float p1 = exp2_hw(fmaf(sc[kh][8 * hh + 2 * i + 1], f, off));
-                    ps += p0 + p1;
+                    const float x0 = sc[kh][8 * hh + 2 * i], x1 = sc[kh][8 * hh + 2 * i + 1];
+                    float p0, p1;
+                    if constexpr (apart) {  // the weights for their sum, and times the values' powers of two
+                        ps += exp2_hw(x0 + off_sum) + exp2_hw(x1 + off_sum);
+                        p0 = exp2_hw(x0 - (float)byte_of(vs, 2 * i) + off);
+                        p1 = exp2_hw(x1 - (float)byte_of(vs, 2 * i + 1) + off);
+                    } else {
+                        p0 = exp2_hw(fmaf(x0, f, off));
+                        p1 = exp2_hw(fmaf(x1, f, off));
+                        ps += p0 + p1;
+                    }
                     uint32_t hi, lo;
                     split2(p0, p1, hi, lo);
                     hw[i] = hi;
@@ -589,7 +665,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
                     acc[db] = mfma16(lo, ph, acc[db]);
                 }
             }
-        l = fmaf(ps, pow2(-less), l);
+        l = apart ? l + ps : fmaf(ps, pow2(-(int)less), l);
         if (evo & 1) {  // values that are not finite, zeros in the tile: what sees one is no number
             const int left = limit - kb * KB;
             const uint64_t sees = left >= 64 ? ~uint64_t(0) : (left > 0 ? (uint64_t(1) << left) - 1 : 0);
@@ -605,49 +681,33 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
                     if (odd[32 * db + 8 * (v >> 2) + 4 * g + (v & 3)] & sees) acc[db][v] = NAN;
         }
     };
-    // Block kb from the buffers kc and vc, the next one on its way into kn and vn: four arrays, so that the compiler sees that it need
-    // not wait for the copies before it reads.
-    auto step = [&](const uint8_t *kc, const uint8_t *vc, uint8_t *kn, uint8_t *vn, int kb) __attribute__((always_inline)) {
+    // The powers of two of block kb, and whether one serves all of its rows.
+    int eko = 0, evo = 0;
+    auto even = [&](int kb) {
         if (kb >= shifts_at + 64) {
             shifts_at += 64;
             hold_shifts();
         }
+        eko = __builtin_amdgcn_readlane(key_shifts, kb - shifts_at);
+        evo = __builtin_amdgcn_readlane(value_shifts, kb - shifts_at);
+        return !((eko | evo) & 2);
+    };
+    // Block kb from the buffers kc and vc, the next one on its way into kn and vn: four arrays, so that the compiler sees that it need
+    // not wait for the copies before it reads.
+    auto step = [&](const uint8_t *kc, const uint8_t *vc, uint8_t *kn, uint8_t *vn, int kb, int eko, int evo) __attribute__((always_inline)) {
         __builtin_amdgcn_s_waitcnt(0);  // this wavefront's copies of block kb have landed
         __syncthreads();                // everyone's have, and block kb - 1's buffers are no longer read
-        const int evo = __builtin_amdgcn_readlane(value_shifts, kb - shifts_at);
-        const int ek = __builtin_amdgcn_readlane(key_shifts, kb - shifts_at);
         if (kb + 1 < kb1) {
             copy(tiles + (kb + 1) * kb_bytes, kn);
             copy(tiles + (kb + 1) * kb_bytes + HALF, vn);
         }
-        block(Flag<false>{}, kc, vc, kb, ek, evo);
+        block_of(Flag<false>{}, Flag<false>{}, kc, vc, kb, eko, evo);
     };
+    int kb = kb0;
     if (direct) {
-        if constexpr (DIRECT)
-            for (int kb = kb0; kb < kb1; kb++) {
-                uint32_t big_k = 0, big_v = 0, raw_v = 0;
-#pragma unroll
-                for (int i = 0; i < HELD; i++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const uint32_t y = value_rows[i][e];
-                        big_k = max(big_k, finite_bits(key_rows[i][e >> 2][e & 3]));
-                        big_v = max(big_v, finite_bits(y));
-                        raw_v = max(raw_v, y & 0x7fffffffu);
-                    }
-                const float most_k = wave_max(__uint_as_float(big_k)), most_v = wave_max(__uint_as_float(big_v));
-                const bool any = __any(raw_v >= 0x7f800000u);
-                if (lane == 0) most_here[wave] = floatx4{most_k, most_v, any ? 1.0f : 0.0f, 0.0f};
-                __syncthreads();  // everyone's maxima are there, and block kb - 1's buffers are no longer read
-                floatx4 m = most_here[0];
-#pragma unroll
-                for (int w = 1; w < WAVES; w++)
-#pragma unroll
-                    for (int e = 0; e < 3; e++) m[e] = fmaxf(m[e], most_here[w][e]);
-                const int ek = __builtin_amdgcn_readfirstlane(shift_below(m[0]));
-                const int ev = __builtin_amdgcn_readfirstlane(shift_below(m[1]));
-                const bool odd = __builtin_amdgcn_readfirstlane(m[2] != 0.0f);
-                const float fk = pow2(ek), fv = pow2(ev);
+        if constexpr (DIRECT) {
+            // the rows in registers as halves in the buffers, with these powers of two
+            auto split_rows = [&](const float (&fk)[HELD], float fv, bool odd) __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < HELD; i++) {
                     const int u = tid + 256 * i, c = u % CHUNKS, r = u / CHUNKS, dim = u % D, kc = u / D;
@@ -655,7 +715,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
                     halfx8 wh, wl;
 #pragma unroll
                     for (int e = 0; e < 8; e++) w[e] = __uint_as_float(key_rows[i][e >> 2][e & 3]);
-                    split8(w, fk, wh, wl);
+                    split8(w, fk[i], wh, wl);
                     *reinterpret_cast<halfx8 *>(kt0 + r * 128 + swz(r, c) * 16) = wh;
                     *reinterpret_cast<halfx8 *>(kt0 + r * 128 + (D < 64 ? swz(r, c + CHUNKS) * 16 : 8192 + swz(r, c) * 16)) = wl;
                     uint32_t bits = 0;
@@ -672,36 +732,150 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
                     *reinterpret_cast<halfx8 *>(vt0 + dim * 128 + swz(dim, kc) * 16) = wh;
                     *reinterpret_cast<halfx8 *>(vt0 + D * 128 + dim * 128 + swz(dim, kc) * 16) = wl;
                 }
+            };
+            for (; kb < kb1; kb++) {
+                uint32_t big_k = 0, big_v = 0;
+#pragma unroll
+                for (int i = 0; i < HELD; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        big_k = max(big_k, key_rows[i][e >> 2][e & 3] & 0x7fffffffu);
+                        big_v = max(big_v, value_rows[i][e] & 0x7fffffffu);
+                    }
+                const bool any = __any(big_v >= 0x7f800000u);
+                if (__any(max(big_k, big_v) >= 0x7f800000u)) {  // of the finite ones, then
+                    big_k = big_v = 0;
+#pragma unroll
+                    for (int i = 0; i < HELD; i++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            big_k = max(big_k, finite_bits(key_rows[i][e >> 2][e & 3]));
+                            big_v = max(big_v, finite_bits(value_rows[i][e]));
+                        }
+                }
+                const float most_k = wave_max(__uint_as_float(big_k)), most_v = wave_max(__uint_as_float(big_v));
+                // Where a query of the tile does not see all of the block: the least of its rows by parts that quads of lanes have, four
+                // coordinates of a value, 32 of a key (a row of parts of several sizes then merely has its own power of two). Less one as
+                // an int, so that zeros are not the least.
+                uint32_t least_k = 0x7f7fffffu, least_v = 0x7f7fffffu;
+                if ((kb + 1) * KB > limit_of(row0)) {
+#pragma unroll
+                    for (int i = 0; i < HELD; i++) {
+                        float m = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const uint32_t w = key_rows[i][e >> 2][e & 3];
+                            m = fmaxf(m, fabsf(__uint_as_float(w)));
+                            least_v = min(least_v, __float_as_uint(lanes_max<4>(fabsf(__uint_as_float(value_rows[i][e])))) - 1);
+                        }
+                        least_k = min(least_k, __float_as_uint(lanes_max<4>(m)) - 1);
+                    }
+                    least_k = __float_as_uint(-wave_max(-__uint_as_float(least_k)));
+                    least_v = __float_as_uint(-wave_max(-__uint_as_float(least_v)));
+                    if (any) least_v = 0;
+                }
+                if (lane == 0)
+                    most_here[wave] = floatx4{any ? -most_k : most_k, most_v, __uint_as_float(least_k), __uint_as_float(least_v)};
+                __syncthreads();  // everyone's maxima are there, and block kb - 1's buffers are no longer read
+                floatx4 m = {0.0f, 0.0f, INFINITY, INFINITY};
+                bool odd = false;
+#pragma unroll
+                for (int w = 0; w < WAVES; w++) {
+                    const floatx4 o = most_here[w];
+                    odd = odd || __builtin_signbitf(o[0]);
+                    m = floatx4{fmaxf(m[0], fabsf(o[0])), fmaxf(m[1], o[1]), fminf(m[2], o[2]), fminf(m[3], o[3])};
+                }
+                if (__builtin_amdgcn_readfirstlane(rows_apart(m[2], m[0]) || rows_apart(m[3], m[1]))) break;
+                const int ek = __builtin_amdgcn_readfirstlane(shift_below(m[0]));
+                const int ev = __builtin_amdgcn_readfirstlane(shift_below(m[1]));
+                odd = __builtin_amdgcn_readfirstlane(odd);
+                float fk[HELD];
+#pragma unroll
+                for (int i = 0; i < HELD; i++) fk[i] = pow2(ek);
+                split_rows(fk, pow2(ev), odd);
                 if (kb + 1 < kb1) load_rows(kb + 1);
                 __syncthreads();
-                block(Flag<true>{}, kt0, vt0, kb, ek, 2 * ev + (odd ? 1 : 0));
+                block_of(Flag<true>{}, Flag<false>{}, kt0, vt0, kb, 4 * ek, 4 * ev + (odd ? 1 : 0));
             }
-    } else if constexpr (SINGLE) {
-        for (int kb = kb0; kb < kb1; kb++) {
-            if (kb >= shifts_at + 64) {
-                shifts_at += 64;
-                hold_shifts();
-            }
-            __builtin_amdgcn_s_waitcnt(0);  // as in step
-            __syncthreads();
-            block(Flag<false>{}, kt0, vt0, kb, __builtin_amdgcn_readlane(key_shifts, kb - shifts_at),
-                  __builtin_amdgcn_readlane(value_shifts, kb - shifts_at));
-            if (kb + 1 < kb1) {
-                __syncthreads();  // the buffers are no longer read; the compute unit's other workgroup works meanwhile
-                copy(tiles + (kb + 1) * kb_bytes, kt0);
-                copy(tiles + (kb + 1) * kb_bytes + HALF, vt0);
+            // from the first block whose rows lie apart on: a power of two for each row
+            for (; kb < kb1; kb++) {
+                __syncthreads();  // the buffers are no longer read
+                if (tid < KB) rows_most[tid] = 0;
+                if (tid == 0) most_here[0][2] = 0.0f;
+                __syncthreads();
+                float fk[HELD];
+                uint32_t raw_v = 0;
+#pragma unroll
+                for (int i = 0; i < HELD; i++) {
+                    const int u = tid + 256 * i;
+                    uint32_t big = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        big = max(big, finite_bits(key_rows[i][e >> 2][e & 3]));
+                        raw_v = max(raw_v, value_rows[i][e] & 0x7fffffffu);
+                        atomicMax(&rows_most[8 * (u / D) + e], finite_bits(value_rows[i][e]));
+                    }
+                    const int shift = shift_below(lanes_max<CHUNKS>(__uint_as_float(big)));
+                    fk[i] = pow2(shift);
+                    if (u % CHUNKS == 0) shifts_here[0][u / CHUNKS] = (int8_t)shift;
+                }
+                if (raw_v >= 0x7f800000u) most_here[0][2] = 1.0f;
+                __syncthreads();
+                if (tid < KB) shifts_here[1][tid] = (int8_t)shift_below(__uint_as_float(rows_most[tid]));
+                const bool odd = __builtin_amdgcn_readfirstlane(most_here[0][2] != 0.0f);
+#pragma unroll
+                for (int i = 0; i < HELD; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        const float most = __uint_as_float(rows_most[8 * ((tid + 256 * i) / D) + e]);
+                        value_rows[i][e] = __float_as_uint(__uint_as_float(value_rows[i][e]) * pow2(shift_below(most)));
+                    }
+                split_rows(fk, 1.0f, odd);
+                if (kb + 1 < kb1) load_rows(kb + 1);
+                __syncthreads();
+                block_of(Flag<true>{}, Flag<true>{}, kt0, vt0, kb, 2, 2 + (odd ? 1 : 0));
             }
         }
     } else {
-        int kb = kb0;
-        for (; kb + 1 < kb1; kb += 2) {  // two steps a turn: the buffers' places are constants
-            step(kt0, vt0, kt1, vt1, kb);
-            step(kt1, vt1, kt0, vt0, kb + 1);
+        if constexpr (SINGLE) {
+            for (; kb < kb1 && even(kb); kb++) {
+                __builtin_amdgcn_s_waitcnt(0);  // as in step
+                __syncthreads();
+                block_of(Flag<false>{}, Flag<false>{}, kt0, vt0, kb, eko, evo);
+                if (kb + 1 < kb1) {
+                    __syncthreads();  // the buffers are no longer read; the compute unit's other workgroup works meanwhile
+                    copy(tiles + (kb + 1) * kb_bytes, kt0);
+                    copy(tiles + (kb + 1) * kb_bytes + HALF, vt0);
+                }
+            }
+        } else {
+            for (; kb + 1 < kb1 && even(kb); kb += 2) {  // two steps a turn: the buffers' places are constants
+                const int eko0 = eko, evo0 = evo;
+                if (!even(kb + 1)) break;
+                step(kt0, vt0, kt1, vt1, kb, eko0, evo0);
+                step(kt1, vt1, kt0, vt0, kb + 1, eko, evo);
+            }
+            if (kb + 1 == kb1 && even(kb)) {
+                step(kt0, vt0, kt1, vt1, kb, eko, evo);
+                kb++;
+            }
         }
-        if (kb < kb1) step(kt0, vt0, kt1, vt1, kb);
+        // from the first block whose rows lie apart on, a block after the other
+        for (; kb < kb1; kb++) {
+            even(kb);
+            __builtin_amdgcn_s_waitcnt(0);  // what is on its way has landed
+            __syncthreads();                // and is no longer read
+            copy(tiles + kb * kb_bytes, kt0);
+            copy(tiles + kb * kb_bytes + HALF, vt0);
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            block_of(Flag<false>{}, Flag<true>{}, kt0, vt0, kb, eko, evo);
+        }
     }
     l = half_sum(l);  // lanes l and l ^ 32 have the same queries' sums over different keys
-    const float inv = l > 0.0f ? 1.0f / l : l, unit = pow2(-min(ev, 149));  // 0 and NaN stay
+    const float inv = l > 0.0f ? 1.0f / l : l;  // 0 and NaN stay
+    const float back = ref == -INFINITY ? 1.0f : pow2((int)(unit - ref));
     if (!done || live) {
         float *dst = done ? p.out + ((size_t)(qa + qi) * p.heads + h) * p.hd : p.part_o + (slot * QT + 32 * wave + r32) * p.hd;
 #pragma unroll
@@ -712,7 +886,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 && WAVES == 4 ? 3 : 2) void k_p
                 if (dim < p.hd) {
                     floatx4 o;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[e] = acc[db][4 * v4 + e] * inv * unit;
+                    for (int e = 0; e < 4; e++) o[e] = acc[db][4 * v4 + e] * inv * back;
                     *reinterpret_cast<floatx4u *>(dst + dim) = o;
                 }
             }
@@ -786,8 +960,8 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 struct Plan {
     int waves, runs, blocks, d, log_share;  // d: the heads' width, padded
     int64_t grid;
-    size_t tiles, shifts, odd, tables, part_o, part_ml, cut;
-    size_t bytes() const { return tiles + shifts + odd + 256 + 3 * tables + part_o + part_ml + cut; }
+    size_t tiles, shifts, row_shifts, odd, tables, part_o, part_ml, cut;
+    size_t bytes() const { return tiles + shifts + row_shifts + odd + 256 + 3 * tables + part_o + part_ml + cut; }
 };
 
 Plan plan(const PackedShape &a) {
@@ -809,6 +983,7 @@ Plan plan(const PackedShape &a) {
     const size_t halves = (size_t)blocks * a.kv_heads, places = 2 * (size_t)r.runs * qt;
     r.tiles = up256(halves * r.d * 512);
     r.shifts = up256(halves * 2 * sizeof(int));
+    r.row_shifts = up256(halves * 2 * KB);
     r.odd = up256(halves * r.d * sizeof(uint64_t));
     r.tables = up256(((size_t)a.tables + 1) * sizeof(uint32_t));
     r.part_o = up256(places * a.hd * sizeof(float));
@@ -850,6 +1025,7 @@ void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const
     p.blocks = r.blocks;
     p.tiles = carve(r.tiles);
     p.shifts = reinterpret_cast<int *>(carve(r.shifts));
+    p.row_shifts = reinterpret_cast<int8_t *>(carve(r.row_shifts));
     p.odd = reinterpret_cast<uint64_t *>(carve(r.odd));
     p.plan = reinterpret_cast<PackedPlan *>(carve(256));
     p.first = reinterpret_cast<uint32_t *>(carve(r.tables));

@@ -112,3 +112,73 @@ def test_pages_values_near_the_largest_float(gpu, dev, fmt, hd, lengths, counts,
         # together, of which a head's outputs have three times as much at most.
         check(got[at:at + n].astype(np.float64) / LARGE, out, off, f"format {fmt}, table {t}", 3 * 1.3e-6)
         at += n
+
+
+def by_tables(counts):
+    at = 0
+    for c in counts:
+        yield at, at + c
+        at += c
+
+
+@pytest.mark.parametrize("kind", ["key", "value"])
+@pytest.mark.parametrize("larger", [1e4, 1e8, 1e12, 1e30])
+@pytest.mark.parametrize("counts,heads,kv_heads,hd", SHAPES)
+def test_packed_rows_that_a_query_does_not_see(gpu, counts, heads, kv_heads, hd, larger, kind):
+    """In order: a row of a block far larger than those before it takes nothing from the queries that do not see it, and is what those
+    see that do; with as many queries as rows, and fewer."""
+    rng = np.random.default_rng(hd + heads)
+    n = sum(counts)
+    for queries in (counts, [max(1, c // 3) for c in counts]):
+        q, k, v = inputs(rng, sum(queries), n, heads, kv_heads, hd)
+        rows = [a + int(f * (b - a)) for a, b in by_tables(counts) for f in (0.41, 0.87)]
+        for r in rows:
+            {"key": k, "value": v}[kind][r] *= np.float32(larger)
+        got = gpu.attend_packed(flat(q), flat(k), flat(v), offsets_of(queries), heads, kv_heads, True, offsets_of(counts)).reshape(q.shape)
+        out, off = wanted(q, k, v, queries, counts, True)
+        if kind == "value" or larger < 1e6:  # scores past 2^22 have no fractions to speak of
+            assert np.all(np.isfinite(got)) and np.all(np.abs(got - out) <= off)
+        # where one row outweighs all others the roundings of its weight do not cancel: together only those that see neither
+        for (a, b), (qa, qb) in zip(by_tables(counts), by_tables(queries)):
+            at = qa + np.array([i for i, m in enumerate(P.limits_of(b - a, qb - qa, True)) if not any(a <= r < a + m for r in rows)], int)
+            if len(at):
+                check(got[at], out[at], off[at], f"{kind} {larger}, {qb - qa} over {b - a}")
+
+
+@pytest.mark.parametrize("counts,heads,kv_heads,hd", SHAPES)
+def test_packed_blocks_that_a_query_does_not_see(gpu, counts, heads, kv_heads, hd):
+    """In order: blocks of values 2^140 times those of the blocks before them."""
+    rng = np.random.default_rng(hd)
+    n = sum(counts)
+    q, k, v = inputs(rng, n, n, heads, kv_heads, hd)
+    v *= np.float32(1e-6)
+    for a, b in by_tables(counts):
+        v[a + (b - a) // 128 * 64:b] *= np.float32(2.0**100)
+        v[a + (b - a) // 128 * 64:b] *= np.float32(2.0**40)
+    got = gpu.attend_packed(flat(q), flat(k), flat(v), offsets_of(counts), heads, kv_heads, True).reshape(q.shape).astype(np.float64)
+    out, off = wanted(q, k, v, counts, counts, True)
+    for a, b in by_tables(counts):
+        c = a + (b - a) // 128 * 64
+        if c > a:
+            check(got[a:c] * 1e6, out[a:c] * 1e6, off[a:c] * 1e6, f"{b - a} rows, before")
+        check(got[c:b] * 1e-36, out[c:b] * 1e-36, off[c:b] * 1e-36, f"{b - a} rows, from there on")
+
+
+@pytest.mark.parametrize("counts,heads,kv_heads,hd", SHAPES)
+def test_packed_blocks_that_weigh_nothing(gpu, counts, heads, kv_heads, hd):
+    """A block of values 1e12 times the others', whose scores are 90 below theirs: the others' outputs, to their own precision."""
+    rng = np.random.default_rng(hd)
+    n = sum(counts)
+    for last in (False, True):
+        q, k, v = inputs(rng, n, n, heads, kv_heads, hd)
+        q[:, :, 0], k[:, :, 0] = 8.0, 0.0
+        left = np.ones(n, bool)
+        for a, b in by_tables(counts):
+            at = a + ((b - a - 1) // 64 * 64 if last else 0)
+            left[at:min(at + 64, b)] = False
+        k[~left, :, 0] = -12.0
+        v[~left] *= np.float32(1e12)
+        got = gpu.attend_packed(flat(q), flat(k), flat(v), offsets_of(counts), heads, kv_heads).reshape(q.shape)
+        rows = [int(left[a:b].sum()) for a, b in by_tables(counts)]
+        # what the block adds: e^-80 1e12, at most 2e-23
+        check(got, *wanted(q, k[left], v[left], counts, rows, False), f"the {'last' if last else 'first'} block")
