@@ -371,7 +371,9 @@ int tah_pages_read_dev(tah_dev *dev, const tah_pages *p, const int32_t *starts, 
  * h / (heads / kv_heads); kv_heads divides heads. out [nq][heads * hd], before the output projection; queries from
  * offsets[tables] on are left as they were. Rows on no page are not seen (a length counts as no more than ld * page_rows);
  * a query that sees none gives zeros. A number that is not finite makes NaN of the outputs that see it, and of no others: a key
- * of its head's, a value of its own coordinate's. The _dev form takes every array in device memory as above (lengths and
+ * of its head's, a value of its own coordinate's. Rows that a query does not see take none of its precision; a
+ * term is off by 2^-22 of itself, or by 2^-37 of the largest in the 64 rows around it that the query sees, whichever is more. Scores
+ * of magnitude 2^22 and more have no fractions that count, and may give NaN, as in tah_attend. The _dev form takes every array in device memory as above (lengths and
  * offsets may change between replays of a captured call); the other takes them in host memory, but for the pool, and refuses
  * lengths over ld * page_rows or of rows on no page with TAH_E_ARG. */
 int tah_pages_attend(tah_dev *dev, const tah_pages *p, const int32_t *lengths, const float *q, const int32_t *offsets,
@@ -382,8 +384,8 @@ int tah_pages_attend_dev(tah_dev *dev, const tah_pages *p, const int32_t *length
 /* Attention of packed tables in full precision (tah_attend of several tables at once): queries q [nq][heads * hd] (already
  * scaled) of table t, q_offsets[t] .. q_offsets[t + 1] - 1, over rows kv_offsets[t] .. kv_offsets[t + 1] - 1 of k and v
  * [nkv][kv_heads * hd]; rows q_ld and kv_ld floats apart (0: heads * hd, kv_heads * hd). With causal the last query of a table
- * sees all of its rows, each one before it one less. Heads, rows that see nothing, numbers that are not finite and rows past
- * the last table as for tah_pages_attend; hd a multiple of 16 up to 128. Offsets [tables + 1] run from 0 up; they may be the
+ * sees all of its rows, each one before it one less. Heads, rows that see nothing, numbers that are not finite, precision and rows
+ * past the last table as for tah_pages_attend; hd a multiple of 16 up to 128. Offsets [tables + 1] run from 0 up; they may be the
  * same array. The _dev form takes every array in device memory (4-byte aligned); the other in host memory, and refuses offsets
  * that fall or pass nq or nkv. */
 int tah_attend_packed(tah_dev *dev, const float *q, const float *k, const float *v, const int32_t *q_offsets,

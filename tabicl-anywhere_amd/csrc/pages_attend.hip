@@ -127,8 +127,10 @@ __device__ __forceinline__ floatx4 mfma(halfx8 a, halfx8 b, floatx4 c) {
 // Numbers: ints go in as they are (i8 exact in one half, i16 in two bytes), the key's step multiplies its scores, the value's its
 // weights; f32 goes in as two halves times the block's power of two. Queries and weights are two halves. So a term is two
 // products (i8), three (f32) or four (i16: a low byte is 2^-8 of the largest number, so its product with a low half counts), for
-// f32's error. Weights are held below 2^15 (their maximum raised by blocks that pass it by more than
-// 2^3), times the value's step over a power of two that no step so far passes.
+// f32's error. Weights are held below 2^15 (their maximum raised by blocks that pass it by more than 2^3). A column's sums of values have a
+// unit of their own, 2^(vunit - 12), raised when a block's largest weight times the largest step that the column sees passes it by as much,
+// so that rows that it does not see, or gives no weight, take none of its precision. f32: where columns do not see
+// the same rows of a block each row has a power of two of its own, as ints have their steps.
 //
 // Bound by bytes where tables are long: 64 of up to 20,000 rows, 8 heads of 64 in i8, one query each, 133 us of kernel for 702 MB, 5.3
 // TB/s, what a large copy reaches (vector instructions issue in 55% of the cycles, matrix instructions in 14%). One table of 100,000
@@ -148,6 +150,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
     constexpr int QS = WAIT ? CT * C * 2 * 2 * 64 : 0;  // 16-byte words of a wavefront's
     __shared__ __align__(16) uint8_t store[WAVES * (QS * 16 > HD * 68 ? QS * 16 : HD * 68)];
     __shared__ float mref[WAVES][COLS], msum[WAVES][COLS];
+    // f32, blocks that some columns see in part: the steps of the block's keys and values, each wavefront's own
+    __shared__ __align__(16) float steps_here[WAVES][2][INTS ? 4 : KEYS];
     float (*macc)[HD][17] = reinterpret_cast<float (*)[HD][17]>(store);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int qi = lane & 15, lg = lane >> 4, group = heads / p.heads, hd = p.hd, P = p.rows;
@@ -225,8 +229,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
         // the columns' queries and limits
         halfx8 qh[WAIT ? 1 : CT][C][2], ql[WAIT ? 1 : CT][C][2];
         halfx8 *waiting = reinterpret_cast<halfx8 *>(store) + (size_t)wave * QS + lane;
-        float to_log2[CT], ref[CT], l[CT];
-        int limit[CT], ev = INTS ? -1000 : 1000;
+        // whole numbers, log2: ref, and the values' unit with what follows from both (0 where nothing has been seen)
+        float to_log2[CT], ref[CT], vunit[CT], base[CT], gap[CT], l[CT];
+        int limit[CT];
         floatx4 acc[CT][M];
         int lim_most = 0, lim_least = tw.len;
 #pragma unroll
@@ -266,8 +271,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                     }
                 }
             to_log2[ct] = (BYTES ? 256.0f : 1.0f) * LOG2E * pow2(-eq);
-            ref[ct] = -INFINITY;
-            l[ct] = 0.0f;
+            ref[ct] = vunit[ct] = -INFINITY;
+            base[ct] = gap[ct] = l[ct] = 0.0f;
 #pragma unroll
             for (int m = 0; m < M; m++) acc[ct][m] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
             // where the join finds the unit
@@ -341,6 +346,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
             // of the lane's N keys (values), how many there are
             const int here = whole ? N : (idv >= 0 ? min(max(tw.len - kv, 0), N) : 0);
             const bool all_seen = whole && first + KEYS <= lim_least;
+            const bool in_part = lim_least < min(first + KEYS, tw.len);  // some column does not see all that is there
             // coordinates past the head's width; f32: keys that are not there, and the block's keys' power of two
             int ek = 0;
             if (hd & 63) {
@@ -363,16 +369,34 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
 #pragma unroll
                                 for (int i = 0; i < Raw<FMT, 2>::WORDS; i++) kr[sp][c].w[i] = 0;
                 }
-                uint32_t most = 0;
+                float rows[2 * KS], most = 0.0f;  // the largest of the lane's numbers of a row
 #pragma unroll
-                for (int sp = 0; sp < 2 * KS; sp++)
+                for (int sp = 0; sp < 2 * KS; sp++) {
+                    uint32_t bits = 0;
 #pragma unroll
                     for (int c = 0; c < C; c++)
 #pragma unroll
-                        for (int i = 0; i < Raw<FMT, 2>::WORDS; i++) most = max(most, finite_bits(kr[sp][c].w[i]));
-                ek = shift_below(wave_max(__uint_as_float(most)));
+                        for (int i = 0; i < Raw<FMT, 2>::WORDS; i++) bits = max(bits, finite_bits(kr[sp][c].w[i]));
+                    rows[sp] = __uint_as_float(bits);
+                    most = fmaxf(most, rows[sp]);
+                }
+                most = wave_max(most);
+                if (!in_part) {
+                    ek = shift_below(most);
+                } else {  // each by its own
+#pragma unroll
+                    for (int sp = 0; sp < 2 * KS; sp++) {
+                        const int e = shift_below(half_max(row_max(rows[sp])));
+#pragma unroll
+                        for (int c = 0; c < C; c++)
+#pragma unroll
+                            for (int i = 0; i < Raw<FMT, 2>::WORDS; i++)
+                                kr[sp][c].w[i] = __float_as_uint(__uint_as_float(kr[sp][c].w[i]) * pow2(e));
+                        if (lg == 0) steps_here[wave][0][N * (qi >> 2) + 4 * sp + (qi & 3)] = pow2(-e);
+                    }
+                }
             }
-            const float fk = INTS ? 1.0f : pow2(ek), unk = INTS ? 1.0f : pow2(-ek);
+            const float fk = INTS ? 1.0f : pow2(ek);
             floatx4 sc[2 * KS][CT];  // set sp = 2 s + p
             const floatx4 none = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -403,58 +427,82 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                 __builtin_amdgcn_sched_barrier(0);
                 load_values();
             }
-            // the values' scale: ints by a power of two that no step passes, f32 by one that brings every value below 2^14
-            float vs = 1.0f;
+            // The values' scale: the power of two of the largest step that a column sees. f32 has one step for the block, which brings
+            // every value below 2^14, or in part one for each row.
+            float eb[CT], vs = 1.0f;
             uint32_t odd = 0;  // f32: whether a value is not finite
-            if constexpr (INTS) {
-                float most = 0.0f;
+            if constexpr (!INTS) {
+                uint32_t rows[N], most = 0;
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    if (!whole && j >= here) stv[j >> 2][j & 3] = 0.0f;
-                    most = fmaxf(most, stv[j >> 2][j & 3]);
-                }
-                most = half_max(row_max(most));
-                const int e = most > 0.0f ? __builtin_amdgcn_frexp_expf(most) : -1000;
-                if (e > ev) {
-                    const float f = ev > -1000 ? pow2(ev - e) : 0.0f;
+                for (int i = 0; i < N; i++) {
+                    rows[i] = 0;
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                        for (int m = 0; m < M; m++) acc[ct][m] *= f;
-                    ev = e;
-                }
-                vs = pow2(-max(ev, -126));
-            } else {
-                uint32_t most = 0;
-#pragma unroll
-                for (int m = 0; m < M; m++)
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
+                    for (int m = 0; m < M; m++) {
                         if (!whole && i >= here) vr[m].w[i] = 0;
                         odd = max(odd, vr[m].w[i] & 0x7fffffffu);
-                        most = max(most, finite_bits(vr[m].w[i]));
+                        rows[i] = max(rows[i], finite_bits(vr[m].w[i]));
                     }
-                const int e = shift_below(wave_max(__uint_as_float(most)));
-                if (e < ev) {
-                    const float f = ev < 1000 ? pow2(e - ev) : 0.0f;
-#pragma unroll
-                    for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                        for (int m = 0; m < M; m++) acc[ct][m] *= f;
-                    ev = e;
+                    most = max(most, rows[i]);
                 }
-                vs = pow2(ev);
+                if (in_part) {
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const int e = shift_below(row16_reduce(__uint_as_float(rows[i]), fmaxf));
+#pragma unroll
+                        for (int m = 0; m < M; m++) vr[m].w[i] = __float_as_uint(__uint_as_float(vr[m].w[i]) * pow2(e));
+                        steps_here[wave][1][N * lg + i] = pow2(-e);  // of sixteen lanes the same
+                    }
+                } else {
+                    const int e = shift_below(wave_max(__uint_as_float(most)));
+                    vs = pow2(e);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) eb[ct] = (float)-e;
+                }
+            }
+            if (INTS && !whole)
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (j >= here) stv[j >> 2][j & 3] = 0.0f;
+            auto value_step = [&](int j) {
+                if constexpr (INTS) {
+                    const float f = stv[j >> 2][j & 3];
+                    return f;
+                } else {
+                    return steps_here[wave][1][N * lg + j];
+                }
+            };
+            auto largest_of = [&](int seen) {
+                float most = 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; j++) most = j < seen ? fmaxf(most, value_step(j)) : most;
+                most = half_max(row_max(most));
+                return most > 0.0f ? (float)max(__builtin_amdgcn_frexp_expf(most), -126) : -126.0f;
+            };
+            if (in_part) {
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) eb[ct] = largest_of(limit[ct] - kv);
+            } else if (INTS) {
+                eb[0] = largest_of(N);
+#pragma unroll
+                for (int ct = 1; ct < CT; ct++) eb[ct] = eb[0];
             }
             halfx8 ph[CT][KS], pl[CT][KS];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 float x[N];
-                const float f = INTS ? to_log2[ct] : fminf(fmaxf(to_log2[ct] * unk, 0x1p-126f), 0x1p126f);
+                auto in_log2 = [&](float unk) { return fminf(fmaxf(to_log2[ct] * unk, 0x1p-126f), 0x1p126f); };
+                float f = INTS ? to_log2[ct] : in_log2(pow2(-ek));
 #pragma unroll
                 for (int j = 0; j < N; j++) {
                     x[j] = sc[j >> 2][ct][j & 3];
                     if constexpr (INTS) x[j] *= stk[j >> 2][j & 3];
                 }
+                if constexpr (!INTS)
+                    if (in_part) {
+                        f = 1.0f;
+#pragma unroll
+                        for (int j = 0; j < N; j++) x[j] *= in_log2(steps_here[wave][0][N * lg + j]);
+                    }
                 if (!all_seen) {
                     const int seen = min(here, min(max(limit[ct] - kv, 0), N));
 #pragma unroll
@@ -465,16 +513,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
 #pragma unroll
                 for (int j = 1; j < N; j++) mb = fmaxf(mb, x[j]);
                 mb = half_max(row_max(mb)) * f;
-                const bool grow = mb > ref[ct] + 3.0f;
-                if (__any(grow)) {
-                    const float nref = grow ? mb : ref[ct];
-                    const float alpha = grow ? exp2_hw(ref[ct] - nref) : 1.0f;
-                    l[ct] *= alpha;
+                const float top = mb + eb[ct];  // of weights times steps
+                const bool grow = mb > ref[ct] + 3.0f, grow_values = top > vunit[ct] + 3.0f;
+                if (__any(grow || grow_values)) {
+                    const float nref = grow ? floorf(mb) : ref[ct], nvunit = grow_values ? floorf(top) : vunit[ct];
+                    l[ct] *= grow ? pow2((int)fmaxf(ref[ct] - nref, -200.0f)) : 1.0f;
+                    const float beta = grow_values ? pow2((int)fmaxf(vunit[ct] - nvunit, -200.0f)) : 1.0f;
 #pragma unroll
-                    for (int m = 0; m < M; m++) acc[ct][m] *= alpha;
+                    for (int m = 0; m < M; m++) acc[ct][m] *= beta;
                     ref[ct] = nref;
+                    vunit[ct] = nvunit;
+                    base[ct] = nref == -INFINITY ? 0.0f : 12.0f - nref;
+                    gap[ct] = nref == -INFINITY ? 0.0f : nref - nvunit;
                 }
-                const float off = ref[ct] == -INFINITY ? 0.0f : 12.0f - ref[ct];
+                // what the block's weights are taken larger by (below 2^-60 they are zeros as halves; their sum is taken of them)
+                const float less = fmaxf(gap[ct] + eb[ct], -60.0f), off = base[ct] + less, step = pow2(-(int)eb[ct]);
+                float ps = 0.0f;
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
                     u32x4 hw, lw;
@@ -482,10 +536,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                     for (int i = 0; i < 4; i++) {
                         const int j = 8 * s + 2 * i;
                         float p0 = exp2_hw(fmaf(x[j], f, off)), p1 = exp2_hw(fmaf(x[j + 1], f, off));
-                        l[ct] += p0 + p1;
-                        if constexpr (INTS) {
-                            p0 *= stv[j >> 2][j & 3] * vs;
-                            p1 *= stv[j >> 2][(j + 1) & 3] * vs;
+                        ps += p0 + p1;
+                        if (INTS || in_part) {  // at most 1 where it is seen
+                            p0 *= __builtin_amdgcn_fmed3f(value_step(j) * step, 0.0f, 1.0f);
+                            p1 *= __builtin_amdgcn_fmed3f(value_step(j + 1) * step, 0.0f, 1.0f);
                         }
                         uint32_t a, b;
                         split2(p0, p1, a, b);
@@ -495,6 +549,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                     ph[ct][s] = __builtin_bit_cast(halfx8, hw);
                     pl[ct][s] = __builtin_bit_cast(halfx8, lw);
                 }
+                l[ct] = fmaf(ps, pow2(-(int)less), l[ct]);
             }
             // values that are not finite: zeros in the products, and what sees one is no number
             if constexpr (!INTS) {
@@ -546,12 +601,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
             kb += step;
         }
         at += b1 - b0;
-        // the sums over the weights' sum, in their own units
-        const float uv = (BYTES ? 256.0f : 1.0f) * (INTS ? (ev > -1000 ? pow2(ev) : 0.0f) : pow2(-min(ev, 149)));
+        // the sums over the weights' sum
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             const float lw = half_sum(row_sum(l[ct]));
             const float inv = lw > 0.0f ? 1.0f / lw : lw;  // 0 and NaN stay
+            const float uv = (BYTES ? 256.0f : 1.0f) * pow2(-(int)gap[ct]);
             if (!together) {
                 const size_t own = 2 * (size_t)me + (at - (b1 - b0) == mine ? 0 : 1);
                 const int col = 16 * ct + qi, c = tile * COLS + col, i = c / group;

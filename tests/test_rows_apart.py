@@ -182,3 +182,87 @@ def test_packed_blocks_that_weigh_nothing(gpu, counts, heads, kv_heads, hd):
         rows = [int(left[a:b].sum()) for a, b in by_tables(counts)]
         # what the block adds: e^-80 1e12, at most 2e-23
         check(got, *wanted(q, k[left], v[left], counts, rows, False), f"the {'last' if last else 'first'} block")
+
+
+def asked_often(gpu, dev, pool, table, lengths, q, counts, heads, causal, copies):
+    """The outputs of queries of a few tables, asked `copies` times in one call, so that a wavefront has several of their blocks."""
+    T, n = len(lengths), sum(counts)
+    card, tb = dev.of(pool.bytes), dev.of(np.tile(table, (copies, 1)))
+    ln, of, qd = dev.of(np.tile(np.array(lengths, np.int32), copies)), dev.of(offsets_of(counts * copies)), dev.of(np.tile(q, (copies, 1, 1)))
+    od = dev.of(np.zeros((copies * n,) + q.shape[1:], np.float32))
+    gpu.pages_attend_dev(described(pool, T * copies, table.shape[1], card.ptr, tb.ptr), ln.ptr, qd.ptr, of.ptr, copies * n, heads, od.ptr,
+                         causal)
+    gpu.sync()
+    return od.download((copies, n) + q.shape[1:]).astype(np.float64)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kind", ["key", "value"])
+@pytest.mark.parametrize("larger", [1e4, 1e8, 1e12, 1e30])
+@pytest.mark.parametrize("hd,group,copies", [(64, 1, 1), (64, 4, 150), (128, 2, 150), (48, 1, 300)])
+def test_pages_rows_that_a_query_does_not_see(gpu, dev, fmt, kind, larger, hd, group, copies):
+    """In order: a row far larger than those before it takes nothing from the queries that do not see it."""
+    rng = np.random.default_rng(hd + group)
+    rows, kv_heads, lengths, counts = 32, 2, [100, 37, 130], [20, 18, 40]
+    table = rng.permutation(15).astype(np.int32).reshape(3, 5)
+    pool = P.Pool(fmt, kv_heads, hd, rows, 15, fill=0xFF)
+    large = [[n - 7, n - 15] for n in lengths]
+    for t, n in enumerate(lengths):
+        for i in range(n):
+            k, v = values(rng, 1, kv_heads, hd)[0], values(rng, 1, kv_heads, hd)[0]
+            f = np.float32(larger if i in large[t] else 1.0)
+            pool.write(table[t, i // rows], i % rows, *((k * f, v) if kind == "key" else (k, v * f)))
+    q = (rng.standard_normal((sum(counts), kv_heads * group, hd)) * 0.4).astype(np.float32)
+    got = asked_often(gpu, dev, pool, table, lengths, q, counts, kv_heads * group, True, copies)
+    at = 0
+    for t, n in enumerate(counts):
+        k, v = pool.rows_of(table[t], lengths[t])
+        limits = P.limits_of(lengths[t], n, True)
+        out, off = P.attention(q[at:at + n], k, v, limits)
+        blind = np.array([i for i, m in enumerate(limits) if m <= min(large[t])])
+        for c in sorted({0, 1 % copies, copies // 2, copies - 1}):
+            one = got[c, at:at + n]
+            if kind == "value" or larger < 1e6:
+                assert np.all(np.isfinite(one)) and np.all(np.abs(one - out) <= off)
+            check(one[blind], out[blind], off[blind], f"format {fmt}, {kind} {larger}, table {t}, copy {c}", 3 * 1.3e-6)
+        at += n
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hd,group,copies", [(64, 1, 1), (64, 4, 150), (128, 2, 150)])
+def test_pages_blocks_apart(gpu, dev, fmt, hd, group, copies):
+    """Blocks of values 2^100 times those before them, which the first queries do not see; and such a block whose scores are 90 below
+    the others', which weighs nothing."""
+    rng = np.random.default_rng(hd + group)
+    rows, lengths, counts = 64, [200, 192], [20, 40]
+    table = rng.permutation(8).astype(np.int32).reshape(2, 4)
+    q = (rng.standard_normal((sum(counts), group, hd)) * 0.4).astype(np.float32)
+    q[:, :, 0] = 8.0
+    for weighs in (True, False):
+        pool = P.Pool(fmt, 1, hd, rows, 8, fill=0xFF)
+        # the last 8 rows of the first, the last 32 of the second; or the block from row 64 on
+        large = [lambda i, n: i >= 192, lambda i, n: i >= 160] if weighs else [lambda i, n: 64 <= i < 128] * 2
+        for t, n in enumerate(lengths):
+            k, v = values(rng, n, 1, hd), values(rng, n, 1, hd)
+            k[:, :, 0] = 0.0
+            for i in range(n):
+                if large[t](i, n):
+                    v[i] *= np.float32(2.0**100)
+                    k[i, :, 0] = 0.0 if weighs else -22.5
+                pool.write(table[t, i // rows], i % rows, k[i], v[i])
+        got = asked_often(gpu, dev, pool, table, lengths, q, counts, group, True, copies)
+        at = 0
+        for t, n in enumerate(counts):
+            k, v = pool.rows_of(table[t], lengths[t])
+            limits = P.limits_of(lengths[t], n, True)
+            if not weighs:  # e^-150 2^100, at most 1e-35
+                left = np.array([not large[t](i, lengths[t]) for i in range(lengths[t])])
+                k, v, limits = k[left], v[left], [int(left[:m].sum()) for m in limits]
+            out, off = P.attention(q[at:at + n], k, v, limits)
+            sees = np.array([weighs and any(large[t](i, lengths[t]) for i in range(m)) for m in limits])
+            for c in sorted({0, copies // 2, copies - 1}):
+                one = got[c, at:at + n]
+                assert np.all(np.isfinite(one)) and np.all(np.abs(one - out) <= off)
+                if not np.all(sees):
+                    check(one[~sees], out[~sees], off[~sees], f"format {fmt}, table {t}, copy {c}, weighs {weighs}")
+            at += n
