@@ -371,10 +371,11 @@ int tah_pages_read_dev(tah_dev *dev, const tah_pages *p, const int32_t *starts, 
  * h / (heads / kv_heads); kv_heads divides heads. out [nq][heads * hd], before the output projection; queries from
  * offsets[tables] on are left as they were. Rows on no page are not seen (a length counts as no more than ld * page_rows);
  * a query that sees none gives zeros. A number that is not finite makes NaN of the outputs that see it, and of no others: a key
- * of its head's, a value of its own coordinate's. Rows that a query does not see take none of its precision; a
- * term is off by 2^-22 of itself, or by 2^-37 of the largest in the 64 rows around it that the query sees, whichever is more. Scores
- * of magnitude 2^22 and more have no fractions that count, and may give NaN, as in tah_attend. The _dev form takes every array in device memory as above (lengths and
- * offsets may change between replays of a captured call); the other takes them in host memory, but for the pool, and refuses
+ * of its head's, a value of its own coordinate's. Rows that a query does not see take none of its precision; a key's or value's
+ * number is held to 2^-22 of itself, 2^-26 of its row's largest or 2^-37 of the largest in the 64 rows around it that the query
+ * sees, whichever is most. Scores of magnitude 2^22 and more have no fractions that count, and may give NaN, as in tah_attend.
+ * The _dev form takes every array in device memory as above (lengths and offsets may change between replays of a captured
+ * call); the other takes them in host memory, but for the pool, and refuses
  * lengths over ld * page_rows or of rows on no page with TAH_E_ARG. */
 int tah_pages_attend(tah_dev *dev, const tah_pages *p, const int32_t *lengths, const float *q, const int32_t *offsets,
                      int32_t nq, int32_t heads, int32_t causal, int64_t q_ld, float *out);

@@ -234,6 +234,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
         int limit[CT];
         floatx4 acc[CT][M];
         int lim_most = 0, lim_least = tw.len;
+        bool small = false;  // ints: queries so small that keys' steps may be as large as a product with them does not hold
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             const int col = tile * COLS + 16 * ct + qi, i = col / group;
@@ -271,6 +272,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                     }
                 }
             to_log2[ct] = (BYTES ? 256.0f : 1.0f) * LOG2E * pow2(-eq);
+            small = small || (INTS && most > 0.0f && eq > 60);
             ref[ct] = vunit[ct] = -INFINITY;
             base[ct] = gap[ct] = l[ct] = 0.0f;
 #pragma unroll
@@ -287,6 +289,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
             lim_most = max(lim_most, __shfl_xor(lim_most, d));
             lim_least = min(lim_least, __shfl_xor(lim_least, d));
         }
+        small = __any(small);
         lim_most = __builtin_amdgcn_readfirstlane(lim_most);
         lim_least = __builtin_amdgcn_readfirstlane(lim_least);
         const int last = min((int)b1, (lim_most + KEYS - 1) / KEYS);  // blocks behind every column's limit are not looked at
@@ -493,16 +496,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                 auto in_log2 = [&](float unk) { return fminf(fmaxf(to_log2[ct] * unk, 0x1p-126f), 0x1p126f); };
                 float f = INTS ? to_log2[ct] : in_log2(pow2(-ek));
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    x[j] = sc[j >> 2][ct][j & 3];
-                    if constexpr (INTS) x[j] *= stk[j >> 2][j & 3];
-                }
-                if constexpr (!INTS)
-                    if (in_part) {
-                        f = 1.0f;
+                for (int j = 0; j < N; j++) x[j] = sc[j >> 2][ct][j & 3];
+                if (INTS ? small : in_part) {  // the factors first
+                    f = 1.0f;
 #pragma unroll
-                        for (int j = 0; j < N; j++) x[j] *= in_log2(steps_here[wave][0][N * lg + j]);
-                    }
+                    for (int j = 0; j < N; j++) x[j] *= INTS ? stk[j >> 2][j & 3] * to_log2[ct] : in_log2(steps_here[wave][0][INTS ? 0 : N * lg + j]);
+                } else if constexpr (INTS) {
+#pragma unroll
+                    for (int j = 0; j < N; j++) x[j] *= stk[j >> 2][j & 3];
+                }
                 if (!all_seen) {
                     const int seen = min(here, min(max(limit[ct] - kv, 0), N));
 #pragma unroll

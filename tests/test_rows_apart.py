@@ -266,3 +266,27 @@ def test_pages_blocks_apart(gpu, dev, fmt, hd, group, copies):
                 if not np.all(sees):
                     check(one[~sees], out[~sees], off[~sees], f"format {fmt}, table {t}, copy {c}, weighs {weighs}")
             at += n
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hd,group,causal", [(64, 1, False), (64, 20, True), (128, 2, True)])
+def test_pages_small_queries_of_large_keys(gpu, dev, fmt, hd, group, causal):
+    """Scores of ordinary size, of queries of 1e-34 and keys of 1e34, beside a table of ordinary ones and queries of zeros."""
+    rng = np.random.default_rng(hd)
+    lengths, counts = [150, 90, 70], [4, 3, 2]
+    table = rng.permutation(9).astype(np.int32).reshape(3, 3)
+    pool = P.Pool(fmt, 1, hd, 64, 9, fill=0xFF)
+    q = (rng.standard_normal((sum(counts), group, hd)) * 0.4).astype(np.float32)
+    q[:4] *= np.float32(1e-34)
+    q[8] = 0.0
+    for t, n in enumerate(lengths):
+        for i in range(n):
+            k, v = values(rng, 1, 1, hd)[0], values(rng, 1, 1, hd)[0]
+            pool.write(table[t, i // 64], i % 64, k * np.float32(1e34 if t == 0 else 1.0), v)
+    card = dev.of(pool.bytes)
+    got = gpu.pages_attend(described(pool, 3, 3, card.ptr), table, lengths, flat(q), offsets_of(counts), group, causal).reshape(q.shape)
+    at = 0
+    for t, n in enumerate(counts):
+        out, off = P.attention(q[at:at + n], *pool.rows_of(table[t], lengths[t]), P.limits_of(lengths[t], n, causal))
+        check(got[at:at + n], out, off, f"format {fmt}, table {t}", 3 * 1.3e-6)
+        at += n
