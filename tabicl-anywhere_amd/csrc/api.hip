@@ -1230,7 +1230,7 @@ extern "C" int tah_attend_packed_dev(tah_dev *dev, const float *q, const float *
         if (!aligned4({q, k, v, q_offsets, kv_offsets, out})) throw ArgError{"attend_packed: the pointers have to be 4-byte aligned"};
         if (nq == 0) return TAH_OK;
         Loans loans(dev);
-        void *work = loans.take<uint8_t>(packed_work_bytes(a));
+        void *work = loans.take<uint8_t>(packed_work_bytes(a, (size_t)kv_ld));
         packed_attention(dev->stream, a, q, k, v, q_offsets, kv_offsets, (size_t)q_ld, (size_t)kv_ld, out, work);
         return TAH_OK;
     });
@@ -1252,7 +1252,7 @@ extern "C" int tah_attend_packed(tah_dev *dev, const float *q, const float *k, c
         float *qd = loans.take<float>(a.nq * qw), *od = loans.take<float>(a.nq * qw);
         float *kd = loans.take<float>(a.nkv * kw), *vd = loans.take<float>(a.nkv * kw);
         int32_t *qo = loans.take<int32_t>(tables + (size_t)1), *ko = loans.take<int32_t>(tables + (size_t)1);
-        void *work = loans.take<uint8_t>(packed_work_bytes(a));
+        void *work = loans.take<uint8_t>(packed_work_bytes(a, kw));
         auto rows_in = [&](float *to, const float *from, int rows, size_t width, int64_t ld) {
             if (rows > 0)
                 TAH_HIP(hipMemcpy2DAsync(to, width * 4, from, (size_t)ld * 4, width * 4, rows, hipMemcpyHostToDevice, dev->stream));

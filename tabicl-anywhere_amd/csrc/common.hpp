@@ -309,7 +309,7 @@ struct PackedShape {
     int tables, nq, nkv, heads, kv_heads, hd;
     bool causal;
 };
-size_t packed_work_bytes(const PackedShape &a);
+size_t packed_work_bytes(const PackedShape &a, size_t kv_ld);
 void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const float *k, const float *v, const int32_t *q_offsets,
                       const int32_t *kv_offsets, size_t q_ld, size_t kv_ld, float *out, void *work);
 

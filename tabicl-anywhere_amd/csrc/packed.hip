@@ -36,7 +36,7 @@ struct Packed {
     // if a value is not finite), the rows' own (64 of the keys, 64 of the values), which keys of each coordinate hold values that are
     // not finite; the attention's plan, and per table its first block of rows, and for one head the tiles of queries of the tables
     // before it and those tiles' blocks (tables + 1)
-    int blocks;  // room for so many
+    int blocks;  // room for so many tiles of a head
     uint8_t *tiles;
     int *shifts;
     int8_t *row_shifts;
@@ -56,26 +56,6 @@ struct Packed {
 __device__ __forceinline__ int rows_of(const int32_t *offsets, int t, int rows, int &a) {
     a = min(max(offsets[t], 0), rows);
     return min(max(offsets[t + 1], a), rows) - a;
-}
-
-// The table whose units (size units of its rows) hold unit `at` of all: its number (-1 if there are fewer), and `at` within it.
-// Every lane of a wavefront calls it.
-__device__ __forceinline__ int table_with(const int32_t *offsets, int tables, int rows, int size, uint32_t at, uint32_t &within) {
-    const int lane = threadIdx.x & 63;
-    uint64_t before = 0;
-    for (int t0 = 0; t0 < tables; t0 += 64) {
-        int a = 0;
-        const uint32_t c = t0 + lane < tables ? (uint32_t)((rows_of(offsets, t0 + lane, rows, a) + size - 1) / size) : 0;
-        const uint64_t sum = before + wave_scan(c);  // of 64 tables: below 2^32
-        const uint64_t past = __ballot(sum > at);
-        if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            within = at - (uint32_t)__shfl(sum - c, l);
-            return __builtin_amdgcn_readfirstlane(t0 + l);
-        }
-        before = __shfl(sum, 63);
-    }
-    return -1;
 }
 
 // What beginning and ending a unit costs, in blocks of heads padded to D (8,000 rows in order, 8 heads of 64 that share their keys, 260,
@@ -129,6 +109,33 @@ __device__ __forceinline__ bool few_readers(const Packed &p, int n_q) {
     return p.direct && (int64_t)((n_q + (1 << log) - 1) >> log) * ((p.heads / p.kv_heads) >> p.log_share) <= READERS;
 }
 
+// Blocks that are made into tiles, of a table of n_q queries and n_k rows.
+__device__ __forceinline__ uint32_t tiled_blocks(const Packed &p, int n_q, int n_k) {
+    return few_readers(p, n_q) ? 0 : (uint32_t)((n_k + KB - 1) / KB);
+}
+// `first` of a table whose tiles are past the room that the offsets' promise gives: its queries see no rows
+constexpr uint32_t NO_ROOM = 0x7fffffff;
+
+// The table that tile `at` of all is of: its number (-1 if there are fewer), and the block of its rows. Every lane of a wavefront calls it.
+__device__ __forceinline__ int table_with(const Packed &p, uint32_t at, uint32_t &block) {
+    const int lane = threadIdx.x & 63;
+    uint64_t before = 0;
+    for (int t0 = 0; t0 < p.tables; t0 += 64) {
+        int a = 0;
+        const int t = min(t0 + lane, p.tables - 1);
+        const uint32_t c = t0 + lane < p.tables ? tiled_blocks(p, rows_of(p.qo, t, p.nq, a), rows_of(p.ko, t, p.nkv, a)) : 0;
+        const uint64_t sum = before + wave_scan(c);  // of 64 tables: below 2^32
+        const uint64_t past = __ballot(sum > at);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            block = at - (uint32_t)__shfl(sum - c, l);
+            return __builtin_amdgcn_readfirstlane(t0 + l);
+        }
+        before = __shfl(sum, 63);
+    }
+    return -1;
+}
+
 __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {  // of numbers below 2^50
     const uint32_t lo = wave_scan((uint32_t)v & 0x1ffffffu), hi = wave_scan((uint32_t)(v >> 25));
     return ((uint64_t)hi << 25) + lo;
@@ -152,12 +159,12 @@ __device__ void make_plan(const Packed &p) {
         const bool in = t0 + lane < p.tables;
         int qa = 0, ka = 0;
         const int n_q = rows_of(p.qo, t, p.nq, qa), n_t = rows_of(p.ko, t, p.nkv, ka);
-        const uint32_t nb = in ? (n_t + KB - 1) / KB : 0;
+        const uint32_t nb = in ? tiled_blocks(p, n_q, n_t) : 0;
         const uint64_t before = rows + wave_scan(nb) - nb;  // of 64 tables: below 2^32
-        if (in) p.first[t] = (uint32_t)min(before, (uint64_t)0x7fffffff);
+        const bool room = before + nb <= (uint64_t)p.blocks;
+        if (in) p.first[t] = room ? (uint32_t)before : NO_ROOM;
         rows = lane64(before + nb, 63);
-        // a table past the room that the offsets' promise gives has no rows
-        const Tiles<BEGIN> ts{n_q, before + nb <= (uint64_t)p.blocks ? n_t : 0, p.causal, log_queries};
+        const Tiles<BEGIN> ts{n_q, room ? n_t : 0, p.causal, log_queries};
         const uint64_t tiles = in ? ts.count() : 0, cost = in ? ts.before(ts.count()) : 0;
         const uint64_t tile_sum = units + wave_scan64(tiles), block_sum = blocks + wave_scan64(cost);
         if (in) {
@@ -183,7 +190,7 @@ __device__ void make_plan(const Packed &p) {
             const int t = min(t0 + lane, p.tables - 1);
             int qa = 0, ka = 0;
             const int n_q = rows_of(p.qo, t, p.nq, qa), n_t = rows_of(p.ko, t, p.nkv, ka);
-            const Tiles<BEGIN> ts{n_q, (uint64_t)p.first[t] + (n_t + KB - 1) / KB <= (uint64_t)p.blocks ? n_t : 0, p.causal, log_queries};
+            const Tiles<BEGIN> ts{n_q, p.first[t] != NO_ROOM ? n_t : 0, p.causal, log_queries};
             const uint64_t a = p.tile_sums[t];
             const uint64_t here = __ballot(t0 + lane < p.tables && own >= a && own < a + ts.count());
             if (here) {
@@ -246,10 +253,9 @@ __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     const bool values = blockIdx.z == 1;
     if (blockIdx.x == 0 && h == 0 && !values && tid < 64) p.waves == 8 ? make_plan<256, BEGIN_OF<D>>(p) : make_plan<128, BEGIN_OF<D>>(p);
     uint32_t kb = 0;
-    const int t = table_with(p.ko, p.tables, p.nkv, KB, blockIdx.x, kb);
+    const int t = table_with(p, blockIdx.x, kb);
     if (t < 0) return;
     int a = 0;
-    if (few_readers(p, rows_of(p.qo, t, p.nq, a))) return;
     const int n = min(rows_of(p.ko, t, p.nkv, a) - (int)kb * KB, KB);
     const float *src = (values ? p.v : p.k) + (size_t)(a + (int)kb * KB) * p.kv_ld + (size_t)h * p.hd;
 #pragma unroll
@@ -418,7 +424,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 ? (WAVES == 4 ? 3 : 4) : 2) voi
         first = p.first[t];
         local = in_head - sums[t];
     }
-    const int n_k = (uint64_t)first + (n_t + KB - 1) / KB <= (uint64_t)p.blocks ? n_t : 0;
+    const int n_k = first != NO_ROOM ? n_t : 0;
     const Tiles<BEGIN> ts{n_q, n_k, p.causal, log_queries};
     int tile = 0;
     if (whole) {
@@ -959,12 +965,13 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 // Wavefronts a workgroup, runs, workgroups and the working memory's parts.
 struct Plan {
     int waves, runs, blocks, d, log_share;  // d: the heads' width, padded
+    bool direct;
     int64_t grid;
     size_t tiles, shifts, row_shifts, odd, tables, part_o, part_ml, cut;
     size_t bytes() const { return tiles + shifts + row_shifts + odd + 256 + 3 * tables + part_o + part_ml + cut; }
 };
 
-Plan plan(const PackedShape &a) {
+Plan plan(const PackedShape &a, size_t kv_ld) {
     Plan r;
     r.d = a.hd <= 32 ? 32 : a.hd <= 64 ? 64 : 128;
     // tiles of 256 queries where all of a long table's are full (10,000 rows 619 -> 598 us), else of 128 (five tables of up to 6,007 rows
@@ -978,7 +985,12 @@ Plan plan(const PackedShape &a) {
     while (r.log_share < 5 && (a.heads / a.kv_heads) % (2 << r.log_share) == 0) r.log_share++;
     r.runs = r.waves == 8 ? 256 : r.d == 32 ? 768 : 512;  // what the card holds at once
     r.grid = (a.nq / (qt >> r.log_share) + (int64_t)std::min(a.tables, a.nq)) * (a.heads >> r.log_share) + r.runs + 32;
-    const int64_t blocks = a.nkv / KB + (int64_t)std::min(a.tables, a.nkv);
+    r.direct = r.d <= 64 && r.waves == 4 && kv_ld < (size_t)1 << 22;  // a block's rows within 2^30 bytes
+    // of tables that have tiles, the last one of each in part: where rows are also read where they stand, those of so many queries that
+    // more than READERS tiles of queries read them
+    const int readers = (a.heads / a.kv_heads) >> r.log_share;
+    const int64_t least = r.direct ? (int64_t)(READERS / readers) * (qt >> r.log_share) + 1 : 1;
+    const int64_t blocks = a.nkv / KB + std::min((int64_t)std::min(a.tables, a.nkv), r.direct ? a.nq / least : a.nkv);
     r.blocks = (int)blocks;
     const size_t halves = (size_t)blocks * a.kv_heads, places = 2 * (size_t)r.runs * qt;
     r.tiles = up256(halves * r.d * 512);
@@ -1004,8 +1016,8 @@ void launch(hipStream_t s, const Packed &p, const Plan &r) {
 
 }  // namespace
 
-size_t packed_work_bytes(const PackedShape &a) {
-    const Plan r = plan(a);
+size_t packed_work_bytes(const PackedShape &a, size_t kv_ld) {
+    const Plan r = plan(a, kv_ld);
     // a launch takes fewer than 2^32 threads; the tiles' has 256 a block of rows
     if ((uint64_t)r.grid * (64 * r.waves) >> 32 || r.blocks > 0x7FFFFF || a.nq > 0x7FFFFF00)
         throw ArgError{"attend_packed: more rows than a call takes: fewer tables a call"};
@@ -1014,7 +1026,7 @@ size_t packed_work_bytes(const PackedShape &a) {
 
 void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const float *k, const float *v, const int32_t *q_offsets,
                       const int32_t *kv_offsets, size_t q_ld, size_t kv_ld, float *out, void *work) {
-    const Plan r = plan(a);
+    const Plan r = plan(a, kv_ld);
     uint8_t *at = static_cast<uint8_t *>(work);
     auto carve = [&](size_t bytes) {
         uint8_t *here = at;
@@ -1034,7 +1046,7 @@ void packed_attention(hipStream_t s, const PackedShape &a, const float *q, const
     p.waves = r.waves;
     p.runs = r.runs;
     p.log_share = r.log_share;
-    p.direct = r.d <= 64 && r.waves == 4 && kv_ld < (size_t)1 << 22;  // a block's rows within 2^30 bytes
+    p.direct = r.direct;
     p.part_o = reinterpret_cast<float *>(carve(r.part_o));
     p.part_ml = reinterpret_cast<float2 *>(carve(r.part_ml));
     p.cut = reinterpret_cast<CutUnit *>(carve(r.cut));

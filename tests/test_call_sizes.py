@@ -101,3 +101,23 @@ def test_more_tiles_than_a_launch_takes_are_refused(gpu):
         offsets.b.free()
         q.b.free()
         k.free()
+
+
+def test_many_tables_of_a_row(gpu):
+    """65,536 tables of a row each, 8 heads of 64: within the default working memory, of which tiles of 64 rows a table would take 17
+    GB. Each query's answer is its row."""
+    tables, heads, hd = 65536, 8, 64
+    rng = np.random.default_rng(3)
+    v = rng.standard_normal((tables, heads * hd)).astype(np.float32)
+    at = np.arange(tables + 1, dtype=np.int32)
+    before = gpu.work_budget()
+    gpu.release()
+    gpu.set_work_budget(16 << 30)
+    try:
+        got = gpu.attend_packed(v[::-1], v, v, at, heads, heads, True)
+    finally:
+        gpu.set_work_budget(before)
+    # A number and its weight in two halves each, off by 2^-11 2^-11 of themselves, and the product of their low halves left out, 2^-11
+    # 2^-11: 3 x 2^-22; three products added, a reciprocal (two units) and two products in f32: 7 x 2^-24; 2^-39 of the row's largest
+    # (below 8) where a low half is below fp16's normal numbers.
+    assert np.all(np.abs(got - v) <= (3 * 2.0**-22 + 7 * 2.0**-24) * np.abs(v) + 2.0**-36)
