@@ -290,3 +290,51 @@ def test_pages_small_queries_of_large_keys(gpu, dev, fmt, hd, group, causal):
         out, off = P.attention(q[at:at + n], *pool.rows_of(table[t], lengths[t]), P.limits_of(lengths[t], n, causal))
         check(got[at:at + n], out, off, f"format {fmt}, table {t}", 3 * 1.3e-6)
         at += n
+
+
+@pytest.mark.parametrize("counts,heads,kv_heads,hd,causal", [
+    ([4300], 1, 1, 64, False), ([4300], 2, 1, 32, False), ([2300], 2, 1, 128, True), ([2300], 1, 1, 128, False), ([900, 130], 2, 2, 64, True),
+    ([900, 130], 2, 1, 32, False), ([600, 130], 1, 1, 128, True)])
+def test_packed_rows_of_all_sizes(gpu, counts, heads, kv_heads, hd, causal):
+    """Keys and values of sizes 2^-20 to 1 from row to row, in tiles of 256 and of 128 columns, blocks of even rows before, between and
+    behind."""
+    rng = np.random.default_rng(hd + heads)
+    n = sum(counts)
+    q, k, v = inputs(rng, n, n, heads, kv_heads, hd)
+    f = np.exp2(-rng.integers(0, 21, (2, n, 1, 1))).astype(np.float32)
+    f[:, np.arange(n) // 64 % 5 < 2] = 1.0
+    k, v = k * f[0], v * f[1]
+    got = gpu.attend_packed(flat(q), flat(k), flat(v), offsets_of(counts), heads, kv_heads, causal).reshape(q.shape)
+    some = np.unique(np.concatenate([np.arange(0, n, 31), [n - 1]])) if n > 2000 else np.arange(n)
+    at = 0
+    for c in counts:
+        mine = some[(some >= at) & (some < at + c)]
+        limits = P.limits_of(c, c, causal)
+        out, off = P.attention(q[mine], k[at:at + c], v[at:at + c], [limits[i - at] for i in mine])
+        check(got[mine], out, off, f"{c} rows, heads of {hd}, causal {causal}")
+        at += c
+
+
+@pytest.mark.parametrize("counts,heads,kv_heads,hd", SHAPES)
+def test_packed_rows_apart_and_numbers_that_are_not_finite(gpu, counts, heads, kv_heads, hd):
+    """In order, in one block: a value that is not finite, a key that is not finite and a large row, each behind the other."""
+    rng = np.random.default_rng(hd)
+    n = sum(counts)
+    q, k, v = inputs(rng, n, n, heads, kv_heads, hd)
+    clean_k, clean_v = k.copy(), v.copy()
+    sees_value, sees_key = np.zeros(n, bool), np.zeros(n, bool)
+    blind = np.zeros(n, bool)
+    for a, b in by_tables(counts):
+        v[a + 70, 0, 7], v[a + 75] = np.inf, v[a + 75] * np.float32(1e10)
+        k[a + 80, 0, 3] = np.nan
+        sees_value[a + 70:b], sees_key[a + 80:b], blind[a:a + 70] = True, True, True
+        clean_v[a + 75] *= np.float32(1e10)
+    got = gpu.attend_packed(flat(q), flat(k), flat(v), offsets_of(counts), heads, kv_heads, True).reshape(q.shape)
+    out, off = wanted(q, clean_k, clean_v, counts, counts, True)
+    check(got[blind], out[blind], off[blind], f"{counts}, heads of {hd}")
+    group = heads // kv_heads
+    first = np.arange(heads) < group  # the heads that read the one with such numbers
+    nan = np.zeros(q.shape, bool)
+    nan[:, first, 7] |= sees_value[:, None]
+    nan[:, first] |= sees_key[:, None, None]
+    assert np.all(np.isnan(got[nan])) and np.all(np.abs(got - out)[~nan] <= off[~nan])
