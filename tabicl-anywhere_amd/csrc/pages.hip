@@ -174,9 +174,9 @@ struct Words {
     static constexpr int N = page_width(FMT), ROW = TILE * N / 4 + (N == 4 ? 4 : N);
 };
 
-// the first row of a workgroup: grid (rows / 64 of a part, heads, keys and values of each part), parts where rows are too many for
-// one dimension
-__device__ __forceinline__ int first_row() { return (int)(((blockIdx.z >> 1) * gridDim.x + blockIdx.x) * TILE); }
+// the first row of a workgroup: grid (rows / 64 of a part, heads, keys and values of each part), parts of part_rows where rows are too
+// many for one dimension. The last ones may have none: all are looked at as rows behind the last.
+__device__ __forceinline__ int first_row(int part_rows) { return (int)((blockIdx.z >> 1) * (uint32_t)part_rows + blockIdx.x * TILE); }
 
 // grid (rows / 64, heads, keys and values); 256 threads: four rows and four of each 64 coordinates a lane, sixteen lanes a row.
 // Bound by bytes: 40 tables of up to 1,500 rows, 4 heads of 128 to i16 (180 MB) take 44 us, at the rate of a large copy 35;
@@ -186,15 +186,14 @@ __device__ __forceinline__ int first_row() { return (int)(((blockIdx.z >> 1) * g
 template <int FMT, int C>
 __global__ __launch_bounds__(256) void k_pages_write(PageSet p, const int32_t *__restrict__ starts,
                                                      const int32_t *__restrict__ offsets, const float *__restrict__ k,
-                                                     const float *__restrict__ v, int rows, size_t row_ld) {
+                                                     const float *__restrict__ v, int rows, size_t row_ld, int part_rows) {
     typedef typename Number<FMT>::T T;
     constexpr int N = Words<FMT>::N, ROW = Words<FMT>::ROW, W = page_width(FMT), RUN = 16 / W;
     __shared__ uint32_t tile[64 * C][ROW];
     __shared__ Places pl;
     const int tid = threadIdx.x, l16 = tid & 15, quad = tid >> 4, h = blockIdx.y;
     const bool values = blockIdx.z & 1;
-    const int r0 = first_row(), hd = p.hd, P = p.rows;
-    if (r0 >= rows) return;
+    const int r0 = first_row(part_rows), hd = p.hd, P = p.rows;
     const float *src = (values ? v : k) + (size_t)h * hd;
     floatx4 x[4][C];
 #pragma unroll
@@ -280,15 +279,14 @@ __global__ __launch_bounds__(256) void k_pages_write(PageSet p, const int32_t *_
 template <int FMT, int C>
 __global__ __launch_bounds__(256) void k_pages_read(PageSet p, const int32_t *__restrict__ starts,
                                                     const int32_t *__restrict__ offsets, float *__restrict__ k,
-                                                    float *__restrict__ v, int rows, size_t row_ld) {
+                                                    float *__restrict__ v, int rows, size_t row_ld, int part_rows) {
     typedef typename Number<FMT>::T T;
     constexpr int N = Words<FMT>::N, ROW = Words<FMT>::ROW, W = page_width(FMT), RUN = 16 / W, RUNS = TILE / RUN;
     __shared__ uint32_t tile[64 * C][ROW];
     __shared__ Places pl;
     const int tid = threadIdx.x, l16 = tid & 15, quad = tid >> 4, h = blockIdx.y;
     const bool values = blockIdx.z & 1;
-    const int r0 = first_row(), hd = p.hd, P = p.rows;
-    if (r0 >= rows) return;
+    const int r0 = first_row(part_rows), hd = p.hd, P = p.rows;
     find_places(p, starts, offsets, r0, rows, pl);
     const uint8_t *head = p.pool + (size_t)h * p.head_bytes;
     if (values) {
@@ -364,10 +362,11 @@ void launch_rows(hipStream_t s, const PageSet &p, const int32_t *starts, const i
     // fewer than 2^32 threads in a dimension
     const int tiles = (rows + TILE - 1) / TILE, parts = tiles / MOST_TILES + 1;
     const dim3 grid((tiles + parts - 1) / parts, p.heads, 2 * parts);
+    const int part_rows = (int)grid.x * TILE;
     if (write)
-        hipLaunchKernelGGL((k_pages_write<FMT, C>), grid, dim3(256), 0, s, p, starts, offsets, k, v, rows, row_ld);
+        hipLaunchKernelGGL((k_pages_write<FMT, C>), grid, dim3(256), 0, s, p, starts, offsets, k, v, rows, row_ld, part_rows);
     else
-        hipLaunchKernelGGL((k_pages_read<FMT, C>), grid, dim3(256), 0, s, p, starts, offsets, k, v, rows, row_ld);
+        hipLaunchKernelGGL((k_pages_read<FMT, C>), grid, dim3(256), 0, s, p, starts, offsets, k, v, rows, row_ld, part_rows);
     TAH_LAUNCHED();
 }
 

@@ -665,17 +665,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
     }
 }
 
-// grid (queries x heads, over 4 / PER; in rows of MOST_WGS where there are more); 256 threads: the states that runs of blocks left of a query and head, together: PER
+// grid (queries x heads, over 4 / PER; in rows of `row` where they are more than MOST_WGS); 256 threads: the states that runs of blocks left of a query and head, together: PER
 // wavefronts for each query and head, every PER-th state each. Four where there are few (a state after the other takes longest:
 // the call of one query of 8 heads over 100,000 rows 33 us, with one 42; 7 tables of up to 9,000 23.6 and 27.5), one where there
 // are many (their number does: 24 tables, up to 9 queries each, of 16 heads 62.4 us, with four 65.6). The launch is most of it.
 template <int CT, int PER>
 __global__ __launch_bounds__(256) void k_pages_join(int tables, int hd, const int32_t *__restrict__ offsets, int items,
-                                                    int heads, float *__restrict__ out, Parts parts) {
+                                                    int heads, float *__restrict__ out, Parts parts, uint32_t row) {
     constexpr int COLS = 16 * CT, AHEAD = 8;
     __shared__ float wm[4], wl[4], wo[4][128];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t nth = PER == 4 ? blockIdx.x : (blockIdx.y * gridDim.x + blockIdx.x) * 4 + wave;
+    const uint32_t nth = PER == 4 ? blockIdx.x : (blockIdx.y * row + blockIdx.x) * 4 + wave;
     if (nth >= (uint32_t)items) return;
     const int item = (int)nth, part = PER == 4 ? wave : 0;
     const uint4 unit = parts.units[item];
@@ -802,11 +802,11 @@ void launch(hipStream_t s, const PageSet &p, const int32_t *lengths, const float
     TAH_LAUNCHED();
     const int items = nq * heads;
     if (items <= 1024) {
-        hipLaunchKernelGGL((k_pages_join<CT, 4>), dim3(items), dim3(256), 0, s, p.tables, p.hd, offsets, items, heads, out, parts);
+        hipLaunchKernelGGL((k_pages_join<CT, 4>), dim3(items), dim3(256), 0, s, p.tables, p.hd, offsets, items, heads, out, parts, 0u);
     } else {
-        const int wgs = (items + 3) / 4, rows = (wgs + MOST_WGS - 1) / MOST_WGS;
-        hipLaunchKernelGGL((k_pages_join<CT, 1>), dim3((wgs + rows - 1) / rows, rows), dim3(256), 0, s, p.tables, p.hd, offsets, items,
-                           heads, out, parts);
+        const int wgs = (items + 3) / 4, rows = (wgs + MOST_WGS - 1) / MOST_WGS, row = (wgs + rows - 1) / rows;
+        hipLaunchKernelGGL((k_pages_join<CT, 1>), dim3(row, rows), dim3(256), 0, s, p.tables, p.hd, offsets, items, heads, out, parts,
+                           (uint32_t)row);
     }
     TAH_LAUNCHED();
 }
