@@ -388,7 +388,9 @@ int tah_pages_attend_dev(tah_dev *dev, const tah_pages *p, const int32_t *length
  * sees all of its rows, each one before it one less. Heads, rows that see nothing, numbers that are not finite, precision and rows
  * past the last table as for tah_pages_attend; hd a multiple of 16 up to 128. Offsets [tables + 1] run from 0 up; they may be the
  * same array. The _dev form takes every array in device memory (4-byte aligned); the other in host memory, and refuses offsets
- * that fall or pass nq or nkv. */
+ * that fall or pass nq or nkv. Working memory: about the keys' and values' own size (for heads over 64 wide that of at
+ * least 64 rows a table) and up to 70 MB. Calls of more tiles than a launch takes (2^24 of 128 queries and heads that share keys, a table's last one in part)
+ * are refused. */
 int tah_attend_packed(tah_dev *dev, const float *q, const float *k, const float *v, const int32_t *q_offsets,
                       const int32_t *kv_offsets, int32_t tables, int32_t nq, int32_t nkv, int32_t heads, int32_t kv_heads,
                       int32_t hd, int32_t causal, int64_t q_ld, int64_t kv_ld, float *out);

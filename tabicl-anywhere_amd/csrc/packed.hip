@@ -242,7 +242,7 @@ __device__ __forceinline__ uint32_t lanes_most(uint32_t v) {
 
 // grid (blocks, key/value heads, keys and values); 256 threads: one half tile. Scaled by the power of two that brings its own
 // largest finite number below 2^14, or each row by one of its own (APART). A value that is not finite is a zero in the tile, and its
-// bit is set in `odd`. Bound by bytes: 10,000 rows of 8 heads of 64, 41 MB read and 41 written, 15.6 us, 5.2 TB/s.
+// bit is set in `odd`. Bound by bytes: 10,000 rows of 8 heads of 64, 41 MB read and 41 written, 16.7 us at least (median 17.9), 4.9 TB/s.
 template <int D>
 __global__ __launch_bounds__(256) void k_packed_tiles(Packed p) {
     __shared__ float x[KB][D + 1];
@@ -343,20 +343,21 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const float *p, uint
 // rounds of them are a workgroup's each (all of them where units are short); the blocks of the others, one unit after the other, are
 // cut into equal runs, which end together, for tables of any lengths, causal or not. A run that is not a whole unit leaves a state for
 // k_packed_join. One table of 10,000 rows and 8 heads, 632 units on 512 places: two rounds 720 us, everything in runs 840 (workgroups
-// of an XCD then read different keys at a time, more than its cache holds; whole units read the same ones), as it is 619 (557 with what
+// of an XCD then read different keys at a time, more than its cache holds; whole units read the same ones), as it is 619 (564 with what
 // follows).
 //
 // S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_32x32x16_f16, three products of halves a term, the keys in sigma32 order so that
 // the weights of a block are the values' operand where they stand. Tiles come by DMA into two LDS buffers each for keys and values,
 // a block ahead (one each where two would leave one workgroup of four wavefronts a compute unit), or are made here from rows read a
 // block ahead (few_readers). The softmax is in log2 units against a reference that is raised when a block passes it by more than 3;
-// weights stay below 2^15. A column's sums of values are held in units of their own, 2^(12 - unit): the unit is raised, as the reference is, when a
-// block's largest weight times its values' power of two passes it by more than 3, so that what a column does not see, or gives no
-// weight, takes none of its precision; the block's weights are taken smaller or larger by the difference.
+// weights stay below 2^15. A column's sums of values are held in units of their own, 2^(unit - 12): the unit is raised, as the
+// reference is, when a block's largest weight times its values' power of two passes it by more than 3, so that what a column does not
+// see, or gives no weight, takes none of its precision; the block's weights are taken smaller or larger by the difference.
 //
-// In a long table the matrix pipes are busy 61% of the time and the vector pipes 48%, hardly ever at once:
-// 10,000 rows, 8 heads of 64, 557 us or 1,103 TFLOP/s of the three products, what a large fp16 product reaches here (1,109). Short
-// tables are bound by their start (plan, rows and queries on their way: about 9 us) and by memory.
+// In a long table the matrix pipes are busy 60% of the time and the vector pipes 49%, hardly ever at once: 10,000 rows, 8 heads of 64,
+// 564 us or 1,089 TFLOP/s of the three products, what a large fp16 product reaches here (1,109). Short tables are bound by their start
+// (plan, rows and queries on their way: about 9 us) and by memory. Columns' own units cost a long table 1% (558 us without), looking
+// for rows that lie apart a short one in order 3% (200 of 50 to 100 rows 58 and 60 us; heads of 32 38 and 41, registers).
 template <int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D == 32 ? (WAVES == 4 ? 3 : 4) : 2) void k_packed(Packed p) {
     constexpr int QT = 32 * WAVES, HALF = HALF_BYTES<D>, DC = D / 16, DB = D / 32, BEGIN = BEGIN_OF<D>;
@@ -700,7 +701,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 32 ? (WAVES == 4 ? 3 : 4) : 2) voi
     };
     // Block kb from the buffers kc and vc, the next one on its way into kn and vn: four arrays, so that the compiler sees that it need
     // not wait for the copies before it reads.
-    auto step = [&](const uint8_t *kc, const uint8_t *vc, uint8_t *kn, uint8_t *vn, int kb, int eko, int evo) __attribute__((always_inline)) {
+    auto step = [&](const uint8_t *kc, const uint8_t *vc, uint8_t *kn, uint8_t *vn, int kb, int eko,
+                    int evo) __attribute__((always_inline)) {
         __builtin_amdgcn_s_waitcnt(0);  // this wavefront's copies of block kb have landed
         __syncthreads();                // everyone's have, and block kb - 1's buffers are no longer read
         if (kb + 1 < kb1) {
@@ -976,8 +978,8 @@ Plan plan(const PackedShape &a, size_t kv_ld) {
     r.d = a.hd <= 32 ? 32 : a.hd <= 64 ? 64 : 128;
     // tiles of 256 queries where all of a long table's are full (10,000 rows 619 -> 598 us), else of 128 (five tables of up to 6,007 rows
     // in order 513, with 256 534). Heads over 64 wide: 256 at one workgroup a compute unit or, where tables are short, 128 at two,
-    // with one buffer each for keys and values (100 of up to 300 rows, in order, 155 -> 139 us, 32 of up to 300 66 -> 54; 8,000 rows 357
-    // and 373).
+    // with one buffer each for keys and values (100 of up to 300 rows, in order, 155 -> 139 us, 32 of up to 300 66 -> 54; 8,000
+    // rows, 4 heads, 357 and 373).
     r.waves = (r.d == 128 ? a.nq / 2048 >= a.tables : !a.causal && a.nq / 4096 >= a.tables) ? 8 : 4;
     const int qt = 32 * r.waves;
     // heads that share their keys share tiles too, by powers of two up to a wavefront's columns

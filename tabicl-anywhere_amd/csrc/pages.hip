@@ -179,10 +179,10 @@ struct Words {
 __device__ __forceinline__ int first_row(int part_rows) { return (int)((blockIdx.z >> 1) * (uint32_t)part_rows + blockIdx.x * TILE); }
 
 // grid (rows / 64, heads, keys and values); 256 threads: four rows and four of each 64 coordinates a lane, sixteen lanes a row.
-// Bound by bytes: 40 tables of up to 1,500 rows, 4 heads of 128 to i16 (180 MB) take 44 us, at the rate of a large copy 35;
-// without its stores the kernel takes 25 us (the reads at 4.7 TB/s), without its arithmetic 2 to 4 less. Values are turned in LDS, so
-// that a page's rows of one coordinate are stored 16 bytes at a time. The floats pass the caches by, here and in k_pages_read (written
-// and read back 92 -> 78 us, 10,000 rows of 8 heads of 64 in i8 24.3 -> 24.0): what is wanted next is the pages.
+// Bound by bytes: 40 tables of up to 1,500 rows, 4 heads of 128 to i16 (180 MB) take 43 us at least (median 47), at the rate of a large
+// copy 35; without its stores the kernel takes 25 us (the reads at 4.7 TB/s), without its arithmetic 2 to 4 less. Values are turned in
+// LDS, so that a page's rows of one coordinate are stored 16 bytes at a time. The floats pass the caches by, here and in k_pages_read
+// (written and read back 92 -> 78 us, 10,000 rows of 8 heads of 64 in i8 24.3 -> 24.0): what is wanted next is the pages.
 template <int FMT, int C>
 __global__ __launch_bounds__(256) void k_pages_write(PageSet p, const int32_t *__restrict__ starts,
                                                      const int32_t *__restrict__ offsets, const float *__restrict__ k,

@@ -132,10 +132,11 @@ __device__ __forceinline__ floatx4 mfma(halfx8 a, halfx8 b, floatx4 c) {
 // so that rows that it does not see, or gives no weight, take none of its precision. f32: where columns do not see
 // the same rows of a block each row has a power of two of its own, as ints have their steps.
 //
-// Bound by bytes where tables are long: 64 of up to 20,000 rows, 8 heads of 64 in i8, one query each, 133 us of kernel for 702 MB, 5.3
-// TB/s, what a large copy reaches (vector instructions issue in 55% of the cycles, matrix instructions in 14%). One table of 100,000
-// rows, 28 us, has 3.1 blocks a wavefront: the start (lengths, plan, queries, the first keys and their steps, one after the other)
-// is 8 us of it, all that 1,000 rows take. i16's four products of 16 columns twice and f32's splitting cost more than their bytes.
+// Bound by bytes where tables are long: 64 of up to 20,000 rows, 8 heads of 64 in i8, one query each, 132 us of kernel at least (median
+// 140) for 702 MB, 5.3 TB/s, what a large copy reaches (vector instructions issue in 53% of the cycles, matrix instructions in 14%). One
+// table of 100,000 rows, 26 us, has 6.1 blocks a wavefront, in runs of 7: the start (lengths, plan, queries, the first keys and their
+// steps, one after the other) is 8 us of it, all that 1,000 rows take. i16's four products of 16 columns twice and f32's splitting cost
+// more than their bytes; columns past two sets read the keys again (nine queries of four heads: 36 columns, 1.4 times the bytes).
 // Tried and slower: a block's keys and values read while the one before is worked on (141 -> 153 us, the compiler has no registers
 // for both), three wavefronts a SIMD (176, spilling). Two sets of columns that share what is read: registers allow no third.
 template <int FMT, int C, int CT, int KS>
@@ -500,7 +501,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
                 if (INTS ? small : in_part) {  // the factors first
                     f = 1.0f;
 #pragma unroll
-                    for (int j = 0; j < N; j++) x[j] *= INTS ? stk[j >> 2][j & 3] * to_log2[ct] : in_log2(steps_here[wave][0][INTS ? 0 : N * lg + j]);
+                    for (int j = 0; j < N; j++)
+                        x[j] *= INTS ? stk[j >> 2][j & 3] * to_log2[ct] : in_log2(steps_here[wave][0][INTS ? 0 : N * lg + j]);
                 } else if constexpr (INTS) {
 #pragma unroll
                     for (int j = 0; j < N; j++) x[j] *= stk[j >> 2][j & 3];
@@ -665,10 +667,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_pages_attend(PageSet p, const
     }
 }
 
-// grid (queries x heads, over 4 / PER; in rows of `row` where they are more than MOST_WGS); 256 threads: the states that runs of blocks left of a query and head, together: PER
-// wavefronts for each query and head, every PER-th state each. Four where there are few (a state after the other takes longest:
-// the call of one query of 8 heads over 100,000 rows 33 us, with one 42; 7 tables of up to 9,000 23.6 and 27.5), one where there
-// are many (their number does: 24 tables, up to 9 queries each, of 16 heads 62.4 us, with four 65.6). The launch is most of it.
+// grid (queries x heads, over 4 / PER; in rows of `row` where they are more than MOST_WGS); 256 threads: the states that runs of blocks
+// left of a query and head, together: PER wavefronts for each query and head, every PER-th state each. Four where there are few (a
+// state after the other takes longest: the call of one query of 8 heads over 100,000 rows 33 us, with one 42; 7 tables of up to 9,000
+// 23.6 and 27.5), one where there are many (their number does: 24 tables, up to 9 queries each, of 16 heads 62.4 us, with four 65.6).
+// The launch is most of it.
 template <int CT, int PER>
 __global__ __launch_bounds__(256) void k_pages_join(int tables, int hd, const int32_t *__restrict__ offsets, int items,
                                                     int heads, float *__restrict__ out, Parts parts, uint32_t row) {

@@ -1,4 +1,5 @@
-"""Fitted problems in pages of one pool on the card, so that many are served together and grow a row at a time.
+"""Fitted problems in pages of one pool on the card, so that many are served together and (where rows see only those before them)
+grow a row at a time.
 
 `PagePool` is the host side of `Gpu.pages_write`, `pages_read` and `pages_attend` (`tah_pages` in tah.h): which pages are whose. A
 problem is held by `(prefix, node)` as `hip.CardAttend` holds models, from exact keys and values or from a bundle's stored
@@ -86,7 +87,9 @@ class PagePool:
         self.hold(prefix, node, layers)
 
     def grow(self, prefix: str, node: int, layers) -> None:
-        """More rows of a problem that is held (`LookupError` if it is not), as `hold` takes them, behind those it has."""
+        """More rows of a problem that is held (`LookupError` if it is not), as `hold` takes them, behind those it has. What a fit of
+        all the rows would give only where rows see those before them and no others: a network whose rows all see each other has
+        other keys and values for the rows that were there, and the problem is held anew."""
         with self._lock:
             if (prefix, node) not in self._held:
                 raise LookupError(f"no problem {prefix!r}, {node} in the pool")
