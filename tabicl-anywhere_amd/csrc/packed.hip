@@ -358,6 +358,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const float *p, uint
 // 564 us or 1,089 TFLOP/s of the three products, what a large fp16 product reaches here (1,109). Short tables are bound by their start
 // (plan, rows and queries on their way: about 9 us) and by memory. Columns' own units cost a long table 1% (558 us without), looking
 // for rows that lie apart a short one in order 3% (200 of 50 to 100 rows 58 and 60 us; heads of 32 38 and 41, registers).
+// Heads of up to 32 keep to the registers of three workgroups of four wavefronts a compute unit (10,000 rows in order 209 us, at two
+// 226), or two of eight (10,000 rows 350, at one 361).
 template <int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D == 32 ? (WAVES == 4 ? 3 : 4) : 2) void k_packed(Packed p) {
     constexpr int QT = 32 * WAVES, HALF = HALF_BYTES<D>, DC = D / 16, DB = D / 32, BEGIN = BEGIN_OF<D>;
